@@ -30,13 +30,17 @@ SYMBOLS = (
     "aicomp_rope_kv_append",
     "aicomp_rope_paged_decode_attn",
     "aicomp_rope_paged_decode_attn_sized",
+    "aicomp_qk_norm_rope_kv_append",
+    "aicomp_kv_copy_blocks",
+    "aicomp_paged_score_attn",
+    "aicomp_paged_score_workspace_bytes",
     "aicomp_sample_tokens",
     "aicomp_sample_tokens_split",
     "aicomp_sample_workspace_bytes",
 )
 
 F32, BF16, FP8_E4M3, F16 = 0, 1, 2, 3
-MIN_VERSION = 302            # 0.3.2: the entry points of SYMBOLS above
+MIN_VERSION = 400            # 0.4.0: the entry points of SYMBOLS above
 
 _lock = threading.RLock()       # torch_ops() loads the HIP library while holding it
 _lib = None
@@ -101,6 +105,16 @@ def _declare(lib: C.CDLL) -> None:
     lib.aicomp_sample_tokens.argtypes = [vp, vp, i64, vp, vp, i32, i32, f32, i32, f32, i32, i32, vp]
     lib.aicomp_sample_tokens_split.restype = i32
     lib.aicomp_sample_tokens_split.argtypes = [vp, vp, i64, vp, vp, i32, i32, f32, i32, f32, i32, i32, vp, sz, vp]
+    lib.aicomp_qk_norm_rope_kv_append.restype = i32
+    lib.aicomp_qk_norm_rope_kv_append.argtypes = [vp, vp, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, f32, vp, vp, i64, i64, i32,
+                                                  i32, vp, vp, vp, vp, i64, i32, i32, i32, i32, i64, i32, i32, vp, vp, vp]
+    lib.aicomp_kv_copy_blocks.restype = i32
+    lib.aicomp_kv_copy_blocks.argtypes = [vp, i32, i64, i64, vp, i64, vp]
+    lib.aicomp_paged_score_attn.restype = i32
+    lib.aicomp_paged_score_attn.argtypes = [vp, vp, vp, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, i32, i32, i32, i64, f32, i32,
+                                            i32, vp, vp, f32, vp, i32, vp, vp, i32, vp, sz, vp]
+    lib.aicomp_paged_score_workspace_bytes.restype = sz
+    lib.aicomp_paged_score_workspace_bytes.argtypes = [i32] * 10
     lib.aicomp_sample_workspace_bytes.restype = sz
     lib.aicomp_sample_workspace_bytes.argtypes = [i32, i32, i64, f32, i32, i32, i32]
 

@@ -2,8 +2,10 @@
 // The declarations, with the reference interfaces they replace, are in
 // include/aicomp_kv.h.
 #include "common.h"
+#include "score.h"
 
 #include <algorithm>
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -163,7 +165,7 @@ using namespace aicomp;
 
 extern "C" {
 
-int aicomp_kv_version(void) { return 302; }
+int aicomp_kv_version(void) { return 400; }
 
 const char* aicomp_kv_last_error(void) { return g_err; }
 
@@ -746,6 +748,164 @@ int aicomp_paged_prefill_tile_positions(int num_q_heads, int num_kv_heads, int h
     if (q_dtype == AICOMP_KV_F32 && kv_dtype == AICOMP_KV_F32)
         return prefill_mfma_f32_tile_positions(num_q_heads, num_kv_heads);
     return 0;
+}
+
+int aicomp_qk_norm_rope_kv_append(const void* q_in, void* q_out, int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t qo_token_stride, int64_t qo_head_stride, const void* key, const void* value,
+                                  int64_t kv_token_stride, int64_t kv_head_stride, const float* q_weight,
+                                  const float* k_weight, float eps, const float* cos, const float* sin,
+                                  int64_t table_stride, int64_t table_rows, int rotary_dim, int interleaved,
+                                  const int64_t* positions, void* k_pool, void* v_pool, const int64_t* slot_mapping,
+                                  int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int64_t num_blocks, int in_dtype, int pool_dtype, const float* k_scale,
+                                  const float* v_scale, void* stream) {
+    const char* who = "qk_norm_rope_kv_append";
+    AICOMP_REQUIRE(num_tokens >= 0, AICOMP_KV_EINVAL, "%s: negative token count", who);
+    if (num_tokens == 0) return AICOMP_KV_OK;
+    AICOMP_REQUIRE(q_in && q_out && key && value && k_pool && v_pool && slot_mapping, AICOMP_KV_EINVAL, "%s: null pointer", who);
+    AICOMP_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 && block_size > 0 && num_blocks > 0, AICOMP_KV_EINVAL,
+                   "%s: bad sizes (Hq %d, Hkv %d, D %d, BS %d, blocks %lld)", who, num_q_heads, num_kv_heads, head_dim,
+                   block_size, (long long)num_blocks);
+    AICOMP_REQUIRE(in_dtype == AICOMP_KV_F32 || is_16bit_float(in_dtype), AICOMP_KV_EUNSUPPORTED,
+                   "%s: inputs must be float32, bfloat16 or float16 (got %d)", who, in_dtype);
+    AICOMP_REQUIRE(pool_dtype == in_dtype || pool_dtype == AICOMP_KV_FP8_E4M3, AICOMP_KV_EUNSUPPORTED,
+                   "%s: pool type %d must be the input type %d or fp8-e4m3", who, pool_dtype, in_dtype);
+    AICOMP_REQUIRE(pool_dtype != AICOMP_KV_FP8_E4M3 || (k_scale && v_scale), AICOMP_KV_EINVAL,
+                   "%s: an fp8 pool needs k_scale and v_scale", who);
+    AICOMP_REQUIRE(head_dim % 16 == 0 && head_dim <= 256, AICOMP_KV_EUNSUPPORTED,
+                   "%s: head_dim %d is not a multiple of 16 up to 256", who, head_dim);
+    AICOMP_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, AICOMP_KV_EUNSUPPORTED,
+                   "%s: rotary_dim %d is not a multiple of 16 up to head_dim %d", who, rotary_dim, head_dim);
+    AICOMP_REQUIRE(rotary_dim == 0 || (cos && sin && table_rows > 0 && table_stride >= rotary_dim / 2), AICOMP_KV_EINVAL,
+                   "%s: rotary_dim %d needs cos / sin tables of %d columns", who, rotary_dim, rotary_dim / 2);
+    AICOMP_REQUIRE((!q_weight && !k_weight) || (eps >= 0.f && isfinite(eps)), AICOMP_KV_EINVAL,
+                   "%s: eps must be finite and not negative (got %g)", who, (double)eps);
+    const int64_t v = 16 / dtype_size(in_dtype);       // elements per 16 bytes
+    AICOMP_REQUIRE(q_head_stride >= head_dim && qo_head_stride >= head_dim && kv_head_stride >= head_dim &&
+                   q_token_stride >= 0 && qo_token_stride >= 0 && kv_token_stride >= 0, AICOMP_KV_EINVAL,
+                   "%s: strides overlap rows of %d elements", who, head_dim);
+    AICOMP_REQUIRE((q_token_stride | q_head_stride | qo_token_stride | qo_head_stride | kv_token_stride | kv_head_stride) % v == 0 &&
+                   (rotary_dim == 0 || table_stride % 4 == 0), AICOMP_KV_EUNSUPPORTED,
+                   "%s: strides must be multiples of %lld elements (16 bytes)", who, (long long)v);
+    AICOMP_REQUIRE(((uintptr_t)q_in | (uintptr_t)q_out | (uintptr_t)key | (uintptr_t)value | (uintptr_t)cos | (uintptr_t)sin |
+                    (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0,
+                   AICOMP_KV_EUNSUPPORTED, "%s: pointers must be 16-byte aligned", who);
+    NormRopeArgs a;
+    a.q_in = q_in; a.q_out = q_out;
+    a.q_ts = q_token_stride; a.q_hs = q_head_stride; a.qo_ts = qo_token_stride; a.qo_hs = qo_head_stride;
+    a.key = key; a.value = value; a.kv_ts = kv_token_stride; a.kv_hs = kv_head_stride;
+    a.q_weight = q_weight; a.k_weight = k_weight; a.eps = eps;
+    a.cos_tab = cos; a.sin_tab = sin; a.tab_stride = table_stride; a.tab_rows = table_rows;
+    a.rotary = rotary_dim; a.interleaved = interleaved ? 1 : 0;
+    a.positions = positions; a.k_pool = k_pool; a.v_pool = v_pool; a.slot_mapping = slot_mapping;
+    a.num_tokens = num_tokens; a.hq = num_q_heads; a.hkv = num_kv_heads; a.d = head_dim; a.bs = block_size;
+    a.num_blocks = num_blocks; a.in_dtype = in_dtype; a.pool_dtype = pool_dtype;
+    a.k_scale = k_scale; a.v_scale = v_scale; a.stream = (hipStream_t)stream;
+    return launch_qk_norm_rope_kv_append(a);
+}
+
+int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes, int64_t num_blocks, const int64_t* pairs,
+                          int64_t num_pairs, void* stream) {
+    AICOMP_REQUIRE(num_pools >= 0 && num_pairs >= 0, AICOMP_KV_EINVAL, "copy_blocks: negative sizes");
+    if (num_pools == 0 || num_pairs == 0) return AICOMP_KV_OK;
+    AICOMP_REQUIRE(pools && pairs, AICOMP_KV_EINVAL, "copy_blocks: null pointer");
+    for (int i = 0; i < num_pools; ++i)
+        AICOMP_REQUIRE(pools[i], AICOMP_KV_EINVAL, "copy_blocks: pool %d is a null pointer", i);
+    AICOMP_REQUIRE(block_bytes > 0 && num_blocks > 0, AICOMP_KV_EINVAL, "copy_blocks: bad sizes (block of %lld bytes, %lld blocks)",
+                   (long long)block_bytes, (long long)num_blocks);
+    return launch_copy_blocks(pools, num_pools, block_bytes, num_blocks, pairs, num_pairs, (hipStream_t)stream);
+}
+
+// Tokens of a row's visible keys that one workgroup of a decode call takes, and how many such partitions a row has.
+static int score_partition(const ScoreArgs& a, int longest_context, int& parts) {
+    int64_t span = (int64_t)a.max_blocks * a.bs;
+    if (longest_context > 0) span = std::min<int64_t>(span, longest_context);
+    if (a.window > 0) span = std::min<int64_t>(span, a.window);
+    int ps = 64;
+    for (int cand : {1024, 512, 256, 128})
+        if (a.rows * a.hkv * ((span + cand - 1) / cand) >= 1024) { ps = cand; break; }
+    parts = (int)std::max<int64_t>(1, std::min<int64_t>((span + ps - 1) / ps, 65535));
+    return ps;
+}
+
+static int score_shape(ScoreArgs& a, const char* who) {
+    int rc = check_common(a.hq, a.hkv, a.d, a.bs, a.max_blocks, a.num_blocks, a.q_dtype, a.kv_dtype, a.k_scale, a.v_scale, who);
+    if (rc) return rc;
+    AICOMP_REQUIRE(a.d == 64 || a.d == 128 || a.d == 256, AICOMP_KV_EUNSUPPORTED, "%s: head_dim %d not supported (64, 128, 256)",
+                   who, a.d);
+    AICOMP_REQUIRE((a.q_dtype == AICOMP_KV_F32 && a.kv_dtype == AICOMP_KV_F32) ||
+                   (is_16bit_float(a.q_dtype) && (a.kv_dtype == a.q_dtype || a.kv_dtype == AICOMP_KV_FP8_E4M3)),
+                   AICOMP_KV_EUNSUPPORTED, "%s: unsupported type pair (query %d, pool %d); supported: f32/f32, bf16/bf16, f16/f16, "
+                   "bf16/fp8, f16/fp8", who, a.q_dtype, a.kv_dtype);
+    AICOMP_REQUIRE((int64_t)a.max_blocks * a.bs <= INT32_MAX, AICOMP_KV_EINVAL, "%s: a table of %d blocks of %d tokens", who,
+                   a.max_blocks, a.bs);
+    AICOMP_REQUIRE(a.window >= 0, AICOMP_KV_EINVAL, "%s: negative window", who);
+    return AICOMP_KV_OK;
+}
+
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                          int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context) {
+    if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || block_size <= 0 ||
+        max_blocks_per_seq <= 0 || window < 0 || longest_context < 0)
+        return 0;
+    ScoreArgs a;
+    memset(&a, 0, sizeof(a));
+    a.rows = num_seqs; a.hq = num_q_heads; a.hkv = num_kv_heads; a.d = head_dim; a.bs = block_size;
+    a.max_blocks = max_blocks_per_seq; a.q_dtype = q_dtype; a.kv_dtype = kv_dtype; a.window = window;
+    int parts;
+    score_partition(a, longest_context, parts);
+    return parts > 1 ? split_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, parts) : 0;
+}
+
+int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, const void* v_pool, const int32_t* block_table,
+                            int64_t block_table_stride, const int32_t* context_lens, const int32_t* cu_q_lens, int num_seqs,
+                            int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                            int max_blocks_per_seq, int64_t num_blocks, float scale, int q_dtype, int kv_dtype,
+                            const float* k_scale, const float* v_scale, float softcap, const float* slopes, int window,
+                            const int32_t* first_keys, const int32_t* prefix_lens, int longest_context, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    const char* who = "paged_score_attn";
+    AICOMP_REQUIRE(num_seqs >= 0 && total_q >= 0, AICOMP_KV_EINVAL, "%s: negative sizes", who);
+    if (num_seqs == 0 || total_q == 0) return AICOMP_KV_OK;
+    AICOMP_REQUIRE(out && query && k_pool && v_pool && block_table && context_lens, AICOMP_KV_EINVAL, "%s: null pointer", who);
+    ScoreArgs a;
+    memset(&a, 0, sizeof(a));
+    a.out = out; a.query = query; a.k_pool = k_pool; a.v_pool = v_pool;
+    a.block_table = block_table; a.block_table_stride = block_table_stride;
+    a.context_lens = context_lens; a.cu_q_lens = cu_q_lens; a.num_seqs = num_seqs; a.rows = total_q; a.max_q_len = max_q_len;
+    a.hq = num_q_heads; a.hkv = num_kv_heads; a.d = head_dim; a.bs = block_size; a.max_blocks = max_blocks_per_seq;
+    a.num_blocks = num_blocks; a.scale = scale; a.q_dtype = q_dtype; a.kv_dtype = kv_dtype;
+    a.k_scale = kv_dtype == AICOMP_KV_FP8_E4M3 ? k_scale : nullptr;
+    a.v_scale = kv_dtype == AICOMP_KV_FP8_E4M3 ? v_scale : nullptr;
+    a.cap = softcap; a.slopes = slopes; a.window = window; a.first_keys = first_keys; a.prefix_lens = prefix_lens;
+    a.stream = (hipStream_t)stream;
+    int rc = score_shape(a, who);
+    if (rc) return rc;
+    AICOMP_REQUIRE(max_blocks_per_seq > 0 && block_table_stride >= max_blocks_per_seq, AICOMP_KV_EINVAL,
+                   "%s: block table stride %lld < width %d", who, (long long)block_table_stride, max_blocks_per_seq);
+    AICOMP_REQUIRE(isfinite(scale) && softcap >= 0.f && isfinite(softcap), AICOMP_KV_EINVAL,
+                   "%s: scale must be finite and softcap finite and not negative (got %g, %g)", who, (double)scale, (double)softcap);
+    AICOMP_REQUIRE(longest_context >= 0, AICOMP_KV_EINVAL, "%s: negative longest context", who);
+    AICOMP_REQUIRE(((uintptr_t)query | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0, AICOMP_KV_EUNSUPPORTED,
+                   "%s: pointers must be 16-byte aligned", who);
+    if (cu_q_lens != nullptr) {
+        AICOMP_REQUIRE(max_q_len > 0 && max_q_len <= total_q, AICOMP_KV_EINVAL, "%s: max_q_len %d out of range (total %lld)", who,
+                       max_q_len, (long long)total_q);
+        a.partition_size = INT32_MAX; a.num_parts = 1;
+        return launch_score_generic(a);
+    }
+    AICOMP_REQUIRE(total_q == num_seqs && prefix_lens == nullptr, AICOMP_KV_EINVAL,
+                   "%s: without cu_q_lens there is one row per sequence and no prefix", who);
+    a.partition_size = score_partition(a, longest_context, a.num_parts);
+    if (a.num_parts > 1) {
+        const size_t need = split_workspace_bytes(a.rows, a.hq, a.hkv, a.d, a.num_parts);
+        AICOMP_REQUIRE(workspace && workspace_bytes >= need, AICOMP_KV_EWORKSPACE,
+                       "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+        AICOMP_REQUIRE((uintptr_t)workspace % 16 == 0, AICOMP_KV_EINVAL, "%s: workspace must be 16-byte aligned", who);
+        const SplitWorkspace ws = split_workspace_view(workspace, a.rows, a.hq, a.hkv, a.d, a.num_parts);
+        a.ws_acc = ws.acc; a.ws_ml = ws.ml;
+    }
+    return launch_score_generic(a);
 }
 
 }  // extern "C"

@@ -332,4 +332,29 @@ int launch_rope_kv_append(const void* q_in, void* q_out, int64_t q_ts, int64_t q
                           int64_t num_blocks, int in_dtype, int pool_dtype, const float* k_scale,
                           const float* v_scale, hipStream_t stream);
 
+struct NormRopeArgs {
+    const void* q_in; void* q_out;
+    int64_t q_ts, q_hs, qo_ts, qo_hs;
+    const void* key; const void* value;
+    int64_t kv_ts, kv_hs;
+    const float* q_weight; const float* k_weight;   // NULL: no norm
+    float eps;
+    const float* cos_tab; const float* sin_tab;
+    int64_t tab_stride, tab_rows;
+    int rotary, interleaved;
+    const int64_t* positions;
+    void* k_pool; void* v_pool;
+    const int64_t* slot_mapping;
+    int64_t num_tokens;
+    int hq, hkv, d, bs;
+    int64_t num_blocks;
+    int in_dtype, pool_dtype;
+    const float* k_scale; const float* v_scale;
+    hipStream_t stream;
+};
+int launch_qk_norm_rope_kv_append(const NormRopeArgs& a);
+
+int launch_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes, int64_t num_blocks, const int64_t* pairs,
+                       int64_t num_pairs, hipStream_t stream);
+
 }  // namespace aicomp

@@ -1,4 +1,4 @@
-"""Tensor-level wrappers of the C ABI: the three native ops of the path.
+"""Tensor-level wrappers of the C ABI: the native ops of the path.
 
 ``kv_append``, ``paged_decode_attn`` and ``paged_prefill_attn`` take torch
 tensors on a ROCm device, check them the way a ``TORCH_CHECK`` would
@@ -8,7 +8,9 @@ used for device memory and streams only.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Tuple
+import ctypes
+from contextlib import nullcontext
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
@@ -710,3 +712,238 @@ def sample_tokens(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0
                                             _ptr(scratch), need, _stream(logits))
         _lib.check(rc, lib)
     return (out, probs) if return_probs else out
+
+
+# ------------------------------------------------------------------ normed heads, scores by a rule, moved blocks
+def _guard(t: torch.Tensor):
+    """The tensors' device as the current one: a launch goes to the device that is current."""
+    if t.device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _call_workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
+    """Scratch of one call: the stream's buffer, or, in a call that is recorded into a graph, memory of that graph's own (two
+    graphs may be replayed side by side, whatever stream they were recorded on)."""
+    if nbytes and torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _workspace(device, nbytes)
+
+
+def rotary_pair_tables(inv_freq: torch.Tensor, num_positions: int, attention_scaling: float = 1.0, device=None):
+    """float32 cos / sin tables ``[num_positions, R/2]`` of ``qk_norm_rope_kv_append``, one angle per rotated pair: angles
+    ``position * inv_freq`` in float64, so that those of far positions are exact to float32.  ``inv_freq [R/2]`` as the model's
+    rotary module holds it (frequencies that it scales for long contexts among them), ``attention_scaling`` its factor."""
+    device = inv_freq.device if device is None else device
+    inv = inv_freq.to(device=device, dtype=torch.float64)
+    angles = torch.arange(num_positions, device=device, dtype=torch.float64)[:, None] * inv[None, :]
+    return ((angles.cos() * attention_scaling).to(torch.float32).contiguous(),
+            (angles.sin() * attention_scaling).to(torch.float32).contiguous())
+
+
+def qk_norm_rope_kv_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_weight: Optional[torch.Tensor],
+                           k_weight: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                           positions: Optional[torch.Tensor], k_pool: torch.Tensor, v_pool: torch.Tensor,
+                           slot_mapping: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
+                           k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                           query_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Norm every head of ``query [T, Hq, D]`` and ``key [T, Hkv, D]`` (RMS, weights ``[D]`` float32; ``None``: not normed),
+    rotate the first R elements of each by their positions, and append key and ``value`` to the pools, in one launch.
+
+    ``cos`` / ``sin``: float32 tables ``[P, R/2]`` (``rotary_pair_tables``), or both ``None`` for no rotation; R is a multiple of
+    16.  Pairs are ``(j, j + R/2)``, or neighbours with ``interleaved``.  ``positions [T]`` int64 selects the row of each token
+    (``None``: row t); a token whose position is outside the tables is left alone, one whose slot is outside the pools is
+    not stored.  Computed in float32 and rounded once.  Returns the query (``query_out``, by default ``query`` itself, in place);
+    the inputs may be views into one projection output.
+    """
+    out = query if query_out is None else query_out
+    lib = _lib.load()
+    _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    nb, hkv, bs, d = _check_pools(k_pool, v_pool)
+    _req(query.dim() == 3 and key.dim() == 3 and value.shape == key.shape and out.shape == query.shape,
+         "query/query_out must be [T, Hq, D], key/value [T, Hkv, D]")
+    T, hq, dq = query.shape
+    _req(key.shape == (T, hkv, d) and dq == d,
+         f"key/value {tuple(key.shape)} and query {tuple(query.shape)} do not match pools {tuple(k_pool.shape)}")
+    _req(key.dtype == query.dtype and value.dtype == query.dtype and out.dtype == query.dtype,
+         "query, key, value and query_out must share one dtype")
+    _req(query.dtype in (torch.float32, torch.bfloat16, torch.float16), f"unsupported input dtype {query.dtype}")
+    for t, n in ((query, "query"), (out, "query_out"), (key, "key"), (value, "value")):
+        _req(t.stride(2) == 1, f"{n}: last dimension must be contiguous")
+    _req(key.stride() == value.stride(), "key and value must have equal strides")
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _req(w.dtype == torch.float32 and w.shape == (d,) and w.is_contiguous(), f"{n} must be contiguous float32 [{d}]")
+            _dev(w, query, n)
+    _req((cos is None) == (sin is None), "cos and sin come together")
+    rotary = 0
+    if cos is not None:
+        _req(cos.shape == sin.shape and cos.dim() == 2 and cos.dtype == torch.float32 and sin.dtype == torch.float32
+             and cos.stride(1) == 1 and cos.stride() == sin.stride(),
+             "cos/sin must be float32 [P, R/2] tables with equal strides")
+        rotary = 2 * cos.shape[1]
+        _req(0 < rotary <= d, f"tables of {cos.shape[1]} columns rotate {rotary} elements, head_dim is {d}")
+        _req(positions is not None or cos.shape[0] >= T, "without positions the tables need one row per token")
+        _dev(cos, query, "cos")
+        _dev(sin, query, "sin")
+    if positions is not None:
+        _req(positions.dtype == torch.int64 and positions.numel() == T and positions.is_contiguous(),
+             "positions must be contiguous int64 [T]")
+        _dev(positions, query, "positions")
+    _req(slot_mapping.dtype == torch.int64 and slot_mapping.numel() == T and slot_mapping.is_contiguous(),
+         "slot_mapping must be contiguous int64 [T]")
+    for t, n in ((key, "key"), (value, "value"), (out, "query_out"), (k_pool, "k_pool"), (slot_mapping, "slot_mapping")):
+        _dev(t, query, n)
+    _req(k_pool.dtype in (query.dtype, torch.float8_e4m3fn),
+         f"pool dtype {k_pool.dtype} must be {query.dtype} or float8_e4m3fn")
+    ks, vs = _check_scales(k_scale, v_scale, k_pool, hkv)
+    if T == 0:
+        return out
+    with _guard(query):
+        rc = lib.aicomp_qk_norm_rope_kv_append(
+            query.data_ptr(), out.data_ptr(), query.stride(0), query.stride(1), out.stride(0), out.stride(1),
+            key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), _ptr(q_weight), _ptr(k_weight), float(eps),
+            _ptr(cos), _ptr(sin), cos.stride(0) if rotary else 0, cos.shape[0] if rotary else 0, rotary, int(bool(interleaved)),
+            _ptr(positions), k_pool.data_ptr(), v_pool.data_ptr(), slot_mapping.data_ptr(), T, hq, hkv, d, bs, nb,
+            _dt(query, "query"), _dt(k_pool, "pool"), _ptr(ks), _ptr(vs), _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys, k_scale, v_scale):
+    _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    nb, hkv, bs, d = _check_pools(k_pool, v_pool)
+    _req(query.dim() == 3 and out.shape == query.shape and out.dtype == query.dtype,
+         f"out/query must both be [T, Hq, D]; got {tuple(out.shape)} and {tuple(query.shape)}")
+    T, hq, dq = query.shape
+    _req(dq == d, f"query head_dim {dq} != pool head_dim {d}")
+    _req(query.is_contiguous() and out.is_contiguous(), "query and out must be contiguous")
+    S = context_lens.numel()
+    _req(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == S
+         and block_table.stride(1) == 1, "block_table must be int32 [S, max_blocks], rows contiguous")
+    _req(context_lens.dtype == torch.int32 and context_lens.is_contiguous(), "context_lens must be contiguous int32 [S]")
+    for t, n in ((out, "out"), (k_pool, "k_pool"), (block_table, "block_table"), (context_lens, "context_lens")):
+        _dev(t, query, n)
+    if slopes is not None:
+        _req(slopes.dtype == torch.float32 and slopes.shape == (hq,) and slopes.is_contiguous(),
+             f"slopes must be contiguous float32 [{hq}]")
+        _dev(slopes, query, "slopes")
+    if first_keys is not None:
+        _req(first_keys.dtype == torch.int32 and first_keys.shape == (T,) and first_keys.is_contiguous(),
+             f"first_keys must be contiguous int32 [{T}], one entry per row")
+        _dev(first_keys, query, "first_keys")
+    ks, vs = _check_scales(k_scale, v_scale, k_pool, hkv)
+    return nb, hkv, bs, d, T, hq, S, ks, vs
+
+
+def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                            block_table: torch.Tensor, context_lens: torch.Tensor, scale: float, softcap: float = 0.0,
+                            slopes: Optional[torch.Tensor] = None, window: int = 0,
+                            first_keys: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                            v_scale: Optional[torch.Tensor] = None, longest_context: int = 0,
+                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode_attn`` for scores that follow a rule: one token per sequence, at position ``p = context_lens[b] - 1``.
+
+    ``s_j = scale q.k_j``, then ``softcap * tanh(s / softcap)`` (0: no cap), then ``- slopes[h] * (p - j)`` (``slopes [Hq]``
+    float32); visible are the last ``window`` keys (0: all) from ``first_keys[b]`` (int32) on.  A row without any is zero.
+    ``longest_context``: the host's bound of ``context_lens`` (0: the table's width); it sizes the call, no row is cut by it.
+    In place on ``out [B, Hq, D]``, on the current stream.
+    """
+    lib = _lib.load()
+    nb, hkv, bs, d, B, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
+                                                     k_scale, v_scale)
+    _req(S == B, f"{S} context lengths for {B} rows")
+    qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
+    need = lib.aicomp_paged_score_workspace_bytes(B, hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window),
+                                                  int(longest_context))
+    with _guard(query):
+        if workspace is None:
+            workspace = _call_workspace(query.device, need)
+        else:
+            _req(workspace.is_contiguous(), "workspace must be contiguous")
+            _dev(workspace, query, "workspace")
+        rc = lib.aicomp_paged_score_attn(
+            out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            block_table.stride(0), context_lens.data_ptr(), None, S, B, 1, hq, hkv, d, bs, block_table.shape[1], nb,
+            float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), int(window), _ptr(first_keys), None,
+            int(longest_context), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def score_decode_workspace_bytes(batch: int, hq: int, hkv: int, d: int, bs: int, max_blocks: int, q_dtype: torch.dtype,
+                                 kv_dtype: torch.dtype, window: int = 0, longest_context: int = 0) -> int:
+    """Scratch bytes of ``paged_score_decode_attn`` for these shapes, for a caller that passes ``workspace`` itself."""
+    return _lib.load().aicomp_paged_score_workspace_bytes(batch, hq, hkv, d, bs, max_blocks, _DT[q_dtype], _DT[kv_dtype],
+                                                          int(window), int(longest_context))
+
+
+def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                             block_table: torch.Tensor, context_lens: torch.Tensor, cu_q_lens: torch.Tensor, scale: float,
+                             max_q_len: Optional[int] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                             window: int = 0, first_keys: Optional[torch.Tensor] = None,
+                             prefix_lens: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                             v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_prefill_attn`` for scores that follow a rule: chunks ``query [T, Hq, D]`` whose rows are in the pools already.
+
+    Cap, slopes and window as in ``paged_score_decode_attn`` (the bias falls with ``|p - j|``); ``first_keys [T]`` int32 gives the
+    first key that each row sees (packed documents), ``prefix_lens [S]`` int32 a part at the start of each sequence that all
+    its rows see.  A row without visible keys is zero; rows behind the last sequence are left as they are.
+    """
+    lib = _lib.load()
+    nb, hkv, bs, d, T, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
+                                                     k_scale, v_scale)
+    _req(cu_q_lens.dtype == torch.int32 and cu_q_lens.numel() == S + 1 and cu_q_lens.is_contiguous(),
+         "cu_q_lens must be contiguous int32 [S+1]")
+    _dev(cu_q_lens, query, "cu_q_lens")
+    if prefix_lens is not None:
+        _req(prefix_lens.dtype == torch.int32 and prefix_lens.shape == (S,) and prefix_lens.is_contiguous(),
+             f"prefix_lens must be contiguous int32 [{S}]")
+        _dev(prefix_lens, query, "prefix_lens")
+    if max_q_len is None:
+        cu = cu_q_lens.cpu()
+        max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
+    if max_q_len == 0:
+        return out
+    with _guard(query):
+        rc = lib.aicomp_paged_score_attn(
+            out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            block_table.stride(0), context_lens.data_ptr(), cu_q_lens.data_ptr(), S, T, int(max_q_len), hq, hkv, d, bs,
+            block_table.shape[1], nb, float(scale), _dt(query, "query"), _dt(k_pool, "pool"), _ptr(ks), _ptr(vs),
+            float(softcap), _ptr(slopes), int(window), _ptr(first_keys), _ptr(prefix_lens), 0, None, 0, _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
+    """``pool[dst] = pool[src]`` in every pool ``[num_blocks, ...]`` of ``pools`` (the K and V pools of all layers, alike in shape
+    and type) for each (src, dst) of ``pairs [n, 2]`` int64, in one launch on the current stream.
+
+    No block may be the target of two pairs or the target of one and the source of another; pairs on the host are checked for
+    that and copied to the device, pairs on the device are taken as they are (one outside the pools is skipped).
+    """
+    lib = _lib.load()
+    _req(len(pools) > 0, "copy_blocks needs at least one pool")
+    first = pools[0]
+    _req(first.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    for t in pools:
+        _req(t.shape == first.shape and t.dtype == first.dtype and t.dim() >= 1 and t.is_contiguous(),
+             "pools must be contiguous and alike in shape and type")
+        _dev(t, first, "a pool")
+    _req(pairs.dtype == torch.int64 and pairs.dim() == 2 and pairs.shape[1] == 2, "pairs must be int64 [n, 2]")
+    n, nb = pairs.shape[0], first.shape[0]
+    if n == 0 or first.numel() == 0:
+        return
+    if not pairs.is_cuda:
+        src, dst = pairs[:, 0], pairs[:, 1]
+        _req(bool(((pairs >= 0) & (pairs < nb)).all()), f"a block of pairs is outside the pools of {nb} blocks")
+        _req(dst.unique().numel() == n, "two pairs have the same target block")
+        _req(not bool(torch.isin(dst, src).any()), "a block is the target of one pair and the source of another")
+        pairs = pairs.to(first.device)
+    _dev(pairs, first, "pairs")
+    _req(pairs.is_contiguous(), "pairs must be contiguous")
+    with _guard(first):
+        rc = lib.aicomp_kv_copy_blocks((ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools]), len(pools),
+                                       first.numel() // nb * first.element_size(), nb, pairs.data_ptr(), n, _stream(first))
+    _lib.check(rc, lib)

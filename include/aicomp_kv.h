@@ -46,7 +46,8 @@ extern "C" {
 #define AICOMP_KV_FP8_E4M3  2       /* OCP e4m3 ("e4m3fn"), max finite 448       */
 #define AICOMP_KV_F16       3       /* IEEE binary16                             */
 
-/* Library version (major*10000 + minor*100 + patch).  302 = 0.3.2: added
+/* Library version (major*10000 + minor*100 + patch).  400 = 0.4.0: added aicomp_qk_norm_rope_kv_append,
+ * aicomp_paged_score_attn, aicomp_paged_score_workspace_bytes and aicomp_kv_copy_blocks.  302 = 0.3.2: added
  * aicomp_rope_paged_decode_attn_sized and aicomp_kv_append_prefill_attn_sized.  301 = 0.3.1: added
  * aicomp_rope_paged_decode_attn and aicomp_kv_append_prefill_attn.  300 = 0.3.0: added
  * aicomp_sample_tokens_split and aicomp_sample_workspace_bytes.  200 = 0.2.0: added
@@ -474,6 +475,80 @@ int aicomp_sample_tokens_split(int64_t* out, const void* logits, int64_t row_str
                                size_t workspace_bytes, void* stream);
 size_t aicomp_sample_workspace_bytes(int batch, int vocab, int64_t row_stride, float temperature, int top_k,
                                      int greedy, int logits_dtype);
+
+/*
+ * RMS norm of every query and key head, rotary positions and the KV append in one launch (models that norm their heads, or rotate
+ * a part of them, or neighbours):
+ *   y = x / sqrt(mean(x^2) + eps) * weight            over the D elements of a head
+ *   (a, b) -> (a cos - b sin, b cos + a sin)          for the rotary_dim / 2 pairs among the first rotary_dim elements of y
+ *
+ *   q_in, q_out, key, value, strides, positions, table_rows, slot_mapping, pools, scales   as in aicomp_rope_kv_append
+ *                   (q_out may be q_in; a token whose position is outside the tables is left alone)
+ *   q_weight, k_weight   [D] float; NULL: those heads are not normed
+ *   cos, sin        float tables, row r at r*table_stride, rotary_dim / 2 columns: one angle per pair (NULL if rotary_dim is 0)
+ *   rotary_dim      a multiple of 16, at most head_dim; elements from there on are not rotated; 0: none is
+ *   interleaved     0: pairs (j, j + rotary_dim / 2);  otherwise (2j, 2j + 1)
+ * Computed in float32 and rounded once, to the tensor's type or to the code of an fp8 pool (unlike aicomp_rope_kv_append, which
+ * rounds as an eager evaluation does).  D % 16 == 0 and at most 256; pointers and strides 16-byte aligned.
+ */
+int aicomp_qk_norm_rope_kv_append(const void* q_in, void* q_out,
+                                  int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t qo_token_stride, int64_t qo_head_stride,
+                                  const void* key, const void* value,
+                                  int64_t kv_token_stride, int64_t kv_head_stride,
+                                  const float* q_weight, const float* k_weight, float eps,
+                                  const float* cos, const float* sin, int64_t table_stride, int64_t table_rows,
+                                  int rotary_dim, int interleaved, const int64_t* positions,
+                                  void* k_pool, void* v_pool, const int64_t* slot_mapping,
+                                  int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                                  int block_size, int64_t num_blocks, int in_dtype, int pool_dtype,
+                                  const float* k_scale, const float* v_scale, void* stream);
+
+/*
+ * Attention over the paged pools whose scores follow a rule.  Row at position p of its sequence, key j, head h:
+ *   s = scale * (q . k_j);   softcap > 0: s = softcap * tanh(s / softcap);   slopes: s = s - slopes[h] * |p - j|
+ *   visible: first_keys[row] <= j,  window > 0: p - j < window,  and j <= p or j < prefix_lens[sequence]
+ *   out = softmax of s over the visible keys, times V; a row without visible keys (or all of whose scores are -inf) is zero
+ *
+ *   out, query, pools, block_table, context_lens, scales   as in aicomp_paged_decode_attn (cu_q_lens NULL: one row per
+ *                   sequence at position context_lens - 1, total_q == num_seqs) or aicomp_paged_prefill_attn (rows of sequence s
+ *                   are cu_q_lens[s] .. cu_q_lens[s+1], the last of them at position context_lens - 1; rows behind the last
+ *                   sequence are left as they are)
+ *   softcap         0: none
+ *   slopes          [Hq] float or NULL
+ *   window          0: none
+ *   first_keys      [total_q] int32 or NULL: the first key of each row's document
+ *   prefix_lens     [num_seqs] int32 or NULL: keys below are seen by every row of the sequence (chunks only; at most the context)
+ *   longest_context   what the caller knows of context_lens (0: nothing); it sizes a decode call and bounds nothing
+ *   workspace       aicomp_paged_score_workspace_bytes(...) bytes, 16-byte aligned, needing no initialisation (NULL where that is
+ *                   0, and for chunks); calls that may overlap need separate ones
+ * head_dim 64, 128 or 256; any block size; f32/f32, bf16/bf16, f16/f16, bf16/fp8, f16/fp8 (query / pool); pointers 16-byte aligned.
+ */
+int aicomp_paged_score_attn(void* out, const void* query,
+                            const void* k_pool, const void* v_pool,
+                            const int32_t* block_table, int64_t block_table_stride,
+                            const int32_t* context_lens, const int32_t* cu_q_lens,
+                            int num_seqs, int64_t total_q, int max_q_len,
+                            int num_q_heads, int num_kv_heads, int head_dim,
+                            int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                            float scale, int q_dtype, int kv_dtype,
+                            const float* k_scale, const float* v_scale,
+                            float softcap, const float* slopes, int window,
+                            const int32_t* first_keys, const int32_t* prefix_lens,
+                            int longest_context, void* workspace, size_t workspace_bytes, void* stream);
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                          int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context);
+
+/*
+ * Blocks copied within every pool: pool[dst] = pool[src] for each (src, dst) pair, in one launch (per 128 pools).  What forking a
+ * sequence or compacting the pools takes.
+ *   pools           HOST array of num_pools device pointers (the K and V pools of all layers, alike in size)
+ *   block_bytes     bytes of a block of one pool: Hkv * block_size * D * element size
+ *   pairs           [num_pairs, 2] int64 on the device; a pair outside [0, num_blocks) is skipped.  No block may be the target of
+ *                   two pairs, or the target of one and the source of another
+ */
+int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes, int64_t num_blocks,
+                          const int64_t* pairs, int64_t num_pairs, void* stream);
 
 #ifdef __cplusplus
 }
