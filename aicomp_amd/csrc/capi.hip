@@ -891,6 +891,7 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
     if (cu_q_lens != nullptr) {
         AICOMP_REQUIRE(max_q_len > 0 && max_q_len <= total_q, AICOMP_KV_EINVAL, "%s: max_q_len %d out of range (total %lld)", who,
                        max_q_len, (long long)total_q);
+        if (score_prefill_supported(a)) return launch_score_prefill(a);
         a.partition_size = INT32_MAX; a.num_parts = 1;
         return launch_score_generic(a);
     }

@@ -70,5 +70,7 @@ __device__ __forceinline__ void visible_keys(const ScoreRule& r, int64_t row, in
 
 int launch_score_generic(const ScoreArgs& a);
 int launch_score_merge(const ScoreArgs& a);
+bool score_prefill_supported(const ScoreArgs& a);
+int launch_score_prefill(const ScoreArgs& a);
 
 }  // namespace aicomp
