@@ -816,16 +816,27 @@ int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes
     return launch_copy_blocks(pools, num_pools, block_bytes, num_blocks, pairs, num_pairs, (hipStream_t)stream);
 }
 
-// Tokens of a row's visible keys that one workgroup of a decode call takes, and how many such partitions a row has.
-static int score_partition(const ScoreArgs& a, int longest_context, int& parts) {
-    int64_t span = (int64_t)a.max_blocks * a.bs;
+// How a decode call by a score rule is cut: whether the matrix-core kernels take it, by which schedule, and the partitions of a
+// row's visible keys.  The lines are those of the plain decode calls, for rows as long as the window (or the hint) lets them be.
+struct ScoreCut {
+    bool matrix, balanced;
+    int partition_size, parts;
+};
+
+static ScoreCut score_cut(int64_t rows, int hq, int hkv, int d, int bs, int max_blocks, int q_dtype, int kv_dtype, int window,
+                          int longest_context) {
+    int64_t span = (int64_t)max_blocks * bs;
     if (longest_context > 0) span = std::min<int64_t>(span, longest_context);
-    if (a.window > 0) span = std::min<int64_t>(span, a.window);
-    int ps = 64;
-    for (int cand : {1024, 512, 256, 128})
-        if (a.rows * a.hkv * ((span + cand - 1) / cand) >= 1024) { ps = cand; break; }
-    parts = (int)std::max<int64_t>(1, std::min<int64_t>((span + ps - 1) / ps, 65535));
-    return ps;
+    ScoreCut c;
+    c.matrix = is_16bit_float(q_dtype) && rows <= 65535 && streamk_shape(1, hq, hkv, d, bs, q_dtype, kv_dtype);
+    const bool few = c.matrix && rows <= 1024 && hkv <= 256;           // (what the balanced schedule can hold)
+    // (a window that begins inside a tile reaches into one more)
+    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + (c.matrix ? (d == 64 ? 63 : 31) : 0));
+    const int columns = (int)((span + bs - 1) / bs);
+    c.balanced = few && !grid_call(rows, hq, hkv, d, bs, columns, kv_dtype);
+    c.partition_size = auto_partition(rows, hq, hkv, d, bs, columns, kv_dtype, few);
+    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>((span + c.partition_size - 1) / c.partition_size, 65535));
+    return c;
 }
 
 static int score_shape(ScoreArgs& a, const char* who) {
@@ -848,13 +859,10 @@ size_t aicomp_paged_score_workspace_bytes(int num_seqs, int num_q_heads, int num
     if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || block_size <= 0 ||
         max_blocks_per_seq <= 0 || window < 0 || longest_context < 0)
         return 0;
-    ScoreArgs a;
-    memset(&a, 0, sizeof(a));
-    a.rows = num_seqs; a.hq = num_q_heads; a.hkv = num_kv_heads; a.d = head_dim; a.bs = block_size;
-    a.max_blocks = max_blocks_per_seq; a.q_dtype = q_dtype; a.kv_dtype = kv_dtype; a.window = window;
-    int parts;
-    score_partition(a, longest_context, parts);
-    return parts > 1 ? split_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, parts) : 0;
+    const ScoreCut c = score_cut(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, q_dtype, kv_dtype,
+                                 window, longest_context);
+    if (c.balanced) return decode_streamk_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim);
+    return c.parts > 1 ? split_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, c.parts) : 0;
 }
 
 int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, const void* v_pool, const int32_t* block_table,
@@ -897,16 +905,34 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
     }
     AICOMP_REQUIRE(total_q == num_seqs && prefix_lens == nullptr, AICOMP_KV_EINVAL,
                    "%s: without cu_q_lens there is one row per sequence and no prefix", who);
-    a.partition_size = score_partition(a, longest_context, a.num_parts);
-    if (a.num_parts > 1) {
-        const size_t need = split_workspace_bytes(a.rows, a.hq, a.hkv, a.d, a.num_parts);
+    const ScoreCut c = score_cut(a.rows, a.hq, a.hkv, a.d, a.bs, a.max_blocks, q_dtype, kv_dtype, window, longest_context);
+    a.partition_size = c.partition_size; a.num_parts = c.parts; a.part_align = 1;
+    const size_t need = aicomp_paged_score_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                                                           max_blocks_per_seq, q_dtype, kv_dtype, window, longest_context);
+    if (need > 0) {
         AICOMP_REQUIRE(workspace && workspace_bytes >= need, AICOMP_KV_EWORKSPACE,
                        "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
         AICOMP_REQUIRE((uintptr_t)workspace % 16 == 0, AICOMP_KV_EINVAL, "%s: workspace must be 16-byte aligned", who);
+    }
+    if (a.num_parts > 1 && !c.balanced) {
         const SplitWorkspace ws = split_workspace_view(workspace, a.rows, a.hq, a.hkv, a.d, a.num_parts);
         a.ws_acc = ws.acc; a.ws_ml = ws.ml;
     }
-    return launch_score_generic(a);
+    if (!c.matrix) return launch_score_generic(a);
+    const ScoreRule rule = rule_of(a);
+    DecodeArgs m;
+    memset(&m, 0, sizeof(m));
+    m.out = out; m.query = query; m.k_pool = k_pool; m.v_pool = v_pool;
+    m.block_table = block_table; m.block_table_stride = block_table_stride; m.context_lens = context_lens;
+    m.num_seqs = num_seqs; m.rows = total_q; m.hq = a.hq; m.hkv = a.hkv; m.d = a.d; m.bs = a.bs;
+    m.max_blocks = a.max_blocks; m.num_blocks = num_blocks; m.q_dtype = q_dtype; m.kv_dtype = kv_dtype;
+    m.k_scale = a.k_scale; m.v_scale = a.v_scale; m.partition_size = a.partition_size; m.num_parts = a.num_parts;
+    m.ws.acc = a.ws_acc; m.ws.ml = a.ws_ml;
+    m.stream = a.stream; m.rule = &rule;
+    if (c.balanced) return launch_decode_streamk(m, workspace);
+    rc = launch_decode_mfma(m);
+    a.part_align = a.d == 64 ? 64 : 32;
+    return rc == AICOMP_KV_OK && a.num_parts > 1 ? launch_score_merge(a) : rc;
 }
 
 }  // extern "C"

@@ -265,6 +265,8 @@ inline SplitWorkspace split_workspace_view(void* ws, int64_t rows, int hq, int h
 }
 
 // ------------------------------------------------------- kernel launchers ---
+struct ScoreRule;
+
 struct DecodeArgs {
     void* out;
     const void* query;
@@ -303,6 +305,7 @@ struct DecodeArgs {
     const int32_t* items;
     int num_items;
     bool chunks;                // prefill only: the call is a step's prompt chunks and nothing else
+    const ScoreRule* rule;   // decode only (NULL = none): scores by a rule (score.h), 16-bit queries
     int longest_context;        // prefill only: what the caller knows of context_lens (0: nothing); chooses a kernel, bounds nothing
 };
 

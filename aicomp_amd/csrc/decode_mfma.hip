@@ -44,8 +44,10 @@
 //              workspace; a second, small kernel merges them.
 #include "common.h"
 #include "rope_math.h"
+#include "score.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace aicomp {
 
@@ -84,8 +86,32 @@ struct MfmaParams {
     int64_t q_token_stride, q_head_stride;
 };
 
+struct MfmaRuleParams : MfmaParams {
+    ScoreRule rule;
+};
+
 #include "decode_tile_f32.h"
 #include "decode_tile_f32_quad.h"
+
+// A decode row's scores by the rule: what a lane makes of its products (its column's head), and the first visible key.
+template <typename T, typename Params>
+__device__ __forceinline__ RuleScore rule_score(const Params& p, int kvh, int lane) {
+    RuleScore s;
+    const float ks = T::FP8 ? p.k_scale[kvh] : 1.f;
+    s.cap = p.rule.cap_log2;
+    s.mul = (s.cap > 0.f ? 2.f * LOG2E * p.rule.cap_mul : p.rule.mul) * ks;
+    s.slope = p.rule.slopes != nullptr ? p.rule.slopes[kvh * p.group + min((lane & 15) / T::NPAR, p.group - 1)] * LOG2E : 0.f;
+    s.pos = s.lo = 0;
+    return s;
+}
+// (a row of `len` tokens, its query at the last; no load is waited for where the rule has no borders)
+template <typename Params>
+__device__ __forceinline__ int first_visible(const Params& p, int seq, int len) {
+    if (p.rule.window <= 0 && p.rule.first_keys == nullptr) return 0;
+    int lo, hi;
+    visible_keys(p.rule, seq, seq, len - 1, len, lo, hi);
+    return __builtin_amdgcn_readfirstlane(lo);
+}
 
 // query rows of (sequence, KV head) in the tensor, and its new rows
 template <typename T, typename Params>
@@ -152,9 +178,10 @@ __device__ __forceinline__ void store_new_row(const MfmaParams& p, const typenam
 // ROPE: the query rows come as projected, with strides of their own, and are rotated here, like the new K row: a decode
 // step of a layer is then this launch alone, where the rotary + append launch before it and the rotated query's way
 // through memory cost 3.3 us of device and 6 us of host time (8 rows of 900 tokens, 32 / 8 heads, D 64).
-template <typename T, int NW, bool ROPE>
+// RULE: scores by a rule (score.h); the partitions then begin with the tile of the row's first visible key.
+template <typename T, int NW, bool ROPE, bool RULE = false>
 __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 1)
-paged_decode_mfma_kernel(MfmaParams p) {
+paged_decode_mfma_kernel(std::conditional_t<RULE, MfmaRuleParams, MfmaParams> p) {
     // KV head fastest: the workgroups launched together read the Hkv slices of the same
     // physical blocks, i.e. one contiguous Hkv*4 KB piece of each pool
     constexpr int DQ = T::DQ, TT = T::TT, BPT = T::BPT, NPAR = T::NPAR;
@@ -169,7 +196,11 @@ paged_decode_mfma_kernel(MfmaParams p) {
     const int g4 = lane >> 4;       // MFMA k-group of this lane
     const int G = p.group;
     const int ncol = NPAR * G;      // B-operand columns in use
-    const int start = part * p.partition_size;
+    int start = part * p.partition_size, lo = 0;
+    if constexpr (RULE) {
+        lo = first_visible(p, seq, min(p.context_lens[seq], p.max_blocks * BS));
+        start += lo / TT * TT;
+    }
     const int blk_base = start / BS;
 
     // Prologue loads, all issued before anything waits: the context length (scalar), the
@@ -190,8 +221,8 @@ paged_decode_mfma_kernel(MfmaParams p) {
     const bool pos_ok = pos_in >= 0 && pos_in < p.tab_rows;
     const bool stored = ROPE && pos_ok && slot >= 0 && slot < p.num_blocks * BS;
     __shared__ __attribute__((aligned(16))) typename T::Fmt::raw k_new[ROPE ? NW : 1][ROPE ? DQ : 1];
-    if (start >= len) {
-        if (len <= 0 && part == 0) {   // nothing to attend to: the output row is defined as zero
+    if (start >= len || (RULE && lo >= len)) {
+        if ((RULE ? lo >= len : len <= 0) && part == 0) {   // nothing to attend to: the output row is defined as zero
             auto* o = (typename T::Fmt::raw*)p.out + ((int64_t)seq * p.hq + kvh * G) * DQ;
             for (int i = tid; i < G * DQ; i += blockDim.x) o[i] = 0;
             if constexpr (ROPE) {
@@ -204,14 +235,24 @@ paged_decode_mfma_kernel(MfmaParams p) {
         return;
     }
     // (ROPE: the caller's idea of the lengths sized the grid, and the last partition takes what is left of a row)
-    const int end = ROPE && part + 1 == p.num_parts ? len : min(len, start + p.partition_size);
+    const int end = (ROPE || RULE) && part + 1 == p.num_parts ? len : min(len, start + p.partition_size);
     const int ntiles = (end - start + TT - 1) / TT;
 
     __shared__ float sm_m[NW][16];
     __shared__ float sm_l[NW][16];
     unsigned char* kt = lds + w * KTILE_BYTES;
 
-    const float cmul = p.qk_mul * (T::FP8 ? p.k_scale[kvh] : 1.f);
+    auto score = [&] {
+        if constexpr (RULE) {
+            RuleScore s = rule_score<T>(p, kvh, lane);
+            s.pos = len - 1;
+            s.lo = lo;
+            return s;
+        } else {
+            return p.qk_mul * (T::FP8 ? p.k_scale[kvh] : 1.f);
+        }
+    };
+    const auto cmul = score();
 
     typename T::State st;
     if constexpr (!T::QUAD) clear_state(st);
@@ -243,6 +284,13 @@ paged_decode_mfma_kernel(MfmaParams p) {
         }
         T::q_operand(qf, qf, G, lane);
         int tt = w;
+        if constexpr (RULE) {                     // the tile that the row's first visible key is in
+            if (start + tt * TT < lo && tt + NW < ntiles) {
+                tile_blocks(tt + NW);
+                T::template process<true, true>(st, kv, qf, kt, ko, p, bb, kvh, lane, start + tt * TT, end, cmul);
+                tt += NW;
+            }
+        }
         for (; tt + NW < ntiles; tt += NW) {      // steady state: never the partition's last tile
             tile_blocks(tt + NW);
             T::template process<true, false>(st, kv, qf, kt, ko, p, bb, kvh, lane, start + tt * TT, end, cmul);
@@ -266,7 +314,7 @@ paged_decode_mfma_kernel(MfmaParams p) {
                 T::inject(kv, p, new_row<T>(p.new_key, p, seq, kvh), nv, kvh, lane, tile_start, len, bb);
             }
         }
-        if (tile_start + TT > end)
+        if (tile_start + TT > end || (RULE && tile_start < lo))
             T::template process<false, true>(st, kv, qf, kt, ko, p, bb, kvh, lane, tile_start, end, cmul);
         else
             T::template process<false, false>(st, kv, qf, kt, ko, p, bb, kvh, lane, tile_start, end, cmul);
@@ -475,18 +523,28 @@ struct StreamKParams {
     int64_t new_token_stride, new_head_stride;     // elements
 };
 
-template <int TT>
-__device__ __forceinline__ int sk_tiles(int len, int max_blocks) {
-    len = min(max(len, 0), max_blocks * BS);
-    return (len + TT - 1) / TT;
-}
+struct StreamKRuleParams : StreamKParams {
+    ScoreRule rule;
+};
 
+// tiles of a sequence; by a rule, from the one that its first visible key is in
+template <int TT, bool RULE, typename Params>
+__device__ __forceinline__ int sk_tiles(const Params& p, int seq) {
+    const int len = min(max(p.context_lens[seq], 0), p.max_blocks * BS);
+    if constexpr (RULE) {
+        int lo, hi;
+        visible_keys(p.rule, seq, seq, len - 1, len, lo, hi);
+        return lo < len ? (len + TT - 1) / TT - lo / TT : 0;
+    } else {
+        return (len + TT - 1) / TT;
+    }
+}
 
 // Token pairs (Tile16 with PAIR): every head takes two B-operand columns, one per token parity, and a
 // flush merges the two columns of a head inside the wave and writes one partial of 64 floats per head.
-template <typename T>
+template <typename T, bool RULE = false>
 __global__ void __launch_bounds__(256, 1)     // one workgroup per CU: a wave may use the whole register file
-streamk_decode_kernel(StreamKParams p) {
+streamk_decode_kernel(std::conditional_t<RULE, StreamKRuleParams, StreamKParams> p) {
     constexpr int DQ = T::DQ, TT = T::TT, BPT = T::BPT;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -504,7 +562,7 @@ streamk_decode_kernel(StreamKParams p) {
     if (B <= 64) {
         // every wave scans for itself and reads back only what it wrote: no barrier (the
         // four waves write identical values to the same words)
-        const int mine = lane < B ? sk_tiles<TT>(p.context_lens[lane], p.max_blocks) : 0;
+        const int mine = lane < B ? sk_tiles<TT, RULE>(p, lane) : 0;
         int inc = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -519,7 +577,7 @@ streamk_decode_kernel(StreamKParams p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int sidx = 4 * tid + k;
-            loc[k] = sidx < B ? sk_tiles<TT>(p.context_lens[sidx], p.max_blocks) : 0;
+            loc[k] = sidx < B ? sk_tiles<TT, RULE>(p, sidx) : 0;
             sum += loc[k];
         }
         int inc = sum;
@@ -580,10 +638,22 @@ streamk_decode_kernel(StreamKParams p) {
         return (first_block + lane < p.max_blocks) ? table[first_block + lane] : 0;
     };
 
+    // by a rule: a row's tiles are counted from the one that its first visible key is in
+    auto first_of = [&](int sq) {
+        if constexpr (RULE) return first_visible(p, sq, min(p.context_lens[sq], p.max_blocks * BS));
+        else return 0;
+    };
+    int lo = first_of(seq);
+    auto score = [&] {
+        if constexpr (RULE) return rule_score<T>(p, kvh, lane);        // (a wave stays with its KV head)
+        else return 0.f;
+    };
+    auto rule = score();
+
     int nt = (int)min((int64_t)(row_tiles - t), g1 - g0);          // tiles of the current segment (>= 1)
     typename T::Q qf, qraw;
     T::load_q(qraw, q_rows<T>(p, seq, kvh), G, lane);
-    int tab = load_tab(seq, BPT * t);
+    int tab = load_tab(seq, BPT * (t + lo / TT));
     typename T::Regs kv;
     // the blocks of a tile out of a table slice held one entry per lane
     auto slice_blocks = [&](int slice, int first, int64_t (&bb)[4]) {
@@ -600,10 +670,20 @@ streamk_decode_kernel(StreamKParams p) {
 
     for (int64_t g = g0; g < g1 && seq < B;) {
         const int len = min(p.context_lens[seq], p.max_blocks * BS);
-        const int blk_base = BPT * t;
+        const int t0 = lo / TT;
+        const int blk_base = BPT * (t + t0);
         const int32_t* table = p.block_table + (int64_t)seq * p.block_table_stride;
         int tab_first = 0;
-        const float cmul = p.qk_mul * (T::FP8 ? p.k_scale[kvh] : 1.f);
+        auto mul = [&] {
+            if constexpr (RULE) {
+                rule.pos = len - 1;
+                rule.lo = lo;
+                return rule;
+            } else {
+                return p.qk_mul * (T::FP8 ? p.k_scale[kvh] : 1.f);
+            }
+        };
+        const auto cmul = mul();
         auto tile_blocks = [&](int k, int64_t (&bb)[4]) {              // k-th tile of the segment
             const int i0 = BPT * k;
             if (i0 - tab_first >= 64) {
@@ -622,11 +702,12 @@ streamk_decode_kernel(StreamKParams p) {
             nrow_tiles = nseq < B ? __builtin_amdgcn_readfirstlane(prefix[nseq + 1] - prefix[nseq]) : 0;
         }
         const bool has_next = more && nseq < B;
-        int tabn = 0;
+        int tabn = 0, nlo = 0;
         typename T::Q qn;
         if (has_next) {
             T::load_q(qraw, q_rows<T>(p, nseq, nkvh), G, lane);
-            tabn = load_tab(nseq, 0);
+            nlo = first_of(nseq);
+            tabn = load_tab(nseq, BPT * (nlo / TT));
         }
 
         typename T::State st;
@@ -634,11 +715,18 @@ streamk_decode_kernel(StreamKParams p) {
 
         int64_t bb[4] = {0, 0, 0, 0};
         int k = 0;
+        if constexpr (RULE) {
+            if ((t + t0) * TT < lo && nt > 1) {
+                tile_blocks(1, bb);
+                T::template process<true, true>(st, kv, qf, kt, ko, p, bb, kvh, lane, (t + t0) * TT, len, cmul);
+                k = 1;
+            }
+        }
         for (; k + 1 < nt; ++k) {
             tile_blocks(k + 1, bb);
-            T::template process<true, false>(st, kv, qf, kt, ko, p, bb, kvh, lane, (t + k) * TT, len, cmul);
+            T::template process<true, false>(st, kv, qf, kt, ko, p, bb, kvh, lane, (t + t0 + k) * TT, len, cmul);
         }
-        const int tile_start = (t + k) * TT;
+        const int tile_start = (t + t0 + k) * TT;
         if (p.new_key != nullptr && t + k == row_tiles - 1) {       // the row's newest token lives here
             tile_blocks(k, bb);
             // Same rule as the separate one-token append: the row is stored only where the table names a
@@ -711,7 +799,7 @@ streamk_decode_kernel(StreamKParams p) {
         // ---- next segment
         g += nt;
         if (!has_next) break;
-        seq = nseq; kvh = nkvh; row_tiles = nrow_tiles; t = 0;
+        seq = nseq; kvh = nkvh; row_tiles = nrow_tiles; t = 0; lo = nlo;
         nt = (int)min((int64_t)row_tiles, g1 - g);
         tab = tab_ready;
         qf = qn;
@@ -728,12 +816,13 @@ streamk_decode_kernel(StreamKParams p) {
 // hundreds of partials each) the waves of a head take alternate groups of eight partials and add
 // up through LDS.
 constexpr int RED_WGT = 256;       // weights parked in LDS per wave; rows with more partials recompute the rest
-template <typename E, int DQ>
+struct NoRule {};
+template <typename E, int DQ, typename Rule = NoRule>
 __global__ void __launch_bounds__(1024)
 streamk_reduce_kernel(typename E::raw* __restrict__ out, const float* __restrict__ ws_acc,
                       const float* __restrict__ ws_ml, const int* __restrict__ ws_rows,
                       const int32_t* __restrict__ context_lens, int hq, int hkv, int group,
-                      const float* __restrict__ v_scale, int head_slots) {
+                      const float* __restrict__ v_scale, int head_slots, Rule rule, int max_tokens) {
     constexpr int NV = DQ / 64;                            // output dims per lane
     const int kvh = blockIdx.x, seq = blockIdx.y, wv = threadIdx.x >> 6;
     const int S = (int)(blockDim.x >> 6) / group;          // waves per head
@@ -748,7 +837,14 @@ streamk_reduce_kernel(typename E::raw* __restrict__ out, const float* __restrict
     // written and is not used)
     const int ctx = context_lens[seq];
     const int first = ws_rows[2 * row], last = ws_rows[2 * row + 1];
-    if (ctx <= 0) {                          // no tiles, no partials: the output row is zero (whole workgroup)
+    bool empty = ctx <= 0;
+    if constexpr (std::is_same_v<Rule, ScoreRule>) {
+        int lo, hi;
+        const int len = min(ctx, max_tokens);
+        visible_keys(rule, seq, seq, len - 1, len, lo, hi);
+        empty = empty || lo >= len;
+    }
+    if (empty) {                             // no tiles, no partials: the output row is zero (whole workgroup)
         if (sub == 0) {
 #pragma unroll
             for (int e = 0; e < NV; ++e) o[lane + 64 * e] = 0;
@@ -907,7 +1003,19 @@ int launch_decode_streamk(const DecodeArgs& a, void* workspace) {
         if (fp8) hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, true, PAIR>>), dim3(wgs), dim3(256), 0, a.stream, p);  \
         else hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, false, PAIR>>), dim3(wgs), dim3(256), 0, a.stream, p);    \
     } while (0)
-    if (f32) {
+    StreamKRuleParams rp;
+    if (a.rule != nullptr) {
+        (StreamKParams&)rp = p;
+        rp.rule = *a.rule;
+#define AICOMP_LAUNCH_SK_RULE(E, PAIR)                                                                                              \
+    do {                                                                                                                            \
+        if (fp8) hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, true, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);   \
+        else hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, false, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);      \
+    } while (0)
+        if (pair) { if (f16) AICOMP_LAUNCH_SK_RULE(F16Fmt, true); else AICOMP_LAUNCH_SK_RULE(Bf16Fmt, true); }
+        else { if (f16) AICOMP_LAUNCH_SK_RULE(F16Fmt, false); else AICOMP_LAUNCH_SK_RULE(Bf16Fmt, false); }
+#undef AICOMP_LAUNCH_SK_RULE
+    } else if (f32) {
 #define AICOMP_LAUNCH_SK32(DQ)                                                                                                 \
     do {                                                                                                                       \
         if (group <= 4) hipLaunchKernelGGL((streamk_decode_kernel<TileF32Quad<DQ>>), dim3(wgs), dim3(256), 0, a.stream, p);    \
@@ -922,13 +1030,19 @@ int launch_decode_streamk(const DecodeArgs& a, void* workspace) {
     // waves per head in the merge: one, unless rows are few and long (many partials per row)
     const int64_t per_row = (int64_t)p.waves_per_head / a.rows + 2;
     const int sub = per_row > 8 ? 16 / group : 1;
-#define AICOMP_LAUNCH_RED(E, DQ)                                                                                  \
-    hipLaunchKernelGGL((streamk_reduce_kernel<E, DQ>), dim3(a.hkv, (unsigned)a.rows), dim3(64 * group * sub), 0,  \
+#define AICOMP_LAUNCH_RED_BY(E, DQ, RULE, rule)                                                                   \
+    hipLaunchKernelGGL((streamk_reduce_kernel<E, DQ, RULE>), dim3(a.hkv, (unsigned)a.rows), dim3(64 * group * sub), 0,  \
                        a.stream, (E::raw*)a.out, p.ws_acc, p.ws_ml, p.ws_rows, a.context_lens, a.hq, a.hkv,     \
-                       group, a.v_scale, p.waves_per_head + (int)a.rows)
-    if (f32) { if (a.d == 64) AICOMP_LAUNCH_RED(F32Fmt, 64); else AICOMP_LAUNCH_RED(F32Fmt, 128); }
+                       group, a.v_scale, p.waves_per_head + (int)a.rows, rule, a.max_blocks * a.bs)
+#define AICOMP_LAUNCH_RED(E, DQ)                                                                                  \
+    do {                                                                                                          \
+        if (a.rule != nullptr) AICOMP_LAUNCH_RED_BY(E, DQ, ScoreRule, *a.rule);                                   \
+        else AICOMP_LAUNCH_RED_BY(E, DQ, NoRule, NoRule{});                                                       \
+    } while (0)
+    if (f32) { if (a.d == 64) AICOMP_LAUNCH_RED_BY(F32Fmt, 64, NoRule, NoRule{}); else AICOMP_LAUNCH_RED_BY(F32Fmt, 128, NoRule, NoRule{}); }
     else if (pair) { if (f16) AICOMP_LAUNCH_RED(F16Fmt, 64); else AICOMP_LAUNCH_RED(Bf16Fmt, 64); }
     else { if (f16) AICOMP_LAUNCH_RED(F16Fmt, 128); else AICOMP_LAUNCH_RED(Bf16Fmt, 128); }
+#undef AICOMP_LAUNCH_RED_BY
 #undef AICOMP_LAUNCH_RED
     AICOMP_HIP_LAUNCH_CHECK();
     return AICOMP_KV_OK;
@@ -969,6 +1083,26 @@ int launch_decode_mfma(const DecodeArgs& a) {
     // rows of 1024 tokens of fp8 406 and 464.
     const int tile = a.q_dtype == AICOMP_KV_F32 ? (d64 ? TILE : TILE / 2) : (d64 ? 2 * TILE : TILE);
     const bool wide = a.partition_size > 16 * tile && a.rows * a.hkv * a.num_parts <= 256;
+    if (a.rule != nullptr) {               // (16-bit queries; a split's merge is the caller's)
+        MfmaRuleParams rp;
+        (MfmaParams&)rp = p;
+        rp.rule = *a.rule;
+#define AICOMP_LAUNCH_RULE(...)                                                                                                           \
+    do {                                                                                                                                  \
+        if (wide) hipLaunchKernelGGL((paged_decode_mfma_kernel<__VA_ARGS__, 8, false, true>), grid, dim3(512), 0, a.stream, rp);          \
+        else hipLaunchKernelGGL((paged_decode_mfma_kernel<__VA_ARGS__, 4, false, true>), grid, dim3(256), 0, a.stream, rp);               \
+    } while (0)
+#define AICOMP_LAUNCH_RULE16(E)                                                                     \
+    do {                                                                                            \
+        if (d64) { if (fp8) AICOMP_LAUNCH_RULE(Tile16<E, true, true>); else AICOMP_LAUNCH_RULE(Tile16<E, false, true>); } \
+        else { if (fp8) AICOMP_LAUNCH_RULE(Tile16<E, true, false>); else AICOMP_LAUNCH_RULE(Tile16<E, false, false>); }   \
+    } while (0)
+        if (a.q_dtype == AICOMP_KV_F16) AICOMP_LAUNCH_RULE16(F16Fmt); else AICOMP_LAUNCH_RULE16(Bf16Fmt);
+#undef AICOMP_LAUNCH_RULE16
+#undef AICOMP_LAUNCH_RULE
+        AICOMP_HIP_LAUNCH_CHECK();
+        return AICOMP_KV_OK;
+    }
 #define AICOMP_LAUNCH_GRID(...)                                                                                        \
     do {                                                                                                               \
         if (rope && wide) hipLaunchKernelGGL((paged_decode_mfma_kernel<__VA_ARGS__, 8, true>), grid, dim3(512), 0, a.stream, p); \

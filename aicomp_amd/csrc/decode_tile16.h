@@ -130,6 +130,29 @@ __device__ __forceinline__ void clear_state(WaveStateT<NO>& st) {
     for (int j = 0; j < NO; ++j) st.O[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 }
 
+// What makes a score, in the exponent's units, of a dot product: its multiplier, or a rule (score.h) over the keys from `lo` on.
+struct PlainScore {
+    float mul;
+    static constexpr bool LOW = false;
+    __device__ __forceinline__ float operator()(float s, int) const { return s * mul; }
+    __device__ __forceinline__ bool below(int) const { return false; }
+};
+// cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)): one exponential and one reciprocal more.  The branches are uniform.
+struct RuleScore {
+    float mul;                             // with a cap: 2 log2(e) scale / cap
+    float cap, slope;                      // times log2(e); slope: of this lane's head
+    int pos, lo;
+    static constexpr bool LOW = true;
+    __device__ __forceinline__ float operator()(float s, int tok) const {
+        float x = s * mul;
+        if (cap > 0.f) x = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap);
+        return fmaf(slope, (float)(tok - pos), x);
+    }
+    __device__ __forceinline__ bool below(int tok) const { return tok < lo; }
+};
+__device__ __forceinline__ PlainScore score_of(float mul) { return PlainScore{mul}; }
+__device__ __forceinline__ const RuleScore& score_of(const RuleScore& r) { return r; }
+
 // One 32-token tile: K registers -> LDS -> S^T = K Q^T -> online softmax -> O^T += V^T P^T.
 // NEXT: prefetch the wave's next tile (blocks nb0/nb1) into the same registers.
 // MASK: the tile crosses `end` (of this lane's column) or `v_end` (of all); scores beyond the one are dropped, V rows
@@ -141,12 +164,12 @@ __device__ __forceinline__ void clear_state(WaveStateT<NO>& st) {
 // not finite: there each half of a row is summed by itself and a column takes its own (as many products).
 // LEAN (one-token rows in the prefill kernel): fewer registers; and a key of -inf has no weight, as in that kernel's other
 // rows, where in a shared product it would leave NaN in the other token's score.
-template <typename E, bool FP8, bool NEXT, bool MASK, bool PAIR, bool ONCE, bool LEAN>
+template <typename E, bool FP8, bool NEXT, bool MASK, bool PAIR, bool ONCE, bool LEAN, typename Score>
 __device__ __forceinline__ void process_tile(WaveState& st, TileRegs<FP8>& kr, TileRegs<FP8>& vr,
                                              const uint4 (&qf)[4], unsigned char* kt, const KTileOffsets& ko,
                                              const void* k_pool, const void* v_pool,
                                              int64_t nb0, int64_t nb1, int hkv, int kvh_next, int lane,
-                                             int g4, int tile_start, int end, int v_end, float cmul,
+                                             int g4, int tile_start, int end, int v_end, const Score& score,
                                              int64_t nb2 = 0, int64_t nb3 = 0) {
     constexpr bool HALVES = PAIR && (!ONCE || LEAN);     // a row's score summed over either half by itself
     // ---- K tile -> LDS, then prefetch the next K tile into the same registers
@@ -155,7 +178,10 @@ __device__ __forceinline__ void process_tile(WaveState& st, TileRegs<FP8>& kr, T
         uint4 kk = tile_elems<E, FP8>(kr, i);
         // PAIR, one dot product for a row's two tokens: a token beyond the context must not leave non-finite
         // values in the row
-        if (PAIR && !HALVES && MASK && tile_start + 2 * (4 * i + g4) + ((lane & 15) >> 3) >= v_end) kk = make_uint4(0, 0, 0, 0);
+        if (PAIR && !HALVES && MASK) {
+            const int ktok = tile_start + 2 * (4 * i + g4) + ((lane & 15) >> 3);
+            if (ktok >= v_end || score.below(ktok)) kk = make_uint4(0, 0, 0, 0);
+        }
         *(uint4*)(kt + ko.wr[i & 3] + i * 4 * KROW) = kk;
     }
     if (NEXT) {
@@ -182,15 +208,18 @@ __device__ __forceinline__ void process_tile(WaveState& st, TileRegs<FP8>& kr, T
         }
     }
     // lane (head r16, g4) now holds tokens tile_start + 16a + 4i + g4 in s_a[i]
+    auto tok_of = [&](int k) {
+        const int r = 16 * (k >> 2) + 4 * (k & 3) + g4;
+        return PAIR ? tile_start + 2 * r + (lane & 1) : tile_start + r;
+    };
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { sc[i] = s0[i] * cmul; sc[4 + i] = s1[i] * cmul; }
+    for (int i = 0; i < 4; ++i) { sc[i] = score(s0[i], tok_of(i)); sc[4 + i] = score(s1[i], tok_of(4 + i)); }
     if (MASK) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int r = 16 * (k >> 2) + 4 * (k & 3) + g4;
-            const int tok = PAIR ? tile_start + 2 * r + (lane & 1) : tile_start + r;
-            if (tok >= end) sc[k] = NEG_BIG;
+            const int tok = tok_of(k);
+            if (tok >= end || score.below(tok)) sc[k] = NEG_BIG;
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])),
@@ -227,7 +256,7 @@ __device__ __forceinline__ void process_tile(WaveState& st, TileRegs<FP8>& kr, T
         vv[i] = tile_elems<E, FP8>(vr, i);
         // PAIR: chunks 8..15 of a row belong to the pair's second token
         const int vtok = PAIR ? tile_start + 2 * (4 * i + g4) + ((lane & 15) >> 3) : tile_start + 4 * i + g4;
-        if (MASK && vtok >= v_end) vv[i] = make_uint4(0, 0, 0, 0);
+        if (MASK && (vtok >= v_end || score.below(vtok))) vv[i] = make_uint4(0, 0, 0, 0);
     }
     auto operand = [&](int j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -363,19 +392,20 @@ struct Tile16 {
             load_tile<FP8, ONCE>(t.v, p.v_pool, bb[0], bb[1], p.hkv, kvh, lane);
         }
     }
-    template <bool NEXT, bool MASK, typename Params>
+    // cmul: the score's multiplier, or a RuleScore
+    template <bool NEXT, bool MASK, typename Params, typename Mul>
     __device__ __forceinline__ static void process(State& st, Regs& t, const Q& q, unsigned char* kt, const Offsets& ko,
                                                    const Params& p, const int64_t (&nb)[4], int kvh_next, int lane,
-                                                   int tile_start, int end, float cmul) {
+                                                   int tile_start, int end, const Mul& cmul) {
         process_rows<NEXT, MASK>(st, t, q, kt, ko, p, nb, kvh_next, lane, tile_start, end, end, cmul);
     }
     // columns with ends of their own (rows of a chunk)
-    template <bool NEXT, bool MASK, typename Params>
+    template <bool NEXT, bool MASK, typename Params, typename Mul>
     __device__ __forceinline__ static void process_rows(State& st, Regs& t, const Q& q, unsigned char* kt, const Offsets& ko,
                                                         const Params& p, const int64_t (&nb)[4], int kvh_next, int lane,
-                                                        int tile_start, int end, int v_end, float cmul) {
+                                                        int tile_start, int end, int v_end, const Mul& cmul) {
         process_tile<E, FP8, NEXT, MASK, PAIR, ONCE, LEAN>(st, t.k, t.v, q.r, kt, ko, p.k_pool, p.v_pool, nb[0], nb[1], p.hkv,
-                                               kvh_next, lane, lane >> 4, tile_start, end, v_end, cmul, nb[2], nb[3]);
+                                               kvh_next, lane, lane >> 4, tile_start, end, v_end, score_of(cmul), nb[2], nb[3]);
     }
     template <typename Params>
     __device__ __forceinline__ static void inject(Regs& t, const Params& p, const uint16_t* key, const uint16_t* value,

@@ -34,6 +34,7 @@ struct ScoreArgs {
     const int32_t* first_keys;  // [rows] or NULL
     const int32_t* prefix_lens; // [num_seqs] or NULL (not with decode)
     int partition_size, num_parts;      // decode: tokens per partition of a row's visible keys; the last takes what is left
+    int part_align;             // the first partition begins at the multiple of this at or below the first visible key
     float* ws_acc;              // [rows][Hq][num_parts][D]
     float* ws_ml;               // [rows][Hq][num_parts][2]
     hipStream_t stream;

@@ -230,7 +230,7 @@ template <typename Q_T, int NV>
 __global__ void __launch_bounds__(256)
 score_merge_kernel(Q_T* __restrict__ out, const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
                    const int32_t* __restrict__ context_lens, ScoreRule rule, int64_t pairs, int hq, int group, int max_tokens,
-                   int partition_size, int num_parts, const float* __restrict__ v_scale) {
+                   int partition_size, int num_parts, int part_align, const float* __restrict__ v_scale) {
     constexpr int D = 64 * NV;
     const int lane = threadIdx.x & 63;
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);         // (row, head)
@@ -240,6 +240,7 @@ score_merge_kernel(Q_T* __restrict__ out, const float* __restrict__ ws_acc, cons
     int seq, pos, lo, hi;
     row_of(nullptr, context_lens, 0, max_tokens, rule, row, seq, pos, lo, hi);
     if (lo >= hi) return;                                                    // the main kernel wrote the zero row
+    lo -= lo % part_align;
     const int np = min(num_parts, (int)((hi - lo + (int64_t)partition_size - 1) / partition_size));
     const float* ml = ws_ml + at * num_parts * 2;
     const float* acc = ws_acc + at * num_parts * D + lane;
@@ -300,7 +301,7 @@ void launch_merge_t(const ScoreArgs& a) {
 #define AICOMP_MERGE(NV)                                                                                                       \
     hipLaunchKernelGGL((score_merge_kernel<Q_T, NV>), grid, dim3(256), 0, a.stream, (Q_T*)a.out, a.ws_acc, a.ws_ml,            \
                        a.context_lens, rule_of(a), pairs, a.hq, a.hq / a.hkv, a.max_blocks * a.bs, a.partition_size,           \
-                       a.num_parts, a.v_scale)
+                       a.num_parts, a.part_align, a.v_scale)
     if (a.d == 64) AICOMP_MERGE(1);
     else if (a.d == 128) AICOMP_MERGE(2);
     else AICOMP_MERGE(4);

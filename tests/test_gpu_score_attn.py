@@ -133,6 +133,7 @@ def slopes_of(hq):
 
 RULES = {"none": {}, "cap": {"cap": 5.0}, "slopes": {"slopes": True}, "window": {"window": 70}, "window1": {"window": 1},
          "all": {"cap": 30.0, "slopes": True, "window": 100, "first": True}}
+BOTH = pytest.mark.routing("balanced", "library")       # decode calls on either schedule
 TYPES = [(BF16, None), (F16, None), (F32, None), (BF16, FP8), (F16, FP8)]
 
 
@@ -150,6 +151,7 @@ def rule(name, c, g):
 DECODE_LENS = [[1], [0, 5, 300, 17], [33, 64, 65, 1000, 16, 15]]
 
 
+@BOTH
 @pytest.mark.parametrize("name", list(RULES))
 @pytest.mark.parametrize("dtype,pool", TYPES)
 @pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64), (6, 1, 256), (28, 4, 128)])
@@ -162,6 +164,7 @@ def test_decode(dtype, pool, hq, hkv, d, name):
         check(run_decode(c, **r), c, want, mean_abs, size)
 
 
+@BOTH
 @pytest.mark.parametrize("bs", [8, 16, 32])
 @pytest.mark.parametrize("longest", [0, 100, 4000])
 def test_decode_blocks_and_hints(bs, longest):
@@ -169,6 +172,27 @@ def test_decode_blocks_and_hints(bs, longest):
     c = Case([700, 3, 250], [1, 1, 1], 8, 2, 64, bs=bs, seed=3)
     want, mean_abs, size = expect(c, 20.0, None, 0, None, None)
     check(run_decode(c, cap=20.0, longest_context=longest), c, want, mean_abs, size)
+
+
+@BOTH
+@pytest.mark.parametrize("dtype,pool", [(BF16, None), (F16, FP8)])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (16, 2, 64)])
+def test_decode_of_many_rows(dtype, pool, hq, hkv, d):
+    """Rows that several waves of the balanced schedule share, and waves that cross rows; empty ones among them."""
+    lens = [int(x) for x in torch.randint(0, 700, (70,), generator=torch.Generator().manual_seed(1))]
+    lens[3] = lens[69] = 0
+    c = Case(lens, [1] * 70, hq, hkv, d, dtype=dtype, pool=pool, seed=1)
+    first = torch.randint(-5, 400, (70,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    for r in ({"cap": 20.0}, {"window": 129, "slopes": slopes_of(hq)}, {"first": first, "cap": 8.0}):
+        want, mean_abs, size = expect(c, r.get("cap", 0.0), r.get("slopes"), r.get("window", 0), r.get("first"), None)
+        check(run_decode(c, **r), c, want, mean_abs, size)
+
+
+def test_decode_of_more_rows_than_the_balanced_schedule_holds():
+    lens = [1 + i % 50 for i in range(1100)]
+    c = Case(lens, [1] * 1100, 2, 1, 64, seed=1)
+    want, mean_abs, size = expect(c, 20.0, None, 30, None, None)
+    check(run_decode(c, cap=20.0, window=30), c, want, mean_abs, size)
 
 
 def visible(c, window=0, first=None, prefix=None):
@@ -189,6 +213,7 @@ def visible(c, window=0, first=None, prefix=None):
     return out
 
 
+@BOTH
 @pytest.mark.parametrize("dtype,pool", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_decode_never_looks_at_masked_keys(dtype, pool, d):
@@ -251,6 +276,7 @@ def test_masked_keys_of_a_row_that_others_see(d):
     check(got[1:59], inner, want[1:59], mean_abs[1:59], size[1:59])
 
 
+@BOTH
 def test_cut_to_the_table():
     """A context beyond the table is cut to it (as in the plain decode call)."""
     c = Case([200, 64], [1, 1], 4, 2, 128, seed=4, width=13)
@@ -261,6 +287,7 @@ def test_cut_to_the_table():
     check(run_decode(c, cap=20.0), c, want, mean_abs, size)
 
 
+@BOTH
 def test_bad_table_entries_stay_in_the_pool():
     c = Case([100, 40], [1, 1], 4, 2, 128, seed=4)
     fixed = Case([100, 40], [1, 1], 4, 2, 128, seed=4)
@@ -274,6 +301,7 @@ def test_bad_table_entries_stay_in_the_pool():
     assert torch.equal(run_prefill(c, cap=20.0), run_prefill(fixed, cap=20.0))
 
 
+@BOTH
 def test_saturated_caps():
     """Scores far beyond the cap on both sides, and a cap so small that all weights are alike."""
     c = Case([500], [1], 8, 2, 128, seed=8)
@@ -288,6 +316,7 @@ def test_saturated_caps():
         check(run_prefill(p, cap=cap), p, want, mean_abs, size.clamp(max=2 * cap))
 
 
+@BOTH
 def test_plain_rule_agrees_with_the_plain_operator():
     """No rule at all is causal attention, decode and chunks."""
     c = Case([700, 90, 33], [1, 1, 1], 8, 2, 128, seed=11)

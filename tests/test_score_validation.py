@@ -81,16 +81,18 @@ def test_score_refusals(lib):
     assert attn(lib, cu=P, max_q=5) == EINVAL
 
 
-def test_score_workspace(lib):
+@pytest.mark.routing("balanced", "library")
+def test_score_workspace(lib, decode_routing):
     size = lambda rows, mb, window=0, longest=0: lib.aicomp_paged_score_workspace_bytes(rows, 8, 2, 128, 16, mb, BF16, BF16, window,
                                                                                         longest)
     need = size(4, 256)
-    assert need > 0 and need % (4 * 8 * 130 * 4) == 0
+    assert need > 0
     assert attn(lib, mb=256, stride=256) == EWORKSPACE and str(need) in err(lib)
     assert attn(lib, mb=256, stride=256, ws=P, wsb=need - 1) == EWORKSPACE
     assert attn(lib, mb=256, stride=256, ws=P + 4, wsb=need) == EINVAL and "aligned" in err(lib)
-    assert size(4, 2) == 0                                      # whole rows
-    assert size(4, 256, window=32) == 0 and size(4, 256, longest=32) == 0
+    if decode_routing == "library":                             # whole rows of a small call
+        assert size(4, 2) == 0
+        assert size(4, 256, window=32) == 0 and size(4, 256, longest=32) == 0
     assert size(0, 256) == 0 and size(4, 256, window=-1) == 0
 
 
