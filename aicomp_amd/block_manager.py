@@ -9,7 +9,8 @@ kernels read (``block_table``, ``context_lens``, ``slot_mapping``,
 ``cu_q_lens``).  This module produces them.
 
 ``BlockAllocator``  LIFO free list over the pool's block ids with an owner
-                    check on free (a double free would alias two sequences).
+                    check on free (a double free would alias two sequences); a
+                    block may have several owners (``share``), each of whom frees it.
 ``StepPlanner``     sequences with independent lengths: admit, chunked prompt
                     ingestion under a per-step token budget, one token per
                     running sequence per decode step, preemption of the
@@ -54,7 +55,7 @@ class PlanError(ValueError):
     """A step plan that would make the kernels read or write outside what it owns."""
 
 
-def check_plan(plan: "StepPlan", num_blocks: int, block_size: int) -> None:
+def check_plan(plan: "StepPlan", num_blocks: int, block_size: int, shared: Optional[np.ndarray] = None) -> None:
     """Host-side self-check of a plan, from its host arrays, before anything is launched on it.
 
     The kernels do not fault on a bad plan: an append row whose slot is outside the pool is
@@ -62,6 +63,7 @@ def check_plan(plan: "StepPlan", num_blocks: int, block_size: int) -> None:
     silently wrong attention.  This makes it loud: every slot inside the pool and used once, every
     table entry a sequence needs inside the pool and owned by that sequence alone, lengths within
     the table, chunk rows consistent with the lengths, slots and positions consistent with the table.
+    ``shared`` (a mask over the pool's blocks) names those that several sequences may have: they are read only.
     Raises ``PlanError``.
     """
     bt, cl, cu = plan.host_block_table, plan.host_context_lens, plan.host_cu_q_lens
@@ -101,8 +103,13 @@ def check_plan(plan: "StepPlan", num_blocks: int, block_size: int) -> None:
             raise PlanError(f"sequence row {r}: positions are not {int(cl[r] - new[r])}..{int(cl[r]) - 1}")
         if (slot[cu[r]:cu[r + 1]] != ids[p // block_size].astype(np.int64) * block_size + p % block_size).any():
             raise PlanError(f"sequence row {r}: slots do not follow from its block table")
+    if shared is not None and T and shared[slot // block_size].any():
+        bad = int(np.flatnonzero(shared[slot // block_size])[0])
+        raise PlanError(f"new token {bad}: slot {int(slot[bad])} is in a block that other sequences share")
     if owned:
         allb = np.concatenate(owned)
+        if shared is not None:
+            allb = allb[~shared[allb]]
         if np.unique(allb).size != allb.size:
             raise PlanError("two sequences of the plan share a block")
 
@@ -123,6 +130,7 @@ class BlockAllocator:
         self._free = np.arange(self.num_blocks - 1, -1, -1, dtype=np.int32)
         self._top = self.num_blocks
         self._owned = np.zeros(self.num_blocks, dtype=bool)
+        self._more = np.zeros(self.num_blocks, dtype=np.int32)       # owners beyond the first
 
     @property
     def num_free(self) -> int:
@@ -153,9 +161,40 @@ class BlockAllocator:
             raise ValueError("block id out of range")
         if np.unique(b).size != b.size or not self._owned[b].all():
             raise ValueError("freeing a block that is not allocated (double free)")
+        others = self._more[b] > 0                     # these stay with their other owners
+        if others.any():
+            self._more[b[others]] -= 1
+            b = b[~others]
         self._owned[b] = False
         self._free[self._top:self._top + b.size] = b[::-1].astype(np.int32)
         self._top += b.size
+
+    def share(self, blocks: Iterable[int]) -> None:
+        """One more owner for each of these allocated blocks: ``free`` takes one owner away at a time."""
+        b = np.asarray(blocks if isinstance(blocks, np.ndarray) else list(blocks), dtype=np.int64)
+        if b.size == 0:
+            return
+        if b.min() < 0 or b.max() >= self.num_blocks:
+            raise ValueError("block id out of range")
+        if np.unique(b).size != b.size or not self._owned[b].all():
+            raise ValueError("sharing a block that is not allocated")
+        self._more[b] += 1
+
+    @property
+    def shared(self) -> np.ndarray:
+        """Mask of the blocks that have several owners."""
+        return self._more > 0
+
+    def compact(self) -> np.ndarray:
+        """Move the allocated blocks to the low end of the pool: int64 ``[n, 2]`` pairs (from, to), no block in two of
+        them, for ``ops.copy_blocks``.  The ids above the allocated ones are free afterwards."""
+        used = self.num_used
+        src = np.flatnonzero(self._owned[used:]).astype(np.int64) + used
+        dst = np.flatnonzero(~self._owned[:used]).astype(np.int64)
+        self._owned[dst], self._owned[src] = True, False
+        self._more[dst], self._more[src] = self._more[src], 0
+        self._free[:self._top] = np.arange(self.num_blocks - 1, used - 1, -1, dtype=np.int32)
+        return np.stack([src, dst], axis=1)
 
     def blocks_for(self, num_tokens: int) -> int:
         return -(-int(num_tokens) // self.block_size)
@@ -430,6 +469,45 @@ class StepPlanner:
             return
         self._release_row(r)
 
+    def fork(self, seq_id, new_id) -> np.ndarray:
+        """A second running sequence ``new_id`` with the tokens of ``seq_id`` so far.  Full blocks are shared (both only read
+        them from here on); a partly filled last block is copied: the returned int64 ``[n, 2]`` (source, target) pairs, of
+        which there are none or one, go to ``ops.copy_blocks`` (``PagedAttentionBackend.copy_blocks``) on the stream of
+        the steps, after the last step and before the next one."""
+        if seq_id not in self._row_of:
+            raise ValueError(f"sequence {seq_id!r} is not running")
+        if new_id in self._row_of or new_id in self._waiting_ids:
+            raise ValueError(f"sequence id {new_id!r} is already known")
+        if not self._free_rows:
+            raise ValueError(f"all {self.max_seqs} sequences are in use")
+        a = self._row_of[seq_id]
+        n = int(self._nblk[a])
+        full = int(self._len[a]) // self.block_size
+        mine = self._tab[a, :n].copy()
+        fresh = self.alloc.allocate(n - full)                  # raises OutOfBlocks before anything has changed
+        self.alloc.share(mine[:full])
+        r = self._free_rows.pop()
+        self._row_of[new_id], self._id_of[r] = r, new_id
+        self._tab[r, :full], self._tab[r, full:n] = mine[:full], fresh
+        for state in (self._nblk, self._len, self._prompt, self._orig, self._maxnew):
+            state[r] = state[a]
+        self._live[r] = True
+        self._arr[r] = self._arrivals
+        self._arrivals += 1
+        return np.stack([mine[full:], fresh], axis=1).astype(np.int64)
+
+    def compact(self) -> np.ndarray:
+        """Move every sequence's blocks to the low end of the pool: int64 ``[n, 2]`` (source, target) pairs for
+        ``ops.copy_blocks``, on the stream of the steps, after the last step and before the next one.  Plans made before hold the
+        old block ids and must not run any more."""
+        pairs = self.alloc.compact()
+        if pairs.size:
+            where = np.arange(self.alloc.num_blocks, dtype=np.int32)
+            where[pairs[:, 0]] = pairs[:, 1]
+            for r in np.flatnonzero(self._live):
+                self._tab[r, :self._nblk[r]] = where[self._tab[r, :self._nblk[r]]]
+        return pairs
+
     def _release_row(self, r: int) -> None:
         self.alloc.free(self._tab[r, :self._nblk[r]])
         self._nblk[r] = 0
@@ -655,7 +733,7 @@ class StepPlanner:
                              max_q_len=0, total_new_tokens=T, block_table=None, context_lens=None, cu_q_lens=None,
                              slot_mapping=None, positions=None, preempted=preempted, host_block_table=bt,
                              host_context_lens=cl, host_cu_q_lens=cu, host_slot_mapping=slot, host_positions=posn)
-            check_plan(probe, self.alloc.num_blocks, BS)       # raises before anything reaches the device
+            check_plan(probe, self.alloc.num_blocks, BS, self.alloc.shared)     # raises before anything reaches the device
         self._len[rows] = cl
         self._staging.upload(i, end)
         d32, d64 = self._staging.dev32[i], self._staging.dev64[i]      # (every offset is a multiple of its element size)

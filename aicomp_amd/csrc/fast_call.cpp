@@ -14,7 +14,8 @@
 // Same checks, same errors (RuntimeError), same results as the registered operator.
 //
 // Beside it, the plain calls of aicomp_amd.ops (kv_append, rope_kv_append, paged_decode_attn, rope_paged_decode_attn,
-// paged_prefill_attn, append_prefill_attn, chunks_and_rows, sample_tokens): the same checks made here instead of in Python.  A call that
+// paged_prefill_attn, append_prefill_attn, chunks_and_rows, sample_tokens, qk_norm_rope_kv_append, paged_score_attn,
+// copy_blocks): the same checks made here instead of in Python.  A call that
 // passes them all is launched and returns true; any other returns false without having touched
 // anything, and the Python function goes on to convert what may be converted or to name what is wrong.
 #include <Python.h>
@@ -781,6 +782,148 @@ PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // token per running sequence and nothing else: 52 us of host time at 8 sequences, of which these functions leave 20
 // (most of that the copy's own call, its event and the plan's tensors).
 
+// ---- normed heads, scores by a rule, block copies
+
+PyObject* qk_norm_rope_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        Pools p;
+        double eps;
+        if (nargs != 16)
+            FAIL("qk_norm_rope_kv_append(query, key, value, q_weight, k_weight, cos, sin, positions, k_pool, v_pool, slot_mapping, "
+                 "eps, interleaved, k_scale, v_scale, out)");
+        const at::Tensor *q = plain(args[0]), *key = plain(args[1]), *value = plain(args[2]), *slots = plain(args[10]),
+                         *out = plain(args[15]);
+        auto optional = [&](int i, bool& ok) -> const at::Tensor* {
+            if (args[i] == Py_None) return nullptr;
+            const at::Tensor* t = plain(args[i]);
+            ok = ok && t;
+            return t;
+        };
+        bool ok = true;
+        const at::Tensor *qw = optional(3, ok), *kw = optional(4, ok), *cos = optional(5, ok), *sin = optional(6, ok), *pos = optional(7, ok);
+        if (!ok || !q || !key || !value || !out || !p.get(args[8], args[9]) || !as_double(args[11], eps) || !PyBool_Check(args[12]) ||
+            q->dim() != 3 || key->dim() != 3 || value->sizes() != key->sizes() || out->sizes() != q->sizes() || !cos != !sin)
+            Py_RETURN_FALSE;
+        const int64_t T = q->size(0);
+        const at::ScalarType st = q->scalar_type();
+        const int dt = dtype_code(st);
+        if (T == 0 || dt < 0 || key->size(0) != T || key->size(1) != p.hkv || key->size(2) != p.d || q->size(2) != p.d ||
+            key->scalar_type() != st || value->scalar_type() != st || out->scalar_type() != st || q->stride(2) != 1 ||
+            out->stride(2) != 1 || key->stride(2) != 1 || key->strides() != value->strides())
+            Py_RETURN_FALSE;
+        for (const at::Tensor* w : {qw, kw})
+            if (w && (w->dim() != 1 || !vector_of(w, at::kFloat, p.d, *q))) Py_RETURN_FALSE;
+        if (cos && (cos->dim() != 2 || sin->sizes() != cos->sizes() || cos->scalar_type() != at::kFloat ||
+                    sin->scalar_type() != at::kFloat || cos->stride(1) != 1 || cos->strides() != sin->strides() || cos->size(1) <= 0 ||
+                    2 * cos->size(1) > p.d || (!pos && cos->size(0) < T) || !on(*cos, *q) || !on(*sin, *q)))
+            Py_RETURN_FALSE;
+        if ((pos && !vector_of(pos, at::kLong, T, *q)) || !vector_of(slots, at::kLong, T, *q) || !on(*key, *q) || !on(*value, *q) ||
+            !on(*out, *q) || !on(*p.k, *q) || (p.dt != dt && p.dt != AICOMP_KV_FP8_E4M3) || !p.scales(args[13], args[14]))
+            Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(q->device());
+        void* stream = stream_of(*q);
+        const bool interleaved = args[12] == Py_True;
+        auto data = [](const at::Tensor* t) { return t ? t->data_ptr() : nullptr; };
+        const int rc = unlocked([&] {
+            return aicomp_qk_norm_rope_kv_append(
+                q->data_ptr(), out->data_ptr(), q->stride(0), q->stride(1), out->stride(0), out->stride(1), key->data_ptr(),
+                value->data_ptr(), key->stride(0), key->stride(1), (const float*)data(qw), (const float*)data(kw), (float)eps,
+                (const float*)data(cos), (const float*)data(sin), cos ? cos->stride(0) : 0, cos ? cos->size(0) : 0,
+                cos ? (int)(2 * cos->size(1)) : 0, interleaved, (const int64_t*)data(pos), p.k->data_ptr(), p.v->data_ptr(),
+                (const int64_t*)slots->data_ptr(), T, (int)q->size(1), p.hkv, p.d, p.bs, p.nb, dt, p.dt, p.ks, p.vs, stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+// paged_score_decode_attn (cu and prefix None, max_q 0) and paged_score_prefill_attn
+PyObject* paged_score_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        Pools p;
+        const at::Tensor *out, *q, *table, *ctx;
+        int dt, max_q, window, longest;
+        int64_t S;
+        double scale, softcap;
+        if (nargs != 18)
+            FAIL("paged_score_attn(out, query, k_pool, v_pool, block_table, context_lens, scale, k_scale, v_scale, cu_q_lens, max_q_len, "
+                 "softcap, slopes, window, first_keys, prefix_lens, longest_context, workspace)");
+        if (!attention_args(args, out, q, p, table, ctx, dt, S) || !as_double(args[6], scale) || !p.scales(args[7], args[8]) ||
+            !as_int(args[10], max_q) || !as_double(args[11], softcap) || !as_int(args[13], window) || !as_int(args[16], longest))
+            Py_RETURN_FALSE;
+        const int64_t T = q->size(0), hq = q->size(1);
+        const at::Tensor *cu = nullptr, *slopes = nullptr, *first = nullptr, *prefix = nullptr, *own = nullptr;
+        if (args[9] != Py_None && !vector_of(cu = plain(args[9]), at::kInt, S + 1, *q)) Py_RETURN_FALSE;
+        if (args[12] != Py_None && (!vector_of(slopes = plain(args[12]), at::kFloat, hq, *q) || slopes->dim() != 1)) Py_RETURN_FALSE;
+        if (args[14] != Py_None && (!vector_of(first = plain(args[14]), at::kInt, T, *q) || first->dim() != 1)) Py_RETURN_FALSE;
+        if (args[15] != Py_None && (!vector_of(prefix = plain(args[15]), at::kInt, S, *q) || prefix->dim() != 1)) Py_RETURN_FALSE;
+        if (args[17] != Py_None && (!(own = plain(args[17])) || !own->is_contiguous() || !on(*own, *q))) Py_RETURN_FALSE;
+        if (T > INT_MAX || (cu ? max_q <= 0 : T != S)) Py_RETURN_FALSE;
+        const int width = (int)table->size(1);
+        const c10::DeviceGuard guard(q->device());
+        void* stream = stream_of(*q);
+        at::Tensor scratch;
+        bool shared = false;                           // the module's own scratch, not the caller's
+        if (own) {
+            scratch = *own;
+        } else if (!cu) {
+            const size_t need = aicomp_paged_score_workspace_bytes((int)S, (int)hq, p.hkv, p.d, p.bs, width, dt, p.dt, window, longest);
+            if (need && recording(stream)) {           // memory of the graph's own: two graphs may be replayed side by side
+                scratch = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(q->device()));
+            } else if (need) {
+                shared = true;
+                scratch = cached_scratch(q->device(), stream, need);
+            }
+        }
+        auto data = [](const at::Tensor* t) { return t ? t->data_ptr() : nullptr; };
+        const int rc = unlocked([&] {
+            std::unique_lock<std::mutex> one_at_a_time(scratch_launches(), std::defer_lock);
+            if (shared) one_at_a_time.lock();
+            return aicomp_paged_score_attn(
+                out->data_ptr(), q->data_ptr(), p.k->data_ptr(), p.v->data_ptr(), (const int32_t*)table->data_ptr(), table->stride(0),
+                (const int32_t*)ctx->data_ptr(), (const int32_t*)data(cu), (int)S, T, max_q, (int)hq, p.hkv, p.d, p.bs, width, p.nb,
+                (float)scale, dt, p.dt, p.ks, p.vs, (float)softcap, (const float*)data(slopes), window, (const int32_t*)data(first),
+                (const int32_t*)data(prefix), longest, scratch.defined() ? scratch.data_ptr() : nullptr,
+                scratch.defined() ? (size_t)(scratch.numel() * scratch.element_size()) : 0, stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+PyObject* copy_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        if (nargs != 2) FAIL("copy_blocks(pools, pairs)");
+        const at::Tensor* pairs = plain(args[1]);
+        const bool list = PyList_CheckExact(args[0]);
+        if (!pairs || (!list && !PyTuple_CheckExact(args[0]))) Py_RETURN_FALSE;
+        const Py_ssize_t n = list ? PyList_GET_SIZE(args[0]) : PyTuple_GET_SIZE(args[0]);
+        if (n <= 0 || n > INT_MAX) Py_RETURN_FALSE;
+        std::vector<void*> pools((size_t)n);
+        const at::Tensor* ref = nullptr;
+        at::Tensor first;                              // held: the list may change once the interpreter lock is let go of
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const at::Tensor* t = plain(list ? PyList_GET_ITEM(args[0], i) : PyTuple_GET_ITEM(args[0], i));
+            if (!t) Py_RETURN_FALSE;
+            if (!ref) { first = *t; ref = &first; }
+            if (t->sizes() != ref->sizes() || t->scalar_type() != ref->scalar_type() || t->dim() < 1 || !t->is_contiguous() || !on(*t, *ref))
+                Py_RETURN_FALSE;
+            pools[(size_t)i] = t->data_ptr();
+        }
+        if (pairs->scalar_type() != at::kLong || pairs->dim() != 2 || pairs->size(1) != 2 || pairs->size(0) == 0 || !pairs->is_contiguous() ||
+            !on(*pairs, *ref) || ref->numel() == 0)
+            Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(ref->device());
+        const int rc = aicomp_kv_copy_blocks(pools.data(), (int)n, ref->numel() / ref->size(0) * ref->element_size(), ref->size(0),
+                                             (const int64_t*)pairs->data_ptr(), pairs->size(0), stream_of(*ref));
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
 // A contiguous buffer of at least n elements of `size` bytes, released with the object; null data where it is not one.
 struct Buf {
     Py_buffer b{};
@@ -939,6 +1082,9 @@ PyMethodDef methods[] = {
     {"append_prefill_attn", FAST(append_prefill_attn), "ops.append_prefill_attn of a plain call"},
     {"chunks_and_rows", FAST(chunks_and_rows), "prompt chunks and one-token rows of a step, each through their own kernels"},
     {"sample_tokens", FAST(sample_tokens), "ops.sample_tokens of a plain call: the tokens, or None if it is not one"},
+    {"qk_norm_rope_kv_append", FAST(qk_norm_rope_kv_append), "ops.qk_norm_rope_kv_append of a plain call, out given"},
+    {"paged_score_attn", FAST(paged_score_attn), "ops.paged_score_decode_attn / paged_score_prefill_attn of a plain call"},
+    {"copy_blocks", FAST(copy_blocks), "ops.copy_blocks of a plain call, pairs on the device"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_aicomp_fast", "lean host routes into the paged KV-cache library",

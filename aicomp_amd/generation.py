@@ -18,13 +18,16 @@ sequence, ``clear_cache`` resets.  Differences, all on purpose:
 ``PagedAttentionBackend`` owns one K and one V pool per layer and runs, per layer and
 step, the rotary embedding fused with the append followed by the chunked-prefill
 kernel on the prompt-chunk rows and the decode kernel on the one-token rows; a small
-step of one-token rows alone is one launch (``ops.rope_paged_decode_attn``).
+step of one-token rows alone is one launch (``ops.rope_paged_decode_attn``).  A layer may norm its query and key
+heads (``set_head_norm``) and score by a rule (``set_score_rule``: a cap, a bias by distance, a window); its steps
+then run ``ops.qk_norm_rope_kv_append`` and the ``ops.paged_score_*`` calls.
 """
 from __future__ import annotations
 
 import math
 from typing import Callable, Dict, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import ops
@@ -36,13 +39,16 @@ class PagedAttentionBackend:
 
     ``inv_freq`` (the rotary module's buffer, compiler_fx/modeling_llama.py:130-132) switches
     the rotary embedding on: ``attend`` then takes Q/K as projected and rotates them itself.
-    Without it Q/K must arrive rotated.
+    Without it Q/K must arrive rotated.  With fewer than ``head_dim / 2`` frequencies the rest of each head is not rotated;
+    ``interleaved`` rotates neighbours instead of halves (both are computed in float32 and rounded once, where the
+    rotation of whole heads by halves repeats the roundings of the reference's eager evaluation).
     """
 
     def __init__(self, num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda", kv_dtype: Optional[torch.dtype] = None,
                  inv_freq: Optional[torch.Tensor] = None, max_positions: int = 8192,
-                 attention_scaling: float = 1.0, scale: Optional[float] = None, block_size: int = 16) -> None:
+                 attention_scaling: float = 1.0, scale: Optional[float] = None, block_size: int = 16,
+                 interleaved: bool = False) -> None:
         self.device = torch.device(device)
         self.dtype = dtype
         kv_dtype = kv_dtype or dtype
@@ -53,17 +59,82 @@ class PagedAttentionBackend:
         self.v_scales: List[Optional[torch.Tensor]] = [None] * num_layers
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         self.cos = self.sin = None
-        if inv_freq is not None:
+        self.interleaved = bool(interleaved)
+        # float32 tables of a layer that norms its heads, or of every layer where the rotation is not that of whole heads by halves
+        self._pair_tables = None
+        self._pairs_from = None if inv_freq is None else (inv_freq, max_positions, attention_scaling)
+        self._pairs_only = inv_freq is not None and (self.interleaved or 2 * inv_freq.numel() != head_dim)
+        if inv_freq is not None and not self._pairs_only:
             self.cos, self.sin = ops.rotary_tables(inv_freq, max_positions, dtype, attention_scaling, self.device)
+        if self._pairs_only:
+            self._pairs()
+        self._norms: Dict[int, tuple] = {}
+        self._rules: Dict[int, dict] = {}
         self.plan: Optional[StepPlan] = None
+        self.first_keys: Optional[torch.Tensor] = None
+        self.prefix_lens: Optional[torch.Tensor] = None
+
+    def _pairs(self):
+        if self._pair_tables is None and self._pairs_from is not None:
+            inv_freq, positions, scaling = self._pairs_from
+            self._pair_tables = ops.rotary_pair_tables(inv_freq, positions, scaling, self.device)
+        return self._pair_tables or (None, None)
+
+    @property
+    def num_positions(self) -> Optional[int]:
+        """Rows of the rotary tables, ``None`` without them."""
+        return None if self._pairs_from is None else int(self._pairs_from[1])
+
+    def set_head_norm(self, layer_idx: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                      eps: float = 1e-6) -> None:
+        """RMS norm of every query and key head of a layer before the rotation, weights ``[D]`` (``None``: not that one)."""
+        f32 = lambda w: None if w is None else w.to(self.device, torch.float32).contiguous()
+        self._norms[layer_idx] = (f32(q_weight), f32(k_weight), float(eps))
+        self._pairs()                                  # (built here, not in the first step)
+
+    def set_score_rule(self, layer_idx: int, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: int = 0) -> None:
+        """Scores of a layer: capped by a tanh, less ``slopes[h]`` times the distance, over the last ``window`` keys."""
+        if softcap < 0 or window < 0:
+            raise ValueError(f"softcap and window must not be negative, got {softcap}, {window}")
+        self._rules[layer_idx] = dict(softcap=float(softcap), window=int(window),
+                                      slopes=None if slopes is None else slopes.to(self.device, torch.float32).contiguous())
+
+    def copy_blocks(self, pairs) -> None:
+        """Blocks copied in every layer's pools: what ``StepPlanner.fork`` and ``compact`` return."""
+        pairs = torch.from_numpy(np.ascontiguousarray(pairs, dtype=np.int64))
+        if pairs.shape[0]:
+            ops.copy_blocks(self.k_pools + self.v_pools, pairs)
 
     def set_scales(self, layer_idx: int, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
         """Per-KV-head dequantisation scales of an fp8 pool."""
         self.k_scales[layer_idx] = k_scale.to(self.device, torch.float32).contiguous()
         self.v_scales[layer_idx] = v_scale.to(self.device, torch.float32).contiguous()
 
-    def begin_step(self, plan: StepPlan) -> None:
-        self.plan = plan
+    def begin_step(self, plan: StepPlan, first_keys: Optional[torch.Tensor] = None,
+                   prefix_lens: Optional[torch.Tensor] = None) -> None:
+        """``first_keys [T]`` int32: the first key that each row of the step sees (packed documents); ``prefix_lens [S]`` int32: the
+        part at the start of each sequence that all its rows see.  Both hold for every layer of the step."""
+        self.plan, self.first_keys, self.prefix_lens = plan, first_keys, prefix_lens
+
+    def _score_attend(self, layer_idx: int, out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+        """Attention of a step by the layer's rule: its rows are in the pools, ``q`` is rotated."""
+        plan, kp, vp = self.plan, self.k_pools[layer_idx], self.v_pools[layer_idx]
+        ks, vs = self.k_scales[layer_idx], self.v_scales[layer_idx]
+        rule = self._rules.get(layer_idx, {})
+        npre, S, t = plan.num_prefill_seqs, plan.num_seqs, plan.num_prefill_tokens
+        first, prefix = self.first_keys, self.prefix_lens
+        if npre:
+            ops.paged_score_prefill_attn(out[:t], q[:t], kp, vp, plan.block_table[:npre], plan.context_lens[:npre],
+                                         plan.cu_q_lens[:npre + 1], self.scale, max_q_len=plan.max_q_len,
+                                         first_keys=None if first is None else first[:t],
+                                         prefix_lens=None if prefix is None else prefix[:npre], k_scale=ks, v_scale=vs, **rule)
+        if S > npre:
+            # (a recorded launch is sized for the whole table: the lengths of its replays may grow)
+            longest = 0 if q.is_cuda and torch.cuda.is_current_stream_capturing() else int(plan.host_context_lens[npre:].max())
+            ops.paged_score_decode_attn(out[t:], q[t:], kp, vp, plan.block_table[npre:], plan.context_lens[npre:], self.scale,
+                                        first_keys=None if first is None else first[t:], k_scale=ks, v_scale=vs,
+                                        longest_context=longest, **rule)
+        return out
 
     def attend(self, layer_idx: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
         """``query [T, Hq, D]``, ``key`` / ``value [T, Hkv, D]`` in the plan's row order -> ``[T, Hq, D]``."""
@@ -72,6 +143,23 @@ class PagedAttentionBackend:
             raise RuntimeError("PagedAttentionBackend.attend called outside a step (begin_step first)")
         kp, vp = self.k_pools[layer_idx], self.v_pools[layer_idx]
         ks, vs = self.k_scales[layer_idx], self.v_scales[layer_idx]
+        norm = self._norms.get(layer_idx)
+        ruled = layer_idx in self._rules or self.first_keys is not None or self.prefix_lens is not None
+        if ruled or norm is not None or self._pairs_only:
+            q = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            if norm is not None or self._pairs_only:
+                q_weight, k_weight, eps = norm or (None, None, 0.0)
+                cos, sin = self._pairs()
+                ops.qk_norm_rope_kv_append(query, key, value, q_weight, k_weight, cos, sin, plan.positions, kp, vp,
+                                           plan.slot_mapping, eps, self.interleaved, ks, vs, query_out=q)
+            elif self.cos is not None:
+                ops.rope_kv_append(query, key, value, self.cos, self.sin, plan.positions, kp, vp, plan.slot_mapping, ks, vs,
+                                   query_out=q)
+            else:
+                ops.kv_append(key, value, kp, vp, plan.slot_mapping, ks, vs)
+                q = query.contiguous()
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            return self._score_attend(layer_idx, out, q) if ruled else self._attend(layer_idx, out, q)
         if self.cos is not None and plan.num_prefill_seqs == 0:          # one token per sequence: one launch, if it can be
             out = ops.rope_paged_decode_attn(query, key, value, self.cos, self.sin, plan.positions, kp, vp,
                                              plan.slot_mapping, plan.block_table, plan.context_lens,
@@ -86,13 +174,19 @@ class PagedAttentionBackend:
         q = torch.empty(query.shape, dtype=query.dtype, device=query.device)
         ops.rope_kv_append(query, key, value, self.cos, self.sin, plan.positions, kp, vp, plan.slot_mapping,
                            ks, vs, query_out=q)
+        return self._attend(layer_idx, out, q)
+
+    def _attend(self, layer_idx: int, out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+        """Causal attention of a step whose rows are in the pools."""
+        plan, kp, vp = self.plan, self.k_pools[layer_idx], self.v_pools[layer_idx]
+        ks, vs = self.k_scales[layer_idx], self.v_scales[layer_idx]
         npre, S, t_pre = plan.num_prefill_seqs, plan.num_seqs, plan.num_prefill_tokens
         items = plan.launch_items(q, kp)
         if items is not None:                      # mixed step: chunks and decode rows in one launch
             return ops.paged_prefill_attn(out, q, kp, vp, plan.block_table, plan.context_lens, plan.cu_q_lens,
                                           self.scale, max_q_len=plan.launch_q_len(q.shape[1], kp.shape[1]), k_scale=ks,
                                           v_scale=vs, items=items)
-        if plan.only_chunks and t_pre == query.shape[0]:     # chunks alone, rows alone: the plan's tensors as they are
+        if plan.only_chunks and t_pre == q.shape[0]:         # chunks alone, rows alone: the plan's tensors as they are
             return ops.append_prefill_attn(out, q, None, None, kp, vp, None, plan.block_table, plan.context_lens,
                                            plan.cu_q_lens, self.scale, plan.max_q_len, ks, vs, plan.prefill_items(q, kp),
                                            plan.host_context_lens)
@@ -116,10 +210,12 @@ class ScheduleGeneration:
                  backend: PagedAttentionBackend, planner: StepPlanner) -> None:
         # a token whose position has no row in the rotary tables would be left unrotated and
         # unstored by the fused rotary + append launch: refuse the combination up front
-        cos = getattr(backend, "cos", None)
-        if cos is not None and planner.max_seq_len > cos.shape[0]:
+        cos, positions = getattr(backend, "cos", None), getattr(backend, "num_positions", None)
+        if positions is None and cos is not None:
+            positions = cos.shape[0]
+        if positions is not None and planner.max_seq_len > positions:
             raise ValueError(f"the planner admits sequences of {planner.max_seq_len} tokens but the backend's "
-                             f"rotary tables hold {cos.shape[0]} positions (max_positions)")
+                             f"rotary tables hold {positions} positions (max_positions)")
         self.model = model
         self.backend = backend
         self.planner = planner
@@ -197,6 +293,15 @@ class ScheduleGeneration:
         if len(got) != B:
             raise RuntimeError("not every sequence could be scheduled in this decode step")
         return torch.stack([got[b] for b in self._batch])
+
+    def fork(self, row: int) -> int:
+        """A second sequence with the tokens of batch row ``row`` so far (several continuations of one prompt): the new batch
+        row, the last one.  Its full blocks are shared, its last block is copied in every layer's pools."""
+        new = max(self._batch) + 1
+        self.backend.copy_blocks(self.planner.fork(self._batch[row], new))
+        self._batch.append(new)
+        self._offset[new] = self._offset.get(self._batch[row], 0)
+        return len(self._batch) - 1
 
     def clear_cache(self) -> None:
         """Release every sequence of the current batch (schedule_infer.py:451-454)."""

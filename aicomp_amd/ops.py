@@ -757,6 +757,10 @@ def qk_norm_rope_kv_append(query: torch.Tensor, key: torch.Tensor, value: torch.
     the inputs may be views into one projection output.
     """
     out = query if query_out is None else query_out
+    if _native("aicomp_qk_norm_rope_kv_append") and _FAST.qk_norm_rope_kv_append(
+            query, key, value, q_weight, k_weight, cos, sin, positions, k_pool, v_pool, slot_mapping, eps, interleaved, k_scale,
+            v_scale, out):
+        return out
     lib = _lib.load()
     _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
     nb, hkv, bs, d = _check_pools(k_pool, v_pool)
@@ -849,6 +853,10 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
     ``longest_context``: the host's bound of ``context_lens`` (0: the table's width); it sizes the call, no row is cut by it.
     In place on ``out [B, Hq, D]``, on the current stream.
     """
+    if _native("aicomp_paged_score_attn") and _FAST.paged_score_attn(
+            out, query, k_pool, v_pool, block_table, context_lens, scale, k_scale, v_scale, None, 0, softcap, slopes, window,
+            first_keys, None, longest_context, workspace):
+        return out
     lib = _lib.load()
     nb, hkv, bs, d, B, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
                                                      k_scale, v_scale)
@@ -891,6 +899,10 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
     first key that each row sees (packed documents), ``prefix_lens [S]`` int32 a part at the start of each sequence that all
     its rows see.  A row without visible keys is zero; rows behind the last sequence are left as they are.
     """
+    if _native("aicomp_paged_score_attn") and max_q_len and _FAST.paged_score_attn(
+            out, query, k_pool, v_pool, block_table, context_lens, scale, k_scale, v_scale, cu_q_lens, max_q_len, softcap, slopes,
+            window, first_keys, prefix_lens, 0, None):
+        return out
     lib = _lib.load()
     nb, hkv, bs, d, T, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
                                                      k_scale, v_scale)
@@ -923,6 +935,8 @@ def copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     No block may be the target of two pairs or the target of one and the source of another; pairs on the host are checked for
     that and copied to the device, pairs on the device are taken as they are (one outside the pools is skipped).
     """
+    if _native("aicomp_kv_copy_blocks") and _FAST.copy_blocks(pools, pairs):
+        return
     lib = _lib.load()
     _req(len(pools) > 0, "copy_blocks needs at least one pool")
     first = pools[0]
