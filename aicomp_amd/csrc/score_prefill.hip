@@ -2,9 +2,8 @@
 //
 // Mathematics: online softmax over tiles of 64 keys, one pass.  With a cap,
 //   cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)):
-// the matrix cores deliver 2 log2(e) x / cap (the multiplier is in Q), one exponential, one reciprocal and one multiply-add give the
-// score in the exponent's units with the running maximum already subtracted.  Without a cap they deliver score - maximum (the
-// accumulators start from -maximum).  The bias by distance is one addition and one multiply-add per score.
+// one exponential, one reciprocal and one multiply-add give the score in the exponent's units with the running maximum already
+// subtracted; without a cap it is one multiply-add.  The bias by distance is one addition and one multiply-add more.
 //
 // Work split   one workgroup (4 waves) per (64 or 128 query rows, sequence, head group); a row is a (position, query head)
 //              pair, the heads of a KV head packed side by side where the group divides 16, so that a K/V tile serves all of them.
@@ -14,10 +13,12 @@
 // K/V tiles    64 tokens, double-buffered in LDS, one barrier per tile.  16-bit pools: straight into LDS
 //              (global_load_lds_dwordx4) one tile ahead, rows unpadded, 16-byte chunks swizzled by the row.  fp8 pools: through
 //              registers, widened (exactly) to the query's type on the way.
+// head_dim     64, 128 or 256 (its tiles are 128 KB of LDS, one workgroup to a CU).
 // Per wave     16 or 32 rows.  S^T = K Q^T, rows as columns of the B operand; O^T += V^T P^T with V^T read by the transposing LDS
 //              read, in the token order of the scores, so that P never leaves its lane.
-// Rounding     Q times the multiplier, and the weights, to the 16-bit format of the matrix cores; sums, maxima and outputs
-//              in float32 until the one rounding of the result.
+// Rounding     The weights to the 16-bit format of the matrix cores; everything else in float32 until the one rounding of
+//              the result.  (The scores' multiplier in Q would save an instruction per score, which no time shows, and round
+//              Q once more: against float64 an error of 3.0e-3 where this has 2.1e-3, bf16, a prompt of 8192 under a cap.)
 #include "score.h"
 
 #include <atomic>
@@ -121,7 +122,7 @@ __device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, i
 
 // E: 16-bit format of queries and output; R: column groups of 16 rows per wave; DH: head_dim
 template <typename E, bool FP8, int R, int DH, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, DH == 64 ? 3 : 2)
+__global__ void __launch_bounds__(256, DH == 256 ? 1 : DH == 64 && !BIAS ? 3 : 2)
 score_prefill_kernel(ScorePrefillParams p) {
     constexpr int KROW = 2 * DH;               // bytes of an LDS row
     constexpr int NSL = DH / 32;               // k-slots of a row (QK^T MFMAs per 16 x 16 tile)
@@ -193,7 +194,7 @@ score_prefill_kernel(ScorePrefillParams p) {
 
     // Q as the B operand: column = this lane's row, k-slots = dims 32 s + 8 g4 ..
     const float ks = FP8 ? p.k_scale[kvh] : 1.f;
-    const float qmul = CAP ? 2.f * LOG2E * p.rule.cap_mul * ks : p.rule.mul * ks;
+    const float mul = CAP ? 2.f * LOG2E * p.rule.cap_mul * ks : p.rule.mul * ks;
     uint4 qf[R][NSL];
 #pragma unroll
     for (int c = 0; c < R; ++c) {
@@ -201,10 +202,6 @@ score_prefill_kernel(ScorePrefillParams p) {
 #pragma unroll
         for (int s = 0; s < NSL; ++s) {
             qf[c][s] = *(const uint4*)(qrow + 32 * s + 8 * g4);
-            uint32_t* x = (uint32_t*)&qf[c][s];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                x[i] = E::pack(E::to_f32((uint16_t)(x[i] & 0xffffu)) * qmul, E::to_f32((uint16_t)(x[i] >> 16)) * qmul);
         }
     }
 
@@ -228,14 +225,14 @@ score_prefill_kernel(ScorePrefillParams p) {
     // consecutive lanes share 64-byte segments that spread over a bank line; see prefill_mfma.hip for the measurements).
     auto swz_k = [](int row) {
         const int a = (row >> 2) & 3, b = row & 3;
-        return DH == 128 ? (a | (b << 2)) : (a | ((b >> 1) << 2));
+        return DH >= 128 ? (a | (b << 2)) : (a | ((b >> 1) << 2));
     };
     auto swz_v = [](int row) {
         const int a = (row >> 2) & 3, b = row & 3;
-        return DH == 128 ? ((a | ((b & 1) << 2)) << 1) : (a << 1);
+        return DH >= 128 ? ((a | ((b & 1) << 2)) << 1) : (a << 1);
     };
 
-    // --- 16-bit pools: tile t straight into LDS.  Wave w brings in block w of the tile, four (eight) rows per instruction.
+    // --- 16-bit pools: tile t straight into LDS.  Wave w brings in block w of the tile, 1 KB per instruction.
     constexpr int RPI = 1024 / KROW, NQ = 16 / RPI;
     const uint32_t blk_stride = (uint32_t)p.hkv * (BS * DH * (FP8 ? 1 : 2));
     const char* kp = (const char*)p.k_pool + (int64_t)kvh * (BS * DH * (FP8 ? 1 : 2));
@@ -247,23 +244,29 @@ score_prefill_kernel(ScorePrefillParams p) {
         offk[q] = lrow * KROW + ((lslot ^ swz_k(RPI * q + lrow)) << 4);
         offv[q] = lrow * KROW + ((lslot ^ swz_v(RPI * q + lrow)) << 4);
     }
-    auto fetch_dma = [&](int t, unsigned char* kb, unsigned char* vb) {
+    auto fetch_dma = [&](int t, unsigned char* kb, unsigned char* vb) __attribute__((always_inline)) {
         const int first = NB * t;
         if (t * KT >= kv_lo && (t + 1) * KT <= kv_hi) {                // workgroup-uniform
             const uint32_t blk = min((uint32_t)max(table[first + w], 0), (uint32_t)(p.num_blocks - 1));
             const uint64_t base = (uint64_t)blk * blk_stride;
-            // (opaque lane offsets: each address stays a uniform base plus a 32-bit offset)
-            uint32_t ok[4] = {offk[0], offk[1], offk[NQ > 2 ? 2 : 0], offk[NQ > 2 ? 3 : 1]};
-            uint32_t ov[4] = {offv[0], offv[1], offv[NQ > 2 ? 2 : 0], offv[NQ > 2 ? 3 : 1]};
-            asm volatile("" : "+v"(ok[0]), "+v"(ok[1]), "+v"(ok[2]), "+v"(ok[3]));
-            asm volatile("" : "+v"(ov[0]), "+v"(ov[1]), "+v"(ov[2]), "+v"(ov[3]));
+            // (opaque lane offsets: each address stays a uniform base plus a 32-bit offset; the instruction's own offset, up to
+            // 3 KB, moves the pool's address and that in LDS together)
+            uint32_t ok[NQ], ov[NQ];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                ok[q] = offk[q]; ov[q] = offv[q];
+                asm volatile("" : "+v"(ok[q]), "+v"(ov[q]));
+            }
             const char* ka = kp + base;
             const char* va = vp + base;
 #define AICOMP_DMA_ROWS(addr, o, buf, q)                                                                                   \
             if constexpr (q < NQ)                                                                                          \
-                __builtin_amdgcn_global_load_lds(GLOBAL_PTR(addr + o[q]), LDS_PTR(buf + 16 * w * KROW), 16, 1024 * q, 0);
+                __builtin_amdgcn_global_load_lds(GLOBAL_PTR(addr + (q / 4 * 4096) + o[q < NQ ? q : 0]),                    \
+                                                 LDS_PTR(buf + 16 * w * KROW + q / 4 * 4096), 16, 1024 * (q % 4), 0);
             AICOMP_DMA_ROWS(ka, ok, kb, 0) AICOMP_DMA_ROWS(ka, ok, kb, 1) AICOMP_DMA_ROWS(ka, ok, kb, 2) AICOMP_DMA_ROWS(ka, ok, kb, 3)
+            AICOMP_DMA_ROWS(ka, ok, kb, 4) AICOMP_DMA_ROWS(ka, ok, kb, 5) AICOMP_DMA_ROWS(ka, ok, kb, 6) AICOMP_DMA_ROWS(ka, ok, kb, 7)
             AICOMP_DMA_ROWS(va, ov, vb, 0) AICOMP_DMA_ROWS(va, ov, vb, 1) AICOMP_DMA_ROWS(va, ov, vb, 2) AICOMP_DMA_ROWS(va, ov, vb, 3)
+            AICOMP_DMA_ROWS(va, ov, vb, 4) AICOMP_DMA_ROWS(va, ov, vb, 5) AICOMP_DMA_ROWS(va, ov, vb, 6) AICOMP_DMA_ROWS(va, ov, vb, 7)
 #undef AICOMP_DMA_ROWS
         } else {
             // rows that nobody here sees take the nearest one that somebody does
@@ -285,7 +288,7 @@ score_prefill_kernel(ScorePrefillParams p) {
     };
     // --- fp8 pools: tile t into registers, eight codes per lane and load; then widened into LDS
     constexpr int RPL = 256 / CPR, NL = KT / RPL;              // rows per load of the workgroup, loads per tile and pool
-    auto fetch = [&](int t, Stage<FP8>& st) {
+    auto fetch = [&](int t, Stage<FP8>& st) __attribute__((always_inline)) {
         if constexpr (FP8) {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
@@ -298,7 +301,7 @@ score_prefill_kernel(ScorePrefillParams p) {
             }
         }
     };
-    auto stash = [&](const Stage<FP8>& st, unsigned char* kb, unsigned char* vb) {
+    auto stash = [&](const Stage<FP8>& st, unsigned char* kb, unsigned char* vb) __attribute__((always_inline)) {
         if constexpr (FP8) {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
@@ -313,14 +316,14 @@ score_prefill_kernel(ScorePrefillParams p) {
     const int vrow = 4 * (r16 >> 2) + g4;
 
     // one tile out of LDS
-    auto compute = [&](int t, const unsigned char* kb, const unsigned char* vb) {
+    auto compute = [&](int t, const unsigned char* kb, const unsigned char* vb) __attribute__((always_inline)) {
         const int start = t * KT;
         if (start >= wave_hi || start + KT <= wave_lo) return;         // wave-uniform
         f32x4_t sa[NH][R];
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int c = 0; c < R; ++c) sa[h][c] = CAP ? f32x4_t{0.f, 0.f, 0.f, 0.f} : f32x4_t{-m[c], -m[c], -m[c], -m[c]};
+            for (int c = 0; c < R; ++c) sa[h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < NSL; ++s) {
             uint4 a[NH];
@@ -344,20 +347,21 @@ score_prefill_kernel(ScorePrefillParams p) {
         uint4 pf[R][NH / 2];
         float alpha[R];
         bool grew[R];                                                  // wave-uniform
-        auto softmax = [&](auto mask_tag) {
+        auto softmax = [&](auto mask_tag) __attribute__((always_inline)) {
             constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
             for (int c = 0; c < R; ++c) {
                 float sc[NS];
                 bool dead[NS];
                 const float dist = (float)(start + g4 - pos[c]);       // score k is of key start + g4 + 16 (k / 4) + 4 (k % 4)
-                const float top = cap - m[c];
+                const float top = (CAP ? cap : 0.f) - m[c];
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
                     const int r = 16 * (k >> 2) + 4 * (k & 3);
                     sc[k] = sa[k >> 2][c][k & 3];
-                    if constexpr (CAP) sc[k] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(sc[k])), top);
-                    if constexpr (BIAS) sc[k] = fmaf(-slope[c], fabsf(dist + (float)r), sc[k]);
+                    const float base = BIAS ? fmaf(-slope[c], fabsf(dist + (float)r), top) : top;
+                    if constexpr (CAP) sc[k] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(sc[k] * mul)), base);
+                    else sc[k] = fmaf(sc[k], mul, base);
                     dead[k] = MASK && (uint32_t)(start + g4 - lo[c] + r) >= (uint32_t)(hi[c] - lo[c]);
                     if (MASK && dead[k]) sc[k] = NEG_BIG;
                 }
@@ -438,7 +442,7 @@ score_prefill_kernel(ScorePrefillParams p) {
 
     Stage<FP8> st;
     // Opens the step of tile t: it is in `kb` / `vb` afterwards for every wave, and the next one is on its way into the other pair.
-    auto open = [&](int t, unsigned char* kb, unsigned char* vb, unsigned char* kn, unsigned char* vn) {
+    auto open = [&](int t, unsigned char* kb, unsigned char* vb, unsigned char* kn, unsigned char* vn) __attribute__((always_inline)) {
         if constexpr (FP8) {
             stash(st, kb, vb);                                     // (nobody reads this pair: its readers met at the tile between)
             __syncthreads();
@@ -505,18 +509,15 @@ void launch_rule(const ScorePrefillParams& p, bool cap, bool bias, dim3 grid, hi
 
 template <typename E, bool FP8>
 void launch_shape(const ScorePrefillParams& p, int R, int d, bool cap, bool bias, dim3 grid, hipStream_t stream) {
-    if (d == 64) { if (R == 2) launch_rule<E, FP8, 2, 64>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 64>(p, cap, bias, grid, stream); }
+    if (d == 256) { if (R == 2) launch_rule<E, FP8, 2, 256>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 256>(p, cap, bias, grid, stream); }
+    else if (d == 64) { if (R == 2) launch_rule<E, FP8, 2, 64>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 64>(p, cap, bias, grid, stream); }
     else { if (R == 2) launch_rule<E, FP8, 2, 128>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 128>(p, cap, bias, grid, stream); }
 }
 
 }  // namespace
 
 bool score_prefill_supported(const ScoreArgs& a) {
-    if (a.cu_q_lens == nullptr || !is_16bit_float(a.q_dtype) || a.bs != BS || (a.d != 64 && a.d != 128)) return false;
-    // the score multiplier is rounded into Q: fp16 keeps it within a range where the product stays a normal number for
-    // ordinary queries (bf16 has float's range)
-    const float mul = a.cap > 0.f ? 2.f * a.scale / a.cap : a.scale;
-    if (a.q_dtype == AICOMP_KV_F16 && !(mul >= 0x1p-12f && mul <= 0x1p8f)) return false;
+    if (a.cu_q_lens == nullptr || !is_16bit_float(a.q_dtype) || a.bs != BS) return false;
     const int group = a.hq / a.hkv, gpack = 16 % group == 0 ? group : 1;
     const int64_t qtiles = ((int64_t)a.max_q_len * gpack + 63) / 64;
     return a.num_seqs <= 65535 && qtiles <= 65535 && a.num_blocks <= INT32_MAX && (int64_t)a.hkv * BS * a.d * 2 <= UINT32_MAX;

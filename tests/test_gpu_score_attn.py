@@ -2,10 +2,10 @@
 that leave rows empty, non-finite values where nothing may look, rows behind the last sequence.
 
 Tolerance, per output element and derived from the formats: the result is rounded once (half a step of the output type, u = eps / 2
-relative).  The matrix-core kernels round the query times the score's multiplier to the 16-bit type, which moves a score by at
-most ds = u * max_j scale sum_d |q_d k_jd| (a cap only shrinks it) and a weight by e^(2 ds) - 1 relative to the others, and round the
-weights themselves, u each, so that the mean moves by at most (2 u + e^(2 ds) - 1) times the weighted mean of |v| and of the result.  Float32 sums
-of up to 2000 terms and exponents of up to 2^7 add less than 1e-5 of that; a float32 call has u = 2^-24 for both (1e-5 covers them).
+relative).  The matrix-core kernels round the weights to the 16-bit type, u each, so that the mean moves by at most 2 u times the
+weighted mean of |v| and of the result.  A score is a float32 sum of up to 256 products: off by at most ds = 300 * 2^-24 * max_j scale
+sum_d |q_d k_jd| (a cap only shrinks it), which moves a weight by e^(2 ds) - 1 relative to the others.  Float32 sums of up to 2000
+weights and exponents of up to 2^7 add less than 1e-5 of that; a float32 call rounds no weight.
 """
 import math
 
@@ -93,7 +93,7 @@ def check(got, c, want, mean_abs, size):
     assert bool(torch.isfinite(want).all()) and bool(torch.isfinite(got).all())
     u = torch.finfo(c.dtype).eps / 2
     uq = 0.0 if c.dtype == F32 else u
-    ds = uq * size[..., None]
+    ds = 300 * 2.0 ** -24 * size[..., None]
     tol = u * want.abs() + (2 * uq + torch.expm1(2 * ds) + 1e-5) * (mean_abs + want.abs()) + 1e-30
     if c.dtype == F16:
         tol = tol + 2.0 ** -24                              # (results and weights below the normal numbers)
