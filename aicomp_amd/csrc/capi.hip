@@ -820,6 +820,7 @@ int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes
 // row's visible keys.  The lines are those of the plain decode calls, for rows as long as the window (or the hint) lets them be.
 struct ScoreCut {
     bool matrix, balanced;
+    int tile;                   // tokens of the matrix-core kernels' tiles
     int partition_size, parts;
 };
 
@@ -828,10 +829,11 @@ static ScoreCut score_cut(int64_t rows, int hq, int hkv, int d, int bs, int max_
     int64_t span = (int64_t)max_blocks * bs;
     if (longest_context > 0) span = std::min<int64_t>(span, longest_context);
     ScoreCut c;
-    c.matrix = is_16bit_float(q_dtype) && rows <= 65535 && streamk_shape(1, hq, hkv, d, bs, q_dtype, kv_dtype);
+    c.matrix = rows <= 65535 && streamk_shape(1, hq, hkv, d, bs, q_dtype, kv_dtype);
+    c.tile = q_dtype == AICOMP_KV_F32 ? (d == 64 ? 32 : 16) : (d == 64 ? 64 : 32);
     const bool few = c.matrix && rows <= 1024 && hkv <= 256;           // (what the balanced schedule can hold)
     // (a window that begins inside a tile reaches into one more)
-    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + (c.matrix ? (d == 64 ? 63 : 31) : 0));
+    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + (c.matrix ? c.tile - 1 : 0));
     const int columns = (int)((span + bs - 1) / bs);
     c.balanced = few && !grid_call(rows, hq, hkv, d, bs, columns, kv_dtype);
     c.partition_size = auto_partition(rows, hq, hkv, d, bs, columns, kv_dtype, few);
@@ -931,7 +933,7 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
     m.stream = a.stream; m.rule = &rule;
     if (c.balanced) return launch_decode_streamk(m, workspace);
     rc = launch_decode_mfma(m);
-    a.part_align = a.d == 64 ? 64 : 32;
+    a.part_align = c.tile;
     return rc == AICOMP_KV_OK && a.num_parts > 1 ? launch_score_merge(a) : rc;
 }
 

@@ -305,7 +305,7 @@ struct DecodeArgs {
     const int32_t* items;
     int num_items;
     bool chunks;                // prefill only: the call is a step's prompt chunks and nothing else
-    const ScoreRule* rule;   // decode only (NULL = none): scores by a rule (score.h), 16-bit queries
+    const ScoreRule* rule;      // decode only (NULL = none): scores by a rule (score.h)
     int longest_context;        // prefill only: what the caller knows of context_lens (0: nothing); chooses a kernel, bounds nothing
 };
 

@@ -95,12 +95,14 @@ struct MfmaRuleParams : MfmaParams {
 
 // A decode row's scores by the rule: what a lane makes of its products (its column's head), and the first visible key.
 template <typename T, typename Params>
-__device__ __forceinline__ RuleScore rule_score(const Params& p, int kvh, int lane) {
-    RuleScore s;
+__device__ __forceinline__ auto rule_score(const Params& p, int kvh, int lane) {
+    constexpr bool F32 = sizeof(typename T::Fmt::raw) == 4;
+    std::conditional_t<F32, RuleScoreF32, RuleScore> s;
     const float ks = T::FP8 ? p.k_scale[kvh] : 1.f;
+    const int h = T::QUAD ? lane & 3 : (lane & 15) / T::NPAR;
     s.cap = p.rule.cap_log2;
-    s.mul = (s.cap > 0.f ? 2.f * LOG2E * p.rule.cap_mul : p.rule.mul) * ks;
-    s.slope = p.rule.slopes != nullptr ? p.rule.slopes[kvh * p.group + min((lane & 15) / T::NPAR, p.group - 1)] * LOG2E : 0.f;
+    s.mul = (s.cap > 0.f ? (F32 ? 1.f : 2.f * LOG2E) * p.rule.cap_mul : p.rule.mul) * ks;
+    s.slope = p.rule.slopes != nullptr ? p.rule.slopes[kvh * p.group + min(h, p.group - 1)] * LOG2E : 0.f;
     s.pos = s.lo = 0;
     return s;
 }
@@ -244,7 +246,7 @@ paged_decode_mfma_kernel(std::conditional_t<RULE, MfmaRuleParams, MfmaParams> p)
 
     auto score = [&] {
         if constexpr (RULE) {
-            RuleScore s = rule_score<T>(p, kvh, lane);
+            auto s = rule_score<T>(p, kvh, lane);
             s.pos = len - 1;
             s.lo = lo;
             return s;
@@ -1012,7 +1014,14 @@ int launch_decode_streamk(const DecodeArgs& a, void* workspace) {
         if (fp8) hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, true, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);   \
         else hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, false, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);      \
     } while (0)
-        if (pair) { if (f16) AICOMP_LAUNCH_SK_RULE(F16Fmt, true); else AICOMP_LAUNCH_SK_RULE(Bf16Fmt, true); }
+#define AICOMP_LAUNCH_SK_RULE32(DQ)                                                                                                 \
+    do {                                                                                                                            \
+        if (group <= 4) hipLaunchKernelGGL((streamk_decode_kernel<TileF32Quad<DQ>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);  \
+        else hipLaunchKernelGGL((streamk_decode_kernel<TileF32<DQ>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);                 \
+    } while (0)
+        if (f32) { if (pair) AICOMP_LAUNCH_SK_RULE32(64); else AICOMP_LAUNCH_SK_RULE32(128); }
+#undef AICOMP_LAUNCH_SK_RULE32
+        else if (pair) { if (f16) AICOMP_LAUNCH_SK_RULE(F16Fmt, true); else AICOMP_LAUNCH_SK_RULE(Bf16Fmt, true); }
         else { if (f16) AICOMP_LAUNCH_SK_RULE(F16Fmt, false); else AICOMP_LAUNCH_SK_RULE(Bf16Fmt, false); }
 #undef AICOMP_LAUNCH_SK_RULE
     } else if (f32) {
@@ -1039,7 +1048,7 @@ int launch_decode_streamk(const DecodeArgs& a, void* workspace) {
         if (a.rule != nullptr) AICOMP_LAUNCH_RED_BY(E, DQ, ScoreRule, *a.rule);                                   \
         else AICOMP_LAUNCH_RED_BY(E, DQ, NoRule, NoRule{});                                                       \
     } while (0)
-    if (f32) { if (a.d == 64) AICOMP_LAUNCH_RED_BY(F32Fmt, 64, NoRule, NoRule{}); else AICOMP_LAUNCH_RED_BY(F32Fmt, 128, NoRule, NoRule{}); }
+    if (f32) { if (a.d == 64) AICOMP_LAUNCH_RED(F32Fmt, 64); else AICOMP_LAUNCH_RED(F32Fmt, 128); }
     else if (pair) { if (f16) AICOMP_LAUNCH_RED(F16Fmt, 64); else AICOMP_LAUNCH_RED(Bf16Fmt, 64); }
     else { if (f16) AICOMP_LAUNCH_RED(F16Fmt, 128); else AICOMP_LAUNCH_RED(Bf16Fmt, 128); }
 #undef AICOMP_LAUNCH_RED_BY
@@ -1083,7 +1092,7 @@ int launch_decode_mfma(const DecodeArgs& a) {
     // rows of 1024 tokens of fp8 406 and 464.
     const int tile = a.q_dtype == AICOMP_KV_F32 ? (d64 ? TILE : TILE / 2) : (d64 ? 2 * TILE : TILE);
     const bool wide = a.partition_size > 16 * tile && a.rows * a.hkv * a.num_parts <= 256;
-    if (a.rule != nullptr) {               // (16-bit queries; a split's merge is the caller's)
+    if (a.rule != nullptr) {               // (a split's merge is the caller's)
         MfmaRuleParams rp;
         (MfmaParams&)rp = p;
         rp.rule = *a.rule;
@@ -1097,7 +1106,11 @@ int launch_decode_mfma(const DecodeArgs& a) {
         if (d64) { if (fp8) AICOMP_LAUNCH_RULE(Tile16<E, true, true>); else AICOMP_LAUNCH_RULE(Tile16<E, false, true>); } \
         else { if (fp8) AICOMP_LAUNCH_RULE(Tile16<E, true, false>); else AICOMP_LAUNCH_RULE(Tile16<E, false, false>); }   \
     } while (0)
-        if (a.q_dtype == AICOMP_KV_F16) AICOMP_LAUNCH_RULE16(F16Fmt); else AICOMP_LAUNCH_RULE16(Bf16Fmt);
+        if (a.q_dtype == AICOMP_KV_F32) {
+            if (d64) { if (p.group <= 4) AICOMP_LAUNCH_RULE(TileF32Quad<64>); else AICOMP_LAUNCH_RULE(TileF32<64>); }
+            else { if (p.group <= 4) AICOMP_LAUNCH_RULE(TileF32Quad<128>); else AICOMP_LAUNCH_RULE(TileF32<128>); }
+        } else if (a.q_dtype == AICOMP_KV_F16) AICOMP_LAUNCH_RULE16(F16Fmt);
+        else AICOMP_LAUNCH_RULE16(Bf16Fmt);
 #undef AICOMP_LAUNCH_RULE16
 #undef AICOMP_LAUNCH_RULE
         AICOMP_HIP_LAUNCH_CHECK();

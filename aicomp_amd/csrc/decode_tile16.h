@@ -150,8 +150,17 @@ struct RuleScore {
     }
     __device__ __forceinline__ bool below(int tok) const { return tok < lo; }
 };
+// Float32 tiles: the library's tanh, whose error is that of float32 also where it is multiplied by a large cap.
+struct RuleScoreF32 : RuleScore {          // mul with a cap: scale / cap
+    __device__ __forceinline__ float operator()(float s, int tok) const {
+        float x = s * mul;
+        if (cap > 0.f) x = cap * tanhf(x);
+        return fmaf(slope, (float)(tok - pos), x);
+    }
+};
 __device__ __forceinline__ PlainScore score_of(float mul) { return PlainScore{mul}; }
 __device__ __forceinline__ const RuleScore& score_of(const RuleScore& r) { return r; }
+__device__ __forceinline__ const RuleScoreF32& score_of(const RuleScoreF32& r) { return r; }
 
 // One 32-token tile: K registers -> LDS -> S^T = K Q^T -> online softmax -> O^T += V^T P^T.
 // NEXT: prefetch the wave's next tile (blocks nb0/nb1) into the same registers.

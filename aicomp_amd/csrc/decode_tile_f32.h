@@ -96,10 +96,12 @@ struct TileF32 {
     }
 
     // NEXT: prefetch the wave's next tile (blocks nb) into the same registers; MASK: the tile crosses `end`
-    template <bool NEXT, bool MASK, typename Params>
+    // (cmul: the score's multiplier, or a rule)
+    template <bool NEXT, bool MASK, typename Params, typename Mul>
     __device__ __forceinline__ static void process(State& st, Regs& t, const Q& q, unsigned char* kt, const Offsets& ko,
                                                    const Params& p, const int64_t (&nb)[4], int kvh_next, int lane,
-                                                   int tile_start, int end, float cmul) {
+                                                   int tile_start, int end, const Mul& cmul) {
+        const auto& score = score_of(cmul);
         const int g4 = lane >> 4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) *(uint4*)(kt + write_at(ko, i)) = t.k[i];
@@ -125,8 +127,9 @@ struct TileF32 {
         float sc[NS];
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
-            sc[k] = (s[k >> 2][0][k & 3] + s[k >> 2][1][k & 3]) * cmul;
-            if (MASK && tile_start + 16 * (k >> 2) + 4 * g4 + (k & 3) >= end) sc[k] = NEG_BIG;
+            const int tok = tile_start + 16 * (k >> 2) + 4 * g4 + (k & 3);
+            sc[k] = score(s[k >> 2][0][k & 3] + s[k >> 2][1][k & 3], tok);
+            if (MASK && (tok >= end || score.below(tok))) sc[k] = NEG_BIG;
         }
         float mx = sc[0];
 #pragma unroll
@@ -154,7 +157,7 @@ struct TileF32 {
         for (int i = 0; i < 8; ++i) {
             vv[i] = t.v[i];
             const int tok = tile_start + 16 * (i / (4 * HALVES)) + 4 * g4 + (i / HALVES) % 4;
-            if (MASK && tok >= end) vv[i] = make_uint4(0, 0, 0, 0);
+            if (MASK && (tok >= end || score.below(tok))) vv[i] = make_uint4(0, 0, 0, 0);
         }
         if (NEXT) load_v(t, p, nb, kvh_next, lane);
 #pragma unroll

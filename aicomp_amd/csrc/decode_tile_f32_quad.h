@@ -112,10 +112,14 @@ struct TileF32Quad {
     }
 
     // NEXT: prefetch the wave's next tile (blocks nb) into the same registers; MASK: the tile crosses `end`
-    template <bool NEXT, bool MASK, typename Params>
+    // (cm: the score's multiplier, or a rule)
+    template <bool NEXT, bool MASK, typename Params, typename Mul>
     __device__ __forceinline__ static void process(State& st, Regs& t, const Q& q, unsigned char* kt, const Offsets& ko,
                                                    const Params& p, const int64_t (&nb)[4], int kvh_next, int lane,
-                                                   int tile_start, int end, float cmul) {
+                                                   int tile_start, int end, const Mul& cm) {
+        const auto& score = score_of(cm);
+        constexpr bool RULE = std::decay_t<decltype(score)>::LOW;
+        const float cmul = RULE ? 1.f : score.mul;               // (a rule's scores have theirs already)
 #pragma unroll
         for (int i = 0; i < 8; ++i) *(uint4*)(kt + write_at(ko, i)) = t.k[i];
         if (NEXT) load_rows(t.k, p.k_pool, p, nb, kvh_next, lane);
@@ -137,7 +141,9 @@ struct TileF32Quad {
         // online softmax: the head's reference max moves only when a lane's probabilities of a tile outgrow 2^8
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            if (MASK && tile_start + token(lane, r) >= end) sc[r] = -INFINITY;
+            const int tok = tile_start + token(lane, r);
+            if constexpr (RULE) sc[r] = score(sc[r], tok);
+            if (MASK && (tok >= end || score.below(tok))) sc[r] = -INFINITY;
             e[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], cmul, -st.m));
             sum += e[r];
         }
@@ -167,7 +173,8 @@ struct TileF32Quad {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             vv[i] = t.v[i];
-            if (MASK && tile_start + RPL * i + (lane >> (DQ == 64 ? 4 : 5)) >= end) vv[i] = make_uint4(0, 0, 0, 0);
+            const int vtok = tile_start + RPL * i + (lane >> (DQ == 64 ? 4 : 5));
+            if (MASK && (vtok >= end || score.below(vtok))) vv[i] = make_uint4(0, 0, 0, 0);
         }
         if (NEXT) load_rows(t.v, p.v_pool, p, nb, kvh_next, lane);
         pv<0>(st, vv, e);
