@@ -114,7 +114,7 @@ def _declare(lib: C.CDLL) -> None:
     lib.aicomp_paged_score_attn.argtypes = [vp, vp, vp, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, i32, i32, i32, i64, f32, i32,
                                             i32, vp, vp, f32, vp, i32, vp, vp, i32, vp, sz, vp]
     lib.aicomp_paged_score_workspace_bytes.restype = sz
-    lib.aicomp_paged_score_workspace_bytes.argtypes = [i32] * 10
+    lib.aicomp_paged_score_workspace_bytes.argtypes = [i32, i64] + [i32] * 10
     lib.aicomp_sample_workspace_bytes.restype = sz
     lib.aicomp_sample_workspace_bytes.argtypes = [i32, i32, i64, f32, i32, i32, i32]
 

@@ -856,11 +856,34 @@ static int score_shape(ScoreArgs& a, const char* who) {
     return AICOMP_KV_OK;
 }
 
-size_t aicomp_paged_score_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+// Keys that rows of chunks can see, as far as the host knows; and the workspace where those are divided.
+static int64_t chunk_span(int bs, int max_blocks, int window, int longest_context) {
+    int64_t span = (int64_t)max_blocks * bs;
+    if (longest_context > 0) span = std::min<int64_t>(span, longest_context);
+    return window > 0 ? std::min<int64_t>(span, (int64_t)window + 128) : span;   // (neighbours of a tile, and the tile)
+}
+
+static size_t chunk_workspace_bytes(const ScoreArgs& a) {
+    if (!score_prefill_supported(a)) return 0;
+    // (whether there is a bias decides nothing where keys are divided)
+    const int parts = score_chunk_plan(a.num_seqs, a.rows, a.max_q_len, a.hq, a.hkv, a.d, a.kv_dtype == AICOMP_KV_FP8_E4M3, false,
+                                       a.span).parts;
+    return parts > 1 ? (size_t)a.rows * a.hq * parts * (a.d + 2) * sizeof(float) : 0;
+}
+
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
                                           int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context) {
     if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || block_size <= 0 ||
-        max_blocks_per_seq <= 0 || window < 0 || longest_context < 0)
+        max_blocks_per_seq <= 0 || window < 0 || longest_context < 0 || total_q <= 0 || max_q_len < 0)
         return 0;
+    if (max_q_len > 0) {
+        ScoreArgs a;
+        memset(&a, 0, sizeof(a));
+        a.num_seqs = num_seqs; a.rows = total_q; a.max_q_len = max_q_len; a.hq = num_q_heads; a.hkv = num_kv_heads; a.d = head_dim;
+        a.bs = block_size; a.q_dtype = q_dtype; a.kv_dtype = kv_dtype;
+        a.span = chunk_span(block_size, max_blocks_per_seq, window, longest_context);
+        return chunk_workspace_bytes(a);
+    }
     const ScoreCut c = score_cut(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, q_dtype, kv_dtype,
                                  window, longest_context);
     if (c.balanced) return decode_streamk_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim);
@@ -901,7 +924,18 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
     if (cu_q_lens != nullptr) {
         AICOMP_REQUIRE(max_q_len > 0 && max_q_len <= total_q, AICOMP_KV_EINVAL, "%s: max_q_len %d out of range (total %lld)", who,
                        max_q_len, (long long)total_q);
-        if (score_prefill_supported(a)) return launch_score_prefill(a);
+        if (score_prefill_supported(a)) {
+            a.span = chunk_span(block_size, max_blocks_per_seq, window, longest_context);
+            const size_t need = workspace ? chunk_workspace_bytes(a) : 0;
+            if (need > 0) {
+                AICOMP_REQUIRE(workspace_bytes >= need, AICOMP_KV_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who,
+                               need, workspace_bytes);
+                AICOMP_REQUIRE((uintptr_t)workspace % 16 == 0, AICOMP_KV_EINVAL, "%s: workspace must be 16-byte aligned", who);
+                a.ws_acc = (float*)workspace;
+                a.ws_ml = (float*)((char*)workspace + need / (head_dim + 2) * head_dim);
+            }
+            return launch_score_prefill(a);
+        }
         a.partition_size = INT32_MAX; a.num_parts = 1;
         return launch_score_generic(a);
     }
@@ -909,7 +943,7 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
                    "%s: without cu_q_lens there is one row per sequence and no prefix", who);
     const ScoreCut c = score_cut(a.rows, a.hq, a.hkv, a.d, a.bs, a.max_blocks, q_dtype, kv_dtype, window, longest_context);
     a.partition_size = c.partition_size; a.num_parts = c.parts; a.part_align = 1;
-    const size_t need = aicomp_paged_score_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+    const size_t need = aicomp_paged_score_workspace_bytes(num_seqs, total_q, 0, num_q_heads, num_kv_heads, head_dim, block_size,
                                                            max_blocks_per_seq, q_dtype, kv_dtype, window, longest_context);
     if (need > 0) {
         AICOMP_REQUIRE(workspace && workspace_bytes >= need, AICOMP_KV_EWORKSPACE,

@@ -867,8 +867,8 @@ PyObject* paged_score_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         bool shared = false;                           // the module's own scratch, not the caller's
         if (own) {
             scratch = *own;
-        } else if (!cu) {
-            const size_t need = aicomp_paged_score_workspace_bytes((int)S, (int)hq, p.hkv, p.d, p.bs, width, dt, p.dt, window, longest);
+        } else {
+            const size_t need = aicomp_paged_score_workspace_bytes((int)S, T, cu ? max_q : 0, (int)hq, p.hkv, p.d, p.bs, width, dt, p.dt, window, longest);
             if (need && recording(stream)) {           // memory of the graph's own: two graphs may be replayed side by side
                 scratch = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(q->device()));
             } else if (need) {

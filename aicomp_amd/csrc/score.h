@@ -35,8 +35,9 @@ struct ScoreArgs {
     const int32_t* prefix_lens; // [num_seqs] or NULL (not with decode)
     int partition_size, num_parts;      // decode: tokens per partition of a row's visible keys; the last takes what is left
     int part_align;             // the first partition begins at the multiple of this at or below the first visible key
-    float* ws_acc;              // [rows][Hq][num_parts][D]
-    float* ws_ml;               // [rows][Hq][num_parts][2]
+    int64_t span;               // chunks: a bound of the keys that a row sees, by which its call is laid out (no row is cut by it)
+    float* ws_acc;              // decode: [rows][Hq][num_parts][D]; chunks: [parts][rows][Hq][D], NULL: keys are not divided
+    float* ws_ml;               // decode: [rows][Hq][num_parts][2]; chunks: [parts][rows][Hq][2]
     hipStream_t stream;
 };
 
@@ -72,6 +73,9 @@ __device__ __forceinline__ void visible_keys(const ScoreRule& r, int64_t row, in
 int launch_score_generic(const ScoreArgs& a);
 int launch_score_merge(const ScoreArgs& a);
 bool score_prefill_supported(const ScoreArgs& a);
+// How a chunk call is laid out: column groups of 16 rows per wave, and the parts that the keys of its rows are divided into.
+struct ScoreChunkPlan { int R, parts; };
+ScoreChunkPlan score_chunk_plan(int num_seqs, int64_t total_q, int max_q_len, int hq, int hkv, int d, bool fp8, bool bias, int64_t span);
 int launch_score_prefill(const ScoreArgs& a);
 
 }  // namespace aicomp

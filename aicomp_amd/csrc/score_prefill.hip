@@ -5,7 +5,8 @@
 // one exponential, one reciprocal and one multiply-add give the score in the exponent's units with the running maximum already
 // subtracted; without a cap it is one multiply-add.  The bias by distance is one addition and one multiply-add more.
 //
-// Work split   one workgroup (4 waves) per (64 or 128 query rows, sequence, head group); a row is a (position, query head)
+// Work split   one workgroup (4 waves) per (64 or 128 query rows, sequence, head group), or, with few rows, per one of the parts that
+//              their keys are divided into (a second kernel joins the parts); a row is a (position, query head)
 //              pair, the heads of a KV head packed side by side where the group divides 16, so that a K/V tile serves all of them.
 //              Every row's visible keys are one interval [lo, hi): a workgroup walks the tiles between the smallest lo and the
 //              largest hi of its rows, a wave computes those between its own, and only tiles that cross a row's
@@ -21,6 +22,7 @@
 //              Q once more: against float64 an error of 3.0e-3 where this has 2.1e-3, bf16, a prompt of 8192 under a cap.)
 #include "score.h"
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -32,6 +34,7 @@ constexpr int BS = 16;
 constexpr int KT = 64;                 // tokens per tile
 constexpr int NB = KT / BS;            // blocks per tile
 constexpr float NEG_BIG = -1.0e30f;
+constexpr int PART_TILES = 4;          // least tiles of a part where the keys are divided
 
 struct ScorePrefillParams {
     void* out;
@@ -48,6 +51,11 @@ struct ScorePrefillParams {
     const float* k_scale;
     const float* v_scale;
     ScoreRule rule;
+    // divided keys (parts > 1): sums, reference and weight of part i of (row, head) at [(i rows + row) hq + head]
+    int hgroups, parts;
+    int64_t rows;
+    float* ws_acc;
+    float2* ws_ml;
 };
 
 template <bool FP8> struct Stage;              // registers of one K and one V tile (fp8 pools)
@@ -65,8 +73,9 @@ __device__ __forceinline__ int wave_min(int x) {
 
 // One row key by key, by a whole wave: what the matrix cores cannot give where a key that the row does not see, but a neighbour
 // does, has a value that is not finite (a weight of 0 times it is not 0).
-template <typename E, bool FP8, int DH>
-__device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, int head, int kvh, int pos, int lo, int hi, int lane) {
+template <typename E, bool FP8, int DH, bool PARTS>
+__device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, int head, int kvh, int pos, int lo, int hi, int part,
+                          int lane) {
     constexpr int NV = DH / 64;
     typedef typename E::elem Elem;
     const uint16_t* q = (const uint16_t*)p.query + (q_row * p.hq + head) * DH;
@@ -114,6 +123,13 @@ __device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, i
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+    if (PARTS && p.parts > 1) {
+        const int64_t slot = (part * p.rows + q_row) * p.hq + head;
+#pragma unroll
+        for (int e = 0; e < NV; ++e) p.ws_acc[slot * DH + lane + 64 * e] = acc[e];
+        if (lane == 0) p.ws_ml[slot] = make_float2(m, l);
+        return;
+    }
     const float inv = (FP8 ? p.v_scale[kvh] : 1.f) / l;
     uint16_t* o = (uint16_t*)p.out + (q_row * p.hq + head) * DH + lane;
 #pragma unroll
@@ -122,7 +138,7 @@ __device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, i
 
 // E: 16-bit format of queries and output; R: column groups of 16 rows per wave; DH: head_dim
 template <typename E, bool FP8, int R, int DH, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, DH == 256 ? 1 : DH == 64 && !BIAS ? 3 : 2)
+__global__ void __launch_bounds__(256, DH == 256 ? 1 : DH == 64 ? 3 : 2)
 score_prefill_kernel(ScorePrefillParams p) {
     constexpr int KROW = 2 * DH;               // bytes of an LDS row
     constexpr int NSL = DH / 32;               // k-slots of a row (QK^T MFMAs per 16 x 16 tile)
@@ -132,7 +148,7 @@ score_prefill_kernel(ScorePrefillParams p) {
     constexpr int TILE_BYTES = KT * KROW;
     constexpr int WROWS = 16 * R;              // rows per wave
     constexpr int NS = 4 * NH;                 // scores per lane and column group
-    const int hgroup = blockIdx.x, seq = blockIdx.y;
+    const int part = R == 1 ? blockIdx.x / p.hgroups : 0, hgroup = R == 1 ? blockIdx.x % p.hgroups : blockIdx.x, seq = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
@@ -181,8 +197,19 @@ score_prefill_kernel(ScorePrefillParams p) {
     int kv_hi = max(max(span[1][0], span[1][1]), max(span[1][2], span[1][3]));
     kv_lo = __builtin_amdgcn_readfirstlane(kv_lo);
     kv_hi = __builtin_amdgcn_readfirstlane(kv_hi);
-    if (kv_lo >= kv_hi) {                                      // nothing visible to any row: zero rows
-        for (int i = tid; i < 4 * WROWS * CPR; i += 256) {
+    int t_first = kv_lo / KT, t_end = (kv_hi + KT - 1) / KT;
+    const bool divided = R == 1 && p.parts > 1;
+    if (divided) {
+        const int per = max((t_end - t_first + p.parts - 1) / p.parts, PART_TILES);
+        t_end -= part * per;
+        t_first = max(t_first, t_end - per);
+    }
+    if (kv_lo >= kv_hi || t_first >= t_end) {                  // nothing visible to any row: zero rows
+        for (int i = tid; divided && i < 4 * WROWS; i += 256) {
+            const int at = q0 + i / p.gpack;
+            if (at < n) p.ws_ml[(part * p.rows + q_begin + at) * p.hq + hgroup * p.gpack + i % p.gpack] = make_float2(NEG_BIG, 0.f);
+        }
+        for (int i = tid; !divided && i < 4 * WROWS * CPR; i += 256) {
             const int row = i / CPR, at = q0 + row / p.gpack;
             if (at < n)
                 *(uint4*)((uint16_t*)p.out + ((int64_t)(q_begin + at) * p.hq + hgroup * p.gpack + row % p.gpack) * DH + 8 * (i % CPR)) =
@@ -190,7 +217,6 @@ score_prefill_kernel(ScorePrefillParams p) {
         }
         return;
     }
-    const int t_first = kv_lo / KT, t_end = (kv_hi + KT - 1) / KT;
 
     // Q as the B operand: column = this lane's row, k-slots = dims 32 s + 8 g4 ..
     const float ks = FP8 ? p.k_scale[kvh] : 1.f;
@@ -481,7 +507,18 @@ score_prefill_kernel(ScorePrefillParams p) {
         uint64_t again = __ballot(row_valid[c] && lo[c] < hi[c] && l - l == 0.f && !(worst == 0.f));
         again |= again >> 32;
         again = (again | (again >> 16)) & 0xffff;                      // rows, by column
-        if (row_valid[c] && !((again >> r16) & 1)) {
+        if (divided) {
+            if (row_valid[c] && !((again >> r16) & 1)) {
+                const int64_t slot = (part * p.rows + q_begin + pos[c] - prior) * p.hq + head[c];
+                if (g4 == 0) p.ws_ml[slot] = make_float2(m[c], l);
+                if (l != 0.f) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) *(f32x4_t*)(p.ws_acc + slot * DH + 16 * j + 4 * g4) = O[c][j];
+                }
+            }
+            lo[c] = max(lo[c], t_first * KT);
+            hi[c] = min(hi[c], t_end * KT);
+        } else if (row_valid[c] && !((again >> r16) & 1)) {
             const bool none = l == 0.f;                                // (no visible key, or all of weight 0)
             const float inv = (FP8 ? p.v_scale[kvh] : 1.f) / l;
             uint16_t* o = (uint16_t*)p.out + ((int64_t)(q_begin + pos[c] - prior) * p.hq + head[c]) * DH + 4 * g4;
@@ -493,10 +530,50 @@ score_prefill_kernel(ScorePrefillParams p) {
         for (; again; again &= again - 1) {                            // wave-uniform
             const int r = __builtin_ctzll(again);
             const int at = __builtin_amdgcn_readlane(pos[c], r);
-            score_row<E, FP8, DH>(p, seq, q_begin + at - prior, __builtin_amdgcn_readlane(head[c], r), kvh, at,
-                                  __builtin_amdgcn_readlane(lo[c], r), __builtin_amdgcn_readlane(hi[c], r), lane);
+            score_row<E, FP8, DH, R == 1>(p, seq, q_begin + at - prior, __builtin_amdgcn_readlane(head[c], r), kvh, at,
+                                  __builtin_amdgcn_readlane(lo[c], r), __builtin_amdgcn_readlane(hi[c], r), part, lane);
         }
     }
+}
+
+// The parts of divided rows joined: out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i over the parts in which the row sees keys.
+// DH / 4 lanes per (row, head), 16-byte loads; every part's loads are in flight together.
+template <typename E, int DH>
+__global__ void __launch_bounds__(256) score_prefill_join_kernel(ScorePrefillParams p) {
+    constexpr int LPR = DH / 4;
+    const int seq = blockIdx.y, begin = p.cu_q_lens[seq], n = p.cu_q_lens[seq + 1] - begin;
+    const int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;      // (row of the chunk, head)
+    if (at >= (int64_t)n * p.hq) return;
+    const int64_t first = begin * (int64_t)p.hq + at, step = p.rows * p.hq;
+    const int e = 4 * (threadIdx.x % LPR);
+    float mx = NEG_BIG, den = 0.f;
+    for (int i = 0; i < p.parts; ++i) {
+        const float2 ml = p.ws_ml[first + i * step];
+        if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
+    }
+    f32x4_t num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < p.parts; ++i) {
+        const float2 ml = p.ws_ml[first + i * step];
+        const f32x4_t a = *(const f32x4_t*)(p.ws_acc + (first + i * step) * DH + e);
+        if (ml.y != 0.f) {                                     // (a part without keys wrote no sums)
+            const float w = exp2f(ml.x - mx);
+            den = fmaf(w, ml.y, den);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) num[k] = fmaf(w, a[k], num[k]);
+        }
+    }
+    const float inv = (p.v_scale != nullptr ? p.v_scale[(int)(at % p.hq) / p.group] : 1.f) / den;
+    *(uint2*)((uint16_t*)p.out + first * DH + e) =
+        den == 0.f ? make_uint2(0, 0) : make_uint2(E::pack(num[0] * inv, num[1] * inv), E::pack(num[2] * inv, num[3] * inv));
+}
+
+template <typename E>
+void launch_join(const ScorePrefillParams& p, const ScoreArgs& a) {
+    const dim3 grid((unsigned)(((int64_t)a.max_q_len * a.hq + 1024 / a.d - 1) / (1024 / a.d)), (unsigned)a.num_seqs);
+    if (a.d == 64) hipLaunchKernelGGL((score_prefill_join_kernel<E, 64>), grid, dim3(256), 0, a.stream, p);
+    else if (a.d == 128) hipLaunchKernelGGL((score_prefill_join_kernel<E, 128>), grid, dim3(256), 0, a.stream, p);
+    else hipLaunchKernelGGL((score_prefill_join_kernel<E, 256>), grid, dim3(256), 0, a.stream, p);
 }
 
 template <typename E, bool FP8, int R, int DH>
@@ -510,17 +587,50 @@ void launch_rule(const ScorePrefillParams& p, bool cap, bool bias, dim3 grid, hi
 template <typename E, bool FP8>
 void launch_shape(const ScorePrefillParams& p, int R, int d, bool cap, bool bias, dim3 grid, hipStream_t stream) {
     if (d == 256) { if (R == 2) launch_rule<E, FP8, 2, 256>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 256>(p, cap, bias, grid, stream); }
-    else if (d == 64) { if (R == 2) launch_rule<E, FP8, 2, 64>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 64>(p, cap, bias, grid, stream); }
+    else if (d == 64) {
+        if constexpr (!FP8) {              // (see score_chunk_plan)
+            if (R == 2 && cap) { hipLaunchKernelGGL((score_prefill_kernel<E, FP8, 2, 64, true, false>), grid, dim3(256), 0, stream, p); return; }
+            if (R == 2) { hipLaunchKernelGGL((score_prefill_kernel<E, FP8, 2, 64, false, false>), grid, dim3(256), 0, stream, p); return; }
+        }
+        launch_rule<E, FP8, 1, 64>(p, cap, bias, grid, stream);
+    }
     else { if (R == 2) launch_rule<E, FP8, 2, 128>(p, cap, bias, grid, stream); else launch_rule<E, FP8, 1, 128>(p, cap, bias, grid, stream); }
 }
 
 }  // namespace
 
 bool score_prefill_supported(const ScoreArgs& a) {
-    if (a.cu_q_lens == nullptr || !is_16bit_float(a.q_dtype) || a.bs != BS) return false;
+    if (!is_16bit_float(a.q_dtype) || a.bs != BS) return false;
     const int group = a.hq / a.hkv, gpack = 16 % group == 0 ? group : 1;
     const int64_t qtiles = ((int64_t)a.max_q_len * gpack + 63) / 64;
     return a.num_seqs <= 65535 && qtiles <= 65535 && a.num_blocks <= INT32_MAX && (int64_t)a.hkv * BS * a.d * 2 <= UINT32_MAX;
+}
+
+// 128 rows to a workgroup (R = 2) read a tile from LDS once for twice the rows, where they leave no CU without its workgroups; 64 rows
+// in smaller calls, with fp8 pools or a bias at head_dim 64 too (there 128 take the registers of a second or third workgroup on a CU).
+// us, 64 against 128 rows, 32 / 8 heads under a cap: prompts of 4 and 8 x 1024, head_dim 64: 41.4 against 41.3, 77 against 73 (fp8: 46
+// against 59 for the first); 2048 and 2000 + 2048 tokens, head_dim 128: 64 against 64, 152 against 129; 512 after 2048: 54 against 72;
+// head_dim 256, 16 / 8 heads: 2048 and 3000 tokens 110 against 119, 191 against 166; 64 with a bias alone, 8192 tokens: 347 against 351.
+//
+// Where even those are too few for two to a CU (head_dim 256: one), the keys are divided: i parts take the tiles' time / i and then a second kernel, which
+// costs about 4 us, 0.6 us per part and the parts' sums at 3 TB/s both ways.  256 new tokens behind 2048, head_dim 128: 48 us in one
+// part, 36 in 2 or 4, 41 in 8; 64 behind 4000: 79 in one, 28 in 8, 35 in 16; 512 from none: 16 in one, 25 in 2.
+ScoreChunkPlan score_chunk_plan(int num_seqs, int64_t total_q, int max_q_len, int hq, int hkv, int d, bool fp8, bool bias, int64_t span) {
+    const int group = hq / hkv, gpack = 16 % group == 0 ? group : 1;
+    auto workgroups = [&](int rows) {
+        const int64_t per = rows / gpack;
+        return std::max<int64_t>(1, hq / gpack * std::min(num_seqs * ((max_q_len + per - 1) / per), total_q / per + num_seqs));
+    };
+    if (workgroups(128) >= (d == 64 ? 1024 : d == 128 ? 512 : 320) && !(d == 64 && (fp8 || bias))) return ScoreChunkPlan{2, 1};
+    const double tile_us = d == 64 ? 0.9 : d == 128 ? 1.3 : 2.4, tiles = (double)((span + KT - 1) / KT);
+    const int most = (int)std::min({(int64_t)(d == 256 ? 256 : 512) / workgroups(64), (span + PART_TILES * KT - 1) / (PART_TILES * KT), (int64_t)16});
+    ScoreChunkPlan plan{1, 1};
+    double best = tiles * tile_us;
+    for (int i = 2; i <= most; ++i) {
+        const double us = tiles * tile_us / i + 4 + i * (0.6 + 8e-3 * total_q * hq * d / 3e3);
+        if (us < best) { best = us; plan.parts = i; }
+    }
+    return plan;
 }
 
 int launch_score_prefill(const ScoreArgs& a) {
@@ -543,9 +653,14 @@ int launch_score_prefill(const ScoreArgs& a) {
         cached_cus.store(cus, std::memory_order_relaxed);
     }
     p.num_cus = num_cus;
-    const int R = (int64_t)a.max_q_len * p.gpack >= 128 ? 2 : 1;
+    const ScoreChunkPlan plan = score_chunk_plan(a.num_seqs, a.rows, a.max_q_len, a.hq, a.hkv, a.d,
+                                                 a.kv_dtype == AICOMP_KV_FP8_E4M3, a.slopes != nullptr, a.span);
+    const int R = plan.R;
+    p.hgroups = a.hq / p.gpack;
+    p.parts = a.ws_acc != nullptr ? plan.parts : 1;
+    p.rows = a.rows; p.ws_acc = a.ws_acc; p.ws_ml = (float2*)a.ws_ml;
     const int pos_per_wg = 64 * R / p.gpack;
-    dim3 grid((unsigned)(a.hq / p.gpack), (unsigned)a.num_seqs, (unsigned)((a.max_q_len + pos_per_wg - 1) / pos_per_wg));
+    dim3 grid((unsigned)(p.hgroups * p.parts), (unsigned)a.num_seqs, (unsigned)((a.max_q_len + pos_per_wg - 1) / pos_per_wg));
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, cap = a.cap > 0.f, bias = a.slopes != nullptr;
     if (a.q_dtype == AICOMP_KV_F16) {
         if (fp8) launch_shape<F16Fmt, true>(p, R, a.d, cap, bias, grid, a.stream);
@@ -553,6 +668,9 @@ int launch_score_prefill(const ScoreArgs& a) {
     } else {
         if (fp8) launch_shape<Bf16Fmt, true>(p, R, a.d, cap, bias, grid, a.stream);
         else launch_shape<Bf16Fmt, false>(p, R, a.d, cap, bias, grid, a.stream);
+    }
+    if (p.parts > 1) {
+        if (a.q_dtype == AICOMP_KV_F16) launch_join<F16Fmt>(p, a); else launch_join<Bf16Fmt>(p, a);
     }
     AICOMP_HIP_LAUNCH_CHECK();
     return AICOMP_KV_OK;

@@ -862,7 +862,7 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
                                                      k_scale, v_scale)
     _req(S == B, f"{S} context lengths for {B} rows")
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
-    need = lib.aicomp_paged_score_workspace_bytes(B, hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window),
+    need = lib.aicomp_paged_score_workspace_bytes(B, B, 0, hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window),
                                                   int(longest_context))
     with _guard(query):
         if workspace is None:
@@ -883,7 +883,7 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
 def score_decode_workspace_bytes(batch: int, hq: int, hkv: int, d: int, bs: int, max_blocks: int, q_dtype: torch.dtype,
                                  kv_dtype: torch.dtype, window: int = 0, longest_context: int = 0) -> int:
     """Scratch bytes of ``paged_score_decode_attn`` for these shapes, for a caller that passes ``workspace`` itself."""
-    return _lib.load().aicomp_paged_score_workspace_bytes(batch, hq, hkv, d, bs, max_blocks, _DT[q_dtype], _DT[kv_dtype],
+    return _lib.load().aicomp_paged_score_workspace_bytes(batch, batch, 0, hq, hkv, d, bs, max_blocks, _DT[q_dtype], _DT[kv_dtype],
                                                           int(window), int(longest_context))
 
 
@@ -918,12 +918,15 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
         max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
     if max_q_len == 0:
         return out
+    qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
+    need = lib.aicomp_paged_score_workspace_bytes(S, T, int(max_q_len), hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window), 0)
     with _guard(query):
+        workspace = _call_workspace(query.device, need)
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
             block_table.stride(0), context_lens.data_ptr(), cu_q_lens.data_ptr(), S, T, int(max_q_len), hq, hkv, d, bs,
-            block_table.shape[1], nb, float(scale), _dt(query, "query"), _dt(k_pool, "pool"), _ptr(ks), _ptr(vs),
-            float(softcap), _ptr(slopes), int(window), _ptr(first_keys), _ptr(prefix_lens), 0, None, 0, _stream(query))
+            block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), int(window),
+            _ptr(first_keys), _ptr(prefix_lens), 0, _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream(query))
     _lib.check(rc, lib)
     return out
 

@@ -519,9 +519,10 @@ int aicomp_qk_norm_rope_kv_append(const void* q_in, void* q_out,
  *   window          0: none
  *   first_keys      [total_q] int32 or NULL: the first key of each row's document
  *   prefix_lens     [num_seqs] int32 or NULL: keys below are seen by every row of the sequence (chunks only; at most the context)
- *   longest_context   what the caller knows of context_lens (0: nothing); it sizes a decode call and bounds nothing
- *   workspace       aicomp_paged_score_workspace_bytes(...) bytes, 16-byte aligned, needing no initialisation (NULL where that is
- *                   0, and for chunks); calls that may overlap need separate ones
+ *   longest_context   what the caller knows of context_lens (0: nothing); it sizes the call and bounds nothing
+ *   workspace       aicomp_paged_score_workspace_bytes(...) bytes (its max_q_len is 0 for decode calls), 16-byte aligned, needing
+ *                   no initialisation; NULL where that is 0, and for chunks, whose keys are then not divided among workgroups
+ *                   (slower where the rows are few).  Calls that may overlap need separate ones
  * head_dim 64, 128 or 256; any block size; f32/f32, bf16/bf16, f16/f16, bf16/fp8, f16/fp8 (query / pool); pointers 16-byte aligned.
  */
 int aicomp_paged_score_attn(void* out, const void* query,
@@ -536,7 +537,7 @@ int aicomp_paged_score_attn(void* out, const void* query,
                             float softcap, const float* slopes, int window,
                             const int32_t* first_keys, const int32_t* prefix_lens,
                             int longest_context, void* workspace, size_t workspace_bytes, void* stream);
-size_t aicomp_paged_score_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
                                           int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context);
 
 /*

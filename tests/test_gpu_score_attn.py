@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from aicomp_amd import ops
+from aicomp_amd import _lib, ops
 from oracle.score_oracle import score_attention
 
 pytestmark = pytest.mark.gpu
@@ -351,3 +351,100 @@ def test_ops_refusals():
     with pytest.raises(RuntimeError, match="prefix_lens"):
         ops.paged_score_prefill_attn(out, q, k, v, t, lens, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 0.1,
                                      prefix_lens=torch.zeros(2, dtype=torch.int32, device="cuda"))
+
+
+def wide(c, g):
+    """Every term of the rule, and a window that is worth dividing."""
+    return {**rule("all", c, g), "window": 900}
+
+
+FEW = [([700, 40, 0, 1333], [33, 40, 0, 2], 8, 2, 128, 16), ([2100], [17], 8, 8, 64, 16), ([900, 1800], [5, 70], 6, 2, 256, 16)]
+
+
+@pytest.mark.parametrize("shape", FEW, ids=["ragged", "one", "d256"])
+@pytest.mark.parametrize("types", [(BF16, None), (F16, FP8)], ids=["bf16", "f16-fp8"])
+@pytest.mark.parametrize("name", list(RULES) + ["wide"])
+def test_prefill_few_rows_divides_their_keys(shape, types, name):
+    """With a workspace the keys of few rows are divided among workgroups, without one they are not: both are right, and what the
+    keys that no row sees hold changes neither."""
+    ctx, new, hq, hkv, d, bs = shape
+    c = Case(ctx, new, hq, hkv, d, bs, *types, seed=11, rows_behind=3)
+    g = torch.Generator().manual_seed(5)
+    r = wide(c, g) if name == "wide" else rule(name, c, g)
+    full = {"cap": 0.0, "slopes": None, "window": 0, "first": None, **r}
+    prefix = torch.tensor([300] * len(ctx), dtype=torch.int32) if name in ("all", "wide") else None
+    want, mean, size = expect(c, full["cap"], full["slopes"], full["window"], full["first"], prefix)
+    n = sum(new)
+    lib = _lib.load()
+    q, lens = c.q.cuda(), torch.tensor(ctx, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32, device="cuda")
+    k, v, table = c.k.cuda(), c.v.cuda(), c.table.cuda()
+    t = [cuda(x) for x in (c.ks, c.vs, full["slopes"], full["first"], prefix)]
+    ptr = lambda x: None if x is None else x.data_ptr()
+    qd, kd = ops._DT[c.dtype], ops._DT[c.pool_dtype]
+    need = lib.aicomp_paged_score_workspace_bytes(len(ctx), c.total, max(new), hq, hkv, d, bs, table.shape[1], qd, kd, full["window"], 0)
+    assert need > 0 or full["window"]                                       # (a short window is one part)
+    for own in (need, 0):
+        ws = torch.full((max(own, 16),), 0xff, dtype=torch.uint8, device="cuda")              # (not a number, read as float)
+        out = torch.full_like(q, 7.0)
+        rc = lib.aicomp_paged_score_attn(
+            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), table.stride(0), lens.data_ptr(), cu.data_ptr(),
+            len(ctx), c.total, max(new), hq, hkv, d, bs, table.shape[1], k.shape[0], c.scale, qd, kd, ptr(t[0]), ptr(t[1]),
+            full["cap"], ptr(t[2]), full["window"], ptr(t[3]), ptr(t[4]), 0, ws.data_ptr() if own else None, own,
+            torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, lib)
+        got = out.cpu()
+        assert bool((got[n:] == 7.0).all())
+        check(got[:n], c, want, mean, size)
+
+
+def test_divided_keys_that_are_not_finite():
+    """Infinite values of keys that only neighbours see: in the last rows' parts, every row of the call has its own keys."""
+    c = Case([2000], [40], 8, 2, 128, seed=3)
+    for j in (5, 700, 1970, 1999):                                          # (visible to some of the 40 rows)
+        blk = int(c.table[0, j // 16])
+        c.v[blk, :, j % 16] = math.inf
+    first = torch.full((40,), 6, dtype=torch.int32)                         # key 5: to no row
+    first[7:20] = 701                                                       # key 700: not to these
+    first[20:30] = 1971                                                     # key 1970: not to these
+    got = run_prefill(c, 5.0, first=first)[:40].double()
+    clean = Case([2000], [40], 8, 2, 128, seed=3)
+    want, mean, size = expect(clean, 5.0, None, 0, first, None)
+    sees = torch.zeros(40, dtype=torch.bool)
+    for j in (5, 700, 1970, 1999):
+        pos = torch.arange(1960, 2000)
+        sees |= (first <= j) & (j <= pos)
+    assert bool(sees.any()) and not bool(sees.all())
+    assert bool((got[sees] == math.inf).all())
+    check(got[~sees], c, want[~sees], mean[~sees], size[~sees])
+
+
+def test_divided_chunks_in_two_graphs():
+    """Two captured calls of divided keys, replayed side by side on two streams: each has scratch of its own."""
+    cases = [Case([1500, 900], [30, 9], 8, 2, 128, seed=s) for s in (21, 22)]
+    want, graphs, outs, keep = [], [], [], []
+    stream = torch.cuda.Stream()
+    for c in cases:
+        want.append(run_prefill(c, 5.0))
+        q, k, v, table = c.q.cuda(), c.k.cuda(), c.v.cuda(), c.table.cuda()
+        lens = torch.tensor(c.ctx, dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, 30, 39], dtype=torch.int32, device="cuda")
+        out = torch.full_like(q, 7.0)
+        keep.append((q, k, v, table, lens, cu))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            ops.paged_score_prefill_attn(out, q, k, v, table, lens, cu, c.scale, 30, 5.0)
+        graphs.append(g), outs.append(out)
+    for _ in range(3):
+        for out in outs:
+            out.fill_(7.0)
+        torch.cuda.synchronize()
+        side = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(10):
+            for g, s in zip(graphs, side):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out.cpu(), w)

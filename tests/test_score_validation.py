@@ -83,7 +83,7 @@ def test_score_refusals(lib):
 
 @pytest.mark.routing("balanced", "library")
 def test_score_workspace(lib, decode_routing):
-    size = lambda rows, mb, window=0, longest=0: lib.aicomp_paged_score_workspace_bytes(rows, 8, 2, 128, 16, mb, BF16, BF16, window,
+    size = lambda rows, mb, window=0, longest=0: lib.aicomp_paged_score_workspace_bytes(rows, rows, 0, 8, 2, 128, 16, mb, BF16, BF16, window,
                                                                                         longest)
     need = size(4, 256)
     assert need > 0
@@ -94,6 +94,19 @@ def test_score_workspace(lib, decode_routing):
         assert size(4, 2) == 0
         assert size(4, 256, window=32) == 0 and size(4, 256, longest=32) == 0
     assert size(0, 256) == 0 and size(4, 256, window=-1) == 0
+
+
+def test_score_chunk_workspace(lib):
+    size = lambda seqs, total, longest, mb, window=0, bound=0, dt=BF16, bs=16: lib.aicomp_paged_score_workspace_bytes(
+        seqs, total, longest, 8, 2, 128, bs, mb, dt, dt, window, bound)
+    need = size(1, 4, 4, 256)
+    assert need > 0 and need % (4 * 8 * 130 * 4) == 0                       # sums, reference and weight of every part
+    assert size(1, 4, 4, 2) == 0 and size(1, 4, 4, 256, window=32) == 0 and size(1, 4, 4, 256, bound=32) == 0      # short rows
+    assert size(16, 65536, 4096, 256) == 0                                  # many rows
+    assert size(1, 4, 4, 256, dt=F32) == 0 and size(1, 4, 4, 256, bs=32) == 0
+    assert size(1, 0, 4, 256) == 0 and size(1, 4, -1, 256) == 0
+    assert attn(lib, cu=P, mb=256, stride=256, total=4, max_q=4, ws=P, wsb=need - 1) == EWORKSPACE and str(need) in err(lib)
+    assert attn(lib, cu=P, mb=256, stride=256, total=4, max_q=4, ws=P + 4, wsb=need) == EINVAL and "aligned" in err(lib)
 
 
 def test_copy_refusals(lib):
