@@ -3,6 +3,10 @@
 // What forking a sequence (its last, partly filled block; full ones are shared) and compacting a pool come to.  A block of
 // one pool is one contiguous piece of Hkv * block_size * D elements, so the copy is bound by HBM, and for a fork, a
 // piece of some KB per pool, by the launch: the pools' addresses travel in the kernel's arguments.
+//
+// One block in each of 64 pools (2 MB): 2.3 us on the device (10 with uint4 as the vector, whose array the compiler moves to LDS, the
+// workgroup's shape being read from host memory for it).  500 pairs in each of 32 pools, 1.05 GB read and written: 188 us, 5.6 TB/s
+// (198 without the nontemporal hint: nothing here is read again).
 #include "common.h"
 
 #include <algorithm>
@@ -13,6 +17,8 @@ namespace {
 
 constexpr int MAX_POOLS = 128;             // per launch: 1 KB of arguments
 constexpr int UNROLL = 4;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct CopyParams {
     void* pools[MAX_POOLS];
@@ -36,13 +42,13 @@ copy_blocks_kernel(CopyParams p) {
     if (i0 + 256 * (UNROLL - 1) < p.vecs) {
         V r[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) r[u] = from[i0 + 256 * u];
+        for (int u = 0; u < UNROLL; ++u) r[u] = __builtin_nontemporal_load(from + i0 + 256 * u);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) to[i0 + 256 * u] = r[u];
+        for (int u = 0; u < UNROLL; ++u) __builtin_nontemporal_store(r[u], to + i0 + 256 * u);
     } else {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (i0 + 256 * u < p.vecs) to[i0 + 256 * u] = from[i0 + 256 * u];
+            if (i0 + 256 * u < p.vecs) __builtin_nontemporal_store(__builtin_nontemporal_load(from + i0 + 256 * u), to + i0 + 256 * u);
     }
 }
 
@@ -67,7 +73,7 @@ int launch_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes, i
         for (int64_t k = 0; k < num_pairs; k += per_launch) {
             p.pairs = pairs + 2 * k;
             dim3 grid((unsigned)(std::min(num_pairs - k, per_launch) * pieces), (unsigned)n);
-            if (width == 16) hipLaunchKernelGGL(copy_blocks_kernel<uint4>, grid, dim3(256), 0, stream, p);
+            if (width == 16) hipLaunchKernelGGL(copy_blocks_kernel<u32x4>, grid, dim3(256), 0, stream, p);
             else if (width == 4) hipLaunchKernelGGL(copy_blocks_kernel<uint32_t>, grid, dim3(256), 0, stream, p);
             else hipLaunchKernelGGL(copy_blocks_kernel<uint8_t>, grid, dim3(256), 0, stream, p);
             AICOMP_HIP_LAUNCH_CHECK();
