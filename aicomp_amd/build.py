@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaicomp_kv.so")
 SOURCES = ["capi.hip", "kv_append.hip", "decode_generic.hip", "decode_mfma.hip", "prefill_mfma.hip",
            "prefill_mfma_f32.hip", "prefill_tiled.hip", "rope_append.hip", "sample.hip", "qk_norm_rope.hip",
-           "block_copy.hip", "score_generic.hip", "score_prefill.hip"]
+           "block_copy.hip", "score_generic.hip", "score_prefill.hip", "score_prefill_f32.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17",

@@ -865,9 +865,7 @@ static int64_t chunk_span(int bs, int max_blocks, int window, int longest_contex
 
 static size_t chunk_workspace_bytes(const ScoreArgs& a) {
     if (!score_prefill_supported(a)) return 0;
-    // (whether there is a bias decides nothing where keys are divided)
-    const int parts = score_chunk_plan(a.num_seqs, a.rows, a.max_q_len, a.hq, a.hkv, a.d, a.kv_dtype == AICOMP_KV_FP8_E4M3, false,
-                                       a.span).parts;
+    const int parts = score_chunk_plan(a).parts;
     return parts > 1 ? (size_t)a.rows * a.hq * parts * (a.d + 2) * sizeof(float) : 0;
 }
 

@@ -75,7 +75,7 @@ int launch_score_merge(const ScoreArgs& a);
 bool score_prefill_supported(const ScoreArgs& a);
 // How a chunk call is laid out: column groups of 16 rows per wave, and the parts that the keys of its rows are divided into.
 struct ScoreChunkPlan { int R, parts; };
-ScoreChunkPlan score_chunk_plan(int num_seqs, int64_t total_q, int max_q_len, int hq, int hkv, int d, bool fp8, bool bias, int64_t span);
+ScoreChunkPlan score_chunk_plan(const ScoreArgs& a);
 int launch_score_prefill(const ScoreArgs& a);
 
 }  // namespace aicomp

@@ -20,121 +20,21 @@
 // Rounding     The weights to the 16-bit format of the matrix cores; everything else in float32 until the one rounding of
 //              the result.  (The scores' multiplier in Q would save an instruction per score, which no time shows, and round
 //              Q once more: against float64 an error of 3.0e-3 where this has 2.1e-3, bf16, a prompt of 8192 under a cap.)
-#include "score.h"
+#include "score_prefill.h"
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace aicomp {
 
 namespace {
 
-constexpr int BS = 16;
 constexpr int KT = 64;                 // tokens per tile
 constexpr int NB = KT / BS;            // blocks per tile
-constexpr float NEG_BIG = -1.0e30f;
-constexpr int PART_TILES = 4;          // least tiles of a part where the keys are divided
-
-struct ScorePrefillParams {
-    void* out;
-    const void* query;
-    const void* k_pool;
-    const void* v_pool;
-    const int32_t* block_table;
-    int64_t block_table_stride;
-    const int32_t* context_lens;
-    const int32_t* cu_q_lens;
-    int hq, hkv, group, gpack, max_blocks;
-    int num_blocks;
-    int num_cus;
-    const float* k_scale;
-    const float* v_scale;
-    ScoreRule rule;
-    // divided keys (parts > 1): sums, reference and weight of part i of (row, head) at [(i rows + row) hq + head]
-    int hgroups, parts;
-    int64_t rows;
-    float* ws_acc;
-    float2* ws_ml;
-};
 
 template <bool FP8> struct Stage;              // registers of one K and one V tile (fp8 pools)
 template <> struct Stage<false> {};
 template <> struct Stage<true> { uint2 k[8], v[8]; };
-
-#define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
-#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
-
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
-}
-
-// One row key by key, by a whole wave: what the matrix cores cannot give where a key that the row does not see, but a neighbour
-// does, has a value that is not finite (a weight of 0 times it is not 0).
-template <typename E, bool FP8, int DH, bool PARTS>
-__device__ void score_row(const ScorePrefillParams& p, int seq, int64_t q_row, int head, int kvh, int pos, int lo, int hi, int part,
-                          int lane) {
-    constexpr int NV = DH / 64;
-    typedef typename E::elem Elem;
-    const uint16_t* q = (const uint16_t*)p.query + (q_row * p.hq + head) * DH;
-    const bool capped = p.rule.cap_log2 > 0.f;
-    const float mul = (capped ? p.rule.cap_mul : p.rule.mul) * (FP8 ? p.k_scale[kvh] : 1.f);
-    const float slope = p.rule.slopes != nullptr ? p.rule.slopes[head] * LOG2E : 0.f;
-    auto key_row = [&](int j) {
-        const int64_t blk = max(0, min(p.block_table[(int64_t)seq * p.block_table_stride + j / BS], p.num_blocks - 1));
-        return ((blk * p.hkv + kvh) * BS + j % BS) * DH;
-    };
-    float m = NEG_BIG, l = 0.f, acc[NV] = {};
-    for (int base = lo; base < hi; base += 64) {
-        const int j = min(base + lane, hi - 1);
-        const int64_t at = key_row(j);
-        float s = 0.f;
-        for (int d = 0; d < DH; ++d) {
-            float k;
-            if constexpr (FP8) k = fp8_to_f32(((const uint8_t*)p.k_pool)[at + d]);
-            else k = load_elem<Elem>((const Elem*)p.k_pool + at + d);
-            s = fmaf(E::to_f32(q[d]), k, s);
-        }
-        s *= mul;
-        if (capped) s = p.rule.cap_log2 * tanhf(s);
-        s = fmaf(-slope, fabsf((float)(pos - j)), s);
-        const bool live = base + lane < hi;
-        float mx = live ? s : NEG_BIG;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const float m_new = fmaxf(m, mx), alpha = exp2f(m - m_new), pr = live ? exp2f(s - m_new) : 0.f;
-        m = m_new;
-        l = l * alpha + pr;
-#pragma unroll
-        for (int e = 0; e < NV; ++e) acc[e] *= alpha;
-        for (int k = 0; k < min(64, hi - base); ++k) {
-            const float w = __shfl(pr, k);
-            const int64_t v_at = key_row(base + k) + lane;
-#pragma unroll
-            for (int e = 0; e < NV; ++e) {
-                float v;
-                if constexpr (FP8) v = fp8_to_f32(((const uint8_t*)p.v_pool)[v_at + 64 * e]);
-                else v = load_elem<Elem>((const Elem*)p.v_pool + v_at + 64 * e);
-                acc[e] = fmaf(w, v, acc[e]);
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
-    if (PARTS && p.parts > 1) {
-        const int64_t slot = (part * p.rows + q_row) * p.hq + head;
-#pragma unroll
-        for (int e = 0; e < NV; ++e) p.ws_acc[slot * DH + lane + 64 * e] = acc[e];
-        if (lane == 0) p.ws_ml[slot] = make_float2(m, l);
-        return;
-    }
-    const float inv = (FP8 ? p.v_scale[kvh] : 1.f) / l;
-    uint16_t* o = (uint16_t*)p.out + (q_row * p.hq + head) * DH + lane;
-#pragma unroll
-    for (int e = 0; e < NV; ++e) o[64 * e] = l == 0.f ? 0 : E::from_f32(acc[e] * inv);
-}
 
 // E: 16-bit format of queries and output; R: column groups of 16 rows per wave; DH: head_dim
 template <typename E, bool FP8, int R, int DH, bool CAP, bool BIAS>
@@ -200,7 +100,7 @@ score_prefill_kernel(ScorePrefillParams p) {
     int t_first = kv_lo / KT, t_end = (kv_hi + KT - 1) / KT;
     const bool divided = R == 1 && p.parts > 1;
     if (divided) {
-        const int per = max((t_end - t_first + p.parts - 1) / p.parts, PART_TILES);
+        const int per = max((t_end - t_first + p.parts - 1) / p.parts, PART_KEYS / KT);
         t_end -= part * per;
         t_first = max(t_first, t_end - per);
     }
@@ -536,46 +436,6 @@ score_prefill_kernel(ScorePrefillParams p) {
     }
 }
 
-// The parts of divided rows joined: out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i over the parts in which the row sees keys.
-// DH / 4 lanes per (row, head), 16-byte loads; every part's loads are in flight together.
-template <typename E, int DH>
-__global__ void __launch_bounds__(256) score_prefill_join_kernel(ScorePrefillParams p) {
-    constexpr int LPR = DH / 4;
-    const int seq = blockIdx.y, begin = p.cu_q_lens[seq], n = p.cu_q_lens[seq + 1] - begin;
-    const int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;      // (row of the chunk, head)
-    if (at >= (int64_t)n * p.hq) return;
-    const int64_t first = begin * (int64_t)p.hq + at, step = p.rows * p.hq;
-    const int e = 4 * (threadIdx.x % LPR);
-    float mx = NEG_BIG, den = 0.f;
-    for (int i = 0; i < p.parts; ++i) {
-        const float2 ml = p.ws_ml[first + i * step];
-        if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
-    }
-    f32x4_t num = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < p.parts; ++i) {
-        const float2 ml = p.ws_ml[first + i * step];
-        const f32x4_t a = *(const f32x4_t*)(p.ws_acc + (first + i * step) * DH + e);
-        if (ml.y != 0.f) {                                     // (a part without keys wrote no sums)
-            const float w = exp2f(ml.x - mx);
-            den = fmaf(w, ml.y, den);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) num[k] = fmaf(w, a[k], num[k]);
-        }
-    }
-    const float inv = (p.v_scale != nullptr ? p.v_scale[(int)(at % p.hq) / p.group] : 1.f) / den;
-    *(uint2*)((uint16_t*)p.out + first * DH + e) =
-        den == 0.f ? make_uint2(0, 0) : make_uint2(E::pack(num[0] * inv, num[1] * inv), E::pack(num[2] * inv, num[3] * inv));
-}
-
-template <typename E>
-void launch_join(const ScorePrefillParams& p, const ScoreArgs& a) {
-    const dim3 grid((unsigned)(((int64_t)a.max_q_len * a.hq + 1024 / a.d - 1) / (1024 / a.d)), (unsigned)a.num_seqs);
-    if (a.d == 64) hipLaunchKernelGGL((score_prefill_join_kernel<E, 64>), grid, dim3(256), 0, a.stream, p);
-    else if (a.d == 128) hipLaunchKernelGGL((score_prefill_join_kernel<E, 128>), grid, dim3(256), 0, a.stream, p);
-    else hipLaunchKernelGGL((score_prefill_join_kernel<E, 256>), grid, dim3(256), 0, a.stream, p);
-}
-
 template <typename E, bool FP8, int R, int DH>
 void launch_rule(const ScorePrefillParams& p, bool cap, bool bias, dim3 grid, hipStream_t stream) {
     if (cap && bias) hipLaunchKernelGGL((score_prefill_kernel<E, FP8, R, DH, true, true>), grid, dim3(256), 0, stream, p);
@@ -600,10 +460,10 @@ void launch_shape(const ScorePrefillParams& p, int R, int d, bool cap, bool bias
 }  // namespace
 
 bool score_prefill_supported(const ScoreArgs& a) {
-    if (!is_16bit_float(a.q_dtype) || a.bs != BS) return false;
+    if (a.bs != BS) return false;
     const int group = a.hq / a.hkv, gpack = 16 % group == 0 ? group : 1;
     const int64_t qtiles = ((int64_t)a.max_q_len * gpack + 63) / 64;
-    return a.num_seqs <= 65535 && qtiles <= 65535 && a.num_blocks <= INT32_MAX && (int64_t)a.hkv * BS * a.d * 2 <= UINT32_MAX;
+    return a.num_seqs <= 65535 && qtiles <= 65535 && a.num_blocks <= INT32_MAX && (int64_t)a.hkv * BS * a.d * 4 <= UINT32_MAX;
 }
 
 // 128 rows to a workgroup (R = 2) read a tile from LDS once for twice the rows, where they leave no CU without its workgroups; 64 rows
@@ -612,53 +472,34 @@ bool score_prefill_supported(const ScoreArgs& a) {
 // against 59 for the first); 2048 and 2000 + 2048 tokens, head_dim 128: 64 against 64, 152 against 129; 512 after 2048: 54 against 72;
 // head_dim 256, 16 / 8 heads: 2048 and 3000 tokens 110 against 119, 191 against 166; 64 with a bias alone, 8192 tokens: 347 against 351.
 //
-// Where even those are too few for two to a CU (head_dim 256: one), the keys are divided: i parts take the tiles' time / i and then a second kernel, which
-// costs about 4 us, 0.6 us per part and the parts' sums at 3 TB/s both ways.  256 new tokens behind 2048, head_dim 128: 48 us in one
-// part, 36 in 2 or 4, 41 in 8; 64 behind 4000: 79 in one, 28 in 8, 35 in 16; 512 from none: 16 in one, 25 in 2.
-ScoreChunkPlan score_chunk_plan(int num_seqs, int64_t total_q, int max_q_len, int hq, int hkv, int d, bool fp8, bool bias, int64_t span) {
-    const int group = hq / hkv, gpack = 16 % group == 0 ? group : 1;
+// Where even those are too few for two to a CU (head_dim 256: one), the keys are divided: i parts take the tiles' time / i and then a
+// second kernel, which costs about 4 us, 0.6 us per part and the parts' sums at 3 TB/s both ways.  256 new tokens behind 2048, head_dim
+// 128: 48 us in one part, 36 in 2 or 4, 41 in 8; 64 behind 4000: 79 in one, 28 in 8, 35 in 16; 512 from none: 16 in one, 25 in 2.
+ScoreChunkPlan score_chunk_plan(const ScoreArgs& a) {
+    const int group = a.hq / a.hkv, gpack = 16 % group == 0 ? group : 1;
+    const bool f32 = a.q_dtype == AICOMP_KV_F32, fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3;
     auto workgroups = [&](int rows) {
         const int64_t per = rows / gpack;
-        return std::max<int64_t>(1, hq / gpack * std::min(num_seqs * ((max_q_len + per - 1) / per), total_q / per + num_seqs));
+        return std::max<int64_t>(1, a.hq / gpack * std::min(a.num_seqs * ((a.max_q_len + per - 1) / per), a.rows / per + a.num_seqs));
     };
-    if (workgroups(128) >= (d == 64 ? 1024 : d == 128 ? 512 : 320) && !(d == 64 && (fp8 || bias))) return ScoreChunkPlan{2, 1};
-    const double tile_us = d == 64 ? 0.9 : d == 128 ? 1.3 : 2.4, tiles = (double)((span + KT - 1) / KT);
-    const int most = (int)std::min({(int64_t)(d == 256 ? 256 : 512) / workgroups(64), (span + PART_TILES * KT - 1) / (PART_TILES * KT), (int64_t)16});
+    if (!f32 && !(a.d == 64 && (fp8 || a.slopes != nullptr)) && workgroups(128) >= (a.d == 64 ? 1024 : a.d == 128 ? 512 : 320))
+        return ScoreChunkPlan{2, 1};
+    // (the bias decides nothing below here: the size of a workspace does not know of it)
+    const double tile_us = (f32 ? 3.2 : 1.) * (a.d == 64 ? 0.9 : a.d == 128 ? 1.3 : 2.4), tiles = (double)((a.span + 63) / 64);
+    const int64_t most = std::min({(a.d == 256 ? 256 : 512) / workgroups(64), (a.span + PART_KEYS - 1) / PART_KEYS, (int64_t)16});
     ScoreChunkPlan plan{1, 1};
     double best = tiles * tile_us;
-    for (int i = 2; i <= most; ++i) {
-        const double us = tiles * tile_us / i + 4 + i * (0.6 + 8e-3 * total_q * hq * d / 3e3);
+    for (int i = 2; i <= (int)most; ++i) {
+        const double us = tiles * tile_us / i + 4 + i * (0.6 + 8e-6 * a.rows * a.hq * a.d / 3);
         if (us < best) { best = us; plan.parts = i; }
     }
     return plan;
 }
 
 int launch_score_prefill(const ScoreArgs& a) {
-    ScorePrefillParams p;
-    p.out = a.out; p.query = a.query; p.k_pool = a.k_pool; p.v_pool = a.v_pool;
-    p.block_table = a.block_table; p.block_table_stride = a.block_table_stride;
-    p.context_lens = a.context_lens; p.cu_q_lens = a.cu_q_lens;
-    p.hq = a.hq; p.hkv = a.hkv; p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks;
-    p.gpack = 16 % p.group == 0 ? p.group : 1;
-    p.k_scale = a.k_scale; p.v_scale = a.v_scale;
-    p.rule = rule_of(a);
-    static std::atomic<int> cached_cus{-1};                    // (of the first device used: every GPU of a node is the same part)
-    int num_cus = cached_cus.load(std::memory_order_relaxed);
-    if (num_cus < 0) {
-        int dev = 0, cus = 0;
-        if (hipGetDevice(&dev) != hipSuccess ||
-            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 0)
-            cus = 0;
-        num_cus = cus;
-        cached_cus.store(cus, std::memory_order_relaxed);
-    }
-    p.num_cus = num_cus;
-    const ScoreChunkPlan plan = score_chunk_plan(a.num_seqs, a.rows, a.max_q_len, a.hq, a.hkv, a.d,
-                                                 a.kv_dtype == AICOMP_KV_FP8_E4M3, a.slopes != nullptr, a.span);
-    const int R = plan.R;
-    p.hgroups = a.hq / p.gpack;
-    p.parts = a.ws_acc != nullptr ? plan.parts : 1;
-    p.rows = a.rows; p.ws_acc = a.ws_acc; p.ws_ml = (float2*)a.ws_ml;
+    if (a.q_dtype == AICOMP_KV_F32) return launch_score_prefill_f32(a);
+    const ScorePrefillParams p = chunk_params(a);
+    const int R = score_chunk_plan(a).R;
     const int pos_per_wg = 64 * R / p.gpack;
     dim3 grid((unsigned)(p.hgroups * p.parts), (unsigned)a.num_seqs, (unsigned)((a.max_q_len + pos_per_wg - 1) / pos_per_wg));
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, cap = a.cap > 0.f, bias = a.slopes != nullptr;
@@ -669,9 +510,7 @@ int launch_score_prefill(const ScoreArgs& a) {
         if (fp8) launch_shape<Bf16Fmt, true>(p, R, a.d, cap, bias, grid, a.stream);
         else launch_shape<Bf16Fmt, false>(p, R, a.d, cap, bias, grid, a.stream);
     }
-    if (p.parts > 1) {
-        if (a.q_dtype == AICOMP_KV_F16) launch_join<F16Fmt>(p, a); else launch_join<Bf16Fmt>(p, a);
-    }
+    if (p.parts > 1) { if (a.q_dtype == AICOMP_KV_F16) launch_join<F16Fmt>(p, a); else launch_join<Bf16Fmt>(p, a); }
     AICOMP_HIP_LAUNCH_CHECK();
     return AICOMP_KV_OK;
 }

@@ -362,7 +362,7 @@ FEW = [([700, 40, 0, 1333], [33, 40, 0, 2], 8, 2, 128, 16), ([2100], [17], 8, 8,
 
 
 @pytest.mark.parametrize("shape", FEW, ids=["ragged", "one", "d256"])
-@pytest.mark.parametrize("types", [(BF16, None), (F16, FP8)], ids=["bf16", "f16-fp8"])
+@pytest.mark.parametrize("types", [(BF16, None), (F16, FP8), (F32, None)], ids=["bf16", "f16-fp8", "f32"])
 @pytest.mark.parametrize("name", list(RULES) + ["wide"])
 def test_prefill_few_rows_divides_their_keys(shape, types, name):
     """With a workspace the keys of few rows are divided among workgroups, without one they are not: both are right, and what the

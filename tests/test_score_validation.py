@@ -103,7 +103,7 @@ def test_score_chunk_workspace(lib):
     assert need > 0 and need % (4 * 8 * 130 * 4) == 0                       # sums, reference and weight of every part
     assert size(1, 4, 4, 2) == 0 and size(1, 4, 4, 256, window=32) == 0 and size(1, 4, 4, 256, bound=32) == 0      # short rows
     assert size(16, 65536, 4096, 256) == 0                                  # many rows
-    assert size(1, 4, 4, 256, dt=F32) == 0 and size(1, 4, 4, 256, bs=32) == 0
+    assert size(1, 4, 4, 256, dt=F32) > 0 and size(1, 4, 4, 256, bs=32) == 0
     assert size(1, 0, 4, 256) == 0 and size(1, 4, -1, 256) == 0
     assert attn(lib, cu=P, mb=256, stride=256, total=4, max_q=4, ws=P, wsb=need - 1) == EWORKSPACE and str(need) in err(lib)
     assert attn(lib, cu=P, mb=256, stride=256, total=4, max_q=4, ws=P + 4, wsb=need) == EINVAL and "aligned" in err(lib)
