@@ -93,6 +93,11 @@ struct MfmaRuleParams : MfmaParams {
 #include "decode_tile_f32.h"
 #include "decode_tile_f32_quad.h"
 
+// A tile form whose rows' scores follow a rule (score.h).
+template <typename T> struct Ruled : T {};
+template <typename T> constexpr bool ruled = false;
+template <typename T> constexpr bool ruled<Ruled<T>> = true;
+
 // A decode row's scores by the rule: what a lane makes of its products (its column's head), and the first visible key.
 template <typename T, typename Params>
 __device__ __forceinline__ auto rule_score(const Params& p, int kvh, int lane) {
@@ -180,10 +185,11 @@ __device__ __forceinline__ void store_new_row(const MfmaParams& p, const typenam
 // ROPE: the query rows come as projected, with strides of their own, and are rotated here, like the new K row: a decode
 // step of a layer is then this launch alone, where the rotary + append launch before it and the rotated query's way
 // through memory cost 3.3 us of device and 6 us of host time (8 rows of 900 tokens, 32 / 8 heads, D 64).
-// RULE: scores by a rule (score.h); the partitions then begin with the tile of the row's first visible key.
-template <typename T, int NW, bool ROPE, bool RULE = false>
+// Ruled tiles: the partitions begin with the tile of the row's first visible key.
+template <typename T, int NW, bool ROPE>
 __global__ void __launch_bounds__(64 * NW, NW == 4 ? 2 : 1)
-paged_decode_mfma_kernel(std::conditional_t<RULE, MfmaRuleParams, MfmaParams> p) {
+paged_decode_mfma_kernel(std::conditional_t<ruled<T>, MfmaRuleParams, MfmaParams> p) {
+    constexpr bool RULE = ruled<T>;
     // KV head fastest: the workgroups launched together read the Hkv slices of the same
     // physical blocks, i.e. one contiguous Hkv*4 KB piece of each pool
     constexpr int DQ = T::DQ, TT = T::TT, BPT = T::BPT, NPAR = T::NPAR;
@@ -544,9 +550,10 @@ __device__ __forceinline__ int sk_tiles(const Params& p, int seq) {
 
 // Token pairs (Tile16 with PAIR): every head takes two B-operand columns, one per token parity, and a
 // flush merges the two columns of a head inside the wave and writes one partial of 64 floats per head.
-template <typename T, bool RULE = false>
+template <typename T>
 __global__ void __launch_bounds__(256, 1)     // one workgroup per CU: a wave may use the whole register file
-streamk_decode_kernel(std::conditional_t<RULE, StreamKRuleParams, StreamKParams> p) {
+streamk_decode_kernel(std::conditional_t<ruled<T>, StreamKRuleParams, StreamKParams> p) {
+    constexpr bool RULE = ruled<T>;
     constexpr int DQ = T::DQ, TT = T::TT, BPT = T::BPT;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -1011,13 +1018,13 @@ int launch_decode_streamk(const DecodeArgs& a, void* workspace) {
         rp.rule = *a.rule;
 #define AICOMP_LAUNCH_SK_RULE(E, PAIR)                                                                                              \
     do {                                                                                                                            \
-        if (fp8) hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, true, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);   \
-        else hipLaunchKernelGGL((streamk_decode_kernel<Tile16<E, false, PAIR>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);      \
+        if (fp8) hipLaunchKernelGGL((streamk_decode_kernel<Ruled<Tile16<E, true, PAIR>>>), dim3(wgs), dim3(256), 0, a.stream, rp);   \
+        else hipLaunchKernelGGL((streamk_decode_kernel<Ruled<Tile16<E, false, PAIR>>>), dim3(wgs), dim3(256), 0, a.stream, rp);      \
     } while (0)
 #define AICOMP_LAUNCH_SK_RULE32(DQ)                                                                                                 \
     do {                                                                                                                            \
-        if (group <= 4) hipLaunchKernelGGL((streamk_decode_kernel<TileF32Quad<DQ>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);  \
-        else hipLaunchKernelGGL((streamk_decode_kernel<TileF32<DQ>, true>), dim3(wgs), dim3(256), 0, a.stream, rp);                 \
+        if (group <= 4) hipLaunchKernelGGL((streamk_decode_kernel<Ruled<TileF32Quad<DQ>>>), dim3(wgs), dim3(256), 0, a.stream, rp);  \
+        else hipLaunchKernelGGL((streamk_decode_kernel<Ruled<TileF32<DQ>>>), dim3(wgs), dim3(256), 0, a.stream, rp);                 \
     } while (0)
         if (f32) { if (pair) AICOMP_LAUNCH_SK_RULE32(64); else AICOMP_LAUNCH_SK_RULE32(128); }
 #undef AICOMP_LAUNCH_SK_RULE32
@@ -1098,8 +1105,8 @@ int launch_decode_mfma(const DecodeArgs& a) {
         rp.rule = *a.rule;
 #define AICOMP_LAUNCH_RULE(...)                                                                                                           \
     do {                                                                                                                                  \
-        if (wide) hipLaunchKernelGGL((paged_decode_mfma_kernel<__VA_ARGS__, 8, false, true>), grid, dim3(512), 0, a.stream, rp);          \
-        else hipLaunchKernelGGL((paged_decode_mfma_kernel<__VA_ARGS__, 4, false, true>), grid, dim3(256), 0, a.stream, rp);               \
+        if (wide) hipLaunchKernelGGL((paged_decode_mfma_kernel<Ruled<__VA_ARGS__>, 8, false>), grid, dim3(512), 0, a.stream, rp);          \
+        else hipLaunchKernelGGL((paged_decode_mfma_kernel<Ruled<__VA_ARGS__>, 4, false>), grid, dim3(256), 0, a.stream, rp);               \
     } while (0)
 #define AICOMP_LAUNCH_RULE16(E)                                                                     \
     do {                                                                                            \

@@ -475,6 +475,7 @@ bool score_prefill_supported(const ScoreArgs& a) {
 // Where even those are too few for two to a CU (head_dim 256: one), the keys are divided: i parts take the tiles' time / i and then a
 // second kernel, which costs about 4 us, 0.6 us per part and the parts' sums at 3 TB/s both ways.  256 new tokens behind 2048, head_dim
 // 128: 48 us in one part, 36 in 2 or 4, 41 in 8; 64 behind 4000: 79 in one, 28 in 8, 35 in 16; 512 from none: 16 in one, 25 in 2.
+// float32, the same: 204, 115 in 2, 100 in 4; 356, 63 in 8.
 ScoreChunkPlan score_chunk_plan(const ScoreArgs& a) {
     const int group = a.hq / a.hkv, gpack = 16 % group == 0 ? group : 1;
     const bool f32 = a.q_dtype == AICOMP_KV_F32, fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3;
@@ -485,7 +486,7 @@ ScoreChunkPlan score_chunk_plan(const ScoreArgs& a) {
     if (!f32 && !(a.d == 64 && (fp8 || a.slopes != nullptr)) && workgroups(128) >= (a.d == 64 ? 1024 : a.d == 128 ? 512 : 320))
         return ScoreChunkPlan{2, 1};
     // (the bias decides nothing below here: the size of a workspace does not know of it)
-    const double tile_us = (f32 ? 3.2 : 1.) * (a.d == 64 ? 0.9 : a.d == 128 ? 1.3 : 2.4), tiles = (double)((a.span + 63) / 64);
+    const double tile_us = (f32 ? 4.2 : 1.) * (a.d == 64 ? 0.9 : a.d == 128 ? 1.3 : 2.4), tiles = (double)((a.span + 63) / 64);
     const int64_t most = std::min({(a.d == 256 ? 256 : 512) / workgroups(64), (a.span + PART_KEYS - 1) / PART_KEYS, (int64_t)16});
     ScoreChunkPlan plan{1, 1};
     double best = tiles * tile_us;

@@ -12,6 +12,8 @@
 //              read has the A operands of four.  O^T += V^T P^T: lane (r, g) reads dims 64 f + 4 r .. + 3 of token 4 g + e, and B is
 //              the weight that the lane holds.
 // Bound by     the float32 matrix instruction, which shares the vector ALU's multipliers: what a score costs beside it adds to it.
+//              2048 new tokens, 32 / 8 heads of 128, a cap: 329 us, 104 TFLOP/s, where a large product reaches 153 (on the vector
+//              units 2880); head_dim 64 under a cap and with a bias alone 199 and 190.
 #include "score_prefill.h"
 
 namespace aicomp {
