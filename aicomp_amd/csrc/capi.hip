@@ -869,8 +869,9 @@ static size_t chunk_workspace_bytes(const ScoreArgs& a) {
     return parts > 1 ? (size_t)a.rows * a.hq * parts * (a.d + 2) * sizeof(float) : 0;
 }
 
-size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
-                                          int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context) {
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int block_size, int max_blocks_per_seq, int q_dtype, int kv_dtype,
+                                          int window, int longest_context) {
     if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || block_size <= 0 ||
         max_blocks_per_seq <= 0 || window < 0 || longest_context < 0 || total_q <= 0 || max_q_len < 0)
         return 0;
@@ -914,8 +915,11 @@ int aicomp_paged_score_attn(void* out, const void* query, const void* k_pool, co
     if (rc) return rc;
     AICOMP_REQUIRE(max_blocks_per_seq > 0 && block_table_stride >= max_blocks_per_seq, AICOMP_KV_EINVAL,
                    "%s: block table stride %lld < width %d", who, (long long)block_table_stride, max_blocks_per_seq);
-    AICOMP_REQUIRE(isfinite(scale) && softcap >= 0.f && isfinite(softcap), AICOMP_KV_EINVAL,
+    AICOMP_REQUIRE(isfinite(3.f * scale) && softcap >= 0.f && isfinite(softcap), AICOMP_KV_EINVAL,
                    "%s: scale must be finite and softcap finite and not negative (got %g, %g)", who, (double)scale, (double)softcap);
+    // (cap - 2 cap / (1 + e^(2 x / cap)) is good to 2^-22 cap: 2.4e-4 of a weight at 1024, half the rounding of float16)
+    AICOMP_REQUIRE(softcap <= 1024.f && (softcap == 0.f || isfinite(3.f * scale / softcap)), AICOMP_KV_EUNSUPPORTED,
+                   "%s: softcap %g is beyond 1024, or scale / softcap overflows", who, (double)softcap);
     AICOMP_REQUIRE(longest_context >= 0, AICOMP_KV_EINVAL, "%s: negative longest context", who);
     AICOMP_REQUIRE(((uintptr_t)query | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0, AICOMP_KV_EUNSUPPORTED,
                    "%s: pointers must be 16-byte aligned", who);

@@ -722,6 +722,11 @@ def _guard(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
+def _int32(value, name: str) -> int:
+    _req(-2 ** 31 <= int(value) < 2 ** 31, f"{name} {value} does not fit 32 bits")
+    return int(value)
+
+
 def _call_workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
     """Scratch of one call: the stream's buffer, or, in a call that is recorded into a graph, memory of that graph's own (two
     graphs may be replayed side by side, whatever stream they were recorded on)."""
@@ -861,9 +866,10 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
     nb, hkv, bs, d, B, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
                                                      k_scale, v_scale)
     _req(S == B, f"{S} context lengths for {B} rows")
+    window, longest_context = _int32(window, "window"), _int32(longest_context, "longest_context")
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
-    need = lib.aicomp_paged_score_workspace_bytes(B, B, 0, hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window),
-                                                  int(longest_context))
+    need = lib.aicomp_paged_score_workspace_bytes(B, B, 0, hq, hkv, d, bs, block_table.shape[1], qd, kd, window,
+                                                  longest_context)
     with _guard(query):
         if workspace is None:
             workspace = _call_workspace(query.device, need)
@@ -873,8 +879,8 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
             block_table.stride(0), context_lens.data_ptr(), None, S, B, 1, hq, hkv, d, bs, block_table.shape[1], nb,
-            float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), int(window), _ptr(first_keys), None,
-            int(longest_context), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), window, _ptr(first_keys), None,
+            longest_context, _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
             _stream(query))
     _lib.check(rc, lib)
     return out
@@ -884,7 +890,7 @@ def score_decode_workspace_bytes(batch: int, hq: int, hkv: int, d: int, bs: int,
                                  kv_dtype: torch.dtype, window: int = 0, longest_context: int = 0) -> int:
     """Scratch bytes of ``paged_score_decode_attn`` for these shapes, for a caller that passes ``workspace`` itself."""
     return _lib.load().aicomp_paged_score_workspace_bytes(batch, batch, 0, hq, hkv, d, bs, max_blocks, _DT[q_dtype], _DT[kv_dtype],
-                                                          int(window), int(longest_context))
+                                                          _int32(window, "window"), _int32(longest_context, "longest_context"))
 
 
 def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -918,14 +924,15 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
         max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
     if max_q_len == 0:
         return out
+    max_q_len, window = _int32(max_q_len, "max_q_len"), _int32(window, "window")
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
-    need = lib.aicomp_paged_score_workspace_bytes(S, T, int(max_q_len), hq, hkv, d, bs, block_table.shape[1], qd, kd, int(window), 0)
+    need = lib.aicomp_paged_score_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, window, 0)
     with _guard(query):
         workspace = _call_workspace(query.device, need)
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
-            block_table.stride(0), context_lens.data_ptr(), cu_q_lens.data_ptr(), S, T, int(max_q_len), hq, hkv, d, bs,
-            block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), int(window),
+            block_table.stride(0), context_lens.data_ptr(), cu_q_lens.data_ptr(), S, T, max_q_len, hq, hkv, d, bs,
+            block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), window,
             _ptr(first_keys), _ptr(prefix_lens), 0, _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream(query))
     _lib.check(rc, lib)
     return out

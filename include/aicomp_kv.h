@@ -514,7 +514,7 @@ int aicomp_qk_norm_rope_kv_append(const void* q_in, void* q_out,
  *                   sequence at position context_lens - 1, total_q == num_seqs) or aicomp_paged_prefill_attn (rows of sequence s
  *                   are cu_q_lens[s] .. cu_q_lens[s+1], the last of them at position context_lens - 1; rows behind the last
  *                   sequence are left as they are)
- *   softcap         0: none
+ *   softcap         0: none; at most 1024
  *   slopes          [Hq] float or NULL
  *   window          0: none
  *   first_keys      [total_q] int32 or NULL: the first key of each row's document
@@ -537,8 +537,9 @@ int aicomp_paged_score_attn(void* out, const void* query,
                             float softcap, const float* slopes, int window,
                             const int32_t* first_keys, const int32_t* prefix_lens,
                             int longest_context, void* workspace, size_t workspace_bytes, void* stream);
-size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
-                                          int max_blocks_per_seq, int q_dtype, int kv_dtype, int window, int longest_context);
+size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int block_size, int max_blocks_per_seq, int q_dtype, int kv_dtype,
+                                          int window, int longest_context);
 
 /*
  * Blocks copied within every pool: pool[dst] = pool[src] for each (src, dst) pair, in one launch (per 128 pools).  What forking a

@@ -4,7 +4,7 @@ that leave rows empty, non-finite values where nothing may look, rows behind the
 Tolerance, per output element and derived from the formats: the result is rounded once (half a step of the output type, u = eps / 2
 relative).  The matrix-core kernels round the weights to the 16-bit type, u each, so that the mean moves by at most 2 u times the
 weighted mean of |v| and of the result.  A score is a float32 sum of up to 256 products: off by at most ds = 300 * 2^-24 * max_j scale
-sum_d |q_d k_jd| (a cap only shrinks it), which moves a weight by e^(2 ds) - 1 relative to the others.  Float32 sums of up to 2000
+sum_d |q_d k_jd| (a cap only shrinks it; cap - 2 cap / (1 + e^y) itself adds up to 4 half steps of float32 at cap), which moves a weight by e^(2 ds) - 1 relative to the others.  Float32 sums of up to 2000
 weights and exponents of up to 2^7 add less than 1e-5 of that; a float32 call rounds no weight.
 """
 import math
@@ -89,11 +89,11 @@ def expect(c, cap, slopes, window, first, prefix):
     return torch.cat(outs), torch.cat(means), torch.cat(sizes)
 
 
-def check(got, c, want, mean_abs, size):
+def check(got, c, want, mean_abs, size, cap=0.0):
     assert bool(torch.isfinite(want).all()) and bool(torch.isfinite(got).all())
     u = torch.finfo(c.dtype).eps / 2
     uq = 0.0 if c.dtype == F32 else u
-    ds = 300 * 2.0 ** -24 * size[..., None]
+    ds = 300 * 2.0 ** -24 * size[..., None] + 4 * 2.0 ** -24 * cap
     tol = u * want.abs() + (2 * uq + torch.expm1(2 * ds) + 1e-5) * (mean_abs + want.abs()) + 1e-30
     if c.dtype == F16:
         tol = tol + 2.0 ** -24                              # (results and weights below the normal numbers)
@@ -448,3 +448,16 @@ def test_divided_chunks_in_two_graphs():
         torch.cuda.synchronize()
         for out, w in zip(outs, want):
             assert torch.equal(out.cpu(), w)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=["bf16", "f16", "f32", "bf16-fp8", "f16-fp8"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cap", [1024.0, 0.01])
+def test_largest_and_small_caps(types, d, cap):
+    """A cap so large that it changes little, and one so small that nearly all scores are at it."""
+    c = Case([300, 65, 1], [1, 1, 1], 8, 2, d, 16, *types, seed=31)
+    want, mean, size = expect(c, cap, None, 0, None, None)
+    check(run_decode(c, cap), c, want, mean, size, cap)
+    c = Case([300, 65, 40], [70, 65, 1], 8, 2, d, 16, *types, seed=32)
+    want, mean, size = expect(c, cap, None, 0, None, None)
+    check(run_prefill(c, cap), c, want, mean, size, cap)

@@ -81,6 +81,23 @@ def test_score_refusals(lib):
     assert attn(lib, cu=P, max_q=5) == EINVAL
 
 
+def test_score_caps(lib):
+    for cu in (None, P):
+        assert attn(lib, cu=cu, total=4, cap=1025.0) == EUNSUPPORTED and "softcap" in err(lib)
+        assert attn(lib, cu=cu, total=4, cap=1e-40) == EUNSUPPORTED and "overflows" in err(lib)      # 3 * 0.1 / 1e-40 = 3e39
+        assert attn(lib, cu=cu, total=4, scale=3e38) == EINVAL
+    assert attn(lib, cap=INF) == EINVAL and attn(lib, cap=-1.0) == EINVAL and attn(lib, cap=NAN) == EINVAL
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    """A window of 2^32 + 5 is not one of 5."""
+    for name in ("window", "longest_context"):
+        for bad in (2 ** 32 + 5, 2 ** 31, -2 ** 33):
+            with pytest.raises(RuntimeError, match=name):
+                ops._int32(bad, name)
+    assert ops._int32(2 ** 31 - 1, "window") == 2 ** 31 - 1 and ops._int32(0, "window") == 0
+
+
 @pytest.mark.routing("balanced", "library")
 def test_score_workspace(lib, decode_routing):
     size = lambda rows, mb, window=0, longest=0: lib.aicomp_paged_score_workspace_bytes(rows, rows, 0, 8, 2, 128, 16, mb, BF16, BF16, window,
