@@ -3,11 +3,13 @@
 //
 // One workgroup (4 waves) per (query row, KV head, partition of the row's visible keys).  A K/V row is read by LPR consecutive
 // lanes, 16 bytes each (8 of an fp8 row), so that a wave's load is 64 / LPR whole rows; each lane group runs an online softmax
-// of its own over the tokens that it visits (running maximum and sum in float32, exponents in base 2), all heads of the group
+// of its own over the tokens that it visits (reference and sum in float32, exponents in base 2), all heads of the group
 // share a loaded chunk, and the groups' states are merged by shuffles, the waves' through LDS.
 //
-// Bound by the vector ALU: 2 D multiply-adds and an exponential per score and head, spread over few lanes.  64 rows of 512 .. 4096
-// tokens, 16 / 8 heads of 256, bf16 under a cap: 579 us, 2 TB/s.
+// Bound by the loads in flight for groups of one to four heads, by the vector ALU (2 D multiply-adds a score, and what a score takes
+// itself in every lane of its group) above.  64 rows of 512 .. 4096 tokens, head_dim 256, bf16 under a cap: 16 / 8 heads 288 us, 4.2 TB/s
+// (583 with one token in flight, two of four heads computed for nothing, sums through the LDS's lane moves and a maximum per
+// token); 32 / 4 heads 545; one row of 4096, 24.
 #include "score.h"
 
 namespace aicomp {
@@ -80,7 +82,22 @@ __device__ __forceinline__ bool row_of(const int32_t* cu, const int32_t* ctx_len
 
 constexpr float NEG_BIG = -1.0e30f;
 
-template <typename KV_T, typename Q_T, int D, int GMAX>
+// Sum over LPR consecutive lanes, in each of them: within sixteen by the vector ALU's own lane moves.
+template <int CTRL> __device__ __forceinline__ float add_moved(float s) {
+    return s + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, s), CTRL, 0xf, 0xf, true));
+}
+template <int LPR> __device__ __forceinline__ float lanes_sum(float s) {
+    if constexpr (LPR >= 2) s = add_moved<0xB1>(s);            // lanes 1 0 3 2
+    if constexpr (LPR >= 4) s = add_moved<0x4E>(s);            // lanes 2 3 0 1
+    if constexpr (LPR >= 8) s = add_moved<0x141>(s);           // half rows mirrored
+    if constexpr (LPR >= 16) s = add_moved<0x140>(s);          // rows mirrored
+    if constexpr (LPR >= 32) s += __shfl_xor(s, 16);
+    if constexpr (LPR >= 64) s += __shfl_xor(s, 32);
+    return s;
+}
+
+// U: tokens of a lane group whose loads are in flight together
+template <typename KV_T, typename Q_T, int D, int GMAX, int U>
 __global__ void __launch_bounds__(256)
 score_generic_kernel(GenericScoreParams p) {
     constexpr int N = RowChunk<KV_T>::N;
@@ -136,36 +153,51 @@ score_generic_kernel(GenericScoreParams p) {
 
     const int32_t* table = p.block_table + (int64_t)seq * p.block_table_stride;
     typedef typename RowChunk<KV_T>::Raw Raw;
-    for (int tok0 = start; tok0 < end; tok0 += NW * TPW) {
-        const int tok = tok0 + w * TPW + sub;
-        const bool valid = tok < end;
-        const int at = min(tok, end - 1);                       // clamped: always loadable
-        int64_t blk = table[at / p.bs];
-        blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
-        const int64_t base = ((blk * p.hkv + kvh) * p.bs + at % p.bs) * D + lr * N;
-        const Raw kr = *(const Raw*)((const KV_T*)p.k_pool + base);
-        const Raw vr = *(const Raw*)((const KV_T*)p.v_pool + base);
-        float k[N], v[N];
-        RowChunk<KV_T>::unpack(kr, k);
-        RowChunk<KV_T>::unpack(vr, v);
-        const float dist = fabsf((float)(pos - tok));
+    for (int64_t tok0 = start; tok0 < end; tok0 += NW * TPW * U) {
+        Raw kr[U], vr[U];
 #pragma unroll
-        for (int g = 0; g < GMAX; ++g) {
-            float s = 0.f;
+        for (int u = 0; u < U; ++u) {
+            const int at = (int)min(tok0 + (w * U + u) * TPW + sub, (int64_t)end - 1);        // clamped: always loadable
+            int64_t blk = table[at / p.bs];
+            blk = blk < 0 ? 0 : (blk >= p.num_blocks ? p.num_blocks - 1 : blk);
+            const int64_t base = ((blk * p.hkv + kvh) * p.bs + at % p.bs) * D + lr * N;
+            kr[u] = *(const Raw*)((const KV_T*)p.k_pool + base);
+            vr[u] = *(const Raw*)((const KV_T*)p.v_pool + base);
+        }
 #pragma unroll
-            for (int e = 0; e < N; ++e) s = fmaf(q[g][e], k[e], s);
+        for (int u = 0; u < U; ++u) {
+            const int64_t tok = tok0 + (w * U + u) * TPW + sub;
+            float k[N], v[N];
+            RowChunk<KV_T>::unpack(kr[u], k);
+            RowChunk<KV_T>::unpack(vr[u], v);
+            const float dist = fabsf((float)(pos - tok));
 #pragma unroll
-            for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o);
-            s *= mul;
-            if (capped) s = p.rule.cap_log2 * tanhf(s);
-            s = fmaf(-slope[g], dist, s);
-            if (valid) {
-                const float m_new = fmaxf(m[g], s);
-                const float alpha = exp2f(m[g] - m_new), pr = exp2f(s - m_new);
-                m[g] = m_new;
-                l[g] = l[g] * alpha + pr;
+            for (int g = 0; g < GMAX; ++g) {
+                float s = 0.f;
 #pragma unroll
-                for (int e = 0; e < N; ++e) acc[g][e] = fmaf(pr, v[e], acc[g][e] * alpha);
+                for (int e = 0; e < N; ++e) s = fmaf(q[g][e], k[e], s);
+                s = lanes_sum<LPR>(s) * mul;
+                if (capped) {
+                    // (16-bit queries: the form of the matrix-core kernels, good to 2^-22 of the cap)
+                    if constexpr (sizeof(Q_T) == 2)
+                        s = fmaf(-2.f * p.rule.cap_log2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * s)), p.rule.cap_log2);
+                    else s = p.rule.cap_log2 * tanhf(s);
+                }
+                s = fmaf(-slope[g], dist, s);
+                const bool up = tok < end && s > m[g] + 8.f;                 // the reference moves by more than 2^8 only
+                if (__any(up)) {
+                    const float m_new = up ? s : m[g], alpha = __builtin_amdgcn_exp2f(m[g] - m_new);
+                    m[g] = m_new;
+                    l[g] *= alpha;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[g][e] *= alpha;
+                }
+                if (tok < end) {
+                    const float pr = __builtin_amdgcn_exp2f(s - m[g]);
+                    l[g] += pr;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[g][e] = fmaf(pr, v[e], acc[g][e]);
+                }
             }
         }
     }
@@ -281,13 +313,13 @@ score_merge_kernel(Q_T* __restrict__ out, const float* __restrict__ ws_acc, cons
 template <typename KV_T, typename Q_T, int D>
 void launch_d(const ScoreArgs& a, const GenericScoreParams& p) {
     const int group = a.hq / a.hkv;
-    if (group <= 4) {
-        dim3 grid((unsigned)a.rows, (unsigned)a.hkv, (unsigned)a.num_parts);
-        hipLaunchKernelGGL((score_generic_kernel<KV_T, Q_T, D, 4>), grid, dim3(256), 0, a.stream, p);
-    } else {
-        dim3 grid((unsigned)a.rows, (unsigned)(a.hkv * ((group + 7) / 8)), (unsigned)a.num_parts);
-        hipLaunchKernelGGL((score_generic_kernel<KV_T, Q_T, D, 8>), grid, dim3(256), 0, a.stream, p);
-    }
+    const dim3 grid((unsigned)a.rows, (unsigned)(a.hkv * ((group + 7) / 8)), (unsigned)a.num_parts);
+    // us, 1, 2, 4 and 8 tokens in flight, 64 rows of 512 .. 4096, head_dim 256, 8 KV heads: groups of two 400, 311, 293, 307 (fp8 355,
+    // 251, 253, 214); groups of four, 4 KV heads, 255, 308, 288
+    constexpr int U = sizeof(KV_T) == 1 ? 8 : 4;
+    if (group <= 2) hipLaunchKernelGGL((score_generic_kernel<KV_T, Q_T, D, 2, U>), grid, dim3(256), 0, a.stream, p);
+    else if (group <= 4) hipLaunchKernelGGL((score_generic_kernel<KV_T, Q_T, D, 4, 1>), grid, dim3(256), 0, a.stream, p);
+    else hipLaunchKernelGGL((score_generic_kernel<KV_T, Q_T, D, 8, 1>), grid, dim3(256), 0, a.stream, p);
 }
 
 template <typename KV_T, typename Q_T>
