@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from aicomp_amd import _lib, ops
+from helpers import kernels_of
 from oracle.score_oracle import score_attention
 
 pytestmark = pytest.mark.gpu
@@ -461,3 +462,83 @@ def test_largest_and_small_caps(types, d, cap):
     c = Case([300, 65, 40], [70, 65, 1], 8, 2, d, 16, *types, seed=32)
     want, mean, size = expect(c, cap, None, 0, None, None)
     check(run_prefill(c, cap), c, want, mean, size, cap)
+
+
+# calls that take 128 rows to a workgroup: (query heads, KV heads, sequences' new tokens, tokens before them)
+LARGE = {64: (16, 4, [300] * 27 + [37, 1, 129], 70), 128: (16, 4, [300] * 14 + [37, 1, 129], 100), 256: (8, 2, [300] * 17 + [37, 1, 65], 40)}
+
+
+def large_case(d, dtype, pool, seed):
+    hq, hkv, new, before = LARGE[d]
+    return Case([n + before for n in new], new, hq, hkv, d, dtype=dtype, pool=pool, seed=seed, rows_behind=2)
+
+
+def one_by_one(c, **r):
+    """The same rows, a call for each sequence: few workgroups, 64 rows to each."""
+    outs, t = [], 0
+    for s, n in enumerate(c.new):
+        one = Case.__new__(Case)
+        one.__dict__.update(c.__dict__)
+        one.ctx, one.new, one.table, one.q, one.total = [c.ctx[s]], [n], c.table[s:s + 1].contiguous(), c.q[t:t + n], n
+        part = {**r}
+        for name in ("first", "prefix"):
+            if part.get(name) is not None:
+                part[name] = part[name][t:t + n] if name == "first" else part[name][s:s + 1]
+        outs.append(run_prefill(one, **part))
+        t += n
+    return torch.cat(outs)
+
+
+@pytest.mark.parametrize("name", ["none", "cap", "slopes", "window", "all"])
+@pytest.mark.parametrize("dtype,pool", [(BF16, None), (F16, None), (BF16, FP8), (F32, None)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_chunks(dtype, pool, d, name):
+    """Every row against the calls of single sequences, rows here and there against float64."""
+    c = large_case(d, dtype, pool, 41)
+    g = torch.Generator().manual_seed(8)
+    r = rule(name, c, g)
+    if name == "all":
+        r["prefix"] = torch.full((len(c.new),), 90, dtype=torch.int32)
+    got = []
+    names = [n for n in kernels_of(lambda: got.append(run_prefill(c, **r))) if "score_prefill" in n]
+    wide = dtype != F32 and not (d == 64 and (pool is not None or "slopes" in r))
+    assert len(names) == 1 and (f", 2, {d}," in names[0]) == wide, names
+    got = got[0]
+    total = sum(c.new)
+    assert bool((got[total:] == 7.0).all())
+    other = one_by_one(c, **r)
+    starts = [sum(c.new[:s]) for s in range(len(c.new))]
+    picks = sorted({t for s, n in enumerate(c.new[-4:], len(c.new) - 4) for t in (starts[s], starts[s] + n // 2, starts[s] + n - 1)} |
+                   set(torch.randint(0, total, (40,), generator=g).tolist()))
+    wants, means, sizes = [], [], []
+    for t in picks:
+        s = max(i for i, b in enumerate(starts) if b <= t)
+        k, v = c.rows(s)
+        w, m, z = score_attention(c.q[t:t + 1], k, v, c.ctx[s] - c.new[s] + t - starts[s], c.scale, r.get("cap", 0.0), r.get("slopes"),
+                                  r.get("window", 0), None if r.get("first") is None else r["first"][t:t + 1],
+                                  0 if r.get("prefix") is None else int(r["prefix"][s]))
+        wants.append(w), means.append(m), sizes.append(z)
+    want, mean, size = torch.cat(wants), torch.cat(means), torch.cat(sizes)
+    check(got[picks], c, want, mean, size)
+    check(other[picks], c, want, mean, size)
+    # (two right results differ by two tolerances at most: of |v| up to 6 the mean is at most 6 and so is the result, 9 for both; sizes
+    # up to 30 give e^(2 ds) - 1 = 1.08e-3)
+    u = torch.finfo(dtype).eps / 2 if dtype != F32 else 0.0
+    tol = 2 * (u * other.double().abs() + (2 * u + 1.1e-3) * 9.0)
+    assert bool(((got[:total].double() - other.double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_chunks_with_values_that_are_not_finite(d):
+    """Keys of some rows alone, infinite, in a call of 128 rows to a workgroup: as in the calls of single sequences."""
+    c = large_case(d, BF16, None, 43)
+    for s in range(0, len(c.new) - 3, 3):
+        for j in (c.ctx[s] - 1, 50 + s, c.ctx[s] // 2):
+            c.v[int(c.table[s, j // 16]), :, j % 16] = math.inf
+    r = {"cap": 5.0, "window": 40}
+    got, other = run_prefill(c, **r)[:sum(c.new)], one_by_one(c, **r)
+    finite = torch.isfinite(got)
+    assert torch.equal(finite, torch.isfinite(other)) and not bool(finite.all()) and bool(finite.any())
+    u = 2.0 ** -8
+    tol = 2 * (u * other.double().abs() + (2 * u + 1.1e-3) * 9.0)
+    assert bool(((got.double() - other.double()).abs() <= tol)[finite].all())
