@@ -542,3 +542,25 @@ def test_large_chunks_with_values_that_are_not_finite(d):
     u = 2.0 ** -8
     tol = 2 * (u * other.double().abs() + (2 * u + 1.1e-3) * 9.0)
     assert bool(((got.double() - other.double()).abs() <= tol)[finite].all())
+
+
+@pytest.mark.routing("library")
+@pytest.mark.parametrize("name", ["cap", "slopes", "all"])
+@pytest.mark.parametrize("dtype,pool,hq,hkv,d,longest", [
+    (BF16, None, 8, 2, 128, 600), (F16, None, 4, 4, 128, 513), (F16, FP8, 16, 2, 128, 640), (BF16, None, 8, 2, 64, 1100),
+    (F32, None, 8, 2, 64, 640), (F32, None, 16, 2, 64, 600), (F32, None, 8, 2, 128, 400), (F32, None, 16, 2, 128, 448)])
+def test_decode_rows_of_eight_waves(decode_routing, dtype, pool, hq, hkv, d, longest, name):
+    """Rows that are whole and long in few workgroups."""
+    c = Case([longest, 1, longest - 17, 65, 255, 256, 257], [1] * 7, hq, hkv, d, dtype=dtype, pool=pool, seed=51)
+    g = torch.Generator().manual_seed(9)
+    r = rule(name, c, g)
+    if name == "all":
+        r["window"] = longest - 40
+    tile = (64 if d == 64 else 32) // (2 if dtype == F32 else 1)    # a window reaches into a tile more; eight waves beyond 16 tiles
+    waves = 8 if min(longest, r.get("window", longest) + tile - 1) > 16 * tile else 4
+    assert waves == 8 or (longest, name) == (513, "all")
+    got = []
+    names = [n for n in kernels_of(lambda: got.append(run_decode(c, longest_context=longest, **r))) if "paged_decode" in n]
+    assert len(names) == 1 and f"{waves}, false>" in names[0] and "Ruled" in names[0], names
+    want, mean, size = expect(c, r.get("cap", 0.0), r.get("slopes"), r.get("window", 0), r.get("first"), None)
+    check(got[0], c, want, mean, size)
