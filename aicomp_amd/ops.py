@@ -9,6 +9,7 @@ used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
+import threading
 from contextlib import nullcontext
 from typing import Dict, Optional, Sequence, Tuple
 
@@ -722,6 +723,10 @@ def _guard(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
+# Calls of two threads on one stream share its scratch: the kernels of one are launched before those of the next.
+_score_calls = threading.Lock()
+
+
 def _int32(value, name: str) -> int:
     _req(-2 ** 31 <= int(value) < 2 ** 31, f"{name} {value} does not fit 32 bits")
     return int(value)
@@ -853,7 +858,7 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
                             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``paged_decode_attn`` for scores that follow a rule: one token per sequence, at position ``p = context_lens[b] - 1``.
 
-    ``s_j = scale q.k_j``, then ``softcap * tanh(s / softcap)`` (0: no cap), then ``- slopes[h] * (p - j)`` (``slopes [Hq]``
+    ``s_j = scale q.k_j``, then ``softcap * tanh(s / softcap)`` (0: no cap; at most 1024), then ``- slopes[h] * (p - j)`` (``slopes [Hq]``
     float32); visible are the last ``window`` keys (0: all) from ``first_keys[b]`` (int32) on.  A row without any is zero.
     ``longest_context``: the host's bound of ``context_lens`` (0: the table's width); it sizes the call, no row is cut by it.
     In place on ``out [B, Hq, D]``, on the current stream.
@@ -870,7 +875,7 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
     need = lib.aicomp_paged_score_workspace_bytes(B, B, 0, hq, hkv, d, bs, block_table.shape[1], qd, kd, window,
                                                   longest_context)
-    with _guard(query):
+    with _guard(query), _score_calls:
         if workspace is None:
             workspace = _call_workspace(query.device, need)
         else:
@@ -927,7 +932,7 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
     max_q_len, window = _int32(max_q_len, "max_q_len"), _int32(window, "window")
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
     need = lib.aicomp_paged_score_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, window, 0)
-    with _guard(query):
+    with _guard(query), _score_calls:
         workspace = _call_workspace(query.device, need)
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),

@@ -1,6 +1,7 @@
 """Normed heads, scores by a rule and forked sequences as a decoder uses them: through the backend and the planner, against a plain
 float32 model without a cache; recorded into graphs; by the native and the ctypes host routes; on other streams."""
 import math
+import threading
 
 import pytest
 import torch
@@ -284,3 +285,46 @@ def test_what_the_native_route_declines_is_refused_by_name(device, change):
         a[n] = f(a[n])
     with pytest.raises(RuntimeError):
         _step(a)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@BOTH
+def test_two_threads_on_one_stream(device, monkeypatch, native):
+    """Divided decode rows and divided chunks of two threads: each thread's results are those of its calls alone."""
+    if not native:
+        monkeypatch.setattr(ops, "_FAST", None)
+    cases = []
+    for seed in (1, 2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        pools = [torch.randn(400, 2, 16, 128, device=device, generator=g).bfloat16() for _ in range(2)]
+        q = torch.randn(40, 8, 128, device=device, generator=g).bfloat16()
+        table = torch.randperm(400, device=device, generator=g).to(torch.int32).view(2, 200)
+        lens = torch.tensor([3000, 1700], dtype=torch.int32, device=device)
+        cu = torch.tensor([0, 30, 40], dtype=torch.int32, device=device)
+
+        def call(q=q, pools=pools, table=table, lens=lens, cu=cu):
+            a, b = torch.empty_like(q[:2]), torch.empty_like(q)
+            ops.paged_score_decode_attn(a, q[:2], *pools, table, lens, 0.09, 30.0)
+            ops.paged_score_prefill_attn(b, q, *pools, table, lens, cu, 0.09, 30, 30.0)
+            return a, b
+        cases.append(call)
+    want = [c() for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            for _ in range(50):
+                got[i].append(cases[i]())
+        except Exception as e:                                          # (reported by the test, not by the thread)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
