@@ -508,7 +508,8 @@ int aicomp_qk_norm_rope_kv_append(const void* q_in, void* q_out,
  * Attention over the paged pools whose scores follow a rule.  Row at position p of its sequence, key j, head h:
  *   s = scale * (q . k_j);   softcap > 0: s = softcap * tanh(s / softcap);   slopes: s = s - slopes[h] * |p - j|
  *   visible: first_keys[row] <= j,  window > 0: p - j < window,  and j <= p or j < prefix_lens[sequence]
- *   out = softmax of s over the visible keys, times V; a row without visible keys (or all of whose scores are -inf) is zero
+ *   out = softmax of s over the visible keys, times V; a row without visible keys is zero.  Keys that a row does not see may hold
+ *   anything; one that it sees and whose score is not finite may make the row, at head_dim 64 its neighbour's score too, not a number
  *
  *   out, query, pools, block_table, context_lens, scales   as in aicomp_paged_decode_attn (cu_q_lens NULL: one row per
  *                   sequence at position context_lens - 1, total_q == num_seqs) or aicomp_paged_prefill_attn (rows of sequence s
