@@ -65,6 +65,17 @@ inline ScorePrefillParams chunk_params(const ScoreArgs& a) {
 #define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
 
+// Sequence and query tile of a workgroup.  Where two of a grid share a CU from the start (prefill_tile_of_slice), they are an expensive
+// and a cheap tile of one sequence there; here the second is of the sequence at the other end of the batch, whose contexts or windows
+// may be of another length (4 x 512 behind 0 .. 2048, a window of 1024: 54.6 -> 52.3 us).
+__device__ __forceinline__ void place_of(const ScorePrefillParams& p, int& seq, int& qtile) {
+    const int per = gridDim.x * gridDim.y;
+    qtile = prefill_tile_of_slice(blockIdx.z, gridDim.z, p.num_cus, per);
+    seq = blockIdx.y;
+    if (p.num_cus > 0 && p.num_cus % per == 0 && gridDim.z * per <= 2 * p.num_cus && (int)blockIdx.z >= p.num_cus / per)
+        seq = gridDim.y - 1 - seq;
+}
+
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));

@@ -22,7 +22,7 @@
 //              Q once more: against float64 an error of 3.0e-3 where this has 2.1e-3, bf16, a prompt of 8192 under a cap.)
 // Bound by     the issue of vector and matrix instructions, which do not overlap: of a prompt of 8192, 32 / 8 heads of 128 under a cap,
 //              37 % and 62 % of the cycles, 600 us, 0.92 PFLOP/s (a large product reaches 1.26).  head_dim 64 the same 405 us; 4 x 512
-//              with a window of 1024, 54 us; head_dim 256, 4096 tokens of 16 / 8 heads, 300 us.
+//              with a window of 1024, 52 us; head_dim 256, 4096 tokens of 16 / 8 heads, 300 us.
 #include "score_prefill.h"
 
 #include <algorithm>
@@ -51,7 +51,7 @@ score_prefill_kernel(ScorePrefillParams p) {
     constexpr int TILE_BYTES = KT * KROW;
     constexpr int WROWS = 16 * R;              // rows per wave
     constexpr int NS = 4 * NH;                 // scores per lane and column group
-    const int part = R == 1 ? blockIdx.x / p.hgroups : 0, hgroup = R == 1 ? blockIdx.x % p.hgroups : blockIdx.x, seq = blockIdx.y;
+    const int part = R == 1 ? blockIdx.x / p.hgroups : 0, hgroup = R == 1 ? blockIdx.x % p.hgroups : blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
@@ -63,7 +63,8 @@ score_prefill_kernel(ScorePrefillParams p) {
     __shared__ __attribute__((aligned(16))) unsigned char v1[TILE_BYTES];
     __shared__ int span[2][4];
 
-    const int qtile = prefill_tile_of_slice(blockIdx.z, gridDim.z, p.num_cus, gridDim.x * gridDim.y);
+    int seq, qtile;
+    place_of(p, seq, qtile);
     const int q_begin = p.cu_q_lens[seq];
     const int n = p.cu_q_lens[seq + 1] - q_begin;
     const int ctx = min(p.context_lens[seq], p.max_blocks * BS);

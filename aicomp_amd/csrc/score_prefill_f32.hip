@@ -30,7 +30,7 @@ score_prefill_f32_kernel(ScorePrefillParams p) {
     constexpr int NF = DH / 64;
     constexpr int CPR = DH / 4;                // 16-byte chunks per row
     constexpr int TILE_BYTES = KT * KROW;
-    const int part = blockIdx.x / p.hgroups, hgroup = blockIdx.x % p.hgroups, seq = blockIdx.y;
+    const int part = blockIdx.x / p.hgroups, hgroup = blockIdx.x % p.hgroups;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
@@ -42,7 +42,8 @@ score_prefill_f32_kernel(ScorePrefillParams p) {
     __shared__ __attribute__((aligned(16))) unsigned char v1[TILE_BYTES];
     __shared__ int span[2][4];
 
-    const int qtile = prefill_tile_of_slice(blockIdx.z, gridDim.z, p.num_cus, gridDim.x * gridDim.y);
+    int seq, qtile;
+    place_of(p, seq, qtile);
     const int q_begin = p.cu_q_lens[seq];
     const int n = p.cu_q_lens[seq + 1] - q_begin;
     const int ctx = min(p.context_lens[seq], p.max_blocks * BS);
