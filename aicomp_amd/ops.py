@@ -124,6 +124,11 @@ def kv_append(key: torch.Tensor, value: torch.Tensor, k_pool: torch.Tensor, v_po
 # split-K scratch, one growing buffer per (device, stream)
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 
+# A call with scratch is two launches, and on one stream two of them must not interleave: the second call's partials would replace
+# the first's before its merge reads them.  Two host threads on one stream can get there (ctypes lets go of the interpreter lock),
+# so every call that takes a buffer of the above holds this from then to the end of its launches.
+_scratch_calls = threading.RLock()
+
 
 def _workspace(device: torch.device, nbytes: int, stream: Optional[int] = None) -> Optional[torch.Tensor]:
     if nbytes == 0:
@@ -208,9 +213,6 @@ def paged_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tens
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
     need = lib.aicomp_paged_decode_workspace_bytes(B, hq, hkv, d, bs, block_table.shape[1], qd, kd,
                                                    partition_size)
-    if workspace is None:
-        workspace = _workspace(query.device, need)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     if new_key is not None:
         _req(new_value is not None and new_key.shape == (B, hkv, d) and new_value.shape == (B, hkv, d)
              and new_key.dtype == query.dtype and new_value.dtype == query.dtype,
@@ -219,20 +221,24 @@ def paged_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tens
         _dev(new_value, query, "new_value")
         if new_key.stride(2) != 1 or new_key.stride() != new_value.stride():
             new_key, new_value = new_key.contiguous(), new_value.contiguous()
-        rc = lib.aicomp_paged_decode_attn_append(
-            out.data_ptr(), query.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
-            new_key.stride(0), new_key.stride(1), k_pool.data_ptr(), v_pool.data_ptr(),
-            block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), B, hq, hkv, d, bs,
-            block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), partition_size,
-            _ptr(workspace), ws_bytes, _stream(query))
-        _lib.check(rc, lib)
-        return out
-    rc = lib.aicomp_paged_decode_attn(out.data_ptr(), query.data_ptr(), k_pool.data_ptr(),
-                                      v_pool.data_ptr(), block_table.data_ptr(),
-                                      block_table.stride(0), context_lens.data_ptr(), B, hq, hkv, d,
-                                      bs, block_table.shape[1], nb, float(scale), qd, kd,
-                                      _ptr(ks), _ptr(vs), partition_size, _ptr(workspace),
-                                      ws_bytes, _stream(query))
+    with _scratch_calls:
+        if workspace is None:
+            workspace = _workspace(query.device, need)
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        if new_key is not None:
+            rc = lib.aicomp_paged_decode_attn_append(
+                out.data_ptr(), query.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
+                new_key.stride(0), new_key.stride(1), k_pool.data_ptr(), v_pool.data_ptr(),
+                block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), B, hq, hkv, d, bs,
+                block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), partition_size,
+                _ptr(workspace), ws_bytes, _stream(query))
+        else:
+            rc = lib.aicomp_paged_decode_attn(out.data_ptr(), query.data_ptr(), k_pool.data_ptr(),
+                                              v_pool.data_ptr(), block_table.data_ptr(),
+                                              block_table.stride(0), context_lens.data_ptr(), B, hq, hkv, d,
+                                              bs, block_table.shape[1], nb, float(scale), qd, kd,
+                                              _ptr(ks), _ptr(vs), partition_size, _ptr(workspace),
+                                              ws_bytes, _stream(query))
     _lib.check(rc, lib)
     return out
 
@@ -294,23 +300,25 @@ class PreparedDecode:
              and query.is_contiguous() and out.is_contiguous(),
              f"out/query must be contiguous {self.q_shape} {self.q_dtype} tensors on {self.device}")
         ctx = self.context_lens if context_lens is None else context_lens
-        stream = _current_stream(self.device)
-        ws = _workspace(self.device, self.need, stream)
-        ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
-        if new_key is None:
-            rc = self.lib.aicomp_paged_decode_attn(out.data_ptr(), query.data_ptr(), *self._head, ctx.data_ptr(),
-                                                   *self._tail, ws_ptr, ws_bytes, stream)
-        else:
+        if new_key is not None:
             _req(new_value is not None and new_key.shape == self.kv_shape and new_value.shape == self.kv_shape
                  and new_key.dtype == self.q_dtype and new_value.dtype == self.q_dtype
                  and new_key.device == self.device and new_value.device == self.device,
                  f"new_key/new_value must both be {self.kv_shape} of the query dtype on {self.device}")
             if new_key.stride(2) != 1 or new_key.stride() != new_value.stride():
                 new_key, new_value = new_key.contiguous(), new_value.contiguous()
-            rc = self.lib.aicomp_paged_decode_attn_append(
-                out.data_ptr(), query.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
-                new_key.stride(0), new_key.stride(1), *self._head, ctx.data_ptr(), *self._tail,
-                ws_ptr, ws_bytes, stream)
+        stream = _current_stream(self.device)
+        with _scratch_calls:
+            ws = _workspace(self.device, self.need, stream)
+            ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+            if new_key is None:
+                rc = self.lib.aicomp_paged_decode_attn(out.data_ptr(), query.data_ptr(), *self._head, ctx.data_ptr(),
+                                                       *self._tail, ws_ptr, ws_bytes, stream)
+            else:
+                rc = self.lib.aicomp_paged_decode_attn_append(
+                    out.data_ptr(), query.data_ptr(), new_key.data_ptr(), new_value.data_ptr(),
+                    new_key.stride(0), new_key.stride(1), *self._head, ctx.data_ptr(), *self._tail,
+                    ws_ptr, ws_bytes, stream)
         _lib.check(rc, self.lib)
         return out
 
@@ -338,19 +346,20 @@ class PreparedDecode:
              f"key/value must both be [{B}, {hkv} or {hkv}*group, 1, {D}] of the query dtype on {self.device}")
         if key.stride(3) != 1 or key.stride() != value.stride():
             key, value = key.contiguous(), value.contiguous()
-        stream = _current_stream(self.device)
-        ws = _workspace(self.device, self.need, stream)
-        ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
-        if ready is not None:
-            ready()
         tail = self._tail
         if width is not None and 0 < width < tail[5]:
             tail = tail[:5] + (width,) + tail[6:]
-        rc = self.lib.aicomp_paged_decode_attn_append(
-            out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
-            key.stride(0), D if hkv == 1 else key.stride(1) * hstep, *self._head,     # (one head's stride may be 0, and is not taken)
-            context_lens if isinstance(context_lens, int) else context_lens.data_ptr(), *tail,
-            ws_ptr, ws_bytes, stream)
+        stream = _current_stream(self.device)
+        with _scratch_calls:
+            ws = _workspace(self.device, self.need, stream)
+            ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+            if ready is not None:
+                ready()
+            rc = self.lib.aicomp_paged_decode_attn_append(
+                out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                key.stride(0), D if hkv == 1 else key.stride(1) * hstep, *self._head,     # (one head's stride may be 0, and is not taken)
+                context_lens if isinstance(context_lens, int) else context_lens.data_ptr(), *tail,
+                ws_ptr, ws_bytes, stream)
         _lib.check(rc, self.lib)
         return out
 
@@ -723,10 +732,6 @@ def _guard(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
-# Calls of two threads on one stream share its scratch: the kernels of one are launched before those of the next.
-_score_calls = threading.Lock()
-
-
 def _int32(value, name: str) -> int:
     _req(-2 ** 31 <= int(value) < 2 ** 31, f"{name} {value} does not fit 32 bits")
     return int(value)
@@ -875,7 +880,7 @@ def paged_score_decode_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torc
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
     need = lib.aicomp_paged_score_workspace_bytes(B, B, 0, hq, hkv, d, bs, block_table.shape[1], qd, kd, window,
                                                   longest_context)
-    with _guard(query), _score_calls:
+    with _guard(query), _scratch_calls:
         if workspace is None:
             workspace = _call_workspace(query.device, need)
         else:
@@ -932,7 +937,7 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
     max_q_len, window = _int32(max_q_len, "max_q_len"), _int32(window, "window")
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
     need = lib.aicomp_paged_score_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, window, 0)
-    with _guard(query), _score_calls:
+    with _guard(query), _scratch_calls:
         workspace = _call_workspace(query.device, need)
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
