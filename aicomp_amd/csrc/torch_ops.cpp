@@ -114,9 +114,16 @@ void kv_append(const at::Tensor& key, const at::Tensor& value, at::Tensor& k_poo
 
 // Scratch the ops keep for callers that pass none: one growing buffer per (device, stream), like
 // the Python wrappers'.  A decode call's scratch needs no initialisation and holds nothing between
-// calls, and calls on one stream run one after the other, so reuse is safe.  The map is never
+// calls, and calls on one stream run one after the other, so reuse is safe as long as the two launches of
+// a call stay together: scratch_launches() is held over them (the dispatcher lets go of the interpreter lock, and
+// two host threads may be on one stream).  The map is never
 // destroyed (tensors freed at process exit, after the allocator, would fault).
-at::Tensor& cached_scratch(const at::Tensor& ref, size_t bytes) {
+std::mutex& scratch_launches() {
+    static auto* mu = new std::mutex();
+    return *mu;
+}
+
+at::Tensor cached_scratch(const at::Tensor& ref, size_t bytes) {
     static std::mutex mu;
     static auto* table = new std::map<std::pair<int, void*>, at::Tensor>();
     std::lock_guard<std::mutex> lock(mu);
@@ -161,7 +168,9 @@ void decode_impl(at::Tensor& out, const at::Tensor& query, const at::Tensor* new
     at::Tensor own;
     size_t ws_bytes = 0;
     void* ws = decode_workspace(workspace, own, query, B, hq, p, (int)block_table.size(1), qd, kd, (int)partition_size, ws_bytes);
+    std::unique_lock<std::mutex> one_at_a_time(scratch_launches(), std::defer_lock);
     if (new_key == nullptr) {
+        if (own.defined()) one_at_a_time.lock();
         check_rc(aicomp_paged_decode_attn(out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                           block_table.data_ptr<int32_t>(), block_table.stride(0),
                                           context_lens.data_ptr<int32_t>(), B, hq, p.hkv, p.d, p.bs,
@@ -175,6 +184,7 @@ void decode_impl(at::Tensor& out, const at::Tensor& query, const at::Tensor* new
                 nk.device() == query.device() && nv.device() == query.device(),
                 "new_key/new_value must both be [", B, ", ", p.hkv, ", ", p.d, "] of the query dtype on ", query.device());
     if (nk.stride(2) != 1 || nk.strides() != nv.strides()) { nk = nk.contiguous(); nv = nv.contiguous(); }
+    if (own.defined()) one_at_a_time.lock();
     check_rc(aicomp_paged_decode_attn_append(out.data_ptr(), query.data_ptr(), nk.data_ptr(), nv.data_ptr(), nk.stride(0),
                                              nk.stride(1), k_pool.data_ptr(), v_pool.data_ptr(),
                                              block_table.data_ptr<int32_t>(), block_table.stride(0),
@@ -276,6 +286,8 @@ at::Tensor decode_step(const at::Tensor& query_in, const at::Tensor& key, const 
     size_t ws_bytes = 0;
     void* ws = decode_workspace(workspace, own, query, B, hq, p, width, qd, kd, 0, ws_bytes);
     at::Tensor out = at::empty_like(query);
+    std::unique_lock<std::mutex> one_at_a_time(scratch_launches(), std::defer_lock);
+    if (own.defined()) one_at_a_time.lock();
     check_rc(aicomp_paged_decode_attn_append(out.data_ptr(), query.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride(0),
                                              p.hkv == 1 ? p.d : k.stride(1) * hstep, k_pool.data_ptr(), v_pool.data_ptr(),
                                              block_table.data_ptr<int32_t>(), block_table.stride(0),
