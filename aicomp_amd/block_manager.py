@@ -385,7 +385,8 @@ class StepPlanner:
        step's token budget ``max_num_batched_tokens``);
     2. running sequences still inside their prompt, then waiting ones in arrival
        order, get a chunk of at most ``prefill_chunk`` tokens while the budget and
-       the pool allow;
+       the pool allow; a first chunk is never shorter than the request's ``prefix_len``, and
+       a request whose prefix is more than is left of the step's budget waits;
     3. if a running sequence needs a block and none is free, the youngest running
        sequence is preempted: its blocks are released and it re-enters the head of
        the waiting queue, to be recomputed from its prompt plus what it generated.
@@ -418,7 +419,7 @@ class StepPlanner:
         self.device = torch.device(device)
         self.num_preemptions = 0
         self._arrivals = 0
-        # waiting queue: (seq_id, tokens to ingest, original prompt length, max_new_tokens, arrival)
+        # waiting queue: (seq_id, tokens to ingest, original prompt length, max_new_tokens, arrival, prefix length)
         self.waiting: Deque[tuple] = deque()
         self._waiting_ids = set()
         # running sequences, by row
@@ -433,6 +434,7 @@ class StepPlanner:
         self._orig = np.zeros(max_seqs, dtype=np.int32)       # the request's own prompt length
         self._maxnew = np.zeros(max_seqs, dtype=np.int64)     # -1: unbounded
         self._arr = np.zeros(max_seqs, dtype=np.int64)
+        self._prefix = np.zeros(max_seqs, dtype=np.int32)     # tokens that one chunk has to ingest together
         self._live = np.zeros(max_seqs, dtype=bool)
         self._row_state = (self._live, self._len, self._prompt, self._orig, self._nblk, self._maxnew, self._arr)
         # packed layout (bytes): slot_mapping int64 [T] | positions int64 [T] | block_table int32 [S*MB] |
@@ -441,9 +443,14 @@ class StepPlanner:
         self._staging = _Staging(cap, self.device, staging_depth)
 
     # ------------------------------------------------------------------ requests
-    def add_request(self, seq_id, prompt_len: int, max_new_tokens: Optional[int] = None) -> None:
+    def add_request(self, seq_id, prompt_len: int, max_new_tokens: Optional[int] = None, prefix_len: int = 0) -> None:
+        """Queue a sequence.  ``prefix_len``: tokens at its start whose rows all see each other
+        (``PagedAttentionBackend.begin_step(prefix_lens=...)``); they are ingested by one chunk, whatever ``prefill_chunk`` is."""
         if prompt_len <= 0:
             raise ValueError(f"prompt_len must be positive, got {prompt_len}")
+        if not 0 <= prefix_len <= min(prompt_len, self.max_num_batched_tokens):
+            raise ValueError(f"prefix_len {prefix_len} must be within the prompt of {prompt_len} tokens and a step's "
+                             f"{self.max_num_batched_tokens}")
         if max_new_tokens is not None and max_new_tokens < 0:
             raise ValueError(f"max_new_tokens must be non-negative, got {max_new_tokens}")
         total = prompt_len + (max_new_tokens or 0)
@@ -454,7 +461,7 @@ class StepPlanner:
         if seq_id in self._row_of or seq_id in self._waiting_ids:
             raise ValueError(f"sequence id {seq_id!r} is already known")
         self.waiting.append((seq_id, int(prompt_len), int(prompt_len),
-                             -1 if max_new_tokens is None else int(max_new_tokens), self._arrivals))
+                             -1 if max_new_tokens is None else int(max_new_tokens), self._arrivals, int(prefix_len)))
         self._waiting_ids.add(seq_id)
         self._arrivals += 1
 
@@ -489,7 +496,7 @@ class StepPlanner:
         r = self._free_rows.pop()
         self._row_of[new_id], self._id_of[r] = r, new_id
         self._tab[r, :full], self._tab[r, full:n] = mine[:full], fresh
-        for state in (self._nblk, self._len, self._prompt, self._orig, self._maxnew):
+        for state in (self._nblk, self._len, self._prompt, self._orig, self._maxnew, self._prefix):
             state[r] = state[a]
         self._live[r] = True
         self._arr[r] = self._arrivals
@@ -555,7 +562,7 @@ class StepPlanner:
         sid = self._id_of[r]
         # recompute later: everything cached so far must be ingested again
         redo = int(self._len[r]) if self._len[r] >= self._prompt[r] else int(self._prompt[r])
-        self.waiting.appendleft((sid, redo, int(self._orig[r]), int(self._maxnew[r]), int(self._arr[r])))
+        self.waiting.appendleft((sid, redo, int(self._orig[r]), int(self._maxnew[r]), int(self._arr[r]), int(self._prefix[r])))
         self._waiting_ids.add(sid)
         del self._row_of[sid]
         self._release_row(r)
@@ -643,8 +650,10 @@ class StepPlanner:
             chunks.append((r, n))
             budget -= n
         while self.waiting and budget > 0 and self._free_rows:
-            sid, todo, orig, maxnew, arrival = self.waiting[0]
-            n = min(self.prefill_chunk, todo, budget)
+            sid, todo, orig, maxnew, arrival, prefix = self.waiting[0]
+            n = min(max(self.prefill_chunk, prefix), todo, budget)
+            if n < prefix:
+                break
             if not self.alloc.can_allocate(self.alloc.blocks_for(n)):
                 break
             self.waiting.popleft()
@@ -655,7 +664,7 @@ class StepPlanner:
             self._live[r] = True
             self._len[r] = 0
             self._nblk[r] = 0
-            self._prompt[r], self._orig[r], self._maxnew[r], self._arr[r] = todo, orig, maxnew, arrival
+            self._prompt[r], self._orig[r], self._maxnew[r], self._arr[r], self._prefix[r] = todo, orig, maxnew, arrival, prefix
             self._grow_row(r, n)
             chunks.append((r, n))
             budget -= n

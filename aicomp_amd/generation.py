@@ -110,10 +110,28 @@ class PagedAttentionBackend:
         self.k_scales[layer_idx] = k_scale.to(self.device, torch.float32).contiguous()
         self.v_scales[layer_idx] = v_scale.to(self.device, torch.float32).contiguous()
 
-    def begin_step(self, plan: StepPlan, first_keys: Optional[torch.Tensor] = None,
-                   prefix_lens: Optional[torch.Tensor] = None) -> None:
+    def begin_step(self, plan: StepPlan, first_keys: Optional[torch.Tensor] = None, prefix_lens=None) -> None:
         """``first_keys [T]`` int32: the first key that each row of the step sees (packed documents); ``prefix_lens [S]`` int32: the
-        part at the start of each sequence that all its rows see.  Both hold for every layer of the step."""
+        part at the start of each sequence that all its rows see, on the host (a sequence, an array, a CPU tensor; a tensor on the
+        device is read back, which waits for it).  Both hold for every layer of the step.
+
+        All rows of a prefix see each other, so it has to be ingested by one step: one that reaches beyond its sequence's
+        context in this step is refused (``StepPlanner.add_request(..., prefix_len=...)`` keeps it in one chunk)."""
+        if prefix_lens is not None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("begin_step with prefix_lens goes before the recording of a step: their values are looked at")
+            lens = torch.as_tensor(prefix_lens)
+            host = lens.cpu().numpy()
+            if lens.shape != (plan.num_seqs,) or host.dtype.kind not in "iu":
+                raise ValueError(f"prefix_lens must be {plan.num_seqs} whole numbers, one per sequence of the step; got "
+                                 f"{host.dtype} {tuple(lens.shape)}")
+            beyond = np.flatnonzero(host > plan.host_context_lens)
+            if beyond.size:
+                r = int(beyond[0])
+                raise ValueError(f"sequence {plan.seq_ids[r]!r}: its prefix of {int(host[r])} tokens is not in this step, which ends at "
+                                 f"{int(plan.host_context_lens[r])}; a prefix is ingested in one chunk "
+                                 f"(StepPlanner.add_request(..., prefix_len={int(host[r])}))")
+            prefix_lens = lens.to(self.device, torch.int32).contiguous()
         self.plan, self.first_keys, self.prefix_lens = plan, first_keys, prefix_lens
 
     def _score_attend(self, layer_idx: int, out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
