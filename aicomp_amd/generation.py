@@ -141,17 +141,18 @@ class PagedAttentionBackend:
         rule = self._rules.get(layer_idx, {})
         npre, S, t = plan.num_prefill_seqs, plan.num_seqs, plan.num_prefill_tokens
         first, prefix = self.first_keys, self.prefix_lens
+        # (a recorded launch is sized for the whole table: the lengths of its replays may grow)
+        sized = not (q.is_cuda and torch.cuda.is_current_stream_capturing())
         if npre:
             ops.paged_score_prefill_attn(out[:t], q[:t], kp, vp, plan.block_table[:npre], plan.context_lens[:npre],
                                          plan.cu_q_lens[:npre + 1], self.scale, max_q_len=plan.max_q_len,
                                          first_keys=None if first is None else first[:t],
-                                         prefix_lens=None if prefix is None else prefix[:npre], k_scale=ks, v_scale=vs, **rule)
+                                         prefix_lens=None if prefix is None else prefix[:npre], k_scale=ks, v_scale=vs,
+                                         longest_context=int(plan.host_context_lens[:npre].max()) if sized else 0, **rule)
         if S > npre:
-            # (a recorded launch is sized for the whole table: the lengths of its replays may grow)
-            longest = 0 if q.is_cuda and torch.cuda.is_current_stream_capturing() else int(plan.host_context_lens[npre:].max())
             ops.paged_score_decode_attn(out[t:], q[t:], kp, vp, plan.block_table[npre:], plan.context_lens[npre:], self.scale,
                                         first_keys=None if first is None else first[t:], k_scale=ks, v_scale=vs,
-                                        longest_context=longest, **rule)
+                                        longest_context=int(plan.host_context_lens[npre:].max()) if sized else 0, **rule)
         return out
 
     def attend(self, layer_idx: int, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> torch.Tensor:

@@ -908,16 +908,20 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
                              max_q_len: Optional[int] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
                              window: int = 0, first_keys: Optional[torch.Tensor] = None,
                              prefix_lens: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
-                             v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+                             v_scale: Optional[torch.Tensor] = None, longest_context: int = 0) -> torch.Tensor:
     """``paged_prefill_attn`` for scores that follow a rule: chunks ``query [T, Hq, D]`` whose rows are in the pools already.
 
     Cap, slopes and window as in ``paged_score_decode_attn`` (the bias falls with ``|p - j|``); ``first_keys [T]`` int32 gives the
     first key that each row sees (packed documents), ``prefix_lens [S]`` int32 a part at the start of each sequence that all
     its rows see.  A row without visible keys is zero; rows behind the last sequence are left as they are.
+
+    ``longest_context``: the host's bound of ``context_lens`` (0: the table's width).  By it the keys of few rows are divided among
+    workgroups or not, and no row is cut: 64 and 512 new tokens from none, 32 / 8 heads of 128, a cap, in a table of 8192 tokens,
+    take 6.8 and 15.2 us with it and 14.2 and 22.8 without.
     """
     if _native("aicomp_paged_score_attn") and max_q_len and _FAST.paged_score_attn(
             out, query, k_pool, v_pool, block_table, context_lens, scale, k_scale, v_scale, cu_q_lens, max_q_len, softcap, slopes,
-            window, first_keys, prefix_lens, 0, None):
+            window, first_keys, prefix_lens, longest_context, None):
         return out
     lib = _lib.load()
     nb, hkv, bs, d, T, hq, S, ks, vs = _score_checks(out, query, k_pool, v_pool, block_table, context_lens, slopes, first_keys,
@@ -934,16 +938,19 @@ def paged_score_prefill_attn(out: torch.Tensor, query: torch.Tensor, k_pool: tor
         max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
     if max_q_len == 0:
         return out
-    max_q_len, window = _int32(max_q_len, "max_q_len"), _int32(window, "window")
+    max_q_len, window, longest_context = (_int32(x, n) for x, n in ((max_q_len, "max_q_len"), (window, "window"),
+                                                                    (longest_context, "longest_context")))
     qd, kd = _dt(query, "query"), _dt(k_pool, "pool")
-    need = lib.aicomp_paged_score_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, window, 0)
+    need = lib.aicomp_paged_score_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, window,
+                                                  longest_context)
     with _guard(query), _scratch_calls:
         workspace = _call_workspace(query.device, need)
         rc = lib.aicomp_paged_score_attn(
             out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
             block_table.stride(0), context_lens.data_ptr(), cu_q_lens.data_ptr(), S, T, max_q_len, hq, hkv, d, bs,
             block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), float(softcap), _ptr(slopes), window,
-            _ptr(first_keys), _ptr(prefix_lens), 0, _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream(query))
+            _ptr(first_keys), _ptr(prefix_lens), longest_context, _ptr(workspace), 0 if workspace is None else workspace.numel(),
+            _stream(query))
     _lib.check(rc, lib)
     return out
 
