@@ -55,6 +55,37 @@ def score_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first_pos
     return out, mean_abs, size
 
 
+def score_attention_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first_pos: int, scale: float, cap: float = 0.0,
+                         slopes: Optional[torch.Tensor] = None, window: int = 0, first_keys: Optional[torch.Tensor] = None,
+                         prefix: int = 0):
+    """``score_attention`` of all rows of a head at once, for thousands of rows: the same values but for the order of sums."""
+    n, hq, d = q.shape
+    ctx, hkv, _ = k.shape
+    q, k, v = q.double(), k.double(), v.double()
+    j, p = torch.arange(ctx), torch.arange(first_pos, first_pos + n)[:, None]
+    seen = (j <= p) | (j < prefix)
+    if window:
+        seen &= p - j < window
+    if first_keys is not None:
+        seen &= j >= first_keys[:, None]
+    some = seen.any(1)
+    out = torch.zeros(n, hq, d, dtype=torch.float64)
+    mean_abs = torch.zeros_like(out)
+    size = torch.zeros(n, hq, dtype=torch.float64)
+    for h in range(hq):
+        kk, vv = k[:, h // (hq // hkv)], v[:, h // (hq // hkv)]
+        s = q[:, h] @ kk.T * scale
+        if cap:
+            s = cap * torch.tanh(s / cap)
+        if slopes is not None:
+            s = s - float(slopes[h]) * (p - j).abs().double()
+        w = torch.softmax(torch.where(seen, s, -torch.inf)[some], -1)
+        out[some, h] = w @ vv
+        mean_abs[some, h] = w @ vv.abs()
+        size[some, h] = torch.where(seen, q[:, h].abs() @ kk.abs().T, 0.0).amax(1)[some] * abs(scale)
+    return out, mean_abs, size
+
+
 def norm_rope(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, angles: Optional[torch.Tensor], interleaved: bool):
     """``x [T, H, D]``, ``angles [T, R/2]`` (or None) -> float64."""
     x = x.double()
