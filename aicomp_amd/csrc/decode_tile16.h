@@ -137,7 +137,8 @@ struct PlainScore {
     __device__ __forceinline__ float operator()(float s, int) const { return s * mul; }
     __device__ __forceinline__ bool below(int) const { return false; }
 };
-// cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)): one exponential and one reciprocal more.  The branches are uniform.
+// cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)): one exponential and one reciprocal more, good to 2^-22 of the cap (a cap is at
+// most 1024, where that moves a weight by half a rounding of float16).  The branches are uniform.
 struct RuleScore {
     float mul;                             // with a cap: 2 log2(e) scale / cap
     float cap, slope;                      // times log2(e); slope: of this lane's head
@@ -253,7 +254,9 @@ __device__ __forceinline__ void process_tile(WaveState& st, TileRegs<FP8>& kr, T
 #pragma unroll
         for (int j = 0; j < 8; ++j) st.O[j] *= alpha;
     }
-    // P^T as the B operand: k-slot 4a + i <-> token 16a + 4i + g4, this lane's own values
+    // P^T as the B operand: k-slot 4a + i <-> token 16a + 4i + g4, this lane's own values, rounded to the 16-bit type that the matrix
+    // cores take (half a step each, against float64 2.0e-3 of a bf16 batch where the rounding of its result alone leaves 1.7e-3;
+    // the weights in two parts would be twice the products).  Their sum is that of the float32 weights.
     uint4 pw;
     pw.x = E::pack(pr[0], pr[1]); pw.y = E::pack(pr[2], pr[3]);
     pw.z = E::pack(pr[4], pr[5]); pw.w = E::pack(pr[6], pr[7]);

@@ -7,9 +7,12 @@
 // share a loaded chunk, and the groups' states are merged by shuffles, the waves' through LDS.
 //
 // Bound by the loads in flight for groups of one to four heads, by the vector ALU (2 D multiply-adds a score, and what a score takes
-// itself in every lane of its group) above.  64 rows of 512 .. 4096 tokens, head_dim 256, bf16 under a cap: 16 / 8 heads 288 us, 4.2 TB/s
+// itself in every lane of its group) above.  64 rows of 512 .. 4096 tokens, head_dim 256, bf16 under a cap: 16 / 8 heads 271 us, 4.5 TB/s
 // (583 with one token in flight, two of four heads computed for nothing, sums through the LDS's lane moves and a maximum per
-// token); 32 / 4 heads 545; one row of 4096, 24.
+// token); 16 / 4 and 32 / 4 heads 256 and 560, where the bytes take 116; one row of 4096, 24.  Block sizes other than 16 (D 128, 32 / 8
+// heads) 225, head_dim 64 117, where the tiles of blocks of 16 take 97 and 54.
+// Chunks come here for their block size alone, a workgroup per row and KV head that reads the row's keys for itself: 512 and 2048
+// tokens from none, D 128, a cap, blocks of 8 or 32: 115 and 1304 us, where blocks of 16 take 15 and 62; 64 behind 4000 271, and 27.
 #include "score.h"
 
 namespace aicomp {

@@ -20,9 +20,12 @@
 // Rounding     The weights to the 16-bit format of the matrix cores; everything else in float32 until the one rounding of
 //              the result.  (The scores' multiplier in Q would save an instruction per score, which no time shows, and round
 //              Q once more: against float64 an error of 3.0e-3 where this has 2.1e-3, bf16, a prompt of 8192 under a cap.)
-// Bound by     the issue of vector and matrix instructions, which do not overlap: of a prompt of 8192, 32 / 8 heads of 128 under a cap,
-//              37 % and 62 % of the cycles, 600 us, 0.92 PFLOP/s (a large product reaches 1.26).  head_dim 64 the same 405 us; 4 x 512
-//              with a window of 1024, 52 us; head_dim 256, 4096 tokens of 16 / 8 heads, 300 us.
+// Bound by     the issue of vector and matrix instructions, which overlap little: of a prompt of 8192, 32 / 8 heads of 128 under a cap,
+//              the matrix cores hold 39 % of the cycles, vector instructions 56 % (8.5 a score, of which three, exponentials and
+//              a reciprocal, take two slots each), and 9 % of them both; 600 us, 0.92 PFLOP/s (a large product reaches 1.26).  fp8
+//              pools 724 us: the codes' widening and waits.  head_dim 64 the same 405 us: half the products for the same scores, vector
+//              79 %.  4 x 512 with a window of 1024, 52 us (26 % and 46 %).  head_dim 256, 4096 tokens of 16 / 8 heads, 300 us:
+//              19 % and 24 %, one wave to a SIMD has no other to run beside.
 #include "score_prefill.h"
 
 #include <algorithm>

@@ -11,9 +11,10 @@
 // S^T = K Q^T  v_mfma_f32_16x16x4_f32; the k index of MFMA 4 q + e in lane group g is dim 16 q + 4 g + e, so that one 16-byte LDS
 //              read has the A operands of four.  O^T += V^T P^T: lane (r, g) reads dims 64 f + 4 r .. + 3 of token 4 g + e, and B is
 //              the weight that the lane holds.
-// Bound by     the float32 matrix instruction, which shares the vector ALU's multipliers: what a score costs beside it adds to it.
-//              2048 new tokens, 32 / 8 heads of 128, a cap: 329 us, 104 TFLOP/s, where a large product reaches 153 (on the vector
-//              units 2880); head_dim 64 under a cap and with a bias alone 199 and 190.
+// Bound by     the float32 matrix instruction, beside which no vector instruction runs: 2048 new tokens, 32 / 8 heads of 128: it holds 71 %
+//              of the cycles, the vector ALU 5 % (11 % under a cap) and both none; the rest are waits of two rounds of workgroups
+//              unlike in length.  326 us under a cap, 322 without any term, 105 TFLOP/s, where a large product reaches 153 (on the vector
+//              units 2880).  head_dim 64: a cap 198, a bias alone 180, neither 176; 65 % and 8 %.
 #include "score_prefill.h"
 
 namespace aicomp {
