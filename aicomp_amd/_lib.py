@@ -37,10 +37,17 @@ SYMBOLS = (
     "aicomp_sample_tokens",
     "aicomp_sample_tokens_split",
     "aicomp_sample_workspace_bytes",
+    "aicomp_latent_kv_append",
+    "aicomp_paged_latent_attn",
+    "aicomp_paged_latent_workspace_bytes",
+    "aicomp_latent_prompt_attn",
+    "aicomp_paged_tree_attn",
+    "aicomp_paged_tree_workspace_bytes",
+    "aicomp_kv_keep_rows",
 )
 
 F32, BF16, FP8_E4M3, F16 = 0, 1, 2, 3
-MIN_VERSION = 400            # 0.4.0: the entry points of SYMBOLS above
+MIN_VERSION = 500            # 0.5.0: the entry points of SYMBOLS above
 
 _lock = threading.RLock()       # torch_ops() loads the HIP library while holding it
 _lib = None
@@ -115,6 +122,24 @@ def _declare(lib: C.CDLL) -> None:
                                             i32, vp, vp, f32, vp, i32, vp, vp, i32, vp, sz, vp]
     lib.aicomp_paged_score_workspace_bytes.restype = sz
     lib.aicomp_paged_score_workspace_bytes.argtypes = [i32, i64] + [i32] * 10
+    lib.aicomp_latent_kv_append.restype = i32
+    lib.aicomp_latent_kv_append.argtypes = [vp, i64, vp, f32, vp, vp, i64, i64, i32, vp, vp, vp, i64, i64, i64, i64, vp, i64, vp, vp,
+                                            i64, i32, i32, i32, i32, i64, i32, vp]
+    lib.aicomp_paged_latent_attn.restype = i32
+    lib.aicomp_paged_latent_attn.argtypes = [vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i64, i32, i32, i32, i32, i32, i32, i64, f32, i32,
+                                             i32, vp, sz, vp]
+    lib.aicomp_paged_latent_workspace_bytes.restype = sz
+    lib.aicomp_paged_latent_workspace_bytes.argtypes = [i32, i64] + [i32] * 8
+    lib.aicomp_latent_prompt_attn.restype = i32
+    lib.aicomp_latent_prompt_attn.argtypes = [vp, vp, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp, i32, i64, i64, i32, i32, i32, i32, i32,
+                                              f32, i32, vp]
+    lib.aicomp_paged_tree_attn.restype = i32
+    lib.aicomp_paged_tree_attn.argtypes = [vp, vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i64, i32, i32, i32, i32, i32, i32, i64, f32,
+                                           i32, i32, vp, vp, i32, vp, sz, vp]
+    lib.aicomp_paged_tree_workspace_bytes.restype = sz
+    lib.aicomp_paged_tree_workspace_bytes.argtypes = [i32, i64] + [i32] * 9
+    lib.aicomp_kv_keep_rows.restype = i32
+    lib.aicomp_kv_keep_rows.argtypes = [vp, i32, i64, i32, i32, i64, vp, i64, i32, vp, vp, vp, i32, i64, vp]
     lib.aicomp_sample_workspace_bytes.restype = sz
     lib.aicomp_sample_workspace_bytes.argtypes = [i32, i32, i64, f32, i32, i32, i32]
 

@@ -165,7 +165,7 @@ using namespace aicomp;
 
 extern "C" {
 
-int aicomp_kv_version(void) { return 400; }
+int aicomp_kv_version(void) { return 500; }
 
 const char* aicomp_kv_last_error(void) { return g_err; }
 

@@ -988,3 +988,291 @@ def copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
         rc = lib.aicomp_kv_copy_blocks((ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools]), len(pools),
                                        first.numel() // nb * first.element_size(), nb, pairs.data_ptr(), n, _stream(first))
     _lib.check(rc, lib)
+
+
+# ------------------------------------------------------------------ latent rows, trees of drafts, accepted rows
+def latent_kv_append(latent: torch.Tensor, weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+                     positions: Optional[torch.Tensor], pool: torch.Tensor, slot_mapping: torch.Tensor, eps: float = 1e-6,
+                     interleaved: bool = False, query: Optional[torch.Tensor] = None, query_out: Optional[torch.Tensor] = None,
+                     rows_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """The cache rows of latent attention: norm the latent part of ``latent [T, C + D]`` (RMS, ``weight [C]`` float32; ``None``: as it
+    is), rotate its last D elements by the tokens' positions, and store the row at ``slot_mapping`` in ``pool
+    [num_blocks, block_size, C + D]``; rotate ``query [T, H, D]`` (the part of the queries that is rotated) too, in one launch.
+
+    ``cos`` / ``sin``: float32 tables ``[P, D/2]`` (``rotary_pair_tables``); pairs are ``(j, j + D/2)``, or neighbours with
+    ``interleaved``.  ``positions [T]`` int64 selects the row of each token (``None``: row t); a token whose position is outside the
+    tables is left alone, one whose slot is outside the pool is not stored.  ``query_out`` (by default ``query`` itself, in place) may
+    be a slice of a wider query tensor; ``rows_out [T, C + D]`` takes the rows a second time, for their expansion
+    (``latent_prompt_attn``).  Computed in float32 and rounded once.  Returns the rotated queries.
+    """
+    out = query if query_out is None else query_out
+    lib = _lib.load()
+    _req(latent.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    _req(pool.dim() == 3 and pool.is_contiguous(), f"pool must be contiguous [num_blocks, block_size, C + D]; got {tuple(pool.shape)}")
+    _req(latent.dim() == 2 and latent.shape[1] == pool.shape[2] and latent.stride(1) == 1,
+         f"latent must be [T, {pool.shape[2]}], rows contiguous; got {tuple(latent.shape)}")
+    T, width = latent.shape
+    _req(cos.shape == sin.shape and cos.dim() == 2 and cos.dtype == torch.float32 and sin.dtype == torch.float32
+         and cos.stride(1) == 1 and cos.stride() == sin.stride(), "cos/sin must be float32 [P, D/2] tables with equal strides")
+    rope = 2 * cos.shape[1]
+    _req(0 < rope < width, f"tables of {cos.shape[1]} columns rotate {rope} elements of a row of {width}")
+    _req(positions is not None or cos.shape[0] >= T, "without positions the tables need one row per token")
+    _req(latent.dtype in (torch.float32, torch.bfloat16, torch.float16) and pool.dtype == latent.dtype,
+         f"latent and pool must share a type of float32, bfloat16, float16; got {latent.dtype} and {pool.dtype}")
+    if weight is not None:
+        _req(weight.dtype == torch.float32 and weight.shape == (width - rope,) and weight.is_contiguous(),
+             f"weight must be contiguous float32 [{width - rope}]")
+        _dev(weight, latent, "weight")
+    if positions is not None:
+        _req(positions.dtype == torch.int64 and positions.shape == (T,) and positions.is_contiguous(),
+             "positions must be contiguous int64 [T]")
+        _dev(positions, latent, "positions")
+    _req(slot_mapping.dtype == torch.int64 and slot_mapping.shape == (T,) and slot_mapping.is_contiguous(),
+         "slot_mapping must be contiguous int64 [T]")
+    heads = 0
+    if query is not None:
+        _req(query.dim() == 3 and query.shape[0] == T and query.shape[2] == rope and out.shape == query.shape
+             and query.dtype == latent.dtype and out.dtype == latent.dtype,
+             f"query/query_out must be [T, H, {rope}] of the rows' type; got {tuple(query.shape)} and {tuple(out.shape)}")
+        _req(query.stride(2) == 1 and out.stride(2) == 1, "query/query_out: last dimension must be contiguous")
+        _dev(query, latent, "query")
+        _dev(out, latent, "query_out")
+        heads = query.shape[1]
+    else:
+        _req(query_out is None, "query_out without a query")
+    if rows_out is not None:
+        _req(rows_out.shape == latent.shape and rows_out.dtype == latent.dtype and rows_out.stride(1) == 1,
+             f"rows_out must be [T, {width}] of the rows' type, rows contiguous")
+        _dev(rows_out, latent, "rows_out")
+    for t, n in ((cos, "cos"), (sin, "sin"), (pool, "pool"), (slot_mapping, "slot_mapping")):
+        _dev(t, latent, n)
+    if T == 0:
+        return out
+    strides = [n for t in (query, out) for n in (_step(t, 0), t.stride(1) if t.shape[1] > 1 else rope)] if heads else [0] * 4
+    with _guard(latent):
+        rc = lib.aicomp_latent_kv_append(
+            latent.data_ptr(), _row_stride(latent), _ptr(weight), float(eps), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0],
+            int(bool(interleaved)), _ptr(positions), query.data_ptr() if heads else None, out.data_ptr() if heads else None, *strides,
+            _ptr(rows_out), 0 if rows_out is None else _row_stride(rows_out), pool.data_ptr(), slot_mapping.data_ptr(), T, heads,
+            width - rope, rope, pool.shape[1], pool.shape[0], _dt(latent, "latent"), _stream(latent))
+    _lib.check(rc, lib)
+    return out
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Stride of the rows; a single row's is its width (what torch keeps there is any number)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _step(t: torch.Tensor, dim: int) -> int:
+    """Stride of a dimension, 0 of one of a single element."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def tree_masks(parents: Sequence[Sequence[int]]):
+    """The masks of trees of drafted tokens for ``paged_tree_attn`` and ``paged_latent_attn``: ``parents[s][b]`` is the draft (below b)
+    that draft b of sequence s follows, or -1 for one that follows the cached tokens; a draft sees its ancestors and itself.  An int64
+    numpy array ``[sum of drafts, words]``, bit b % 64 of word b / 64 for draft b; as many words as the largest tree takes."""
+    import numpy as np
+    words = -(-max([len(p) for p in parents], default=0) // 64) or 1
+    masks = np.zeros((sum(len(p) for p in parents), words), dtype=np.uint64)
+    at = 0
+    for p in parents:
+        for b, q in enumerate(p):
+            if not -1 <= q < b:
+                raise ValueError(f"draft {b} follows draft {q}: a parent comes before its children (-1: none)")
+            if q >= 0:
+                masks[at + b] = masks[at + q]
+            masks[at + b, b // 64] |= np.uint64(1) << np.uint64(b % 64)
+        at += len(p)
+    return masks.view(np.int64)
+
+
+def _rows_checks(out, query, block_table, context_lens, cu_q_lens, masks, max_q_len):
+    """What the paged calls of query rows check alike; the bound of the sequences' rows."""
+    T, S = query.shape[0], context_lens.numel()
+    _req(query.is_contiguous() and out.is_contiguous(), "query and out must be contiguous")
+    _req(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == S
+         and block_table.stride(1) == 1, "block_table must be int32 [S, max_blocks], rows contiguous")
+    _req(context_lens.dtype == torch.int32 and context_lens.is_contiguous(), "context_lens must be contiguous int32 [S]")
+    for t, n in ((out, "out"), (block_table, "block_table"), (context_lens, "context_lens")):
+        _dev(t, query, n)
+    if cu_q_lens is None:
+        _req(S == T, f"{S} context lengths for {T} rows (cu_q_lens divides rows among sequences)")
+        _req(masks is None, "tree_masks need cu_q_lens")
+        return 1
+    _req(cu_q_lens.dtype == torch.int32 and cu_q_lens.numel() == S + 1 and cu_q_lens.is_contiguous(),
+         "cu_q_lens must be contiguous int32 [S+1]")
+    _dev(cu_q_lens, query, "cu_q_lens")
+    if masks is not None:
+        _req(masks.dtype == torch.int64 and masks.dim() == 2 and masks.shape[0] == T and masks.shape[1] > 0 and masks.is_contiguous(),
+             f"tree_masks must be contiguous int64 [{T}, words], one row per row of the query")
+        _dev(masks, query, "tree_masks")
+    if max_q_len is None:
+        cu = cu_q_lens.cpu()
+        max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
+    return _int32(max_q_len, "max_q_len")
+
+
+def paged_latent_attn(out: torch.Tensor, query: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor,
+                      context_lens: torch.Tensor, scale: float, cu_q_lens: Optional[torch.Tensor] = None,
+                      max_q_len: Optional[int] = None, tree_masks: Optional[torch.Tensor] = None,
+                      longest_context: int = 0) -> torch.Tensor:
+    """Attention over paged latent rows, absorbed: ``out[t, h] = softmax(scale q[t, h] . row_j) row_j[:C]``.
+
+    ``query [T, H, C + D]`` (each head's key projection multiplied in already, its rotated part behind), ``out [T, H, C]``, ``pool
+    [num_blocks, block_size, C + D]``.  One token per sequence; or, with ``cu_q_lens [S+1]``, the last tokens of each sequence, causal,
+    or by ``tree_masks [T, words]`` (``tree_masks``) the drafts of a tree over what is cached before them.  A row that sees nothing is
+    zero; rows behind the last sequence are left as they are.  ``max_q_len``: the host's bound of the sequences' tokens (``None``: read
+    back from ``cu_q_lens``); ``longest_context``: its bound of ``context_lens`` (0: the table's width), which sizes the call and cuts
+    no row.  In place on ``out``, on the current stream.
+    """
+    lib = _lib.load()
+    _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    _req(pool.dim() == 3 and pool.is_contiguous(), f"pool must be contiguous [num_blocks, block_size, C + D]; got {tuple(pool.shape)}")
+    _req(query.dim() == 3 and out.dim() == 3 and out.shape[:2] == query.shape[:2] and query.shape[2] == pool.shape[2]
+         and out.shape[2] <= query.shape[2], f"query must be [T, H, {pool.shape[2]}] and out [T, H, C]; got {tuple(query.shape)} "
+         f"and {tuple(out.shape)}")
+    _req(out.dtype == query.dtype and pool.dtype == query.dtype, "query, out and pool must share one type")
+    _dev(pool, query, "pool")
+    max_q_len = _rows_checks(out, query, block_table, context_lens, cu_q_lens, tree_masks, max_q_len)
+    T, H, width = query.shape
+    if T == 0 or max_q_len == 0:
+        return out
+    S, C, bs, dt = context_lens.numel(), out.shape[2], pool.shape[1], _dt(query, "query")
+    longest_context = _int32(longest_context, "longest_context")
+    need = lib.aicomp_paged_latent_workspace_bytes(S, T, max_q_len, H, C, width - C, bs, block_table.shape[1], dt, longest_context)
+    with _guard(query), _scratch_calls:
+        workspace = _call_workspace(query.device, need)
+        rc = lib.aicomp_paged_latent_attn(
+            out.data_ptr(), query.data_ptr(), pool.data_ptr(), block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(),
+            _ptr(cu_q_lens), _ptr(tree_masks), 0 if tree_masks is None else tree_masks.shape[1], S, T, max_q_len, H, C, width - C, bs,
+            block_table.shape[1], pool.shape[0], float(scale), dt, longest_context, _ptr(workspace),
+            0 if workspace is None else workspace.numel(), _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def paged_tree_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                    context_lens: torch.Tensor, cu_q_lens: torch.Tensor, tree_masks: torch.Tensor, scale: float,
+                    max_q_len: Optional[int] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    longest_context: int = 0) -> torch.Tensor:
+    """Attention of trees of drafted tokens ``query [T, Hq, D]`` over the paged pools, which hold their rows already.
+
+    Drafts ``cu_q_lens[s]:cu_q_lens[s+1]`` are the last of the ``context_lens[s]`` tokens of sequence s.  Each sees all tokens before
+    them, and draft b of its sequence if bit b % 64 of word b / 64 of its row of ``tree_masks [T, words]`` (int64; ``tree_masks``) is
+    set.  A row that sees nothing is zero; rows behind the last sequence are left as they are.  ``max_q_len``, ``longest_context`` as
+    in ``paged_latent_attn``.  In place on ``out``, on the current stream.
+    """
+    lib = _lib.load()
+    _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    nb, hkv, bs, d = _check_pools(k_pool, v_pool)
+    _req(query.dim() == 3 and out.shape == query.shape and out.dtype == query.dtype,
+         f"out/query must both be [T, Hq, D]; got {tuple(out.shape)} and {tuple(query.shape)}")
+    T, hq, dq = query.shape
+    _req(dq == d, f"query head_dim {dq} != pool head_dim {d}")
+    _dev(k_pool, query, "k_pool")
+    _req(cu_q_lens is not None and tree_masks is not None, "paged_tree_attn needs cu_q_lens and tree_masks")
+    max_q_len = _rows_checks(out, query, block_table, context_lens, cu_q_lens, tree_masks, max_q_len)
+    ks, vs = _check_scales(k_scale, v_scale, k_pool, hkv)
+    if T == 0 or max_q_len == 0:
+        return out
+    S, qd, kd, longest_context = context_lens.numel(), _dt(query, "query"), _dt(k_pool, "pool"), _int32(longest_context, "longest_context")
+    need = lib.aicomp_paged_tree_workspace_bytes(S, T, max_q_len, hq, hkv, d, bs, block_table.shape[1], qd, kd, longest_context)
+    with _guard(query), _scratch_calls:
+        workspace = _call_workspace(query.device, need)
+        rc = lib.aicomp_paged_tree_attn(
+            out.data_ptr(), query.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            context_lens.data_ptr(), cu_q_lens.data_ptr(), tree_masks.data_ptr(), tree_masks.shape[1], S, T, max_q_len, hq, hkv, d, bs,
+            block_table.shape[1], nb, float(scale), qd, kd, _ptr(ks), _ptr(vs), longest_context, _ptr(workspace),
+            0 if workspace is None else workspace.numel(), _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def latent_prompt_attn(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor, rope_key: torch.Tensor, value: torch.Tensor,
+                       cu_q_lens: torch.Tensor, cu_k_lens: torch.Tensor, scale: float, max_q_len: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of prompts over expanded latent rows: head h's key is ``key[u, h]`` with ``rope_key[u]`` behind it.
+
+    ``query [Tq, H, N + D]``, ``key [Tk, H, N]``, ``rope_key [Tk, D]`` (shared by the heads), ``value [Tk, H, V]``, ``out [Tq, H, V]``;
+    key, value and rope_key may be slices of wider tensors.  Tokens ``cu_q_lens[s]:cu_q_lens[s+1]`` are the last of the keys
+    ``cu_k_lens[s]:cu_k_lens[s+1]`` of sequence s; one with fewer keys than queries gets zero rows, and rows behind the last sequence are
+    left as they are.  ``max_q_len``: the host's bound of the sequences' queries (``None``: read back).  In place on ``out``, on the
+    current stream.
+    """
+    lib = _lib.load()
+    _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    _req(query.dim() == 3 and out.dim() == 3 and key.dim() == 3 and value.dim() == 3 and rope_key.dim() == 2,
+         "query/out/key/value must be [T, H, elements] and rope_key [T, elements]")
+    Tq, H, width = query.shape
+    Tk, N, D, V = key.shape[0], key.shape[2], rope_key.shape[1], value.shape[2]
+    _req(key.shape == (Tk, H, N) and value.shape == (Tk, H, V) and rope_key.shape[0] == Tk and N + D == width and out.shape == (Tq, H, V),
+         f"query {tuple(query.shape)}, key {tuple(key.shape)}, rope_key {tuple(rope_key.shape)}, value {tuple(value.shape)} and out "
+         f"{tuple(out.shape)} do not match")
+    _req(query.is_contiguous() and out.is_contiguous(), "query and out must be contiguous")
+    for t, n in ((out, "out"), (key, "key"), (rope_key, "rope_key"), (value, "value")):
+        _req(t.dtype == query.dtype and t.stride(-1) == 1, f"{n} must be of {query.dtype}, its last dimension contiguous")
+        _dev(t, query, n)
+    S = cu_q_lens.numel() - 1
+    for t, n in ((cu_q_lens, "cu_q_lens"), (cu_k_lens, "cu_k_lens")):
+        _req(t.dtype == torch.int32 and t.dim() == 1 and t.numel() == S + 1 and S >= 0 and t.is_contiguous(),
+             f"{n} must be contiguous int32 [S+1]")
+        _dev(t, query, n)
+    if max_q_len is None:
+        cu = cu_q_lens.cpu()
+        max_q_len = int((cu[1:] - cu[:-1]).max()) if S else 0
+    max_q_len = _int32(max_q_len, "max_q_len")
+    if Tq == 0 or S == 0 or max_q_len == 0:
+        return out
+    with _guard(query):
+        rc = lib.aicomp_latent_prompt_attn(
+            out.data_ptr(), query.data_ptr(), key.data_ptr(), _step(key, 0), _step(key, 1), rope_key.data_ptr(), _step(rope_key, 0),
+            value.data_ptr(), _step(value, 0), _step(value, 1), cu_q_lens.data_ptr(), cu_k_lens.data_ptr(), S, Tq, Tk, max_q_len, H, N, D,
+            V, float(scale), _dt(query, "query"), _stream(query))
+    _lib.check(rc, lib)
+    return out
+
+
+def keep_rows(pools: Sequence[torch.Tensor], block_table: torch.Tensor, first: torch.Tensor, keep: torch.Tensor,
+              cu_keep: torch.Tensor) -> None:
+    """The cache rows of accepted drafts moved together: in every pool, the row of token ``first[s] + keep[i]`` of sequence s becomes
+    that of token ``first[s] + i`` for the i-th entry ``keep[cu_keep[s]:cu_keep[s+1]]``, in one launch on the current stream.
+
+    ``pools``: the K and V pools ``[num_blocks, Hkv, block_size, D]`` of all layers, or pools of latent rows
+    ``[num_blocks, block_size, C + D]``, alike in shape and type.  ``block_table [S, max_blocks]`` int32 on the device; ``first [S]``,
+    ``keep [n]`` and ``cu_keep [S+1]`` int32: on the host they are checked (``keep`` ascends from 0 or more in every sequence) and copied,
+    on the device they are taken as they are.  Tokens beyond the table, or in blocks outside the pools, are left alone.
+    """
+    lib = _lib.load()
+    _req(len(pools) > 0, "keep_rows needs at least one pool")
+    p = pools[0]
+    _req(p.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
+    for t in pools:
+        _req(t.shape == p.shape and t.dtype == p.dtype and t.dim() in (3, 4) and t.is_contiguous(),
+             "pools must be contiguous [num_blocks, Hkv, block_size, D] or [num_blocks, block_size, C + D], alike in shape and type")
+        _dev(t, p, "a pool")
+    S, n = first.numel(), keep.numel()
+    _req(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == S and block_table.stride(1) == 1,
+         "block_table must be int32 [S, max_blocks], rows contiguous")
+    for t, name, size in ((first, "first", S), (keep, "keep", n), (cu_keep, "cu_keep", S + 1)):
+        _req(t.dtype == torch.int32 and t.shape == (size,) and t.is_contiguous(), f"{name} must be contiguous int32 [{size}]")
+    _dev(block_table, p, "block_table")
+    _req(first.device == keep.device == cu_keep.device, "first, keep and cu_keep must be on one device")
+    if not first.is_cuda:
+        _req(bool((first >= 0).all()), "first must not be negative")
+        _req(int(cu_keep[0]) == 0 and int(cu_keep[-1]) == n and bool((cu_keep[1:] >= cu_keep[:-1]).all()),
+             f"cu_keep must be prefix sums from 0 to {n}")
+        starts = torch.zeros(n + 1, dtype=torch.bool)
+        starts[cu_keep.long()] = True
+        _req(bool((keep >= 0).all()) and bool(((keep[1:] > keep[:-1]) | starts[1:n]).all()),
+             "keep must ascend from 0 or more in every sequence")
+        first, keep, cu_keep = (t.to(p.device) for t in (first, keep, cu_keep))
+    _dev(first, p, "first, keep and cu_keep")
+    if n == 0 or p.numel() == 0 or block_table.shape[1] == 0:
+        return
+    with _guard(p):
+        rc = lib.aicomp_kv_keep_rows(
+            (ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools]), len(pools), p.shape[-1] * p.element_size(),
+            p.shape[1] if p.dim() == 4 else 1, p.shape[-2], p.shape[0], block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], first.data_ptr(), keep.data_ptr(), cu_keep.data_ptr(), S, n, _stream(p))
+    _lib.check(rc, lib)

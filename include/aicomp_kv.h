@@ -46,7 +46,9 @@ extern "C" {
 #define AICOMP_KV_FP8_E4M3  2       /* OCP e4m3 ("e4m3fn"), max finite 448       */
 #define AICOMP_KV_F16       3       /* IEEE binary16                             */
 
-/* Library version (major*10000 + minor*100 + patch).  400 = 0.4.0: added aicomp_qk_norm_rope_kv_append,
+/* Library version (major*10000 + minor*100 + patch).  500 = 0.5.0: added aicomp_latent_kv_append,
+ * aicomp_paged_latent_attn, aicomp_paged_latent_workspace_bytes, aicomp_latent_prompt_attn, aicomp_paged_tree_attn,
+ * aicomp_paged_tree_workspace_bytes and aicomp_kv_keep_rows.  400 = 0.4.0: added aicomp_qk_norm_rope_kv_append,
  * aicomp_paged_score_attn, aicomp_paged_score_workspace_bytes and aicomp_kv_copy_blocks.  302 = 0.3.2: added
  * aicomp_rope_paged_decode_attn_sized and aicomp_kv_append_prefill_attn_sized.  301 = 0.3.1: added
  * aicomp_rope_paged_decode_attn and aicomp_kv_append_prefill_attn.  300 = 0.3.0: added
@@ -552,6 +554,119 @@ size_t aicomp_paged_score_workspace_bytes(int num_seqs, int64_t total_q, int max
  */
 int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes, int64_t num_blocks,
                           const int64_t* pairs, int64_t num_pairs, void* stream);
+
+/*
+ * Latent attention: all heads of a token share one cache row of latent_dim + rope_dim elements, in one pool
+ * [num_blocks, block_size, latent_dim + rope_dim] of the tensors' type.  This call makes and stores the rows, and rotates the queries'
+ * part that the rotation concerns:
+ *   row = [ c / sqrt(mean(c^2) + eps) * weight | rotated(k) ],   latent = [ c | k ],   q_out = rotated(q_in)
+ *
+ *   latent          [T, latent_dim + rope_dim], row t at t*latent_stride
+ *   weight          [latent_dim] float; NULL: c is stored as it is
+ *   cos, sin        float tables, row r at r*table_stride, rope_dim / 2 columns: one angle per pair
+ *   interleaved     0: pairs (j, j + rope_dim / 2);  otherwise (2j, 2j + 1)
+ *   positions       [T] int64 table row of each token, or NULL: row t; a token whose position is outside is left alone
+ *   q_in, q_out     [T, num_heads, rope_dim], element (t,h,d) at t*token_stride + h*head_stride + d; q_out may be q_in; both NULL: none
+ *   rows_out        the rows once more, row t at t*rows_stride; NULL: not wanted
+ *   slot_mapping    [T] int64 as in aicomp_kv_append (a row outside the pool is not stored; queries and rows_out are written)
+ * Computed in float32 and rounded once.  F32, BF16, F16; latent_dim (at most 1024) and rope_dim multiples of 16; pointers and strides
+ * 16-byte aligned.
+ */
+int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const float* weight, float eps,
+                            const float* cos, const float* sin, int64_t table_stride, int64_t table_rows,
+                            int interleaved, const int64_t* positions,
+                            const void* q_in, void* q_out, int64_t q_token_stride, int64_t q_head_stride,
+                            int64_t qo_token_stride, int64_t qo_head_stride,
+                            void* rows_out, int64_t rows_stride, void* pool, const int64_t* slot_mapping,
+                            int64_t num_tokens, int num_heads, int latent_dim, int rope_dim,
+                            int block_size, int64_t num_blocks, int dtype, void* stream);
+
+/*
+ * Attention over the paged latent rows, absorbed form: a query holds its head's key projection already, so that a row is the key
+ * of every head and its first latent_dim elements are the value.
+ *   s = scale * (q . row_j)  over latent_dim + rope_dim elements;   out = softmax(s) row_j[0 .. latent_dim)
+ *
+ *   out             [T, num_heads, latent_dim];  query [T, num_heads, latent_dim + rope_dim]; contiguous
+ *   context_lens, block_table   as in aicomp_paged_decode_attn (cu_q_lens NULL: one token per sequence, total_q == num_seqs) or
+ *                   aicomp_paged_prefill_attn (tokens of sequence s are cu_q_lens[s] .. cu_q_lens[s+1], its last ones, at most
+ *                   max_q_len; rows behind the last sequence are left as they are)
+ *   tree_masks      NULL: causal.  [T, mask_words] int64: the tokens of a sequence in this call are drafts of a tree; a token sees what
+ *                   was cached before them, and draft b of its sequence if bit b % 64 of its word b / 64 is set
+ *   longest_context what the caller knows of context_lens (0: nothing); it sizes the call and bounds nothing
+ *   workspace       aicomp_paged_latent_workspace_bytes(...) bytes (max_q_len 1 without cu_q_lens), 16-byte aligned, needing no
+ *                   initialisation; may be NULL where that is 0.  Calls that may overlap need separate ones
+ * A row that sees nothing is zero, as are the rows of a sequence whose context is shorter than its tokens here.  Keys that a row does
+ * not see may hold anything; a row that sees an element that is not finite may be not a number as a whole.
+ * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16.  Matrix cores: 16 bits, 512 + 64, blocks of 16.
+ */
+int aicomp_paged_latent_attn(void* out, const void* query, const void* pool,
+                             const int32_t* block_table, int64_t block_table_stride,
+                             const int32_t* context_lens, const int32_t* cu_q_lens,
+                             const int64_t* tree_masks, int mask_words,
+                             int num_seqs, int64_t total_q, int max_q_len,
+                             int num_heads, int latent_dim, int rope_dim,
+                             int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                             float scale, int dtype, int longest_context,
+                             void* workspace, size_t workspace_bytes, void* stream);
+size_t aicomp_paged_latent_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_heads, int latent_dim, int rope_dim,
+                                           int block_size, int max_blocks_per_seq, int dtype, int longest_context);
+
+/*
+ * Causal attention of prompts over expanded latent rows: keys and values that a projection made of them, dense.
+ *   s = scale * (q[0 .. nope_dim) . key_j + q[nope_dim ..) . rope_key_j);   out = softmax(s) value_j
+ *
+ *   out             [total_q, num_heads, value_dim];  query [total_q, num_heads, nope_dim + rope_dim]; contiguous
+ *   key, value      [total_k, num_heads, nope_dim / value_dim], element (u,h,d) at u*token_stride + h*head_stride + d (both may be
+ *                   slices of one projection);  rope_key [total_k, rope_dim], row u at u*rope_token_stride, shared by the heads
+ *   cu_q_lens, cu_k_lens   [num_seqs+1] int32: tokens of sequence s are rows cu_q_lens[s] .. of the queries and cu_k_lens[s] .. of
+ *                   the keys, the queries the last of its keys; one with fewer keys than queries gets zero rows, rows behind the last
+ *                   sequence are left as they are
+ *   max_q_len       bound of the sequences' queries
+ * F32, BF16, F16; dims multiples of 16.  Matrix cores: 16 bits, 128 + 64 and 128.  Pointers and strides 16-byte aligned.
+ */
+int aicomp_latent_prompt_attn(void* out, const void* query,
+                              const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                              const void* rope_key, int64_t rope_token_stride,
+                              const void* value, int64_t value_token_stride, int64_t value_head_stride,
+                              const int32_t* cu_q_lens, const int32_t* cu_k_lens, int num_seqs,
+                              int64_t total_q, int64_t total_k, int max_q_len,
+                              int num_heads, int nope_dim, int rope_dim, int value_dim,
+                              float scale, int dtype, void* stream);
+
+/*
+ * Attention of trees of drafted tokens over the paged pools: the tokens of sequence s in this call, whose K/V rows are in the pools
+ * already, see what was cached before them, and each other by tree_masks (as in aicomp_paged_latent_attn).
+ *   out, query, pools, block_table, context_lens, cu_q_lens, scales   as in aicomp_paged_prefill_attn
+ *   longest_context, workspace   as in aicomp_paged_latent_attn, with aicomp_paged_tree_workspace_bytes
+ * head_dim 64, 128 or 256; any block size; f32/f32, bf16/bf16, f16/f16, bf16/fp8, f16/fp8 (query / pool); pointers 16-byte aligned.
+ */
+int aicomp_paged_tree_attn(void* out, const void* query, const void* k_pool, const void* v_pool,
+                           const int32_t* block_table, int64_t block_table_stride,
+                           const int32_t* context_lens, const int32_t* cu_q_lens,
+                           const int64_t* tree_masks, int mask_words,
+                           int num_seqs, int64_t total_q, int max_q_len,
+                           int num_q_heads, int num_kv_heads, int head_dim,
+                           int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                           float scale, int q_dtype, int kv_dtype,
+                           const float* k_scale, const float* v_scale, int longest_context,
+                           void* workspace, size_t workspace_bytes, void* stream);
+size_t aicomp_paged_tree_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                                         int block_size, int max_blocks_per_seq, int q_dtype, int kv_dtype, int longest_context);
+
+/*
+ * What is left of a tree of drafts once some are accepted: in every pool, the row of token first[s] + keep[i] of sequence s becomes that
+ * of token first[s] + i, for i-th entry of cu_keep[s] .. cu_keep[s+1], in one launch (per 128 pools).
+ *   pools           HOST array of num_pools device pointers, pools [num_blocks, num_kv_heads, block_size, row] of row_bytes per row
+ *                   (a pool of latent rows: num_kv_heads 1)
+ *   first           [num_seqs] int32: the position of each tree's first draft
+ *   keep, cu_keep   [total_keep] int32, strictly ascending from 0 or more within a sequence; [num_seqs+1] int32 prefix sums
+ * A token beyond the table, or whose table entry is outside the pool, is neither read nor written.  No block of the pools may be
+ * in two sequences between first and the last token kept.
+ */
+int aicomp_kv_keep_rows(void* const* pools, int num_pools, int64_t row_bytes, int num_kv_heads, int block_size, int64_t num_blocks,
+                        const int32_t* block_table, int64_t block_table_stride, int max_blocks_per_seq,
+                        const int32_t* first, const int32_t* keep, const int32_t* cu_keep,
+                        int num_seqs, int64_t total_keep, void* stream);
 
 #ifdef __cplusplus
 }
