@@ -30,6 +30,24 @@ static int check_rows(const RowAttnArgs& a, const char* who) {
     return AICOMP_KV_OK;
 }
 
+// The call of checked arguments.
+static int attend(const RowAttnArgs& a, size_t workspace_bytes, const char* who) {
+    if (!row_attn_mfma_supported(a)) return launch_rows_generic(a);
+    const size_t need = row_attn_mfma_workspace_bytes(a);
+    AICOMP_REQUIRE(need == 0 || (a.workspace && workspace_bytes >= need), AICOMP_KV_EWORKSPACE,
+                   "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace ? workspace_bytes : (size_t)0);
+    AICOMP_REQUIRE(need == 0 || (uintptr_t)a.workspace % 16 == 0, AICOMP_KV_EINVAL, "%s: workspace must be 16-byte aligned", who);
+    return launch_row_attn_mfma(a);
+}
+
+// The sizes of a call, for its workspace: 0 for what the call refuses.
+static size_t workspace_of(const RowAttnArgs& a) {
+    if (a.num_seqs <= 0 || a.rows <= 0 || a.max_q_len <= 0 || a.max_q_len > a.rows || a.hq <= 0 || a.hkv <= 0 || a.hq % a.hkv ||
+        a.bs <= 0 || a.max_blocks <= 0 || a.longest_context < 0 || !row_attn_mfma_supported(a))
+        return 0;
+    return row_attn_mfma_workspace_bytes(a);
+}
+
 extern "C" {
 
 int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const float* weight, float eps, const float* cos, const float* sin,
@@ -71,7 +89,12 @@ int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const flo
 
 size_t aicomp_paged_latent_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_heads, int latent_dim, int rope_dim,
                                            int block_size, int max_blocks_per_seq, int dtype, int longest_context) {
-    return 0;
+    RowAttnArgs a;
+    memset(&a, 0, sizeof(a));
+    a.num_seqs = num_seqs; a.rows = total_q; a.max_q_len = max_q_len; a.hq = num_heads; a.hkv = 1; a.dk = latent_dim + rope_dim;
+    a.dv = latent_dim; a.v_row = a.dk; a.bs = block_size; a.max_blocks = max_blocks_per_seq; a.q_dtype = a.kv_dtype = dtype;
+    a.longest_context = longest_context;
+    return workspace_of(a);
 }
 
 int aicomp_paged_latent_attn(void* out, const void* query, const void* pool, const int32_t* block_table, int64_t block_table_stride,
@@ -95,12 +118,17 @@ int aicomp_paged_latent_attn(void* out, const void* query, const void* pool, con
     a.kv_dtype = dtype; a.longest_context = longest_context; a.workspace = workspace; a.stream = (hipStream_t)stream;
     const int rc = check_rows(a, who);
     if (rc) return rc;
-    return launch_rows_generic(a);
+    return attend(a, workspace_bytes, who);
 }
 
 size_t aicomp_paged_tree_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
                                          int block_size, int max_blocks_per_seq, int q_dtype, int kv_dtype, int longest_context) {
-    return 0;
+    RowAttnArgs a;
+    memset(&a, 0, sizeof(a));
+    a.num_seqs = num_seqs; a.rows = total_q; a.max_q_len = max_q_len; a.hq = num_q_heads; a.hkv = num_kv_heads;
+    a.dk = a.dv = a.v_row = head_dim; a.bs = block_size; a.max_blocks = max_blocks_per_seq; a.q_dtype = q_dtype; a.kv_dtype = kv_dtype;
+    a.longest_context = longest_context;
+    return workspace_of(a);
 }
 
 int aicomp_paged_tree_attn(void* out, const void* query, const void* k_pool, const void* v_pool, const int32_t* block_table,
@@ -132,7 +160,7 @@ int aicomp_paged_tree_attn(void* out, const void* query, const void* k_pool, con
     a.longest_context = longest_context; a.workspace = workspace; a.stream = (hipStream_t)stream;
     const int rc = check_rows(a, who);
     if (rc) return rc;
-    return launch_rows_generic(a);
+    return attend(a, workspace_bytes, who);
 }
 
 int aicomp_latent_prompt_attn(void* out, const void* query, const void* key, int64_t key_token_stride, int64_t key_head_stride,

@@ -58,6 +58,9 @@ struct PromptAttnArgs {
 };
 
 int launch_rows_generic(const RowAttnArgs& a);
+bool row_attn_mfma_supported(const RowAttnArgs& a);
+size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a);
+int launch_row_attn_mfma(const RowAttnArgs& a);
 int launch_prompt_generic(const PromptAttnArgs& a);
 
 struct LatentAppendArgs {

@@ -1,0 +1,558 @@
+// Attention of query rows over cached rows (row_attn.h) on the matrix cores: latent rows of 512 + 64 elements, trees of drafts over K and
+// V pools of head_dim 64, 128 and 256; 16-bit rows, and fp8 ones under them; blocks of 16 tokens.
+//
+// The rows of a sequence and KV head, (token, head) pairs one after the other, are cut into tiles of 16 R rows, and the keys into
+// tiles of 32.  A workgroup has a row tile; its four waves take the key tiles in turn, each with its own piece of LDS, its own running
+// reference m, sum l and output O, and nothing to wait for but its own loads:
+//   S^T = K Q^T      16 x 16 x 32 products; a lane then has four keys of a row per 16, the order in which
+//   O^T += V^T P^T   takes its weights from registers, V^T out of LDS by transposing reads
+// The reference moves when a score passes it by 2^8, so most tiles leave O as it is.  Rows of a tile are swizzled in 16-byte chunks
+// (chunk c of key k at c ^ f(k)), so that both reads spread over the banks.  Tiles come from the pool straight into LDS.
+//
+// Work is divided evenly: all (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of
+// equal length, whatever the sequences' lengths are.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by
+// it; of others it leaves (m, l, O) in the workspace, and a second kernel joins them.
+#include "row_attn.h"
+
+#include <algorithm>
+
+namespace aicomp {
+
+namespace {
+
+constexpr int BS = 16;                 // tokens per block
+constexpr int KT = 32;                 // keys per tile
+constexpr float NEG_BIG = -1.0e30f;
+constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both formats' range
+
+#define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
+#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+
+struct RowParams {
+    void* out;
+    const void* query;
+    const void* k_pool;
+    const void* v_pool;
+    const int32_t* block_table;
+    int64_t block_table_stride;
+    const int32_t* context_lens;
+    const int32_t* cu_q_lens;
+    const int64_t* masks;
+    int mask_words;
+    int num_seqs;
+    int rows, max_q_len;
+    int hq, hkv, group, max_blocks, num_blocks;
+    float mul;                         // scale * log2(e)
+    const float* k_scale;
+    const float* v_scale;
+    int workers;                       // workgroups
+    int least;                         // key tiles that a workgroup has at least
+    int row_tiles;                     // of the longest sequence (the join's grid)
+    float* ws_acc;                     // [2 workers][16 R][DV]
+    float2* ws_ml;                     // [2 workers][16 R]
+};
+
+// A sequence as the line of work sees it.
+struct Seq {
+    int begin, n, ctx, prior;          // ctx: 0 where its tokens are more than its context
+    int row_tiles, key_tiles;
+    __device__ __forceinline__ int64_t items(const RowParams& p) const { return (int64_t)p.hkv * row_tiles; }
+};
+
+template <int ROWS> __device__ __forceinline__ Seq load_seq(const RowParams& p, int s) {
+    Seq q;
+    q.begin = p.cu_q_lens ? max(0, p.cu_q_lens[s]) : s;
+    q.n = p.cu_q_lens ? min(min(p.cu_q_lens[s + 1], p.rows) - q.begin, p.max_q_len) : 1;
+    q.n = max(0, q.n);
+    q.ctx = min(p.context_lens[s], p.max_blocks * BS);
+    q.prior = q.ctx - q.n;
+    if (q.prior < 0) q.ctx = 0;
+    q.row_tiles = (q.n * p.group + ROWS - 1) / ROWS;
+    q.key_tiles = max(1, (q.ctx + KT - 1) / KT);
+    return q;
+}
+
+// The line's length, over all threads of the workgroup; `mine`: the part of it before this thread's sequences, first .. last - 1.
+template <int ROWS> __device__ __forceinline__ int64_t line_of(const RowParams& p, int64_t* sums, int& first, int& last, int64_t& mine) {
+    const int per = (p.num_seqs + 255) / 256, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    first = min((int)threadIdx.x * per, p.num_seqs);
+    last = min(first + per, p.num_seqs);
+    int64_t own = 0;
+    for (int s = first; s < last; ++s) {
+        const Seq q = load_seq<ROWS>(p, s);
+        own += q.items(p) * q.key_tiles;
+    }
+    int64_t up = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up((long long)up, o);
+        if (lane >= o) up += x;
+    }
+    if (lane == 63) sums[w] = up;
+    __syncthreads();
+    mine = up - own;
+    for (int i = 0; i < w; ++i) mine += sums[i];
+    return sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+__device__ __forceinline__ int64_t piece_of(const RowParams& p, int64_t line) {
+    return max((int64_t)p.least, (line + p.workers - 1) / p.workers);
+}
+
+// Which of the 32 keys from `start` on a row sees.  Causal: those below `limit`; else by its mask words from key `prior` on.
+__device__ __forceinline__ uint32_t window_of(const int64_t* words, int num_words, int start, int prior, int ctx, int limit) {
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+    if (words == nullptr) return below(limit - start);
+    const int o = start - prior;                                   // bit of the first key
+    auto bits = [&](int from) -> uint32_t {                        // from >= 0
+        const int k = from >> 6, b = from & 63;
+        const uint64_t lo = k < num_words ? (uint64_t)words[k] : 0, hi = b > 32 && k + 1 < num_words ? (uint64_t)words[k + 1] : 0;
+        return (uint32_t)(lo >> b | (b > 32 ? hi << (64 - b) : 0));
+    };
+    const uint32_t w = o >= 0 ? bits(o) : o <= -32 ? ~0u : bits(0) << -o | below(-o);
+    return w & below(ctx - start);
+}
+
+// E: 16-bit format of queries and output; DK / DV: elements of a key / value row; R: groups of 16 rows; LATENT: a value is the
+// first part of its key's row.  OCC: workgroups per CU.
+template <typename E, bool FP8, int DK, int DV, bool LATENT, int R, int OCC>
+__global__ void __launch_bounds__(256, OCC)
+row_attn_kernel(RowParams p) {
+    constexpr int ROWS = 16 * R;
+    constexpr int KROW = 2 * DK, VROW = LATENT ? KROW : 2 * DV;    // bytes of a row in LDS
+    constexpr int NS = DK / 32, NJ = DV / 16;
+    constexpr int TILE = KT * KROW + (LATENT ? 0 : KT * VROW);     // bytes per wave
+    constexpr int VBASE = LATENT ? 0 : KT * KROW;
+    constexpr int CH = LATENT ? 128 : DV / R;                      // columns that the waves' outputs are joined by at a time
+    constexpr int PER8 = KROW / 128;                               // 1 KB loads per 8 keys
+    constexpr bool WIDE = !LATENT && DV >= 128;                    // V rows of whole bank lines
+    constexpr int NVA = WIDE ? 8 : 4;                              // V addresses that are no immediates of each other
+    static_assert(4 * ROWS * (CH + 4) * 4 <= 4 * TILE, "the join takes the tiles' place");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * TILE];
+    __shared__ int64_t sums[4];
+    __shared__ int64_t start_off;
+    __shared__ int start_seq;
+    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g4 = lane >> 4;
+    // neighbours on the line, which share keys, on one XCD (workgroups go to the eight in turn)
+    const int worker = (p.workers & 7) ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (p.workers >> 3) + ((int)blockIdx.x >> 3);
+
+    int first, last;
+    int64_t mine;
+    const int64_t line = line_of<ROWS>(p, sums, first, last, mine), piece = piece_of(p, line);
+    int64_t at = worker * piece;
+    const int64_t end = min(line, at + piece);
+    if (at >= end) return;
+    for (int s = first; s < last; ++s) {
+        const Seq q = load_seq<ROWS>(p, s);
+        const int64_t all = q.items(p) * q.key_tiles;
+        if (at >= mine && at < mine + all) { start_seq = s; start_off = at - mine; }
+        mine += all;
+    }
+    __syncthreads();
+    int seq = __builtin_amdgcn_readfirstlane(start_seq);
+    int64_t off = start_off;
+
+    auto fk = [](int key) { return key & 7; };
+    auto fv = [](int key) { return LATENT ? key & 7 : WIDE ? 2 * (key & 7) : key & 6; };
+    unsigned char* const tile = lds + w * TILE;
+    // reads of a tile: chunk 4 s + g4 of key r16; column chunk 2 j + h of the keys 4 g4 + (r16 / 4)
+    uint32_t ka[2], va[NVA];
+    const int vkey = 4 * g4 + (r16 >> 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ka[i] = r16 * KROW + (((4 * i + g4) ^ fk(r16)) << 4);
+#pragma unroll
+    for (int i = 0; i < NVA; ++i) va[i] = VBASE + vkey * VROW + (((2 * i + ((r16 >> 1) & 1)) ^ fv(vkey)) << 4) + (r16 & 1) * 8;
+    // loads of a tile: lane's 16 bytes of each 1 KB of eight keys
+    uint32_t offk[FP8 ? 1 : PER8], offv[FP8 || LATENT ? 1 : PER8];
+    if constexpr (!FP8) {
+#pragma unroll
+        for (int m = 0; m < PER8; ++m) {
+            const int chunk = 64 * m + lane, key = chunk / (KROW / 16), slot = chunk % (KROW / 16);
+            offk[m] = key * KROW + ((slot ^ fk(key)) << 4);
+            if constexpr (!LATENT) offv[m] = key * KROW + ((slot ^ fv(key)) << 4);
+        }
+    }
+    constexpr int PARTS = DK / 16, KPL = 64 / PARTS, NLD = KT / KPL;       // fp8: 16 codes to a lane, keys per load
+    uint4 sk[FP8 ? NLD : 1], sv[FP8 ? NLD : 1];
+
+    while (at < end) {
+        Seq q = load_seq<ROWS>(p, seq);
+        const int64_t all = q.items(p) * q.key_tiles;
+        if (off >= all) { off = 0; ++seq; continue; }                      // (a sequence without tokens, or the next one)
+        const int item = (int)(off / q.key_tiles), t0 = (int)(off - (int64_t)item * q.key_tiles);
+        const int t1 = (int)min((int64_t)q.key_tiles, t0 + (end - at));
+        const int kvh = item / q.row_tiles, rtile = item - kvh * q.row_tiles;
+        const int nrows = q.n * p.group;
+
+        // rows of this lane's columns (beyond the last: that one, computed and not stored)
+        uint4 qf[R][NS];
+        int limit[R];
+        const int64_t* words[R];
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            const int row = min(rtile * ROWS + 16 * c + r16, nrows - 1), i = row / p.group;
+            limit[c] = q.prior + i + 1;
+            words[c] = p.masks ? p.masks + (int64_t)(q.begin + i) * p.mask_words : nullptr;
+            const uint16_t* src = (const uint16_t*)p.query + ((int64_t)(q.begin + i) * p.hq + kvh * p.group + row % p.group) * DK;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) qf[c][s] = *(const uint4*)(src + 32 * s + 8 * g4);
+        }
+        // keys that all rows here see, and that some may
+        const int i_first = rtile * ROWS / p.group, i_last = (min(rtile * ROWS + ROWS, nrows) - 1) / p.group;
+        const int full = p.masks ? q.prior : q.prior + i_first + 1;
+        const int some = q.ctx == 0 ? 0 : p.masks ? q.ctx : q.prior + i_last + 1;
+        const float mul = p.mul * (FP8 ? p.k_scale[kvh] : 1.f);
+
+        float m[R], l[R];
+        f32x4_t O[R][NJ];
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            m[c] = NEG_BIG; l[c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) O[c][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
+        typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
+        const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)seq * p.block_table_stride);
+        const int last_block = (q.ctx - 1) / BS;                           // (blocks behind it are not this sequence's)
+        auto block_base = [&](int t, int half) -> int64_t {                // element index of the block's first row
+            const int b = table[min(2 * t + half, last_block)];
+            return ((int64_t)max(0, min(b, p.num_blocks - 1)) * p.hkv + kvh) * (BS * DK);
+        };
+        auto fetch_dma = [&](int t) __attribute__((always_inline)) {
+            if constexpr (!FP8) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int64_t base = block_base(t, half) * 2;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const char* kp = (const char*)p.k_pool + base + g * 8 * KROW;
+                        const char* vp = (const char*)p.v_pool + base + g * 8 * KROW;
+                        unsigned char* to = tile + (2 * half + g) * 8 * KROW;
+#pragma unroll
+                        for (int m_ = 0; m_ < PER8; ++m_) {
+                            __builtin_amdgcn_global_load_lds(GLOBAL_PTR(kp + offk[m_]), LDS_PTR(to + 1024 * m_), 16, 0, 0);
+                            if constexpr (!LATENT)
+                                __builtin_amdgcn_global_load_lds(GLOBAL_PTR(vp + offv[m_]), LDS_PTR(to + VBASE + 1024 * m_), 16, 0, 0);
+                        }
+                    }
+                }
+            }
+        };
+        auto fetch = [&](int t) __attribute__((always_inline)) {
+            if constexpr (FP8) {
+#pragma unroll
+                for (int i = 0; i < NLD; ++i) {
+                    const int64_t from = block_base(t, KPL * i / BS) + (KPL * i % BS) * DK;
+                    sk[i] = *(const uint4*)((const char*)p.k_pool + from + lane * 16);
+                    sv[i] = *(const uint4*)((const char*)p.v_pool + from + lane * 16);
+                }
+            }
+        };
+        auto stash = [&]() __attribute__((always_inline)) {
+            if constexpr (FP8) {
+#pragma unroll
+                for (int i = 0; i < NLD; ++i) {
+                    const int key = KPL * i + lane / PARTS, c = 2 * (lane % PARTS);
+                    *(uint4*)(tile + key * KROW + ((c ^ fk(key)) << 4)) = E::from_fp8(make_uint2(sk[i].x, sk[i].y));
+                    *(uint4*)(tile + key * KROW + (((c + 1) ^ fk(key)) << 4)) = E::from_fp8(make_uint2(sk[i].z, sk[i].w));
+                    *(uint4*)(tile + VBASE + key * VROW + ((c ^ fv(key)) << 4)) = E::from_fp8(make_uint2(sv[i].x, sv[i].y));
+                    *(uint4*)(tile + VBASE + key * VROW + (((c + 1) ^ fv(key)) << 4)) = E::from_fp8(make_uint2(sv[i].z, sv[i].w));
+                }
+            }
+        };
+
+        int t = t0 + w;
+        const int t_end = min(t1, (some + KT - 1) / KT);
+        if (FP8 && t < t_end) fetch(t);
+        for (; t < t_end; t += 4) {
+            if constexpr (FP8) {
+                stash();
+                if (t + 4 < t_end) fetch(t + 4);
+            } else {
+                __builtin_amdgcn_s_waitcnt(0xC07F);                        // lgkmcnt(0): the tile before has been read
+                fetch_dma(t);
+                __builtin_amdgcn_s_waitcnt(0x0F70);                        // vmcnt(0)
+                asm volatile("" ::: "memory");
+            }
+            const int start = t * KT;
+            const bool masked = start + KT > full;                         // wave-uniform
+            uint64_t bad = 0;                                              // bits 2 k, 2 k + 1: key k's value is not finite
+            if (masked) {
+                // A weight of 0 times a value that is not finite is not 0: such a value becomes 0, and the score of its key not a
+                // number for the rows that see it.  Two lanes to a key.
+                constexpr uint32_t EXP = E::DT == AICOMP_KV_F16 ? 0x7c007c00u : 0x7f807f80u;
+                constexpr uint32_t ONE = E::DT == AICOMP_KV_F16 ? 0x04000400u : 0x00800080u;
+                unsigned char* const mine_v = tile + VBASE + (lane >> 1) * VROW + (lane & 1) * DV;
+                uint32_t acc = 0;
+#pragma unroll 4
+                for (int i = 0; i < DV / 16; ++i) {
+                    const uint4 x = *(const uint4*)(mine_v + 16 * i);
+                    acc |= ((x.x & EXP) + ONE) | ((x.y & EXP) + ONE) | ((x.z & EXP) + ONE) | ((x.w & EXP) + ONE);
+                }
+                bad = __ballot((acc & 0x80008000u) != 0);
+                if (bad && ((bad >> (lane & ~1)) & 3)) {
+                    for (int i = 0; i < DV / 16; ++i) *(uint4*)(mine_v + 16 * i) = make_uint4(0, 0, 0, 0);
+                }
+            }
+
+            f32x4_t sa[2][R];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int c = 0; c < R; ++c) sa[a][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const uint4 a0 = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128);
+                const uint4 a1 = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128 + 16 * KROW);
+#pragma unroll
+                for (int c = 0; c < R; ++c) {
+                    sa[0][c] = E::mfma(a0, qf[c][s], sa[0][c]);
+                    sa[1][c] = E::mfma(a1, qf[c][s], sa[1][c]);
+                }
+            }
+            uint4 pf[R];
+#pragma unroll
+            for (int c = 0; c < R; ++c) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = sa[e >> 2][c][e & 3] * mul;
+                if (masked) {
+                    const uint32_t win = window_of(words[c], p.mask_words, start, q.prior, q.ctx, limit[c]) >> (4 * g4);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = 16 * (e >> 2) + (e & 3);           // + 4 g4
+                        if ((bad >> (2 * key + 8 * g4)) & 3) x[e] = NAN;
+                        if (!((win >> key) & 1)) x[e] = -INFINITY;
+                    }
+                }
+                float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                mx = xor32_max(xor16_max(mx));
+                if (__ballot(mx > m[c] + SLACK)) {                         // wave-uniform
+                    const float m_new = fmaxf(m[c], mx), alpha = __builtin_amdgcn_exp2f(m[c] - m_new);
+                    m[c] = m_new;
+                    l[c] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) O[c][j] *= alpha;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - m[c]);
+                pf[c] = make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
+                l[c] = E::pair_sum(pf[c].x, E::pair_sum(pf[c].y, E::pair_sum(pf[c].z, E::pair_sum(pf[c].w, l[c]))));
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                typedef short v4i16_t __attribute__((ext_vector_type(4)));
+                typedef short v8i16_t __attribute__((ext_vector_type(8)));
+                typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+                const uint32_t o = va[j % NVA] + j / NVA * (32 * NVA);
+                const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(tile + o));
+                const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(tile + o + 16 * VROW));
+                const v8i16_t av = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+                for (int c = 0; c < R; ++c) O[c][j] = E::mfma(__builtin_bit_cast(uint4, av), pf[c], O[c][j]);
+            }
+        }
+
+        // the four waves' outputs joined, through the tiles' LDS
+        float f[R];
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            l[c] += __shfl_xor(l[c], 16);
+            l[c] += __shfl_xor(l[c], 32);
+            if (g4 == 0) { sm_m[w][16 * c + r16] = m[c]; sm_l[w][16 * c + r16] = l[c]; }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == q.key_tiles;
+        const int64_t slot = 2 * (int64_t)worker + (t0 == 0 ? 1 : 0);
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            const int r = 16 * c + r16;
+            f[c] = __builtin_amdgcn_exp2f(m[c] - fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r])));
+        }
+        auto sums_of = [&](int r, float& top, float& sum) __attribute__((always_inline)) {
+            top = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = fmaf(__builtin_amdgcn_exp2f(sm_m[i][r] - top), sm_l[i][r], sum);
+        };
+        if (!whole && tid < ROWS) {
+            float top, sum;
+            sums_of(tid, top, sum);
+            p.ws_ml[slot * ROWS + tid] = make_float2(top, sum);
+        }
+        float* const joint = (float*)lds;
+#pragma unroll
+        for (int ch = 0; ch < DV / CH; ++ch) {
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int j = 0; j < CH / 16; ++j)
+                    *(f32x4_t*)(joint + (w * ROWS + 16 * c + r16) * (CH + 4) + 16 * j + 4 * g4) = O[c][ch * (CH / 16) + j] * f[c];
+            __syncthreads();
+            for (int i = tid; i < ROWS * (CH / 4); i += 256) {
+                const int r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
+                f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col);
+                if (row >= nrows) continue;
+                if (!whole) {
+                    *(f32x4_t*)(p.ws_acc + (slot * ROWS + r) * DV + ch * CH + col) = o;
+                } else {
+                    float top, sum;
+                    sums_of(r, top, sum);
+                    const float inv = (FP8 ? p.v_scale[kvh] : 1.f) / sum;
+                    o *= inv;
+                    if (sum == 0.f) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
+                    *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
+                }
+            }
+            __syncthreads();
+        }
+        off += t1 - t0;
+        at += t1 - t0;
+    }
+}
+
+// Items that several workgroups had: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  1024 / DV rows of an item to a workgroup.
+template <typename E, int DV, int ROWS>
+__global__ void __launch_bounds__(256)
+row_join_kernel(RowParams p) {
+    constexpr int PER = 1024 / DV, LPR = DV / 4;
+    __shared__ int64_t sums[4];
+    __shared__ int64_t before_seq;
+    const int sub = blockIdx.x % (ROWS / PER), item_at = blockIdx.x / (ROWS / PER);
+    const int rtile = item_at % p.row_tiles, kvh = item_at / p.row_tiles % p.hkv, seq = item_at / p.row_tiles / p.hkv;
+    const Seq q = load_seq<ROWS>(p, seq);
+    const int nrows = q.n * p.group;
+    if (rtile * ROWS + sub * PER >= nrows) return;                 // (the whole workgroup)
+    int first, last;
+    int64_t mine;
+    const int64_t line = line_of<ROWS>(p, sums, first, last, mine), piece = piece_of(p, line);
+    for (int s = first; s < last; ++s) {
+        if (s == seq) before_seq = mine;
+        const Seq x = load_seq<ROWS>(p, s);
+        mine += x.items(p) * x.key_tiles;
+    }
+    __syncthreads();
+    const int64_t begin = before_seq + ((int64_t)kvh * q.row_tiles + rtile) * q.key_tiles;
+    const int a = (int)(begin / piece), b = (int)((begin + q.key_tiles - 1) / piece);
+    if (a == b) return;                                            // (one workgroup had it whole)
+    const int r = sub * PER + threadIdx.x / LPR, row = rtile * ROWS + r, col = threadIdx.x % LPR * 4;
+    if (row >= nrows) return;
+    auto slot_of = [&](int k) { return 2 * (int64_t)k + (k == a ? 1 : 0); };
+    float top = NEG_BIG;
+    for (int k = a; k <= b; ++k) top = fmaxf(top, p.ws_ml[slot_of(k) * ROWS + r].x);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int k = a; k <= b; ++k) {
+        const float2 ml = p.ws_ml[slot_of(k) * ROWS + r];
+        const f32x4_t x = *(const f32x4_t*)(p.ws_acc + (slot_of(k) * ROWS + r) * DV + col);
+        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        sum = fmaf(f, ml.y, sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+    }
+    const float inv = (p.v_scale != nullptr ? p.v_scale[kvh] : 1.f) / sum;
+    o *= inv;
+    if (sum == 0.f) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
+    *(uint2*)(dst + col) = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
+}
+
+// How a call is laid out.
+struct RowPlan {
+    int R, occ;
+    int workers, least, row_tiles;
+};
+
+RowPlan row_plan(const RowAttnArgs& a) {
+    const bool latent = a.dk == 576;
+    const int group = a.hq / a.hkv;
+    const int64_t rows = (int64_t)a.max_q_len * group;
+    RowPlan r;
+    if (latent) { r.R = rows <= 16 ? 1 : 2; r.occ = 1; }
+    else {
+        r.R = rows <= 16 ? 1 : rows <= 32 || a.dk == 256 ? 2 : 4;
+        r.occ = r.R == 4 || a.dk == 256 ? 1 : 2;
+    }
+    r.row_tiles = (int)((rows + 16 * r.R - 1) / (16 * r.R));
+    int64_t span = (int64_t)a.max_blocks * BS;
+    if (a.longest_context > 0) span = std::min<int64_t>(span, a.longest_context);
+    r.least = 4;
+    // (rows in all bound the row tiles too, where one long sequence is among many short ones)
+    const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / (16 * r.R) + a.num_seqs);
+    const int64_t tiles = items * ((span + KT - 1) / KT);
+    r.workers = (int)std::min<int64_t>(256 * r.occ, (tiles + r.least - 1) / r.least);
+    return r;
+}
+
+template <typename E, bool FP8, int DK, int DV, bool LATENT, int R, int OCC>
+void launch_variant(const RowParams& p, int64_t join_items, hipStream_t stream) {
+    hipLaunchKernelGGL((row_attn_kernel<E, FP8, DK, DV, LATENT, R, OCC>), dim3((unsigned)p.workers), dim3(256), 0, stream, p);
+    if (p.workers > 1)
+        hipLaunchKernelGGL((row_join_kernel<E, DV, 16 * R>), dim3((unsigned)(join_items * (16 * R * DV / 1024))), dim3(256), 0, stream, p);
+}
+
+template <typename E, bool FP8> void launch_tree(const RowParams& p, const RowPlan& r, int d, int64_t items, hipStream_t stream) {
+    if (d == 64) {
+        if (r.R == 1) launch_variant<E, FP8, 64, 64, false, 1, 2>(p, items, stream);
+        else if (r.R == 2) launch_variant<E, FP8, 64, 64, false, 2, 2>(p, items, stream);
+        else launch_variant<E, FP8, 64, 64, false, 4, 1>(p, items, stream);
+    } else if (d == 128) {
+        if (r.R == 1) launch_variant<E, FP8, 128, 128, false, 1, 2>(p, items, stream);
+        else if (r.R == 2) launch_variant<E, FP8, 128, 128, false, 2, 2>(p, items, stream);
+        else launch_variant<E, FP8, 128, 128, false, 4, 1>(p, items, stream);
+    } else {
+        if (r.R == 1) launch_variant<E, FP8, 256, 256, false, 1, 1>(p, items, stream);
+        else launch_variant<E, FP8, 256, 256, false, 2, 1>(p, items, stream);
+    }
+}
+
+template <typename E> void launch_latent(const RowParams& p, const RowPlan& r, int64_t items, hipStream_t stream) {
+    if (r.R == 1) launch_variant<E, false, 576, 512, true, 1, 1>(p, items, stream);
+    else launch_variant<E, false, 576, 512, true, 2, 1>(p, items, stream);
+}
+
+}  // namespace
+
+// (the join's grid holds less than 2^32 threads; a workgroup's place in a launch and a row are 32 bits)
+bool row_attn_mfma_supported(const RowAttnArgs& a) {
+    if (a.bs != BS || !is_16bit_float(a.q_dtype) || a.num_blocks > INT32_MAX) return false;
+    const bool latent = a.dk == 576 && a.dv == 512 && a.v_row == 576 && a.hkv == 1;
+    if (!latent && (a.dk != a.dv || (a.dk != 64 && a.dk != 128 && a.dk != 256))) return false;
+    const int64_t rows = (int64_t)a.max_q_len * (a.hq / a.hkv), wgs = (rows + 63) * a.hkv * a.num_seqs / 2;
+    return rows <= INT32_MAX / 2 && a.rows <= INT32_MAX && wgs < ((int64_t)1 << 24) && (int64_t)a.num_seqs * a.hkv < ((int64_t)1 << 24);
+}
+
+size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a) {
+    const RowPlan r = row_plan(a);
+    return r.workers > 1 ? (size_t)2 * r.workers * 16 * r.R * (a.dv + 2) * sizeof(float) : 0;
+}
+
+int launch_row_attn_mfma(const RowAttnArgs& a) {
+    const RowPlan r = row_plan(a);
+    RowParams p;
+    p.out = a.out; p.query = a.query; p.k_pool = a.k_pool; p.v_pool = a.v_pool; p.block_table = a.block_table;
+    p.block_table_stride = a.block_table_stride; p.context_lens = a.context_lens; p.cu_q_lens = a.cu_q_lens; p.masks = a.masks;
+    p.mask_words = a.mask_words; p.num_seqs = a.num_seqs; p.rows = (int)a.rows; p.max_q_len = a.max_q_len; p.hq = a.hq; p.hkv = a.hkv;
+    p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
+    p.v_scale = a.v_scale; p.workers = r.workers; p.least = r.least; p.row_tiles = r.row_tiles;
+    p.ws_acc = (float*)a.workspace;
+    p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * 16 * r.R * a.dv);
+    const int64_t items = (int64_t)a.num_seqs * a.hkv * r.row_tiles;
+    const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, f16 = a.q_dtype == AICOMP_KV_F16;
+    if (a.dk == 576) { if (f16) launch_latent<F16Fmt>(p, r, items, a.stream); else launch_latent<Bf16Fmt>(p, r, items, a.stream); }
+    else if (f16) { if (fp8) launch_tree<F16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<F16Fmt, false>(p, r, a.dk, items, a.stream); }
+    else { if (fp8) launch_tree<Bf16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<Bf16Fmt, false>(p, r, a.dk, items, a.stream); }
+    AICOMP_HIP_LAUNCH_CHECK();
+    return AICOMP_KV_OK;
+}
+
+}  // namespace aicomp
