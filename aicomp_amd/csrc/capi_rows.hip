@@ -195,7 +195,7 @@ int aicomp_latent_prompt_attn(void* out, const void* query, const void* key, int
     a.cu_q_lens = cu_q_lens; a.cu_k_lens = cu_k_lens; a.num_seqs = num_seqs; a.rows = total_q; a.keys = total_k; a.max_q_len = max_q_len;
     a.heads = num_heads; a.nope = nope_dim; a.rope = rope_dim; a.dv = value_dim; a.scale = scale; a.dtype = dtype;
     a.stream = (hipStream_t)stream;
-    return launch_prompt_generic(a);
+    return prompt_attn_mfma_supported(a) ? launch_prompt_attn_mfma(a) : launch_prompt_generic(a);
 }
 
 int aicomp_kv_keep_rows(void* const* pools, int num_pools, int64_t row_bytes, int num_kv_heads, int block_size, int64_t num_blocks,

@@ -62,6 +62,8 @@ bool row_attn_mfma_supported(const RowAttnArgs& a);
 size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a);
 int launch_row_attn_mfma(const RowAttnArgs& a);
 int launch_prompt_generic(const PromptAttnArgs& a);
+bool prompt_attn_mfma_supported(const PromptAttnArgs& a);
+int launch_prompt_attn_mfma(const PromptAttnArgs& a);
 
 struct LatentAppendArgs {
     const void* latent; int64_t latent_stride;          // [tokens, latent_dim + rope_dim]

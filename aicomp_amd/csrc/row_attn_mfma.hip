@@ -281,10 +281,10 @@ row_attn_kernel(RowParams p) {
             }
             const int start = t * KT;
             const bool masked = start + KT > full;                         // wave-uniform
-            uint64_t bad = 0;                                              // bits 2 k, 2 k + 1: key k's value is not finite
             if (masked) {
-                // A weight of 0 times a value that is not finite is not 0: such a value becomes 0, and the score of its key not a
-                // number for the rows that see it.  Two lanes to a key.
+                // A weight of 0 times a value that is not finite is not 0: such a value becomes 0, and its key not a number, and with
+                // it the score of the rows that see it (of a latent row, key and value in one, what is left is the key's part).  Two
+                // lanes to a key.
                 constexpr uint32_t EXP = E::DT == AICOMP_KV_F16 ? 0x7c007c00u : 0x7f807f80u;
                 constexpr uint32_t ONE = E::DT == AICOMP_KV_F16 ? 0x04000400u : 0x00800080u;
                 unsigned char* const mine_v = tile + VBASE + (lane >> 1) * VROW + (lane & 1) * DV;
@@ -294,9 +294,10 @@ row_attn_kernel(RowParams p) {
                     const uint4 x = *(const uint4*)(mine_v + 16 * i);
                     acc |= ((x.x & EXP) + ONE) | ((x.y & EXP) + ONE) | ((x.z & EXP) + ONE) | ((x.w & EXP) + ONE);
                 }
-                bad = __ballot((acc & 0x80008000u) != 0);
+                const uint64_t bad = __ballot((acc & 0x80008000u) != 0);
                 if (bad && ((bad >> (lane & ~1)) & 3)) {
                     for (int i = 0; i < DV / 16; ++i) *(uint4*)(mine_v + 16 * i) = make_uint4(0, 0, 0, 0);
+                    *(uint4*)(tile + (lane >> 1) * KROW + (LATENT ? 2 * DV : 0)) = make_uint4(~0u, ~0u, ~0u, ~0u);
                 }
             }
 
@@ -326,7 +327,6 @@ row_attn_kernel(RowParams p) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int key = 16 * (e >> 2) + (e & 3);           // + 4 g4
-                        if ((bad >> (2 * key + 8 * g4)) & 3) x[e] = NAN;
                         if (!((win >> key) & 1)) x[e] = -INFINITY;
                     }
                 }
@@ -337,7 +337,12 @@ row_attn_kernel(RowParams p) {
                     m[c] = m_new;
                     l[c] *= alpha;
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) O[c][j] *= alpha;
+                    for (int j = 0; j < NJ; ++j) {
+                        // (each by itself from and to its accumulator registers: all at once they take the vector registers of the rest)
+                        if constexpr (R * NJ >= 64) asm volatile("" : "+a"(O[c][j]));
+                        O[c][j] *= alpha;
+                        if constexpr (R * NJ >= 64) asm volatile("" : "+a"(O[c][j]));
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - m[c]);
