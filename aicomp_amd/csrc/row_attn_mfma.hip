@@ -12,7 +12,7 @@
 // Work is divided evenly: all (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of
 // equal length, whatever the sequences' lengths are.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by
 // it; of others it leaves (m, l, O) in the workspace, and a second kernel joins them.
-#include "row_attn.h"
+#include "row_line.h"
 
 #include <algorithm>
 
@@ -20,98 +20,7 @@ namespace aicomp {
 
 namespace {
 
-constexpr int BS = 16;                 // tokens per block
 constexpr int KT = 32;                 // keys per tile
-constexpr float NEG_BIG = -1.0e30f;
-constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both formats' range
-
-#define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
-#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
-
-struct RowParams {
-    void* out;
-    const void* query;
-    const void* k_pool;
-    const void* v_pool;
-    const int32_t* block_table;
-    int64_t block_table_stride;
-    const int32_t* context_lens;
-    const int32_t* cu_q_lens;
-    const int64_t* masks;
-    int mask_words;
-    int num_seqs;
-    int rows, max_q_len;
-    int hq, hkv, group, max_blocks, num_blocks;
-    float mul;                         // scale * log2(e)
-    const float* k_scale;
-    const float* v_scale;
-    int workers;                       // workgroups
-    int least;                         // key tiles that a workgroup has at least
-    int row_tiles;                     // of the longest sequence (the join's grid)
-    float* ws_acc;                     // [2 workers][16 R][DV]
-    float2* ws_ml;                     // [2 workers][16 R]
-};
-
-// A sequence as the line of work sees it.
-struct Seq {
-    int begin, n, ctx, prior;          // ctx: 0 where its tokens are more than its context
-    int row_tiles, key_tiles;
-    __device__ __forceinline__ int64_t items(const RowParams& p) const { return (int64_t)p.hkv * row_tiles; }
-};
-
-template <int ROWS> __device__ __forceinline__ Seq load_seq(const RowParams& p, int s) {
-    Seq q;
-    q.begin = p.cu_q_lens ? max(0, p.cu_q_lens[s]) : s;
-    q.n = p.cu_q_lens ? min(min(p.cu_q_lens[s + 1], p.rows) - q.begin, p.max_q_len) : 1;
-    q.n = max(0, q.n);
-    q.ctx = min(p.context_lens[s], p.max_blocks * BS);
-    q.prior = q.ctx - q.n;
-    if (q.prior < 0) q.ctx = 0;
-    q.row_tiles = (q.n * p.group + ROWS - 1) / ROWS;
-    q.key_tiles = max(1, (q.ctx + KT - 1) / KT);
-    return q;
-}
-
-// The line's length, over all threads of the workgroup; `mine`: the part of it before this thread's sequences, first .. last - 1.
-template <int ROWS> __device__ __forceinline__ int64_t line_of(const RowParams& p, int64_t* sums, int& first, int& last, int64_t& mine) {
-    const int per = (p.num_seqs + 255) / 256, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    first = min((int)threadIdx.x * per, p.num_seqs);
-    last = min(first + per, p.num_seqs);
-    int64_t own = 0;
-    for (int s = first; s < last; ++s) {
-        const Seq q = load_seq<ROWS>(p, s);
-        own += q.items(p) * q.key_tiles;
-    }
-    int64_t up = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up((long long)up, o);
-        if (lane >= o) up += x;
-    }
-    if (lane == 63) sums[w] = up;
-    __syncthreads();
-    mine = up - own;
-    for (int i = 0; i < w; ++i) mine += sums[i];
-    return sums[0] + sums[1] + sums[2] + sums[3];
-}
-
-__device__ __forceinline__ int64_t piece_of(const RowParams& p, int64_t line) {
-    return max((int64_t)p.least, (line + p.workers - 1) / p.workers);
-}
-
-// Which of the 32 keys from `start` on a row sees.  Causal: those below `limit`; else by its mask words from key `prior` on.
-__device__ __forceinline__ uint32_t window_of(const int64_t* words, int num_words, int start, int prior, int ctx, int limit) {
-    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
-    if (words == nullptr) return below(limit - start);
-    const int o = start - prior;                                   // bit of the first key
-    auto bits = [&](int from) -> uint32_t {                        // from >= 0
-        const int k = from >> 6, b = from & 63;
-        const uint64_t lo = k < num_words ? (uint64_t)words[k] : 0, hi = b > 32 && k + 1 < num_words ? (uint64_t)words[k + 1] : 0;
-        return (uint32_t)(lo >> b | (b > 32 ? hi << (64 - b) : 0));
-    };
-    const uint32_t w = o >= 0 ? bits(o) : o <= -32 ? ~0u : bits(0) << -o | below(-o);
-    return w & below(ctx - start);
-}
 
 // E: 16-bit format of queries and output; DK / DV: elements of a key / value row; R: groups of 16 rows; LATENT: a value is the
 // first part of its key's row.  OCC: workgroups per CU.
@@ -142,12 +51,12 @@ row_attn_kernel(RowParams p) {
 
     int first, last;
     int64_t mine;
-    const int64_t line = line_of<ROWS>(p, sums, first, last, mine), piece = piece_of(p, line);
+    const int64_t line = line_of<ROWS, KT>(p, sums, first, last, mine), piece = piece_of(p, line);
     int64_t at = worker * piece;
     const int64_t end = min(line, at + piece);
     if (at >= end) return;
     for (int s = first; s < last; ++s) {
-        const Seq q = load_seq<ROWS>(p, s);
+        const Seq q = load_seq<ROWS, KT>(p, s);
         const int64_t all = q.items(p) * q.key_tiles;
         if (at >= mine && at < mine + all) { start_seq = s; start_off = at - mine; }
         mine += all;
@@ -180,7 +89,7 @@ row_attn_kernel(RowParams p) {
     uint4 sk[FP8 ? NLD : 1], sv[FP8 ? NLD : 1];
 
     while (at < end) {
-        Seq q = load_seq<ROWS>(p, seq);
+        Seq q = load_seq<ROWS, KT>(p, seq);
         const int64_t all = q.items(p) * q.key_tiles;
         if (off >= all) { off = 0; ++seq; continue; }                      // (a sequence without tokens, or the next one)
         const int item = (int)(off / q.key_tiles), t0 = (int)(off - (int64_t)item * q.key_tiles);
@@ -424,56 +333,10 @@ row_attn_kernel(RowParams p) {
     }
 }
 
-// Items that several workgroups had: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.  1024 / DV rows of an item to a workgroup.
-template <typename E, int DV, int ROWS>
-__global__ void __launch_bounds__(256)
-row_join_kernel(RowParams p) {
-    constexpr int PER = 1024 / DV, LPR = DV / 4;
-    __shared__ int64_t sums[4];
-    __shared__ int64_t before_seq;
-    const int sub = blockIdx.x % (ROWS / PER), item_at = blockIdx.x / (ROWS / PER);
-    const int rtile = item_at % p.row_tiles, kvh = item_at / p.row_tiles % p.hkv, seq = item_at / p.row_tiles / p.hkv;
-    const Seq q = load_seq<ROWS>(p, seq);
-    const int nrows = q.n * p.group;
-    if (rtile * ROWS + sub * PER >= nrows) return;                 // (the whole workgroup)
-    int first, last;
-    int64_t mine;
-    const int64_t line = line_of<ROWS>(p, sums, first, last, mine), piece = piece_of(p, line);
-    for (int s = first; s < last; ++s) {
-        if (s == seq) before_seq = mine;
-        const Seq x = load_seq<ROWS>(p, s);
-        mine += x.items(p) * x.key_tiles;
-    }
-    __syncthreads();
-    const int64_t begin = before_seq + ((int64_t)kvh * q.row_tiles + rtile) * q.key_tiles;
-    const int a = (int)(begin / piece), b = (int)((begin + q.key_tiles - 1) / piece);
-    if (a == b) return;                                            // (one workgroup had it whole)
-    const int r = sub * PER + threadIdx.x / LPR, row = rtile * ROWS + r, col = threadIdx.x % LPR * 4;
-    if (row >= nrows) return;
-    auto slot_of = [&](int k) { return 2 * (int64_t)k + (k == a ? 1 : 0); };
-    float top = NEG_BIG;
-    for (int k = a; k <= b; ++k) top = fmaxf(top, p.ws_ml[slot_of(k) * ROWS + r].x);
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int k = a; k <= b; ++k) {
-        const float2 ml = p.ws_ml[slot_of(k) * ROWS + r];
-        const f32x4_t x = *(const f32x4_t*)(p.ws_acc + (slot_of(k) * ROWS + r) * DV + col);
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
-        sum = fmaf(f, ml.y, sum);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
-    }
-    const float inv = (p.v_scale != nullptr ? p.v_scale[kvh] : 1.f) / sum;
-    o *= inv;
-    if (sum == 0.f) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
-    *(uint2*)(dst + col) = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
-}
-
-// How a call is laid out.
+// How a call is laid out: rows and keys of a tile, workgroups, key tiles that one has at least.
 struct RowPlan {
-    int R, occ;
+    bool shared;                       // row_attn_shared.hip
+    int R, rows, keys;
     int workers, least, row_tiles;
 };
 
@@ -482,19 +345,18 @@ RowPlan row_plan(const RowAttnArgs& a) {
     const int group = a.hq / a.hkv;
     const int64_t rows = (int64_t)a.max_q_len * group;
     RowPlan r;
-    if (latent) { r.R = rows <= 16 ? 1 : 2; r.occ = 1; }
-    else {
-        r.R = rows <= 16 ? 1 : rows <= 32 || a.dk == 256 ? 2 : 4;
-        r.occ = r.R == 4 || a.dk == 256 ? 1 : 2;
-    }
-    r.row_tiles = (int)((rows + 16 * r.R - 1) / (16 * r.R));
+    r.shared = !latent && rows > 32;
+    r.R = r.shared ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
+    r.rows = (r.shared ? 64 : 16) * r.R;
+    r.keys = r.shared ? 64 : 32;
+    r.least = r.shared ? 2 : 4;
+    r.row_tiles = (int)((rows + r.rows - 1) / r.rows);
     int64_t span = (int64_t)a.max_blocks * BS;
     if (a.longest_context > 0) span = std::min<int64_t>(span, a.longest_context);
-    r.least = 4;
     // (rows in all bound the row tiles too, where one long sequence is among many short ones)
-    const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / (16 * r.R) + a.num_seqs);
-    const int64_t tiles = items * ((span + KT - 1) / KT);
-    r.workers = (int)std::min<int64_t>(256 * r.occ, (tiles + r.least - 1) / r.least);
+    const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / r.rows + a.num_seqs);
+    const int64_t tiles = items * ((span + r.keys - 1) / r.keys);
+    r.workers = (int)std::min<int64_t>(latent || a.dk == 256 ? 256 : 512, (tiles + r.least - 1) / r.least);
     return r;
 }
 
@@ -502,22 +364,13 @@ template <typename E, bool FP8, int DK, int DV, bool LATENT, int R, int OCC>
 void launch_variant(const RowParams& p, int64_t join_items, hipStream_t stream) {
     hipLaunchKernelGGL((row_attn_kernel<E, FP8, DK, DV, LATENT, R, OCC>), dim3((unsigned)p.workers), dim3(256), 0, stream, p);
     if (p.workers > 1)
-        hipLaunchKernelGGL((row_join_kernel<E, DV, 16 * R>), dim3((unsigned)(join_items * (16 * R * DV / 1024))), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((row_join_kernel<E, DV, 16 * R, KT>), dim3((unsigned)(join_items * (16 * R * DV / 1024))), dim3(256), 0, stream, p);
 }
 
 template <typename E, bool FP8> void launch_tree(const RowParams& p, const RowPlan& r, int d, int64_t items, hipStream_t stream) {
-    if (d == 64) {
-        if (r.R == 1) launch_variant<E, FP8, 64, 64, false, 1, 2>(p, items, stream);
-        else if (r.R == 2) launch_variant<E, FP8, 64, 64, false, 2, 2>(p, items, stream);
-        else launch_variant<E, FP8, 64, 64, false, 4, 1>(p, items, stream);
-    } else if (d == 128) {
-        if (r.R == 1) launch_variant<E, FP8, 128, 128, false, 1, 2>(p, items, stream);
-        else if (r.R == 2) launch_variant<E, FP8, 128, 128, false, 2, 2>(p, items, stream);
-        else launch_variant<E, FP8, 128, 128, false, 4, 1>(p, items, stream);
-    } else {
-        if (r.R == 1) launch_variant<E, FP8, 256, 256, false, 1, 1>(p, items, stream);
-        else launch_variant<E, FP8, 256, 256, false, 2, 1>(p, items, stream);
-    }
+    if (d == 64) { if (r.R == 1) launch_variant<E, FP8, 64, 64, false, 1, 2>(p, items, stream); else launch_variant<E, FP8, 64, 64, false, 2, 2>(p, items, stream); }
+    else if (d == 128) { if (r.R == 1) launch_variant<E, FP8, 128, 128, false, 1, 2>(p, items, stream); else launch_variant<E, FP8, 128, 128, false, 2, 2>(p, items, stream); }
+    else { if (r.R == 1) launch_variant<E, FP8, 256, 256, false, 1, 1>(p, items, stream); else launch_variant<E, FP8, 256, 256, false, 2, 1>(p, items, stream); }
 }
 
 template <typename E> void launch_latent(const RowParams& p, const RowPlan& r, int64_t items, hipStream_t stream) {
@@ -532,13 +385,13 @@ bool row_attn_mfma_supported(const RowAttnArgs& a) {
     if (a.bs != BS || !is_16bit_float(a.q_dtype) || a.num_blocks > INT32_MAX) return false;
     const bool latent = a.dk == 576 && a.dv == 512 && a.v_row == 576 && a.hkv == 1;
     if (!latent && (a.dk != a.dv || (a.dk != 64 && a.dk != 128 && a.dk != 256))) return false;
-    const int64_t rows = (int64_t)a.max_q_len * (a.hq / a.hkv), wgs = (rows + 63) * a.hkv * a.num_seqs / 2;
+    const int64_t rows = (int64_t)a.max_q_len * (a.hq / a.hkv), wgs = (rows + 127) * a.hkv * a.num_seqs / 2;
     return rows <= INT32_MAX / 2 && a.rows <= INT32_MAX && wgs < ((int64_t)1 << 24) && (int64_t)a.num_seqs * a.hkv < ((int64_t)1 << 24);
 }
 
 size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a) {
     const RowPlan r = row_plan(a);
-    return r.workers > 1 ? (size_t)2 * r.workers * 16 * r.R * (a.dv + 2) * sizeof(float) : 0;
+    return r.workers > 1 ? (size_t)2 * r.workers * r.rows * (a.dv + 2) * sizeof(float) : 0;
 }
 
 int launch_row_attn_mfma(const RowAttnArgs& a) {
@@ -550,10 +403,11 @@ int launch_row_attn_mfma(const RowAttnArgs& a) {
     p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
     p.v_scale = a.v_scale; p.workers = r.workers; p.least = r.least; p.row_tiles = r.row_tiles;
     p.ws_acc = (float*)a.workspace;
-    p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * 16 * r.R * a.dv);
+    p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * r.rows * a.dv);
     const int64_t items = (int64_t)a.num_seqs * a.hkv * r.row_tiles;
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, f16 = a.q_dtype == AICOMP_KV_F16;
-    if (a.dk == 576) { if (f16) launch_latent<F16Fmt>(p, r, items, a.stream); else launch_latent<Bf16Fmt>(p, r, items, a.stream); }
+    if (r.shared) launch_row_attn_shared(p, f16, fp8, a.dk, r.R, items, a.stream);
+    else if (a.dk == 576) { if (f16) launch_latent<F16Fmt>(p, r, items, a.stream); else launch_latent<Bf16Fmt>(p, r, items, a.stream); }
     else if (f16) { if (fp8) launch_tree<F16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<F16Fmt, false>(p, r, a.dk, items, a.stream); }
     else { if (fp8) launch_tree<Bf16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<Bf16Fmt, false>(p, r, a.dk, items, a.stream); }
     AICOMP_HIP_LAUNCH_CHECK();
