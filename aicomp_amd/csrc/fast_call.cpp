@@ -15,7 +15,7 @@
 //
 // Beside it, the plain calls of aicomp_amd.ops (kv_append, rope_kv_append, paged_decode_attn, rope_paged_decode_attn,
 // paged_prefill_attn, append_prefill_attn, chunks_and_rows, sample_tokens, qk_norm_rope_kv_append, paged_score_attn,
-// copy_blocks): the same checks made here instead of in Python.  A call that
+// copy_blocks, latent_kv_append, paged_latent_attn, paged_tree_attn, latent_prompt_attn, keep_rows): the same checks made here instead of in Python.  A call that
 // passes them all is launched and returns true; any other returns false without having touched
 // anything, and the Python function goes on to convert what may be converted or to name what is wrong.
 #include <Python.h>
@@ -924,6 +924,240 @@ PyObject* copy_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+// ---- latent rows, trees of drafts, accepted rows
+
+// (a dimension of one element has any stride)
+int64_t step_of(const at::Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+PyObject* latent_kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        double eps;
+        if (nargs != 12)
+            FAIL("latent_kv_append(latent, weight, cos, sin, positions, pool, slot_mapping, eps, interleaved, query, out, rows_out)");
+        bool ok = true;
+        auto optional = [&](int i) -> const at::Tensor* {
+            if (args[i] == Py_None) return nullptr;
+            const at::Tensor* t = plain(args[i]);
+            ok = ok && t;
+            return t;
+        };
+        const at::Tensor *x = plain(args[0]), *cos = plain(args[2]), *sin = plain(args[3]), *pool = plain(args[5]), *slots = plain(args[6]);
+        const at::Tensor *w = optional(1), *pos = optional(4), *q = optional(9), *qo = optional(10), *rows = optional(11);
+        if (!ok || !x || !cos || !sin || !pool || !slots || !q != !qo || !as_double(args[7], eps) || !PyBool_Check(args[8]) ||
+            x->dim() != 2 || pool->dim() != 3 || cos->dim() != 2 || !pool->is_contiguous())
+            Py_RETURN_FALSE;
+        const int64_t T = x->size(0), width = x->size(1), rope = 2 * cos->size(1);
+        const at::ScalarType st = x->scalar_type();
+        const int dt = dtype_code(st);
+        if (T == 0 || dt < 0 || pool->size(2) != width || pool->scalar_type() != st || x->stride(1) != 1 || rope <= 0 || rope >= width ||
+            width > INT_MAX || cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || sin->sizes() != cos->sizes() ||
+            cos->stride(1) != 1 || sin->strides() != cos->strides() || (!pos && cos->size(0) < T) || !on(*cos, *x) || !on(*sin, *x) ||
+            !on(*pool, *x) || pool->size(0) == 0 || pool->size(1) == 0 || pool->size(1) > INT_MAX)
+            Py_RETURN_FALSE;
+        if ((w && (w->dim() != 1 || !vector_of(w, at::kFloat, width - rope, *x))) ||
+            (pos && (pos->dim() != 1 || !vector_of(pos, at::kLong, T, *x))) || slots->dim() != 1 || !vector_of(slots, at::kLong, T, *x))
+            Py_RETURN_FALSE;
+        int64_t heads = 0, st4[4] = {0, 0, 0, 0};
+        if (q) {
+            for (const at::Tensor* t : {q, qo})
+                if (t->dim() != 3 || t->size(0) != T || t->size(2) != rope || t->size(1) != q->size(1) || t->scalar_type() != st ||
+                    t->stride(2) != 1 || !on(*t, *x))
+                    Py_RETURN_FALSE;
+            heads = q->size(1);
+            if (heads == 0 || heads > INT_MAX) Py_RETURN_FALSE;
+            st4[0] = step_of(*q, 0); st4[1] = heads > 1 ? q->stride(1) : rope;
+            st4[2] = step_of(*qo, 0); st4[3] = heads > 1 ? qo->stride(1) : rope;
+        }
+        if (rows && (rows->sizes() != x->sizes() || rows->scalar_type() != st || rows->stride(1) != 1 || !on(*rows, *x))) Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(x->device());
+        void* stream = stream_of(*x);
+        const bool interleaved = args[8] == Py_True;
+        auto data = [](const at::Tensor* t) { return t ? t->data_ptr() : nullptr; };
+        const int rc = unlocked([&] {
+            return aicomp_latent_kv_append(
+                x->data_ptr(), T > 1 ? x->stride(0) : width, (const float*)data(w), (float)eps, (const float*)cos->data_ptr(),
+                (const float*)sin->data_ptr(), cos->stride(0), cos->size(0), interleaved, (const int64_t*)data(pos), data(q), data(qo),
+                st4[0], st4[1], st4[2], st4[3], data(rows), rows ? (T > 1 ? rows->stride(0) : width) : 0, pool->data_ptr(),
+                (const int64_t*)slots->data_ptr(), T, (int)heads, (int)(width - rope), (int)rope, (int)pool->size(1), pool->size(0), dt,
+                stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+// Scratch of a call of two launches on `stream`: of a recorded call, memory of the graph's own (two graphs may be replayed side by
+// side); else the stream's buffer, `shared` among its calls.
+at::Tensor call_scratch(const c10::Device& dev, void* stream, size_t need, bool& shared) {
+    shared = false;
+    if (need == 0) return at::Tensor();
+    if (recording(stream)) return at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(dev));
+    shared = true;
+    return cached_scratch(dev, stream, need);
+}
+
+// the masks of a call of T rows, and their words
+bool masks_of(PyObject* o, int64_t T, const at::Tensor& ref, const at::Tensor*& masks, int& words) {
+    masks = nullptr;
+    words = 0;
+    if (o == Py_None) return true;
+    masks = plain(o);
+    if (!masks || masks->scalar_type() != at::kLong || masks->dim() != 2 || masks->size(0) != T || masks->size(1) <= 0 ||
+        masks->size(1) > INT_MAX || !masks->is_contiguous() || !on(*masks, ref))
+        return false;
+    words = (int)masks->size(1);
+    return true;
+}
+
+PyObject* paged_latent_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        int max_q, longest, words;
+        double scale;
+        if (nargs != 10)
+            FAIL("paged_latent_attn(out, query, pool, block_table, context_lens, scale, cu_q_lens, max_q_len, tree_masks, longest_context)");
+        const at::Tensor *out = plain(args[0]), *q = plain(args[1]), *pool = plain(args[2]), *table = plain(args[3]), *ctx = plain(args[4]);
+        if (!out || !q || !pool || !table || !ctx || !as_double(args[5], scale) || !as_int(args[7], max_q) || !as_int(args[9], longest) ||
+            out->dim() != 3 || q->dim() != 3 || pool->dim() != 3 || !pool->is_contiguous() || !q->is_contiguous() || !out->is_contiguous())
+            Py_RETURN_FALSE;
+        const int64_t T = q->size(0), H = q->size(1), width = q->size(2), C = out->size(2), S = ctx->numel();
+        const int dt = dtype_code(q->scalar_type());
+        const at::Tensor *cu = nullptr, *masks;
+        if (T == 0 || dt < 0 || out->size(0) != T || out->size(1) != H || C > width || pool->size(2) != width || T > INT_MAX || H > INT_MAX ||
+            width > INT_MAX || out->scalar_type() != q->scalar_type() || pool->scalar_type() != q->scalar_type() || !on(*out, *q) ||
+            !on(*pool, *q) || !vector_of(ctx, at::kInt, S, *q) || table->scalar_type() != at::kInt || table->dim() != 2 ||
+            table->size(0) != S || table->stride(1) != 1 || table->size(1) > INT_MAX || !on(*table, *q) || pool->size(1) > INT_MAX)
+            Py_RETURN_FALSE;
+        if (args[6] != Py_None && !vector_of(cu = plain(args[6]), at::kInt, S + 1, *q)) Py_RETURN_FALSE;
+        if (!masks_of(args[8], T, *q, masks, words) || (cu ? max_q <= 0 : masks || T != S || max_q != 1)) Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(q->device());
+        void* stream = stream_of(*q);
+        const int bs = (int)pool->size(1), mb = (int)table->size(1);
+        bool shared;
+        const at::Tensor scratch = call_scratch(q->device(), stream, aicomp_paged_latent_workspace_bytes(
+            (int)S, T, max_q, (int)H, (int)C, (int)(width - C), bs, mb, dt, longest), shared);
+        const int rc = unlocked([&] {
+            std::unique_lock<std::mutex> one_at_a_time(scratch_launches(), std::defer_lock);
+            if (shared) one_at_a_time.lock();
+            return aicomp_paged_latent_attn(
+                out->data_ptr(), q->data_ptr(), pool->data_ptr(), (const int32_t*)table->data_ptr(), table->stride(0),
+                (const int32_t*)ctx->data_ptr(), cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                masks ? (const int64_t*)masks->data_ptr() : nullptr, words, (int)S, T, max_q, (int)H, (int)C, (int)(width - C), bs, mb,
+                pool->size(0), (float)scale, dt, longest, scratch.defined() ? scratch.data_ptr() : nullptr,
+                scratch.defined() ? (size_t)scratch.numel() : 0, stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+PyObject* paged_tree_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        Pools p;
+        const at::Tensor *out, *q, *table, *ctx, *cu, *masks;
+        int dt, max_q, longest, words;
+        int64_t S;
+        double scale;
+        if (nargs != 13)
+            FAIL("paged_tree_attn(out, query, k_pool, v_pool, block_table, context_lens, cu_q_lens, tree_masks, scale, max_q_len, k_scale, "
+                 "v_scale, longest_context)");
+        if (!attention_args(args, out, q, p, table, ctx, dt, S) || !vector_of(cu = plain(args[6]), at::kInt, S + 1, *q) ||
+            !masks_of(args[7], q->size(0), *q, masks, words) || !masks || !as_double(args[8], scale) || !as_int(args[9], max_q) ||
+            !p.scales(args[10], args[11]) || !as_int(args[12], longest) || max_q <= 0 || q->size(0) == 0 || q->size(0) > INT_MAX)
+            Py_RETURN_FALSE;
+        const int64_t T = q->size(0);
+        const int hq = (int)q->size(1), mb = (int)table->size(1);
+        const c10::DeviceGuard guard(q->device());
+        void* stream = stream_of(*q);
+        bool shared;
+        const at::Tensor scratch = call_scratch(q->device(), stream, aicomp_paged_tree_workspace_bytes(
+            (int)S, T, max_q, hq, p.hkv, p.d, p.bs, mb, dt, p.dt, longest), shared);
+        const int rc = unlocked([&] {
+            std::unique_lock<std::mutex> one_at_a_time(scratch_launches(), std::defer_lock);
+            if (shared) one_at_a_time.lock();
+            return aicomp_paged_tree_attn(
+                out->data_ptr(), q->data_ptr(), p.k->data_ptr(), p.v->data_ptr(), (const int32_t*)table->data_ptr(), table->stride(0),
+                (const int32_t*)ctx->data_ptr(), (const int32_t*)cu->data_ptr(), (const int64_t*)masks->data_ptr(), words, (int)S, T, max_q,
+                hq, p.hkv, p.d, p.bs, mb, p.nb, (float)scale, dt, p.dt, p.ks, p.vs, longest,
+                scratch.defined() ? scratch.data_ptr() : nullptr, scratch.defined() ? (size_t)scratch.numel() : 0, stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+PyObject* latent_prompt_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        int max_q;
+        double scale;
+        if (nargs != 9) FAIL("latent_prompt_attn(out, query, key, rope_key, value, cu_q_lens, cu_k_lens, scale, max_q_len)");
+        const at::Tensor *out = plain(args[0]), *q = plain(args[1]), *k = plain(args[2]), *r = plain(args[3]), *v = plain(args[4]),
+                         *cu = plain(args[5]), *cuk = plain(args[6]);
+        if (!out || !q || !k || !r || !v || !cu || !cuk || !as_double(args[7], scale) || !as_int(args[8], max_q) || max_q <= 0 ||
+            out->dim() != 3 || q->dim() != 3 || k->dim() != 3 || v->dim() != 3 || r->dim() != 2 || cu->dim() != 1 || cuk->dim() != 1)
+            Py_RETURN_FALSE;
+        const int64_t Tq = q->size(0), H = q->size(1), Tk = k->size(0), N = k->size(2), D = r->size(1), V = v->size(2), S = cu->numel() - 1;
+        const at::ScalarType st = q->scalar_type();
+        const int dt = dtype_code(st);
+        if (Tq == 0 || S <= 0 || S > INT_MAX || H > INT_MAX || N > INT_MAX || D > INT_MAX || V > INT_MAX || dt < 0 || q->size(2) != N + D ||
+            k->size(1) != H || v->size(0) != Tk || v->size(1) != H || r->size(0) != Tk || out->size(0) != Tq || out->size(1) != H ||
+            out->size(2) != V || !q->is_contiguous() || !out->is_contiguous() || !vector_of(cu, at::kInt, S + 1, *q) ||
+            !vector_of(cuk, at::kInt, S + 1, *q))
+            Py_RETURN_FALSE;
+        for (const at::Tensor* t : {out, k, r, v})
+            if (t->scalar_type() != st || t->stride(t->dim() - 1) != 1 || !on(*t, *q)) Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(q->device());
+        void* stream = stream_of(*q);
+        const int rc = unlocked([&] {
+            return aicomp_latent_prompt_attn(
+                out->data_ptr(), q->data_ptr(), k->data_ptr(), step_of(*k, 0), step_of(*k, 1), r->data_ptr(), step_of(*r, 0), v->data_ptr(),
+                step_of(*v, 0), step_of(*v, 1), (const int32_t*)cu->data_ptr(), (const int32_t*)cuk->data_ptr(), (int)S, Tq, Tk, max_q,
+                (int)H, (int)N, (int)D, (int)V, (float)scale, dt, stream);
+        });
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
+PyObject* keep_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    try {
+        if (nargs != 5) FAIL("keep_rows(pools, block_table, first, keep, cu_keep)");
+        const at::Tensor *table = plain(args[1]), *first = plain(args[2]), *keep = plain(args[3]), *cu = plain(args[4]);
+        const bool list = PyList_CheckExact(args[0]);
+        if (!table || !first || !keep || !cu || (!list && !PyTuple_CheckExact(args[0]))) Py_RETURN_FALSE;
+        const Py_ssize_t n = list ? PyList_GET_SIZE(args[0]) : PyTuple_GET_SIZE(args[0]);
+        if (n <= 0 || n > INT_MAX) Py_RETURN_FALSE;
+        std::vector<void*> pools((size_t)n);
+        const at::Tensor* ref = nullptr;
+        at::Tensor held;                               // (the list may change once the interpreter lock is let go of)
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const at::Tensor* t = plain(list ? PyList_GET_ITEM(args[0], i) : PyTuple_GET_ITEM(args[0], i));
+            if (!t) Py_RETURN_FALSE;
+            if (!ref) { held = *t; ref = &held; }
+            if (t->sizes() != ref->sizes() || t->scalar_type() != ref->scalar_type() || !t->is_contiguous() || !on(*t, *ref)) Py_RETURN_FALSE;
+            pools[(size_t)i] = t->data_ptr();
+        }
+        const int64_t S = first->numel(), total = keep->numel(), dims = ref->dim();
+        if ((dims != 3 && dims != 4) || ref->numel() == 0 || total == 0 || S == 0 || S > INT_MAX || table->scalar_type() != at::kInt ||
+            table->dim() != 2 || table->size(0) != S || table->stride(1) != 1 || table->size(1) == 0 || table->size(1) > INT_MAX ||
+            !on(*table, *ref) || first->dim() != 1 || keep->dim() != 1 || cu->dim() != 1 || !vector_of(first, at::kInt, S, *ref) ||
+            !vector_of(keep, at::kInt, total, *ref) || !vector_of(cu, at::kInt, S + 1, *ref) ||
+            (dims == 4 && ref->size(1) > INT_MAX) || ref->size(dims - 2) > INT_MAX)
+            Py_RETURN_FALSE;
+        const c10::DeviceGuard guard(ref->device());
+        const int rc = aicomp_kv_keep_rows(pools.data(), (int)n, ref->size(dims - 1) * ref->element_size(), dims == 4 ? (int)ref->size(1) : 1,
+                                           (int)ref->size(dims - 2), ref->size(0), (const int32_t*)table->data_ptr(), table->stride(0),
+                                           (int)table->size(1), (const int32_t*)first->data_ptr(), (const int32_t*)keep->data_ptr(),
+                                           (const int32_t*)cu->data_ptr(), (int)S, total, stream_of(*ref));
+        DONE(rc);
+    } catch (const std::exception& e) {
+        FAIL("%s", e.what());
+    }
+}
+
 // A contiguous buffer of at least n elements of `size` bytes, released with the object; null data where it is not one.
 struct Buf {
     Py_buffer b{};
@@ -1085,6 +1319,11 @@ PyMethodDef methods[] = {
     {"qk_norm_rope_kv_append", FAST(qk_norm_rope_kv_append), "ops.qk_norm_rope_kv_append of a plain call, out given"},
     {"paged_score_attn", FAST(paged_score_attn), "ops.paged_score_decode_attn / paged_score_prefill_attn of a plain call"},
     {"copy_blocks", FAST(copy_blocks), "ops.copy_blocks of a plain call, pairs on the device"},
+    {"latent_kv_append", FAST(latent_kv_append), "ops.latent_kv_append of a plain call, out given"},
+    {"paged_latent_attn", FAST(paged_latent_attn), "ops.paged_latent_attn of a plain call, max_q_len given"},
+    {"paged_tree_attn", FAST(paged_tree_attn), "ops.paged_tree_attn of a plain call, max_q_len given"},
+    {"latent_prompt_attn", FAST(latent_prompt_attn), "ops.latent_prompt_attn of a plain call, max_q_len given"},
+    {"keep_rows", FAST(keep_rows), "ops.keep_rows of a plain call, all on the device"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_aicomp_fast", "lean host routes into the paged KV-cache library",

@@ -1006,6 +1006,9 @@ def latent_kv_append(latent: torch.Tensor, weight: Optional[torch.Tensor], cos: 
     (``latent_prompt_attn``).  Computed in float32 and rounded once.  Returns the rotated queries.
     """
     out = query if query_out is None else query_out
+    if _native("aicomp_latent_kv_append") and _FAST.latent_kv_append(latent, weight, cos, sin, positions, pool, slot_mapping, eps, interleaved,
+                                                                     query, out, rows_out):
+        return out
     lib = _lib.load()
     _req(latent.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
     _req(pool.dim() == 3 and pool.is_contiguous(), f"pool must be contiguous [num_blocks, block_size, C + D]; got {tuple(pool.shape)}")
@@ -1127,6 +1130,9 @@ def paged_latent_attn(out: torch.Tensor, query: torch.Tensor, pool: torch.Tensor
     back from ``cu_q_lens``); ``longest_context``: its bound of ``context_lens`` (0: the table's width), which sizes the call and cuts
     no row.  In place on ``out``, on the current stream.
     """
+    if _native("aicomp_paged_latent_attn") and _FAST.paged_latent_attn(out, query, pool, block_table, context_lens, scale, cu_q_lens,
+                                                                       1 if cu_q_lens is None else max_q_len, tree_masks, longest_context):
+        return out
     lib = _lib.load()
     _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
     _req(pool.dim() == 3 and pool.is_contiguous(), f"pool must be contiguous [num_blocks, block_size, C + D]; got {tuple(pool.shape)}")
@@ -1164,6 +1170,9 @@ def paged_tree_attn(out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor
     set.  A row that sees nothing is zero; rows behind the last sequence are left as they are.  ``max_q_len``, ``longest_context`` as
     in ``paged_latent_attn``.  In place on ``out``, on the current stream.
     """
+    if _native("aicomp_paged_tree_attn") and _FAST.paged_tree_attn(out, query, k_pool, v_pool, block_table, context_lens, cu_q_lens,
+                                                                   tree_masks, scale, max_q_len, k_scale, v_scale, longest_context):
+        return out
     lib = _lib.load()
     _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
     nb, hkv, bs, d = _check_pools(k_pool, v_pool)
@@ -1200,6 +1209,9 @@ def latent_prompt_attn(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     left as they are.  ``max_q_len``: the host's bound of the sequences' queries (``None``: read back).  In place on ``out``, on the
     current stream.
     """
+    if _native("aicomp_latent_prompt_attn") and _FAST.latent_prompt_attn(out, query, key, rope_key, value, cu_q_lens, cu_k_lens, scale,
+                                                                         max_q_len):
+        return out
     lib = _lib.load()
     _req(query.is_cuda, "tensors must live on a ROCm device (there is no CPU path)")
     _req(query.dim() == 3 and out.dim() == 3 and key.dim() == 3 and value.dim() == 3 and rope_key.dim() == 2,
@@ -1243,6 +1255,8 @@ def keep_rows(pools: Sequence[torch.Tensor], block_table: torch.Tensor, first: t
     ``keep [n]`` and ``cu_keep [S+1]`` int32: on the host they are checked (``keep`` ascends from 0 or more in every sequence) and copied,
     on the device they are taken as they are.  Tokens beyond the table, or in blocks outside the pools, are left alone.
     """
+    if _native("aicomp_kv_keep_rows") and _FAST.keep_rows(pools, block_table, first, keep, cu_keep):
+        return
     lib = _lib.load()
     _req(len(pools) > 0, "keep_rows needs at least one pool")
     p = pools[0]
