@@ -18,6 +18,7 @@ SOURCES = ["capi.hip", "kv_append.hip", "decode_generic.hip", "decode_mfma.hip",
            "prefill_mfma_f32.hip", "prefill_tiled.hip", "rope_append.hip", "sample.hip", "qk_norm_rope.hip",
            "block_copy.hip", "score_generic.hip", "score_prefill.hip", "score_prefill_f32.hip",
            "capi_rows.hip", "latent_append.hip", "keep_rows.hip", "row_attn_generic.hip", "row_attn_mfma.hip", "row_attn_shared.hip",
+           "row_attn_latent.hip",
            "prompt_attn.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

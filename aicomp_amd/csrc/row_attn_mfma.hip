@@ -38,10 +38,8 @@ row_attn_kernel(RowParams p) {
     constexpr int NVA = WIDE ? 8 : 4;                              // V addresses that are no immediates of each other
     static_assert(4 * ROWS * (CH + 4) * 4 <= 4 * TILE, "the join takes the tiles' place");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * TILE];
-    __shared__ int64_t sums[4];
-    __shared__ int64_t start_off;
-    __shared__ int start_seq;
-    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+    __shared__ PieceScratch scratch;
+    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];             // of each wave; then the factors of its output, and of the sum
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -49,21 +47,8 @@ row_attn_kernel(RowParams p) {
     // neighbours on the line, which share keys, on one XCD (workgroups go to the eight in turn)
     const int worker = (p.workers & 7) ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (p.workers >> 3) + ((int)blockIdx.x >> 3);
 
-    int first, last;
-    int64_t mine;
-    const int64_t line = line_of<ROWS, KT>(p, sums, first, last, mine), piece = piece_of(p, line);
-    int64_t at = worker * piece;
-    const int64_t end = min(line, at + piece);
-    if (at >= end) return;
-    for (int s = first; s < last; ++s) {
-        const Seq q = load_seq<ROWS, KT>(p, s);
-        const int64_t all = q.items(p) * q.key_tiles;
-        if (at >= mine && at < mine + all) { start_seq = s; start_off = at - mine; }
-        mine += all;
-    }
-    __syncthreads();
-    int seq = __builtin_amdgcn_readfirstlane(start_seq);
-    int64_t off = start_off;
+    Piece mine;
+    if (!piece_of<ROWS, KT, 256>(p, worker, scratch, mine)) return;
 
     auto fk = [](int key) { return key & 7; };
     auto fv = [](int key) { return LATENT ? key & 7 : WIDE ? 2 * (key & 7) : key & 6; };
@@ -88,14 +73,10 @@ row_attn_kernel(RowParams p) {
     constexpr int PARTS = DK / 16, KPL = 64 / PARTS, NLD = KT / KPL;       // fp8: 16 codes to a lane, keys per load
     uint4 sk[FP8 ? NLD : 1], sv[FP8 ? NLD : 1];
 
-    while (at < end) {
-        Seq q = load_seq<ROWS, KT>(p, seq);
-        const int64_t all = q.items(p) * q.key_tiles;
-        if (off >= all) { off = 0; ++seq; continue; }                      // (a sequence without tokens, or the next one)
-        const int item = (int)(off / q.key_tiles), t0 = (int)(off - (int64_t)item * q.key_tiles);
-        const int t1 = (int)min((int64_t)q.key_tiles, t0 + (end - at));
-        const int kvh = item / q.row_tiles, rtile = item - kvh * q.row_tiles;
-        const int nrows = q.n * p.group;
+    Item it;
+    while (next_item<ROWS, KT>(p, worker, mine, it)) {
+        const Seq q = mine.q;
+        const int kvh = it.kvh, rtile = it.rtile, nrows = q.n * p.group;
 
         // rows of this lane's columns (beyond the last: that one, computed and not stored)
         uint4 qf[R][NS];
@@ -126,7 +107,7 @@ row_attn_kernel(RowParams p) {
         }
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
-        const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)seq * p.block_table_stride);
+        const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
         const int last_block = (q.ctx - 1) / BS;                           // (blocks behind it are not this sequence's)
         auto block_base = [&](int t, int half) -> int64_t {                // element index of the block's first row
             const int b = table[min(2 * t + half, last_block)];
@@ -175,8 +156,8 @@ row_attn_kernel(RowParams p) {
             }
         };
 
-        int t = t0 + w;
-        const int t_end = min(t1, (some + KT - 1) / KT);
+        int t = it.t0 + w;
+        const int t_end = min(it.t1, (some + KT - 1) / KT);
         if (FP8 && t < t_end) fetch(t);
         for (; t < t_end; t += 4) {
             if constexpr (FP8) {
@@ -246,12 +227,7 @@ row_attn_kernel(RowParams p) {
                     m[c] = m_new;
                     l[c] *= alpha;
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        // (each by itself from and to its accumulator registers: all at once they take the vector registers of the rest)
-                        if constexpr (R * NJ >= 64) asm volatile("" : "+a"(O[c][j]));
-                        O[c][j] *= alpha;
-                        if constexpr (R * NJ >= 64) asm volatile("" : "+a"(O[c][j]));
-                    }
+                    for (int j = 0; j < NJ; ++j) O[c][j] *= alpha;
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - m[c]);
@@ -272,8 +248,7 @@ row_attn_kernel(RowParams p) {
             }
         }
 
-        // the four waves' outputs joined, through the tiles' LDS
-        float f[R];
+        // The four waves' outputs joined, through the tiles' LDS: factors first, once per row.
 #pragma unroll
         for (int c = 0; c < R; ++c) {
             l[c] += __shfl_xor(l[c], 16);
@@ -281,55 +256,50 @@ row_attn_kernel(RowParams p) {
             if (g4 == 0) { sm_m[w][16 * c + r16] = m[c]; sm_l[w][16 * c + r16] = l[c]; }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == q.key_tiles;
-        const int64_t slot = 2 * (int64_t)worker + (t0 == 0 ? 1 : 0);
+        if (tid < ROWS) {
+            float top = sm_m[0][tid], sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < R; ++c) {
-            const int r = 16 * c + r16;
-            f[c] = __builtin_amdgcn_exp2f(m[c] - fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r])));
-        }
-        auto sums_of = [&](int r, float& top, float& sum) __attribute__((always_inline)) {
-            top = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
-            sum = 0.f;
+            for (int i = 1; i < 4; ++i) top = fmaxf(top, sm_m[i][tid]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum = fmaf(__builtin_amdgcn_exp2f(sm_m[i][r] - top), sm_l[i][r], sum);
-        };
-        if (!whole && tid < ROWS) {
-            float top, sum;
-            sums_of(tid, top, sum);
-            p.ws_ml[slot * ROWS + tid] = make_float2(top, sum);
+            for (int i = 0; i < 4; ++i) {
+                const float f = __builtin_amdgcn_exp2f(sm_m[i][tid] - top);
+                sum = fmaf(f, sm_l[i][tid], sum);
+                sm_m[i][tid] = f;
+            }
+            sm_l[0][tid] = sum == 0.f ? 0.f : (FP8 ? p.v_scale[kvh] : 1.f) / sum;
+            if (!it.whole) p.ws_ml[it.slot * ROWS + tid] = make_float2(top, sum);
         }
+        __syncthreads();
+        float f[R];
+#pragma unroll
+        for (int c = 0; c < R; ++c) f[c] = sm_m[w][16 * c + r16];
         float* const joint = (float*)lds;
 #pragma unroll
         for (int ch = 0; ch < DV / CH; ++ch) {
+            if (ch > 0) __syncthreads();
 #pragma unroll
             for (int c = 0; c < R; ++c)
 #pragma unroll
                 for (int j = 0; j < CH / 16; ++j)
                     *(f32x4_t*)(joint + (w * ROWS + 16 * c + r16) * (CH + 4) + 16 * j + 4 * g4) = O[c][ch * (CH / 16) + j] * f[c];
             __syncthreads();
-            for (int i = tid; i < ROWS * (CH / 4); i += 256) {
-                const int r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
-                f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col);
+            for (int i0 = 0; i0 < ROWS * (CH / 4); i0 += 256) {
+                const int i = i0 + tid, r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
+                f32x4_t o = *(const f32x4_t*)(joint + r * (CH + 4) + col);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col);
                 if (row >= nrows) continue;
-                if (!whole) {
-                    *(f32x4_t*)(p.ws_acc + (slot * ROWS + r) * DV + ch * CH + col) = o;
+                if (!it.whole) {
+                    *(f32x4_t*)(p.ws_acc + (it.slot * ROWS + r) * DV + ch * CH + col) = o;
                 } else {
-                    float top, sum;
-                    sums_of(r, top, sum);
-                    const float inv = (FP8 ? p.v_scale[kvh] : 1.f) / sum;
-                    o *= inv;
-                    if (sum == 0.f) o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    const float inv = sm_l[0][r];                          // (0: nothing was seen, and O is 0)
                     uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
-                    *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
+                    *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
                 }
             }
-            __syncthreads();
         }
-        off += t1 - t0;
-        at += t1 - t0;
+        __syncthreads();
     }
 }
 
@@ -337,7 +307,7 @@ row_attn_kernel(RowParams p) {
 struct RowPlan {
     bool shared;                       // row_attn_shared.hip
     int R, rows, keys;
-    int workers, least, row_tiles;
+    int workers, least, over, row_tiles;
 };
 
 RowPlan row_plan(const RowAttnArgs& a) {
@@ -345,9 +315,12 @@ RowPlan row_plan(const RowAttnArgs& a) {
     const int group = a.hq / a.hkv;
     const int64_t rows = (int64_t)a.max_q_len * group;
     RowPlan r;
-    r.shared = !latent && rows > 32;
-    r.R = r.shared ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
-    r.rows = (r.shared ? 64 : 16) * r.R;
+    r.shared = rows > (latent ? 16 : 32);
+    // latent rows: 16 R to a workgroup.  64 rows keep fewer registers for the products than 48 and are the better choice only where
+    // 48 would be two tiles
+    if (latent) r.R = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 || rows > 64 ? 3 : 4;
+    else r.R = r.shared ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
+    r.rows = (r.shared && !latent ? 64 : 16) * r.R;
     r.keys = r.shared ? 64 : 32;
     r.least = r.shared ? 2 : 4;
     r.row_tiles = (int)((rows + r.rows - 1) / r.rows);
@@ -355,8 +328,13 @@ RowPlan row_plan(const RowAttnArgs& a) {
     if (a.longest_context > 0) span = std::min<int64_t>(span, a.longest_context);
     // (rows in all bound the row tiles too, where one long sequence is among many short ones)
     const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / r.rows + a.num_seqs);
-    const int64_t tiles = items * ((span + r.keys - 1) / r.keys);
-    r.workers = (int)std::min<int64_t>(latent || a.dk == 256 ? 256 : 512, (tiles + r.least - 1) / r.least);
+    // What an item's start and end cost, in key tiles, counts where workgroups have several items (64 rows of 512 .. 4096 tokens, 16 heads:
+    // 60 us without, 55 with); where items are divided, as many workgroups as there are tiles for are worth more (one row of 700 tokens:
+    // 17 us without, 21 with).
+    const int64_t tiles = (span + r.keys - 1) / r.keys, most = latent || a.dk == 256 ? 256 : 512;
+    r.over = items * 4 >= most ? (r.shared ? 3 : 8) : 0;
+    r.least += r.over;
+    r.workers = (int)std::min<int64_t>(most, (items * (tiles + r.over) + r.least - 1) / r.least);
     return r;
 }
 
@@ -373,11 +351,6 @@ template <typename E, bool FP8> void launch_tree(const RowParams& p, const RowPl
     else { if (r.R == 1) launch_variant<E, FP8, 256, 256, false, 1, 1>(p, items, stream); else launch_variant<E, FP8, 256, 256, false, 2, 1>(p, items, stream); }
 }
 
-template <typename E> void launch_latent(const RowParams& p, const RowPlan& r, int64_t items, hipStream_t stream) {
-    if (r.R == 1) launch_variant<E, false, 576, 512, true, 1, 1>(p, items, stream);
-    else launch_variant<E, false, 576, 512, true, 2, 1>(p, items, stream);
-}
-
 }  // namespace
 
 // (the join's grid holds less than 2^32 threads; a workgroup's place in a launch and a row are 32 bits)
@@ -386,12 +359,15 @@ bool row_attn_mfma_supported(const RowAttnArgs& a) {
     const bool latent = a.dk == 576 && a.dv == 512 && a.v_row == 576 && a.hkv == 1;
     if (!latent && (a.dk != a.dv || (a.dk != 64 && a.dk != 128 && a.dk != 256))) return false;
     const int64_t rows = (int64_t)a.max_q_len * (a.hq / a.hkv), wgs = (rows + 127) * a.hkv * a.num_seqs / 2;
-    return rows <= INT32_MAX / 2 && a.rows <= INT32_MAX && wgs < ((int64_t)1 << 24) && (int64_t)a.num_seqs * a.hkv < ((int64_t)1 << 24);
+    if (rows > INT32_MAX / 2 || a.rows > INT32_MAX || wgs >= ((int64_t)1 << 24) || (int64_t)a.num_seqs * a.hkv >= ((int64_t)1 << 24)) return false;
+    const RowPlan r = row_plan(a);                             // (the whole line, contexts as long as the table)
+    return (int64_t)a.num_seqs * a.hkv * r.row_tiles < ((int64_t)1 << 24) &&
+           (int64_t)a.num_seqs * a.hkv * r.row_tiles * (((int64_t)a.max_blocks * BS + r.keys - 1) / r.keys + r.over) < ((int64_t)1 << 30);
 }
 
 size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a) {
     const RowPlan r = row_plan(a);
-    return r.workers > 1 ? (size_t)2 * r.workers * r.rows * (a.dv + 2) * sizeof(float) : 0;
+    return r.workers > 1 ? (size_t)2 * r.workers * r.rows * (a.dv + 2) * sizeof(float) + (size_t)a.num_seqs * a.hkv * r.row_tiles * sizeof(int2) : 0;
 }
 
 int launch_row_attn_mfma(const RowAttnArgs& a) {
@@ -401,13 +377,16 @@ int launch_row_attn_mfma(const RowAttnArgs& a) {
     p.block_table_stride = a.block_table_stride; p.context_lens = a.context_lens; p.cu_q_lens = a.cu_q_lens; p.masks = a.masks;
     p.mask_words = a.mask_words; p.num_seqs = a.num_seqs; p.rows = (int)a.rows; p.max_q_len = a.max_q_len; p.hq = a.hq; p.hkv = a.hkv;
     p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
-    p.v_scale = a.v_scale; p.workers = r.workers; p.least = r.least; p.row_tiles = r.row_tiles;
+    p.v_scale = a.v_scale; p.workers = r.workers; p.least = r.least; p.over = r.over; p.row_tiles = r.row_tiles;
     p.ws_acc = (float*)a.workspace;
     p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * r.rows * a.dv);
+    p.ws_items = r.workers > 1 ? (int2*)(p.ws_ml + (size_t)2 * r.workers * r.rows) : nullptr;
     const int64_t items = (int64_t)a.num_seqs * a.hkv * r.row_tiles;
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, f16 = a.q_dtype == AICOMP_KV_F16;
-    if (r.shared) launch_row_attn_shared(p, f16, fp8, a.dk, r.R, items, a.stream);
-    else if (a.dk == 576) { if (f16) launch_latent<F16Fmt>(p, r, items, a.stream); else launch_latent<Bf16Fmt>(p, r, items, a.stream); }
+    if (r.shared && a.dk == 576) launch_row_attn_latent(p, f16, r.R, items, a.stream);
+    else if (r.shared) launch_row_attn_shared(p, f16, fp8, a.dk, r.R, items, a.stream);
+    else if (a.dk == 576 && f16) launch_variant<F16Fmt, false, 576, 512, true, 1, 1>(p, items, a.stream);
+    else if (a.dk == 576) launch_variant<Bf16Fmt, false, 576, 512, true, 1, 1>(p, items, a.stream);
     else if (f16) { if (fp8) launch_tree<F16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<F16Fmt, false>(p, r, a.dk, items, a.stream); }
     else { if (fp8) launch_tree<Bf16Fmt, true>(p, r, a.dk, items, a.stream); else launch_tree<Bf16Fmt, false>(p, r, a.dk, items, a.stream); }
     AICOMP_HIP_LAUNCH_CHECK();

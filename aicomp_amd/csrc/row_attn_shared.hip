@@ -29,9 +29,7 @@ row_attn_shared_kernel(RowParams p) {
     __shared__ __attribute__((aligned(1024))) unsigned char v0[KT * ROW];
     __shared__ __attribute__((aligned(1024))) unsigned char k1[KT * ROW];
     __shared__ __attribute__((aligned(1024))) unsigned char v1[KT * ROW];
-    __shared__ int64_t sums[4];
-    __shared__ int64_t start_off;
-    __shared__ int start_seq;
+    __shared__ PieceScratch scratch;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -39,21 +37,8 @@ row_attn_shared_kernel(RowParams p) {
     // neighbours on the line, which share keys, on one XCD (workgroups go to the eight in turn)
     const int worker = (p.workers & 7) ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (p.workers >> 3) + ((int)blockIdx.x >> 3);
 
-    int first, last;
-    int64_t mine;
-    const int64_t line = line_of<ROWS, KT>(p, sums, first, last, mine), piece = piece_of(p, line);
-    int64_t at = worker * piece;
-    const int64_t end = min(line, at + piece);
-    if (at >= end) return;
-    for (int s = first; s < last; ++s) {
-        const Seq q = load_seq<ROWS, KT>(p, s);
-        const int64_t all = q.items(p) * q.key_tiles;
-        if (at >= mine && at < mine + all) { start_seq = s; start_off = at - mine; }
-        mine += all;
-    }
-    __syncthreads();
-    int seq = __builtin_amdgcn_readfirstlane(start_seq);
-    int64_t off = start_off;
+    Piece mine;
+    if (!piece_of<ROWS, KT, 256>(p, worker, scratch, mine)) return;
 
     // chunk c (16 bytes) of key k lies at c ^ f(k) (row_attn_mfma.hip)
     auto fk = [](int key) { return key & 7; };
@@ -68,13 +53,10 @@ row_attn_shared_kernel(RowParams p) {
     }
     constexpr int PARTS = D / 16, KPL = 64 / PARTS, NLD = 16 / KPL;        // fp8: lanes to a row, rows per load, loads of a wave's block
 
-    while (at < end) {
-        const Seq q = load_seq<ROWS, KT>(p, seq);
-        const int64_t all = q.items(p) * q.key_tiles;
-        if (off >= all) { off = 0; ++seq; continue; }          // (a sequence without tokens, or the next one)
-        const int item = (int)(off / q.key_tiles), t0 = (int)(off - (int64_t)item * q.key_tiles);
-        const int t1 = (int)min((int64_t)q.key_tiles, t0 + (end - at));
-        const int kvh = item / q.row_tiles, rtile = item - kvh * q.row_tiles;
+    Item it;
+    while (next_item<ROWS, KT>(p, worker, mine, it)) {
+        const Seq q = mine.q;
+        const int kvh = it.kvh, rtile = it.rtile, t0 = it.t0;
         const int nrows = q.n * p.group, row0 = rtile * ROWS + 16 * R * w;             // of this wave
 
         // rows of this lane's columns (beyond the last: that one, computed and not stored)
@@ -104,7 +86,7 @@ row_attn_shared_kernel(RowParams p) {
         }
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
-        const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)seq * p.block_table_stride);
+        const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
         const int last_block = (q.ctx - 1) / BS;               // (blocks behind it are not this sequence's)
         // wave w brings in block w of a tile
         auto block_base = [&](int t) -> int64_t {              // element index of its first row
@@ -236,7 +218,7 @@ row_attn_shared_kernel(RowParams p) {
         };
 
         // Opens the step of tile t: it is in LDS afterwards for every wave, and the next one is on its way.
-        const int t_end = min(t1, (q.ctx + KT - 1) / KT);      // (0 tiles where the context is none)
+        const int t_end = min(it.t1, (q.ctx + KT - 1) / KT);      // (0 tiles where the context is none)
         auto open = [&](int t, unsigned char* kb, unsigned char* vb, unsigned char* kn, unsigned char* vn) __attribute__((always_inline)) {
             if constexpr (FP8) {
                 stash(kb, vb);                                 // (nobody reads this pair: its readers met at the tile between)
@@ -263,17 +245,15 @@ row_attn_shared_kernel(RowParams p) {
         }
         __syncthreads();                                       // (the buffers are free for the next item)
 
-        const bool whole = t0 == 0 && t1 == q.key_tiles;
-        const int64_t slot = 2 * (int64_t)worker + (t0 == 0 ? 1 : 0);
 #pragma unroll
         for (int c = 0; c < R; ++c) {
             l[c] += __shfl_xor(l[c], 16);
             l[c] += __shfl_xor(l[c], 32);
             const int r = 16 * R * w + 16 * c + r16, row = rtile * ROWS + r;
             if (row >= nrows) continue;
-            if (!whole) {
-                if (g4 == 0) p.ws_ml[slot * ROWS + r] = make_float2(m[c], l[c]);
-                float* dst = p.ws_acc + (slot * ROWS + r) * D + 4 * g4;
+            if (!it.whole) {
+                if (g4 == 0) p.ws_ml[it.slot * ROWS + r] = make_float2(m[c], l[c]);
+                float* dst = p.ws_acc + (it.slot * ROWS + r) * D + 4 * g4;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) *(f32x4_t*)(dst + 16 * j) = O[c][j];
             } else {
@@ -286,8 +266,6 @@ row_attn_shared_kernel(RowParams p) {
                                                                                    E::pack(O[c][j][2] * inv, O[c][j][3] * inv));
             }
         }
-        off += t1 - t0;
-        at += t1 - t0;
     }
 }
 

@@ -2,8 +2,10 @@
 // what a row sees of a tile, and how the pieces of an item are joined.
 //
 // All (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of equal length, whatever
-// the sequences' lengths are.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by it; of others each
-// leaves (m, l, O) of its rows in the workspace: in its slot 0 where it does not have the item's first key tile, else in its slot 1.
+// the sequences' lengths are.  Before an item's key tiles the line has `over` places more, in which nothing is done: what the start and
+// the end of an item cost, in tiles, so that pieces of several items have fewer tiles.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by it; of others each
+// leaves (m, l, O) of its rows in the workspace: in its slot 0 where it does not have the item's first key tile, else in its slot 1.  Who
+// has the first tile says who has the others.
 #pragma once
 
 #include "row_attn.h"
@@ -28,14 +30,17 @@ struct RowParams {
     const float* k_scale;
     const float* v_scale;
     int workers;                       // workgroups
-    int least;                         // key tiles that a workgroup has at least
+    int least;                         // places that a workgroup has at least
+    int over;                          // places of an item before its key tiles
     int row_tiles;                     // of the longest sequence (the join's grid)
     float* ws_acc;                     // [2 workers][rows of a tile][DV]
     float2* ws_ml;                     // [2 workers][rows of a tile]
+    int2* ws_items;                    // [num_seqs][hkv][row_tiles]: the first workgroup that has the item, and how many more do (NULL: one has all)
 };
 
 // d: head_dim; R: groups of 16 rows to a wave; items: of the join's grid
 void launch_row_attn_shared(const RowParams& p, bool f16, bool fp8, int d, int R, int64_t items, hipStream_t stream);
+void launch_row_attn_latent(const RowParams& p, bool f16, int groups, int64_t items, hipStream_t stream);
 
 namespace {
 
@@ -50,7 +55,8 @@ constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both
 struct Seq {
     int begin, n, ctx, prior;          // ctx: 0 where its tokens are more than its context
     int row_tiles, key_tiles;
-    __device__ __forceinline__ int64_t items(const RowParams& p) const { return (int64_t)p.hkv * row_tiles; }
+    __device__ __forceinline__ int items(const RowParams& p) const { return p.hkv * row_tiles; }
+    __device__ __forceinline__ int places(const RowParams& p) const { return items(p) * (key_tiles + p.over); }
 };
 
 // ROWS, KT: rows and keys of a tile
@@ -67,32 +73,98 @@ template <int ROWS, int KT> __device__ __forceinline__ Seq load_seq(const RowPar
     return q;
 }
 
-// The line's length, over all threads of the workgroup; `mine`: the part of it before this thread's sequences, first .. last - 1.
-template <int ROWS, int KT>
-__device__ __forceinline__ int64_t line_of(const RowParams& p, int64_t* sums, int& first, int& last, int64_t& mine) {
-    const int per = (p.num_seqs + 255) / 256, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    first = min((int)threadIdx.x * per, p.num_seqs);
-    last = min(first + per, p.num_seqs);
-    int64_t own = 0;
+// A workgroup's piece of the line: places at .. end - 1, the first of them place `off` of sequence `seq`, `q`.  (A line is less than 2^31
+// places, which the host sees to: 64-bit divisions cost a microsecond each.)
+struct Piece {
+    int at, end, length, seq, off;     // length: of every workgroup's piece
+    Seq q;
+};
+struct PieceScratch {
+    int sums[8];
+    int seq, off;
+    Seq q;
+};
+
+template <int ROWS, int KT, int THREADS>
+__device__ __forceinline__ bool piece_of(const RowParams& p, int worker, PieceScratch& sh, Piece& mine) {
+    const int per = (p.num_seqs + THREADS - 1) / THREADS, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int first = min((int)threadIdx.x * per, p.num_seqs), last = min(first + per, p.num_seqs);
+    Seq q;
+    int own = 0;
     for (int s = first; s < last; ++s) {
-        const Seq q = load_seq<ROWS, KT>(p, s);
-        own += q.items(p) * q.key_tiles;
+        q = load_seq<ROWS, KT>(p, s);
+        own += q.places(p);
     }
-    int64_t up = own;
+    int up = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up((long long)up, o);
+        const int x = __shfl_up(up, o);
         if (lane >= o) up += x;
     }
-    if (lane == 63) sums[w] = up;
+    if (lane == 63) sh.sums[w] = up;
     __syncthreads();
-    mine = up - own;
-    for (int i = 0; i < w; ++i) mine += sums[i];
-    return sums[0] + sums[1] + sums[2] + sums[3];
+    int line = 0, before = up - own;                           // the line's length; the part of it before this thread's sequences
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) {
+        if (i < w) before += sh.sums[i];
+        line += sh.sums[i];
+    }
+    mine.length = max(p.least, (int)(((unsigned)line + p.workers - 1) / (unsigned)p.workers));
+    mine.at = worker * mine.length;
+    mine.end = min(line, mine.at + mine.length);
+    if (mine.at >= mine.end) return false;
+    if (mine.at >= before && mine.at < before + own) {
+        for (int s = first; s < last; ++s) {
+            if (per > 1) q = load_seq<ROWS, KT>(p, s);
+            const int all = q.places(p);
+            if (mine.at >= before && mine.at < before + all) { sh.seq = s; sh.off = mine.at - before; sh.q = q; }
+            before += all;
+        }
+    }
+    __syncthreads();
+    mine.seq = __builtin_amdgcn_readfirstlane(sh.seq);
+    mine.off = __builtin_amdgcn_readfirstlane(sh.off);
+    mine.q.begin = __builtin_amdgcn_readfirstlane(sh.q.begin);
+    mine.q.n = __builtin_amdgcn_readfirstlane(sh.q.n);
+    mine.q.ctx = __builtin_amdgcn_readfirstlane(sh.q.ctx);
+    mine.q.prior = __builtin_amdgcn_readfirstlane(sh.q.prior);
+    mine.q.row_tiles = __builtin_amdgcn_readfirstlane(sh.q.row_tiles);
+    mine.q.key_tiles = __builtin_amdgcn_readfirstlane(sh.q.key_tiles);
+    return true;
 }
 
-__device__ __forceinline__ int64_t piece_of(const RowParams& p, int64_t line) {
-    return max((int64_t)p.least, (line + p.workers - 1) / p.workers);
+// The next item of the piece: key tiles t0 .. t1 - 1 of row tile `rtile` of KV head `kvh`; false if what is left of the piece has none.
+struct Item {
+    int kvh, rtile, t0, t1;
+    bool whole;
+    int64_t slot;                      // of the workspace, unless whole
+};
+template <int ROWS, int KT> __device__ __forceinline__ bool next_item(const RowParams& p, int worker, Piece& mine, Item& it) {
+    while (mine.at < mine.end) {
+        if (mine.off >= mine.q.places(p)) {                    // (sequences without tokens have none)
+            mine.off = 0;
+            mine.q = load_seq<ROWS, KT>(p, ++mine.seq);
+            continue;
+        }
+        const int places = mine.q.key_tiles + p.over, item = (unsigned)mine.off / (unsigned)places;
+        const int from = mine.off - item * places, to = min(places, from + (mine.end - mine.at)), at = mine.at;
+        mine.off += to - from;
+        mine.at += to - from;
+        if (to <= p.over) continue;                            // (its tiles are the next workgroup's)
+        it.t0 = max(0, from - p.over);
+        it.t1 = to - p.over;
+        it.kvh = (unsigned)item / (unsigned)mine.q.row_tiles;
+        it.rtile = item - it.kvh * mine.q.row_tiles;
+        it.whole = it.t0 == 0 && it.t1 == mine.q.key_tiles;
+        it.slot = 2 * (int64_t)worker + (it.t0 == 0 ? 1 : 0);
+        // who has the item, for the join: from this workgroup on, as many more as its further tiles take
+        if (it.t0 == 0 && threadIdx.x == 0 && p.ws_items != nullptr) {
+            const int more = (unsigned)(at - from + places - 1) / (unsigned)mine.length - worker;
+            p.ws_items[(mine.seq * p.hkv + it.kvh) * p.row_tiles + it.rtile] = make_int2(worker, more);
+        }
+        return true;
+    }
+    return false;
 }
 
 // Which of the 32 keys from `start` on a row sees.  Causal: those below `limit`; else by its mask words from key `prior` on.
@@ -114,34 +186,19 @@ template <typename E, int DV, int ROWS, int KT>
 __global__ void __launch_bounds__(256)
 row_join_kernel(RowParams p) {
     constexpr int PER = 1024 / DV, LPR = DV / 4;
-    __shared__ int64_t sums[4];
-    __shared__ int64_t before_seq;
-    const int sub = blockIdx.x % (ROWS / PER), item_at = blockIdx.x / (ROWS / PER);
-    const int rtile = item_at % p.row_tiles, kvh = item_at / p.row_tiles % p.hkv, seq = item_at / p.row_tiles / p.hkv;
+    const int sub = blockIdx.x % (ROWS / PER), item = blockIdx.x / (ROWS / PER);
+    const int rtile = item % p.row_tiles, kvh = item / p.row_tiles % p.hkv, seq = item / p.row_tiles / p.hkv;
     const Seq q = load_seq<ROWS, KT>(p, seq);
-    const int nrows = q.n * p.group;
-    if (rtile * ROWS + sub * PER >= nrows) return;                 // (the whole workgroup)
-    int first, last;
-    int64_t mine;
-    const int64_t line = line_of<ROWS, KT>(p, sums, first, last, mine), piece = piece_of(p, line);
-    for (int s = first; s < last; ++s) {
-        if (s == seq) before_seq = mine;
-        const Seq x = load_seq<ROWS, KT>(p, s);
-        mine += x.items(p) * x.key_tiles;
-    }
-    __syncthreads();
-    const int64_t begin = before_seq + ((int64_t)kvh * q.row_tiles + rtile) * q.key_tiles;
-    const int a = (int)(begin / piece), b = (int)((begin + q.key_tiles - 1) / piece);
-    if (a == b) return;                                            // (one workgroup had it whole)
+    const int2 who = p.ws_items[item];
     const int r = sub * PER + threadIdx.x / LPR, row = rtile * ROWS + r, col = threadIdx.x % LPR * 4;
-    if (row >= nrows) return;
-    auto slot_of = [&](int k) { return 2 * (int64_t)k + (k == a ? 1 : 0); };
+    if (row >= q.n * p.group || who.y == 0) return;            // (no such row: its entry was not written)
+    auto slot_of = [&](int k) { return 2 * (int64_t)(who.x + k) + (k == 0 ? 1 : 0); };
     float top = NEG_BIG;
-    for (int k = a; k <= b; ++k) top = fmaxf(top, p.ws_ml[slot_of(k) * ROWS + r].x);
+    for (int k = 0; k <= who.y; ++k) top = fmaxf(top, p.ws_ml[slot_of(k) * ROWS + r].x);
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll 4
-    for (int k = a; k <= b; ++k) {
+    for (int k = 0; k <= who.y; ++k) {
         const float2 ml = p.ws_ml[slot_of(k) * ROWS + r];
         const f32x4_t x = *(const f32x4_t*)(p.ws_acc + (slot_of(k) * ROWS + r) * DV + col);
         const float f = __builtin_amdgcn_exp2f(ml.x - top);
