@@ -32,14 +32,14 @@ row_attn_kernel(RowParams p) {
     constexpr int NS = DK / 32, NJ = DV / 16;
     constexpr int TILE = KT * KROW + (LATENT ? 0 : KT * VROW);     // bytes per wave
     constexpr int VBASE = LATENT ? 0 : KT * KROW;
-    constexpr int CH = LATENT ? 128 : DV / R;                      // columns that the waves' outputs are joined by at a time
+    constexpr int CH = DV / R;                                     // columns that the waves' outputs are joined by at a time
     constexpr int PER8 = KROW / 128;                               // 1 KB loads per 8 keys
     constexpr bool WIDE = !LATENT && DV >= 128;                    // V rows of whole bank lines
     constexpr int NVA = WIDE ? 8 : 4;                              // V addresses that are no immediates of each other
     static_assert(4 * ROWS * (CH + 4) * 4 <= 4 * TILE, "the join takes the tiles' place");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * TILE];
     __shared__ PieceScratch scratch;
-    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];             // of each wave; then the factors of its output, and of the sum
+    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];             // of each wave
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -78,33 +78,11 @@ row_attn_kernel(RowParams p) {
         const Seq q = mine.q;
         const int kvh = it.kvh, rtile = it.rtile, nrows = q.n * p.group;
 
-        // rows of this lane's columns (beyond the last: that one, computed and not stored)
-        uint4 qf[R][NS];
-        int limit[R];
-        const int64_t* words[R];
-#pragma unroll
-        for (int c = 0; c < R; ++c) {
-            const int row = min(rtile * ROWS + 16 * c + r16, nrows - 1), i = row / p.group;
-            limit[c] = q.prior + i + 1;
-            words[c] = p.masks ? p.masks + (int64_t)(q.begin + i) * p.mask_words : nullptr;
-            const uint16_t* src = (const uint16_t*)p.query + ((int64_t)(q.begin + i) * p.hq + kvh * p.group + row % p.group) * DK;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) qf[c][s] = *(const uint4*)(src + 32 * s + 8 * g4);
-        }
         // keys that all rows here see, and that some may
         const int i_first = rtile * ROWS / p.group, i_last = (min(rtile * ROWS + ROWS, nrows) - 1) / p.group;
         const int full = p.masks ? q.prior : q.prior + i_first + 1;
         const int some = q.ctx == 0 ? 0 : p.masks ? q.ctx : q.prior + i_last + 1;
         const float mul = p.mul * (FP8 ? p.k_scale[kvh] : 1.f);
-
-        float m[R], l[R];
-        f32x4_t O[R][NJ];
-#pragma unroll
-        for (int c = 0; c < R; ++c) {
-            m[c] = NEG_BIG; l[c] = 0.f;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) O[c][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        }
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
         const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
@@ -156,16 +134,39 @@ row_attn_kernel(RowParams p) {
             }
         };
 
+        // the first tile is on its way while the rows are read
         int t = it.t0 + w;
         const int t_end = min(it.t1, (some + KT - 1) / KT);
-        if (FP8 && t < t_end) fetch(t);
+        if (t < t_end) {
+            if constexpr (FP8) fetch(t); else fetch_dma(t);
+        }
+        // rows of this lane's columns (beyond the last: that one, computed and not stored)
+        uint4 qf[R][NS];
+        int limit[R];
+        const int64_t* words[R];
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            const int row = min(rtile * ROWS + 16 * c + r16, nrows - 1), i = row / p.group;
+            limit[c] = q.prior + i + 1;
+            words[c] = p.masks ? p.masks + (int64_t)(q.begin + i) * p.mask_words : nullptr;
+            const uint16_t* src = (const uint16_t*)p.query + ((int64_t)(q.begin + i) * p.hq + kvh * p.group + row % p.group) * DK;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) qf[c][s] = *(const uint4*)(src + 32 * s + 8 * g4);
+        }
+        float m[R], l[R];
+        f32x4_t O[R][NJ];
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            m[c] = NEG_BIG; l[c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) O[c][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
         for (; t < t_end; t += 4) {
             if constexpr (FP8) {
                 stash();
                 if (t + 4 < t_end) fetch(t + 4);
             } else {
-                __builtin_amdgcn_s_waitcnt(0xC07F);                        // lgkmcnt(0): the tile before has been read
-                fetch_dma(t);
                 __builtin_amdgcn_s_waitcnt(0x0F70);                        // vmcnt(0)
                 asm volatile("" ::: "memory");
             }
@@ -196,15 +197,26 @@ row_attn_kernel(RowParams p) {
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int c = 0; c < R; ++c) sa[a][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            // operands are read AHEAD steps before their products (one at a time, a step takes an LDS read's whole latency: 2500 cycles
+            // for the scores of a tile of latent rows, whose products take 600)
+            constexpr int AHEAD = NS < 4 ? NS : 4;
+            uint4 key[AHEAD + 1][2];
+            auto keys_of = [&](int s, uint4* to) __attribute__((always_inline)) {
+                to[0] = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128);
+                to[1] = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128 + 16 * KROW);
+            };
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) keys_of(s, key[s]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                const uint4 a0 = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128);
-                const uint4 a1 = *(const uint4*)(tile + ka[s & 1] + (s >> 1) * 128 + 16 * KROW);
+                if (s + AHEAD < NS) keys_of(s + AHEAD, key[(s + AHEAD) % (AHEAD + 1)]);
 #pragma unroll
                 for (int c = 0; c < R; ++c) {
-                    sa[0][c] = E::mfma(a0, qf[c][s], sa[0][c]);
-                    sa[1][c] = E::mfma(a1, qf[c][s], sa[1][c]);
+                    sa[0][c] = E::mfma(key[s % (AHEAD + 1)][0], qf[c][s], sa[0][c]);
+                    sa[1][c] = E::mfma(key[s % (AHEAD + 1)][1], qf[c][s], sa[1][c]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             uint4 pf[R];
 #pragma unroll
@@ -234,66 +246,71 @@ row_attn_kernel(RowParams p) {
                 pf[c] = make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
                 l[c] = E::pair_sum(pf[c].x, E::pair_sum(pf[c].y, E::pair_sum(pf[c].z, E::pair_sum(pf[c].w, l[c]))));
             }
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                typedef short v4i16_t __attribute__((ext_vector_type(4)));
-                typedef short v8i16_t __attribute__((ext_vector_type(8)));
-                typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+            typedef short v4i16_t __attribute__((ext_vector_type(4)));
+            typedef short v8i16_t __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+            constexpr int VAHEAD = 3;
+            v8i16_t val[VAHEAD + 1];
+            auto value_of = [&](int j) __attribute__((always_inline)) {
                 const uint32_t o = va[j % NVA] + j / NVA * (32 * NVA);
                 const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(tile + o));
                 const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(tile + o + 16 * VROW));
-                const v8i16_t av = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                return v8i16_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            };
 #pragma unroll
-                for (int c = 0; c < R; ++c) O[c][j] = E::mfma(__builtin_bit_cast(uint4, av), pf[c], O[c][j]);
+            for (int j = 0; j < VAHEAD; ++j) val[j] = value_of(j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                if (j + VAHEAD < NJ) val[(j + VAHEAD) % (VAHEAD + 1)] = value_of(j + VAHEAD);
+#pragma unroll
+                for (int c = 0; c < R; ++c) O[c][j] = E::mfma(__builtin_bit_cast(uint4, val[j % (VAHEAD + 1)]), pf[c], O[c][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (!FP8) {
+                if (t + 4 < t_end) {
+                    __builtin_amdgcn_s_waitcnt(0xC07F);                    // lgkmcnt(0): the tile has been read
+                    fetch_dma(t + 4);
+                }
             }
         }
 
-        // The four waves' outputs joined, through the tiles' LDS: factors first, once per row.
+        // The four waves' outputs joined, through the tiles' LDS.
 #pragma unroll
         for (int c = 0; c < R; ++c) {
             l[c] += __shfl_xor(l[c], 16);
             l[c] += __shfl_xor(l[c], 32);
             if (g4 == 0) { sm_m[w][16 * c + r16] = m[c]; sm_l[w][16 * c + r16] = l[c]; }
         }
-        __syncthreads();
-        if (tid < ROWS) {
-            float top = sm_m[0][tid], sum = 0.f;
-#pragma unroll
-            for (int i = 1; i < 4; ++i) top = fmaxf(top, sm_m[i][tid]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f = __builtin_amdgcn_exp2f(sm_m[i][tid] - top);
-                sum = fmaf(f, sm_l[i][tid], sum);
-                sm_m[i][tid] = f;
-            }
-            sm_l[0][tid] = sum == 0.f ? 0.f : (FP8 ? p.v_scale[kvh] : 1.f) / sum;
-            if (!it.whole) p.ws_ml[it.slot * ROWS + tid] = make_float2(top, sum);
-        }
-        __syncthreads();
-        float f[R];
-#pragma unroll
-        for (int c = 0; c < R; ++c) f[c] = sm_m[w][16 * c + r16];
         float* const joint = (float*)lds;
 #pragma unroll
         for (int ch = 0; ch < DV / CH; ++ch) {
-            if (ch > 0) __syncthreads();
+            __syncthreads();                                               // (the tiles, or the columns before, have been read)
 #pragma unroll
             for (int c = 0; c < R; ++c)
 #pragma unroll
                 for (int j = 0; j < CH / 16; ++j)
-                    *(f32x4_t*)(joint + (w * ROWS + 16 * c + r16) * (CH + 4) + 16 * j + 4 * g4) = O[c][ch * (CH / 16) + j] * f[c];
+                    *(f32x4_t*)(joint + (w * ROWS + 16 * c + r16) * (CH + 4) + 16 * j + 4 * g4) = O[c][ch * (CH / 16) + j];
             __syncthreads();
 #pragma unroll
             for (int i0 = 0; i0 < ROWS * (CH / 4); i0 += 256) {
                 const int i = i0 + tid, r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
-                f32x4_t o = *(const f32x4_t*)(joint + r * (CH + 4) + col);
+                float top = sm_m[0][r], sum = 0.f;
 #pragma unroll
-                for (int k = 1; k < 4; ++k) o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col);
+                for (int k = 1; k < 4; ++k) top = fmaxf(top, sm_m[k][r]);
+                f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float f = __builtin_amdgcn_exp2f(sm_m[k][r] - top);
+                    sum = fmaf(f, sm_l[k][r], sum);
+                    o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col) * f;
+                }
                 if (row >= nrows) continue;
                 if (!it.whole) {
                     *(f32x4_t*)(p.ws_acc + (it.slot * ROWS + r) * DV + ch * CH + col) = o;
+                    if (ch == 0 && col == 0) p.ws_ml[it.slot * ROWS + r] = make_float2(top, sum);
                 } else {
-                    const float inv = sm_l[0][r];                          // (0: nothing was seen, and O is 0)
+                    const float inv = sum == 0.f ? 0.f : (FP8 ? p.v_scale[kvh] : 1.f) / sum;   // (0: nothing was seen, and O is 0)
                     uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
                     *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
                 }
