@@ -1,7 +1,7 @@
 // Causal attention of prompts over expanded latent rows on the matrix cores: 16 bits, keys of 128 elements of a head and 64 that all
 // heads share, values of 128.
 //
-// A workgroup has 128 queries of a head, 32 to a wave, and walks the keys in tiles of 64, from the nearest to the farthest, each brought
+// A workgroup has 128 queries of a head (64 in small calls), 32 to a wave, and walks the keys in tiles of 64, from the nearest to the farthest, each brought
 // straight into LDS while the one before is computed:
 //   S^T = K Q^T      six steps of 32 elements, two of them over the shared part; a lane then has four keys of a query per 16
 //   O^T += V^T P^T   weights from registers in that order, V^T out of LDS by transposing reads
@@ -9,6 +9,7 @@
 // The reference of a query moves when a score passes it by 2^8 (row_attn_mfma.hip).
 #include "row_attn.h"
 
+#include <algorithm>
 #include <atomic>
 
 namespace aicomp {
@@ -17,8 +18,6 @@ namespace {
 
 constexpr int NOPE = 128, ROPE = 64, DV = 128;
 constexpr int KT = 64;                 // keys per tile
-constexpr int R = 2;                   // groups of 16 queries per wave
-constexpr int ROWS = 64 * R;
 constexpr int NS = (NOPE + ROPE) / 32, NJ = DV / 16, NH = KT / 16;
 constexpr float NEG_BIG = -1.0e30f, SLACK = 8.f;
 
@@ -39,9 +38,11 @@ struct PromptParams {
     int num_cus;
 };
 
-template <typename E>
+// R: groups of 16 queries per wave
+template <typename E, int R>
 __global__ void __launch_bounds__(256, 2)
 prompt_attn_kernel(PromptParams p) {
+    constexpr int ROWS = 64 * R;
     __shared__ __attribute__((aligned(1024))) unsigned char k0[KT * 2 * NOPE];
     __shared__ __attribute__((aligned(1024))) unsigned char r0[KT * 2 * ROPE];
     __shared__ __attribute__((aligned(1024))) unsigned char v0[KT * 2 * DV];
@@ -49,9 +50,45 @@ prompt_attn_kernel(PromptParams p) {
     __shared__ __attribute__((aligned(1024))) unsigned char r1[KT * 2 * ROPE];
     __shared__ __attribute__((aligned(1024))) unsigned char v1[KT * 2 * DV];
 
-    const int head = blockIdx.x, seq = blockIdx.y;
-    const int qtile = prefill_tile_of_slice(blockIdx.z, gridDim.z, p.num_cus, gridDim.x * gridDim.y);
+    const int head = blockIdx.x;
+    int seq = blockIdx.y, qtile = prefill_tile_of_slice(blockIdx.z, gridDim.z, p.num_cus, gridDim.x * gridDim.y);
     const int tid = threadIdx.x, lane = tid & 63;
+    // Ragged prompts: a tile costs the keys that its last query sees, which differ several-fold, and workgroups start in the order of
+    // the grid.  So the one in place i takes the tile of rank i, the dearest first.  Every workgroup finds it for itself: a tile's rank
+    // is how many tiles of each sequence are dearer, which follows from the sequence's lengths.  (12 prompts of 37 .. 1500 behind 0 ..
+    // 2048, 16 heads: 235 us in the order of the grid, 200 so.)
+    const int nseq = gridDim.y, ntile = gridDim.z;
+    if (nseq > 1 && nseq <= 16 && nseq * ntile <= 512) {                   // grid-uniform
+        int* const tab = (int*)k0;                                         // [nseq][3]: context, prior, tiles; then the one found
+        if (tid < nseq) {
+            const int n = max(0, min(p.cu_q_lens[tid + 1], p.rows) - max(0, p.cu_q_lens[tid]));
+            const int ctx = min(p.cu_k_lens[tid + 1], p.keys) - max(0, p.cu_k_lens[tid]);
+            tab[3 * tid] = ctx;
+            tab[3 * tid + 1] = ctx - n;
+            tab[3 * tid + 2] = min(ntile, (n + ROWS - 1) / ROWS);
+        }
+        if (tid == 0) tab[48] = -1;
+        __syncthreads();
+        // tiles of a sequence that cost more than c
+        auto dearer = [&](int s, int c) {
+            const int ctx = tab[3 * s], prior = tab[3 * s + 1], tiles = tab[3 * s + 2];
+            return ctx <= c ? 0 : max(0, tiles - (c < prior ? 0 : (c - prior) / ROWS));
+        };
+        const int place = blockIdx.y + nseq * blockIdx.z;
+        for (int i = tid; i < nseq * ntile; i += 256) {
+            const int s = i / ntile, t = i - s * ntile;
+            if (t >= tab[3 * s + 2]) continue;
+            const int c = min(tab[3 * s], tab[3 * s + 1] + (t + 1) * ROWS);
+            int rank = 0;
+            for (int o = 0; o < nseq; ++o) rank += o < s ? dearer(o, c - 1) : dearer(o, c);       // (of equal ones, the first sequence's)
+            if (rank == place) { tab[48] = s; tab[49] = t; }
+        }
+        __syncthreads();
+        seq = __builtin_amdgcn_readfirstlane(tab[48]);
+        qtile = __builtin_amdgcn_readfirstlane(tab[49]);
+        if (seq < 0) return;                                               // (more places than tiles)
+        __syncthreads();
+    }
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g4 = lane >> 4;
     const int q_begin = max(0, p.cu_q_lens[seq]), n = min(p.cu_q_lens[seq + 1], p.rows) - q_begin;
@@ -155,19 +192,26 @@ prompt_attn_kernel(PromptParams p) {
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int c = 0; c < R; ++c) sa[h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            uint4 a[NH];
+        // operands are read a step before their products (the order is kept by the barriers)
+        uint4 a[2][NH];
+        auto keys_of = [&](int s, uint4* to) __attribute__((always_inline)) {
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 const int k = 16 * h + r16;
-                a[h] = s < NOPE / 32 ? *(const uint4*)(kb + k * 2 * NOPE + (((4 * s + g4) ^ fk(r16)) << 4))
-                                     : *(const uint4*)(rb + k * 2 * ROPE + (((4 * (s - NOPE / 32) + g4) ^ fk(r16)) << 4));
+                to[h] = s < NOPE / 32 ? *(const uint4*)(kb + k * 2 * NOPE + (((4 * s + g4) ^ fk(r16)) << 4))
+                                      : *(const uint4*)(rb + k * 2 * ROPE + (((4 * (s - NOPE / 32) + g4) ^ fk(r16)) << 4));
             }
+        };
+        keys_of(0, a[0]);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if (s + 1 < NS) keys_of(s + 1, a[(s + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int c = 0; c < R; ++c) sa[h][c] = E::mfma(a[h], qf[c][s], sa[h][c]);
+                for (int c = 0; c < R; ++c) sa[h][c] = E::mfma(a[s & 1][h], qf[c][s], sa[h][c]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         uint4 pf[R][NH / 2];
 #pragma unroll
@@ -203,20 +247,27 @@ prompt_attn_kernel(PromptParams p) {
                 l[c] = E::pair_sum(pf[c][hp].x, E::pair_sum(pf[c][hp].y, E::pair_sum(pf[c][hp].z, E::pair_sum(pf[c][hp].w, l[c]))));
             }
         }
+        typedef short v4i16_t __attribute__((ext_vector_type(4)));
+        typedef short v8i16_t __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+        constexpr int VAHEAD = 5;
+        v8i16_t val[VAHEAD + 1];
+        auto value_of = [&](int u) __attribute__((always_inline)) {            // 16 columns of 32 keys
+            const int j = u >> 1, hp = u & 1;
+            const int o = (32 * hp + vkey) * 2 * DV + (((2 * j + ((r16 >> 1) & 1)) ^ fv(vkey)) << 4) + (r16 & 1) * 8;
+            const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o));
+            const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o + 16 * 2 * DV));
+            return v8i16_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        };
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            typedef short v4i16_t __attribute__((ext_vector_type(4)));
-            typedef short v8i16_t __attribute__((ext_vector_type(8)));
-            typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+        for (int u = 0; u < VAHEAD; ++u) val[u] = value_of(u);
 #pragma unroll
-            for (int hp = 0; hp < NH / 2; ++hp) {
-                const int o = (32 * hp + vkey) * 2 * DV + (((2 * j + ((r16 >> 1) & 1)) ^ fv(vkey)) << 4) + (r16 & 1) * 8;
-                const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o));
-                const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o + 16 * 2 * DV));
-                const v8i16_t av = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        for (int u = 0; u < 2 * NJ; ++u) {
+            if (u + VAHEAD < 2 * NJ) val[(u + VAHEAD) % (VAHEAD + 1)] = value_of(u + VAHEAD);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int c = 0; c < R; ++c) O[c][j] = E::mfma(__builtin_bit_cast(uint4, av), pf[c][hp], O[c][j]);
-            }
+            for (int c = 0; c < R; ++c) O[c][u >> 1] = E::mfma(__builtin_bit_cast(uint4, val[u % (VAHEAD + 1)]), pf[c][u & 1], O[c][u >> 1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -273,12 +324,17 @@ prompt_attn_kernel(PromptParams p) {
     }
 }
 
+template <typename E, int R> void launch(const PromptParams& p, const PromptAttnArgs& a) {
+    const dim3 grid((unsigned)a.heads, (unsigned)a.num_seqs, (unsigned)((a.max_q_len + 64 * R - 1) / (64 * R)));
+    hipLaunchKernelGGL((prompt_attn_kernel<E, R>), grid, dim3(256), 0, a.stream, p);
+}
+
 }  // namespace
 
 bool prompt_attn_mfma_supported(const PromptAttnArgs& a) {
     const int64_t step = (int64_t)1 << 26;                         // (token strides in bytes are 32 bits)
     return is_16bit_float(a.dtype) && a.nope == NOPE && a.rope == ROPE && a.dv == DV && a.num_seqs <= 65535 &&
-           ((int64_t)a.max_q_len + ROWS - 1) / ROWS <= 65535 && a.key_ts < step && a.value_ts < step && a.rope_ts < step;
+           ((int64_t)a.max_q_len + 63) / 64 <= 65535 && a.key_ts < step && a.value_ts < step && a.rope_ts < step;
 }
 
 int launch_prompt_attn_mfma(const PromptAttnArgs& a) {
@@ -303,9 +359,13 @@ int launch_prompt_attn_mfma(const PromptAttnArgs& a) {
         p.num_cus = cus;
         cached_cus.store(cus, std::memory_order_relaxed);
     }
-    const dim3 grid((unsigned)a.heads, (unsigned)a.num_seqs, (unsigned)((a.max_q_len + ROWS - 1) / ROWS));
-    if (a.dtype == AICOMP_KV_F16) hipLaunchKernelGGL(prompt_attn_kernel<F16Fmt>, grid, dim3(256), 0, a.stream, p);
-    else hipLaunchKernelGGL(prompt_attn_kernel<Bf16Fmt>, grid, dim3(256), 0, a.stream, p);
+    // 128 queries to a workgroup read a tile once for twice the queries, where that leaves every CU its workgroups.  us, 64 against 128,
+    // 16 heads: 2048 tokens 46 against 59, 3000 77 against 89, 4096 129 against 124, 8192 412 against 334; 12 prompts of 37 .. 1500
+    // behind 0 .. 2048, 8 heads, 125 against 106
+    const int64_t wgs = a.heads * std::min<int64_t>((int64_t)a.num_seqs * ((a.max_q_len + 127) / 128), a.rows / 128 + a.num_seqs);
+    const bool f16 = a.dtype == AICOMP_KV_F16;
+    if (wgs >= 448) { if (f16) launch<F16Fmt, 2>(p, a); else launch<Bf16Fmt, 2>(p, a); }
+    else { if (f16) launch<F16Fmt, 1>(p, a); else launch<Bf16Fmt, 1>(p, a); }
     AICOMP_HIP_LAUNCH_CHECK();
     return AICOMP_KV_OK;
 }

@@ -155,15 +155,22 @@ row_attn_shared_kernel(RowParams p) {
             for (int h = 0; h < NH; ++h)
 #pragma unroll
                 for (int c = 0; c < R; ++c) sa[h][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            // operands are read a step before their products (the order is kept by the barriers)
+            uint4 a[2][NH];
+            auto keys_of = [&](int s, uint4* to) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < NH; ++h) to[h] = *(const uint4*)(kb + (16 * h + r16) * ROW + (((4 * s + g4) ^ fk(r16)) << 4));
+            };
+            keys_of(0, a[0]);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                uint4 a[NH];
-#pragma unroll
-                for (int h = 0; h < NH; ++h) a[h] = *(const uint4*)(kb + (16 * h + r16) * ROW + (((4 * s + g4) ^ fk(r16)) << 4));
+                if (s + 1 < NS) keys_of(s + 1, a[(s + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
-                    for (int c = 0; c < R; ++c) sa[h][c] = E::mfma(a[h], qf[c][s], sa[h][c]);
+                    for (int c = 0; c < R; ++c) sa[h][c] = E::mfma(a[s & 1][h], qf[c][s], sa[h][c]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             uint4 pf[R][NH / 2];
 #pragma unroll
@@ -200,20 +207,27 @@ row_attn_shared_kernel(RowParams p) {
                     l[c] = E::pair_sum(pf[c][hp].x, E::pair_sum(pf[c][hp].y, E::pair_sum(pf[c][hp].z, E::pair_sum(pf[c][hp].w, l[c]))));
                 }
             }
+            typedef short v4i16_t __attribute__((ext_vector_type(4)));
+            typedef short v8i16_t __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+            constexpr int VAHEAD = FP8 ? 2 : 4;
+            v8i16_t val[VAHEAD + 1];
+            auto value_of = [&](int u) __attribute__((always_inline)) {            // 16 columns of 32 keys
+                const int j = u >> 1, hp = u & 1;
+                const int o = (32 * hp + vkey) * ROW + (((2 * j + ((r16 >> 1) & 1)) ^ fv(vkey)) << 4) + (r16 & 1) * 8;
+                const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o));
+                const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o + 16 * ROW));
+                return v8i16_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            };
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                typedef short v4i16_t __attribute__((ext_vector_type(4)));
-                typedef short v8i16_t __attribute__((ext_vector_type(8)));
-                typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+            for (int u = 0; u < VAHEAD; ++u) val[u] = value_of(u);
 #pragma unroll
-                for (int hp = 0; hp < NH / 2; ++hp) {
-                    const int o = (32 * hp + vkey) * ROW + (((2 * j + ((r16 >> 1) & 1)) ^ fv(vkey)) << 4) + (r16 & 1) * 8;
-                    const v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o));
-                    const v4i16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(vb + o + 16 * ROW));
-                    const v8i16_t av = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+            for (int u = 0; u < 2 * NJ; ++u) {
+                if (u + VAHEAD < 2 * NJ) val[(u + VAHEAD) % (VAHEAD + 1)] = value_of(u + VAHEAD);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int c = 0; c < R; ++c) O[c][j] = E::mfma(__builtin_bit_cast(uint4, av), pf[c][hp], O[c][j]);
-                }
+                for (int c = 0; c < R; ++c) O[c][u >> 1] = E::mfma(__builtin_bit_cast(uint4, val[u % (VAHEAD + 1)]), pf[c][u & 1], O[c][u >> 1]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
 
