@@ -15,7 +15,8 @@ kernels read (``block_table``, ``context_lens``, ``slot_mapping``,
                     ingestion under a per-step token budget, one token per
                     running sequence per decode step, preemption of the
                     youngest sequence when the pool runs dry, release on
-                    finish.  ``schedule()`` returns a ``StepPlan`` whose
+                    finish; steps that check trees of drafted tokens
+                    (``schedule_drafts``, ``keep_drafts``).  ``schedule()`` returns a ``StepPlan`` whose
                     tensors are already on the device: the whole plan is
                     packed into one pinned staging buffer and moved with a
                     single asynchronous copy.  A step of one token per
@@ -35,7 +36,7 @@ from __future__ import annotations
 import os
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Deque, Dict, Iterable, List, Optional
+from typing import Deque, Dict, Iterable, List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -234,6 +235,10 @@ class StepPlan:
     host_cu_q_lens: np.ndarray = None
     host_slot_mapping: np.ndarray = None
     host_positions: np.ndarray = None
+    # a step of drafted tokens (StepPlanner.schedule_drafts): what each row sees of its sequence's rows in this step (ops.tree_masks), and
+    # the trees themselves; positions are then those of the tokens in the text, not in the cache
+    tree_masks: Optional[torch.Tensor] = None
+    parents: Optional[List[List[int]]] = None
     # item lists of this plan, by all that a list follows from (``_list_key``): one list serves every layer of
     # the step.  Not a constructor argument: a plan made by dataclasses.replace starts without any.
     _prefill_items: dict = field(default=None, init=False, repr=False, compare=False)
@@ -318,6 +323,13 @@ class StepPlan:
         too short for the one launch's kernel.  (Others are bit for bit what the one launch gives.)"""
         return self.host_context_lens[:self.num_prefill_seqs] if self.max_q_len < self.launch_q_len(hq, hkv) else None
 
+    def longest_context(self, like: torch.Tensor) -> int:
+        """The longest context, for calls that are sized by it; 0, the table's width, for a call that is recorded into a graph (the
+        lengths of its replays may grow)."""
+        if like.is_cuda and torch.cuda.is_current_stream_capturing():
+            return 0
+        return int(self.host_context_lens.max()) if self.num_seqs else 0
+
     @property
     def num_seqs(self) -> int:
         return len(self.seq_ids)
@@ -337,6 +349,22 @@ class StepPlan:
     @property
     def num_prefill_tokens(self) -> int:
         return int(self.host_cu_q_lens[self.num_prefill_seqs])
+
+
+@dataclass
+class KeptDrafts:
+    """What ``StepPlanner.keep_drafts`` leaves to do in the pools: the arguments of ``ops.keep_rows``, the lengths on the host."""
+    block_table: torch.Tensor             # the plan's
+    first: torch.Tensor                   # [S] int32: the position of each tree's first draft
+    keep: torch.Tensor                    # int32: the drafts kept, ascending in every sequence
+    cu_keep: torch.Tensor                 # [S+1] int32
+
+    @property
+    def moves(self) -> bool:
+        """Whether any row has to move at all (not where the first drafts of every sequence are the ones kept)."""
+        lens = self.cu_keep[1:] - self.cu_keep[:-1]
+        at = torch.arange(self.keep.numel(), dtype=torch.int32) - torch.repeat_interleave(self.cu_keep[:-1], lens)
+        return bool((self.keep != at).any())
 
 
 class _Staging:
@@ -419,6 +447,7 @@ class StepPlanner:
         self.device = torch.device(device)
         self.num_preemptions = 0
         self._arrivals = 0
+        self._drafts: Optional[tuple] = None                  # (plan, rows, lengths before it) of a step of drafts that is still open
         # waiting queue: (seq_id, tokens to ingest, original prompt length, max_new_tokens, arrival, prefix length)
         self.waiting: Deque[tuple] = deque()
         self._waiting_ids = set()
@@ -476,11 +505,16 @@ class StepPlanner:
             return
         self._release_row(r)
 
+    def _no_drafts(self) -> None:
+        if self._drafts is not None:
+            raise ValueError("the last step's drafts are still open: keep_drafts says which of them stay")
+
     def fork(self, seq_id, new_id) -> np.ndarray:
         """A second running sequence ``new_id`` with the tokens of ``seq_id`` so far.  Full blocks are shared (both only read
         them from here on); a partly filled last block is copied: the returned int64 ``[n, 2]`` (source, target) pairs, of
         which there are none or one, go to ``ops.copy_blocks`` (``PagedAttentionBackend.copy_blocks``) on the stream of
         the steps, after the last step and before the next one."""
+        self._no_drafts()
         if seq_id not in self._row_of:
             raise ValueError(f"sequence {seq_id!r} is not running")
         if new_id in self._row_of or new_id in self._waiting_ids:
@@ -507,6 +541,7 @@ class StepPlanner:
         """Move every sequence's blocks to the low end of the pool: int64 ``[n, 2]`` (source, target) pairs for
         ``ops.copy_blocks``, on the stream of the steps, after the last step and before the next one.  Plans made before hold the
         old block ids and must not run any more."""
+        self._no_drafts()
         pairs = self.alloc.compact()
         if pairs.size:
             where = np.arange(self.alloc.num_blocks, dtype=np.int32)
@@ -582,6 +617,7 @@ class StepPlanner:
         """Plan one step.  ``decode`` restricts which running sequences may take their one
         token this step (default: all of them); a driver that ingests a whole batch of prompts
         before its first decode step passes ``()`` until the last prompt is in."""
+        self._no_drafts()
         if (_FAST is not None and decode is None and not self.waiting and not self.check_plans
                 and type(self.alloc) is BlockAllocator):
             plan = self._plan_decode()
@@ -683,6 +719,82 @@ class StepPlanner:
                                np.ones(dec.size + ones.size, dtype=np.int32)])
         return self._pack(rows, lens, len(multi), preempted)
 
+    def schedule_drafts(self, parents: Dict[object, Sequence[int]]) -> StepPlan:
+        """Plan a step that checks drafted tokens: for each of these running sequences, past their prompts, a tree of tokens that
+        follow its last cached one.  ``parents[seq_id][b]`` is the draft (below b) that draft b follows, -1 for one that follows the
+        cached text; usually draft 0 is the token sampled last, whose row is not cached yet, and the only one of those.
+
+        Rows are in the order of the dict, a sequence's drafts in their order, each in a cache slot of its own behind the context;
+        ``positions`` are their places in the text (siblings share one) and ``tree_masks`` says what each sees.  The step is open until
+        ``keep_drafts``; nothing else is planned before.  Raises ``OutOfBlocks`` with nothing changed if the pool cannot hold the
+        drafts (no sequence is preempted for guesses).  ``max_new_tokens`` cuts no tree: the caller keeps as many as it wants.
+        """
+        from . import ops
+        self._no_drafts()
+        if not parents:
+            raise ValueError("no sequences to draft for")
+        trees = [[int(q) for q in tree] for tree in parents.values()]
+        for sid, tree in zip(parents, trees):
+            r = self._row_of.get(sid)
+            if r is None or self._len[r] < self._prompt[r]:
+                raise ValueError(f"sequence {sid!r} is not running, or inside its prompt")
+            if not tree:
+                raise ValueError(f"sequence {sid!r} has no drafts")
+            if int(self._len[r]) + len(tree) > self.max_seq_len:
+                raise ValueError(f"sequence {sid!r} would exceed max_seq_len {self.max_seq_len} with its drafts")
+        masks = ops.tree_masks(trees)                          # (checks the trees)
+        if masks.shape[0] > self.max_num_batched_tokens:
+            raise ValueError(f"{masks.shape[0]} drafts are more than a step's {self.max_num_batched_tokens} tokens")
+        rows = np.asarray([self._row_of[sid] for sid in parents], dtype=np.int64)
+        lens = np.asarray([len(tree) for tree in trees], dtype=np.int32)
+        need = -(-(self._len[rows] + lens) // self.block_size) - self._nblk[rows]
+        fresh, at = self.alloc.allocate(int(np.maximum(need, 0).sum())), 0        # raises OutOfBlocks before anything has changed
+        for r, n in zip(rows, need):
+            if n > 0:
+                self._tab[r, self._nblk[r]:self._nblk[r] + n] = fresh[at:at + n]
+                self._nblk[r] += n
+                at += n
+        depths = np.zeros(masks.shape[0], dtype=np.int64)
+        at = 0
+        for tree in trees:
+            for b, q in enumerate(tree):
+                depths[at + b] = 0 if q < 0 else depths[at + q] + 1
+            at += len(tree)
+        before = self._len[rows].copy()
+        plan = self._pack(rows, lens, rows.size, [], depths)
+        plan.tree_masks, plan.parents = torch.from_numpy(masks).to(self.device), trees
+        self._drafts = (plan, rows, before)
+        return plan
+
+    def keep_drafts(self, plan: StepPlan, kept: Dict[object, Sequence[int]]) -> KeptDrafts:
+        """Close a step of drafts: ``kept[seq_id]`` are the drafts of a sequence that stay, a path of its tree from the cached text on
+        (none, if it is not named).  The sequences continue behind them, blocks that they no longer need are free, and what is
+        returned goes to ``ops.keep_rows`` (``PagedAttentionBackend.keep_drafts``), on the stream of the steps and before the next one."""
+        if self._drafts is None or self._drafts[0] is not plan:
+            raise ValueError("not the plan of the open step of drafts")
+        _, rows, before = self._drafts
+        unknown = [sid for sid in kept if sid not in plan.seq_ids]
+        if unknown:
+            raise ValueError(f"sequence {unknown[0]!r} has no drafts in this step")
+        paths = []
+        for sid, tree in zip(plan.seq_ids, plan.parents):
+            path = [int(b) for b in kept.get(sid, ())]
+            if any(not 0 <= b < len(tree) or tree[b] != (path[i - 1] if i else -1) for i, b in enumerate(path)):
+                raise ValueError(f"sequence {sid!r}: {path} is not a path of its drafts {tree} from the cached text on")
+            paths.append(path)
+        self._drafts = None
+        for i, (sid, r) in enumerate(zip(plan.seq_ids, rows)):
+            if self._row_of.get(sid) != r:                     # (finished meanwhile)
+                paths[i] = []
+                continue
+            self._len[r] = before[i] + len(paths[i])
+            n = self.alloc.blocks_for(int(self._len[r]))
+            self.alloc.free(self._tab[r, n:self._nblk[r]])
+            self._nblk[r] = n
+        i32 = lambda x: torch.from_numpy(np.asarray(x, dtype=np.int32))
+        return KeptDrafts(plan.block_table, i32(before), i32([b for path in paths for b in path]),
+                          i32(np.concatenate([[0], np.cumsum([len(path) for path in paths])])))
+
     def _plan_decode(self) -> Optional[StepPlan]:
         """A step of one token per running sequence (no prompt to ingest, blocks for all), selected and packed natively;
         ``None``, nothing changed, for any other step."""
@@ -709,7 +821,9 @@ class StepPlanner:
             host_context_lens=host[c:c + 4 * S].view(np.int32), host_cu_q_lens=host[c + 4 * S:].view(np.int32),
             host_slot_mapping=host[:8 * S].view(np.int64), host_positions=host[8 * S:16 * S].view(np.int64))
 
-    def _pack(self, rows: np.ndarray, new_lens: np.ndarray, npre: int, preempted: List[object]) -> StepPlan:
+    def _pack(self, rows: np.ndarray, new_lens: np.ndarray, npre: int, preempted: List[object],
+              depths: Optional[np.ndarray] = None) -> StepPlan:
+        # depths: of the tokens of a step of drafts in their trees (positions follow them, and the lengths stay until some are kept)
         S, MB, BS = int(rows.size), self.max_blocks_per_seq, self.block_size
         T = int(new_lens.sum())
         i = self._staging.next()
@@ -743,7 +857,10 @@ class StepPlanner:
                              slot_mapping=None, positions=None, preempted=preempted, host_block_table=bt,
                              host_context_lens=cl, host_cu_q_lens=cu, host_slot_mapping=slot, host_positions=posn)
             check_plan(probe, self.alloc.num_blocks, BS, self.alloc.shared)     # raises before anything reaches the device
-        self._len[rows] = cl
+        if depths is None:
+            self._len[rows] = cl
+        else:
+            posn[:] = np.repeat(start, new_lens) + depths
         self._staging.upload(i, end)
         d32, d64 = self._staging.dev32[i], self._staging.dev64[i]      # (every offset is a multiple of its element size)
         ids = self._id_of
@@ -759,6 +876,14 @@ class StepPlanner:
             host_block_table=bt.copy(), host_context_lens=cl.copy(), host_cu_q_lens=cu.copy(),
             host_slot_mapping=slot.copy(), host_positions=posn.copy(),
         )
+
+
+def tree_attention(plan: StepPlan, out: torch.Tensor, query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, scale: float,
+                   k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One layer's attention for a step of drafts whose rows are in the pools."""
+    from . import ops
+    return ops.paged_tree_attn(out, query, k_pool, v_pool, plan.block_table, plan.context_lens, plan.cu_q_lens, plan.tree_masks, scale,
+                               max_q_len=plan.max_q_len, k_scale=k_scale, v_scale=v_scale, longest_context=plan.longest_context(query))
 
 
 def paged_attention_step(plan: StepPlan, out: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
@@ -777,6 +902,9 @@ def paged_attention_step(plan: StepPlan, out: torch.Tensor, query: torch.Tensor,
     from . import ops
     npre, S = plan.num_prefill_seqs, plan.num_seqs
     t_pre = plan.num_prefill_tokens
+    if plan.tree_masks is not None:
+        ops.kv_append(key, value, k_pool, v_pool, plan.slot_mapping, k_scale, v_scale)
+        return tree_attention(plan, out, query, k_pool, v_pool, scale, k_scale, v_scale)
     items = plan.launch_items(query, k_pool)
     if items is not None:
         # mixed step, decode rows within the measured bounds: every new row appended, then one

@@ -20,7 +20,8 @@ step, the rotary embedding fused with the append followed by the chunked-prefill
 kernel on the prompt-chunk rows and the decode kernel on the one-token rows; a small
 step of one-token rows alone is one launch (``ops.rope_paged_decode_attn``).  A layer may norm its query and key
 heads (``set_head_norm``) and score by a rule (``set_score_rule``: a cap, a bias by distance, a window); its steps
-then run ``ops.qk_norm_rope_kv_append`` and the ``ops.paged_score_*`` calls.
+then run ``ops.qk_norm_rope_kv_append`` and the ``ops.paged_score_*`` calls.  ``LatentAttentionBackend`` is its counterpart for layers
+that cache one latent row a token.  Both take steps of drafted tokens (``ScheduleGeneration.draft_step``).
 """
 from __future__ import annotations
 
@@ -31,7 +32,7 @@ import numpy as np
 import torch
 
 from . import ops
-from .block_manager import StepPlan, StepPlanner
+from .block_manager import KeptDrafts, StepPlan, StepPlanner, tree_attention
 
 
 class PagedAttentionBackend:
@@ -105,6 +106,11 @@ class PagedAttentionBackend:
         if pairs.shape[0]:
             ops.copy_blocks(self.k_pools + self.v_pools, pairs)
 
+    def keep_drafts(self, kept: KeptDrafts) -> None:
+        """The rows of kept drafts moved together in every layer's pools: what ``StepPlanner.keep_drafts`` returns."""
+        if kept.moves:
+            ops.keep_rows(self.k_pools + self.v_pools, kept.block_table, kept.first, kept.keep, kept.cu_keep)
+
     def set_scales(self, layer_idx: int, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
         """Per-KV-head dequantisation scales of an fp8 pool."""
         self.k_scales[layer_idx] = k_scale.to(self.device, torch.float32).contiguous()
@@ -164,7 +170,9 @@ class PagedAttentionBackend:
         ks, vs = self.k_scales[layer_idx], self.v_scales[layer_idx]
         norm = self._norms.get(layer_idx)
         ruled = layer_idx in self._rules or self.first_keys is not None or self.prefix_lens is not None
-        if ruled or norm is not None or self._pairs_only:
+        if ruled and plan.tree_masks is not None:
+            raise RuntimeError(f"layer {layer_idx} scores by a rule: trees of drafts are attended without one")
+        if ruled or norm is not None or self._pairs_only or plan.tree_masks is not None:
             q = torch.empty(query.shape, dtype=query.dtype, device=query.device)
             if norm is not None or self._pairs_only:
                 q_weight, k_weight, eps = norm or (None, None, 0.0)
@@ -196,9 +204,11 @@ class PagedAttentionBackend:
         return self._attend(layer_idx, out, q)
 
     def _attend(self, layer_idx: int, out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
-        """Causal attention of a step whose rows are in the pools."""
+        """Causal attention of a step whose rows are in the pools, or that of its trees of drafts."""
         plan, kp, vp = self.plan, self.k_pools[layer_idx], self.v_pools[layer_idx]
         ks, vs = self.k_scales[layer_idx], self.v_scales[layer_idx]
+        if plan.tree_masks is not None:
+            return tree_attention(plan, out, q, kp, vp, self.scale, ks, vs)
         npre, S, t_pre = plan.num_prefill_seqs, plan.num_seqs, plan.num_prefill_tokens
         items = plan.launch_items(q, kp)
         if items is not None:                      # mixed step: chunks and decode rows in one launch
@@ -222,8 +232,129 @@ class PagedAttentionBackend:
         return out
 
 
+class LatentAttentionBackend:
+    """Per-layer paged pools of latent rows plus the per-step attention call of a decoder layer with latent attention.
+
+    A token's cache row is one latent vector of ``latent_dim`` elements, normed, and ``rope_dim`` rotated ones, shared by all heads.
+    ``set_layer`` gives a layer its norm and the two halves of its up-projection, ``w_k [H, N, C]`` (latent to a head's key) and
+    ``w_v [H, V, C]`` (to its value); they are laid out once.  Prompts that start a sequence are attended in the expanded form (keys and
+    values of every head made by one product, ``ops.latent_prompt_attn``) where N, D and V are multiples of 16; all other rows, one token per
+    sequence, later chunks and trees of drafts, over the latent rows themselves, ``w_k`` multiplied into the queries and ``w_v`` into
+    the output.
+    """
+
+    def __init__(self, num_layers: int, num_blocks: int, latent_dim: int, rope_dim: int, inv_freq: torch.Tensor,
+                 scale: float, dtype: torch.dtype = torch.bfloat16, device="cuda", max_positions: int = 8192,
+                 attention_scaling: float = 1.0, interleaved: bool = False, block_size: int = 16) -> None:
+        self.device, self.dtype = torch.device(device), dtype
+        self.latent_dim, self.rope_dim, self.scale, self.interleaved = int(latent_dim), int(rope_dim), float(scale), bool(interleaved)
+        if 2 * inv_freq.numel() != rope_dim:
+            raise ValueError(f"{inv_freq.numel()} frequencies for {rope_dim} rotated elements")
+        self.pools = [torch.zeros((num_blocks, block_size, latent_dim + rope_dim), dtype=dtype, device=self.device)
+                      for _ in range(num_layers)]
+        self.cos, self.sin = ops.rotary_pair_tables(inv_freq, max_positions, attention_scaling, self.device)
+        self.plan: Optional[StepPlan] = None
+        self._layers: Dict[int, tuple] = {}
+
+    @property
+    def num_positions(self) -> int:
+        return self.cos.shape[0]
+
+    def set_layer(self, layer_idx: int, w_k: torch.Tensor, w_v: torch.Tensor, norm_weight: Optional[torch.Tensor] = None,
+                  eps: float = 1e-6) -> None:
+        if w_k.dim() != 3 or w_v.dim() != 3 or w_k.shape[0] != w_v.shape[0] or w_k.shape[2] != self.latent_dim \
+                or w_v.shape[2] != self.latent_dim:
+            raise ValueError(f"w_k and w_v must be [H, N, {self.latent_dim}] and [H, V, {self.latent_dim}]; got {tuple(w_k.shape)} and "
+                             f"{tuple(w_v.shape)}")
+        H, N, C = w_k.shape
+        w_k, w_v = w_k.to(self.device, self.dtype), w_v.to(self.device, self.dtype)
+        both = torch.cat((w_k, w_v), dim=1).reshape(H * (N + w_v.shape[1]), C)              # rows: a head's key, then its value
+        weight = None if norm_weight is None else norm_weight.to(self.device, torch.float32).contiguous()
+        self._layers[layer_idx] = (w_k.contiguous(), w_v.transpose(1, 2).contiguous(), both.t().contiguous(), weight, float(eps))
+
+    def begin_step(self, plan: StepPlan) -> None:
+        self.plan = plan
+
+    def copy_blocks(self, pairs) -> None:
+        """Blocks copied in every layer's pool: what ``StepPlanner.fork`` and ``compact`` return."""
+        pairs = torch.from_numpy(np.ascontiguousarray(pairs, dtype=np.int64))
+        if pairs.shape[0]:
+            ops.copy_blocks(self.pools, pairs)
+
+    def keep_drafts(self, kept: KeptDrafts) -> None:
+        """The rows of kept drafts moved together in every layer's pool: what ``StepPlanner.keep_drafts`` returns."""
+        if kept.moves:
+            ops.keep_rows(self.pools, kept.block_table, kept.first, kept.keep, kept.cu_keep)
+
+    def _absorbed(self, layer_idx: int, out: torch.Tensor, query: torch.Tensor, q: torch.Tensor, **rows) -> None:
+        """``out [t, H, V]`` of rows over the latent rows: ``query``'s first N elements, multiplied by w_k, go before the rotated ones,
+        which are in ``q [t, H, C + D]`` already."""
+        w_k, w_v, _, _, _ = self._layers[layer_idx]
+        H, N, C = w_k.shape
+        q[..., :C] = torch.bmm(query[..., :N].transpose(0, 1), w_k).transpose(0, 1)
+        o = torch.empty((q.shape[0], H, C), dtype=self.dtype, device=q.device)
+        ops.paged_latent_attn(o, q, self.pools[layer_idx], scale=self.scale, **rows)
+        out.copy_(torch.bmm(o.transpose(0, 1), w_v).transpose(0, 1))
+
+    def attend(self, layer_idx: int, query: torch.Tensor, latent: torch.Tensor) -> torch.Tensor:
+        """``query [T, H, N + D]`` and ``latent [T, C + D]`` as projected, in the plan's row order -> ``[T, H, V]``."""
+        plan, pool = self.plan, self.pools[layer_idx]
+        if plan is None:
+            raise RuntimeError("LatentAttentionBackend.attend called outside a step (begin_step first)")
+        if layer_idx not in self._layers:
+            raise RuntimeError(f"layer {layer_idx} has no weights (set_layer first)")
+        w_k, w_v, w_both, weight, eps = self._layers[layer_idx]
+        H, N, C = w_k.shape
+        V, D = w_v.shape[2], self.rope_dim
+        T, S, npre, t = query.shape[0], plan.num_seqs, plan.num_prefill_seqs, plan.num_prefill_tokens
+        if tuple(query.shape) != (T, H, N + D):
+            raise RuntimeError(f"query must be [T, {H}, {N + D}], got {tuple(query.shape)}")
+        fresh = npre > 0 and plan.tree_masks is None and N % 16 == 0 and D % 16 == 0 and V % 16 == 0 and \
+            bool((plan.host_context_lens[:npre] == plan.new_lens[:npre]).all())
+        # the rotated parts go where they are read: behind the place of the multiplied ones, or by themselves where fresh prompts
+        # need them with the projected ones (rows of C + D for all their heads would be gigabytes that nothing reads)
+        q = torch.empty((T, H, D if fresh else C + D), dtype=self.dtype, device=query.device)
+        rows = torch.empty_like(latent) if fresh else None
+        ops.latent_kv_append(latent, weight, self.cos, self.sin, plan.positions, pool, plan.slot_mapping, eps, self.interleaved,
+                             query[..., N:], q if fresh else q[..., C:], rows)
+        longest = plan.longest_context(query)
+        out = torch.empty((T, H, V), dtype=self.dtype, device=query.device)
+        if fresh:
+            expanded = torch.mm(rows[:t, :C], w_both).view(t, H, N + V)
+            ops.latent_prompt_attn(out[:t], torch.cat((query[:t, :, :N], q[:t]), dim=-1), expanded[..., :N], rows[:t, C:],
+                                   expanded[..., N:], plan.cu_q_lens[:npre + 1], plan.cu_q_lens[:npre + 1], self.scale, plan.max_q_len)
+            if S > npre:
+                q = torch.cat((q.new_empty((T - t, H, C)), q[t:]), dim=-1)
+        elif npre:
+            self._absorbed(layer_idx, out[:t], query[:t], q[:t], block_table=plan.block_table[:npre],
+                           context_lens=plan.context_lens[:npre], cu_q_lens=plan.cu_q_lens[:npre + 1], max_q_len=plan.max_q_len,
+                           tree_masks=plan.tree_masks, longest_context=longest)
+            q = q[t:]
+        if S > npre:
+            self._absorbed(layer_idx, out[t:], query[t:], q, block_table=plan.block_table[npre:],
+                           context_lens=plan.context_lens[npre:], longest_context=longest)
+        return out
+
+
+def accept_drafts(tokens: Sequence[int], parents: Sequence[int], picks: Sequence[int]) -> tuple:
+    """Which drafts of one tree stay: ``tokens[b]`` follows ``tokens[parents[b]]`` (or, at -1, the text), and the model picks
+    ``picks[b]`` after draft b.  Draft 0, which has to follow the text, stays, and from each draft that stays the first child that is the
+    token picked there does.  Returns the drafts that stay and the pick after the last of them, the next token: what a step per token
+    would have given, with as many of its tokens as were guessed."""
+    if len(tokens) != len(parents) or len(picks) != len(tokens) or not len(tokens) or parents[0] != -1:
+        raise ValueError("tokens, parents and picks are those of one tree whose draft 0 follows the text")
+    kept = [0]
+    while True:
+        pick = int(picks[kept[-1]])
+        child = next((b for b in range(kept[-1] + 1, len(tokens)) if parents[b] == kept[-1] and int(tokens[b]) == pick), None)
+        if child is None:
+            return kept, pick
+        kept.append(child)
+
+
 class ScheduleGeneration:
-    """``prefill`` / ``decode_step`` / ``clear_cache`` over a token-major model and a planner."""
+    """``prefill`` / ``decode_step`` / ``clear_cache`` over a token-major model and a planner; ``draft_step`` / ``keep_drafts`` for
+    several guessed tokens a step."""
 
     def __init__(self, model: Callable[[torch.Tensor, torch.Tensor], torch.Tensor],
                  backend: PagedAttentionBackend, planner: StepPlanner) -> None:
@@ -240,6 +371,7 @@ class ScheduleGeneration:
         self.planner = planner
         self._batch: List[object] = []
         self._offset: Dict[object, int] = {}
+        self._draft_plan: Optional[StepPlan] = None
 
     # one planner step: returns {seq_id: logits row of its last new token}
     @torch.no_grad()
@@ -313,6 +445,31 @@ class ScheduleGeneration:
             raise RuntimeError("not every sequence could be scheduled in this decode step")
         return torch.stack([got[b] for b in self._batch])
 
+    @torch.no_grad()
+    def draft_step(self, tokens: Sequence[Sequence[int]], parents: Sequence[Sequence[int]]) -> List[torch.Tensor]:
+        """A tree of drafted tokens per sequence, ``tokens[b]`` with ``parents[b]`` (``StepPlanner.schedule_drafts``): the logits after
+        every draft, one ``[n, V]`` tensor per batch row.  ``keep_drafts`` has to follow."""
+        if len(tokens) != len(self._batch) or len(parents) != len(self._batch):
+            raise ValueError(f"draft_step needs one tree per sequence: got {len(tokens)} for batch {len(self._batch)}")
+        if any(len(t) != len(p) for t, p in zip(tokens, parents)):
+            raise ValueError("draft_step needs one parent per token")
+        plan = self.planner.schedule_drafts({b: p for b, p in zip(self._batch, parents)})
+        ids = torch.as_tensor([int(x) for row in tokens for x in row], dtype=torch.int64).to(self.backend.device)
+        self.backend.begin_step(plan)
+        logits = self.model(ids, plan.positions)
+        self._draft_plan = plan
+        return list(logits.split([len(t) for t in tokens]))
+
+    def keep_drafts(self, kept: Sequence[Sequence[int]]) -> None:
+        """The drafts of the last ``draft_step`` that stay, one path per batch row (``accept_drafts``)."""
+        if self._draft_plan is None:
+            raise ValueError("keep_drafts follows draft_step")
+        if len(kept) != len(self._batch):
+            raise ValueError(f"keep_drafts needs one path per sequence: got {len(kept)} for batch {len(self._batch)}")
+        moved = self.planner.keep_drafts(self._draft_plan, {b: k for b, k in zip(self._batch, kept)})
+        self._draft_plan = None
+        self.backend.keep_drafts(moved)
+
     def fork(self, row: int) -> int:
         """A second sequence with the tokens of batch row ``row`` so far (several continuations of one prompt): the new batch
         row, the last one.  Its full blocks are shared, its last block is copied in every layer's pools."""
@@ -324,6 +481,9 @@ class ScheduleGeneration:
 
     def clear_cache(self) -> None:
         """Release every sequence of the current batch (schedule_infer.py:451-454)."""
+        if self._draft_plan is not None:                       # (a step of drafts that was left open)
+            self.planner.keep_drafts(self._draft_plan, {})
+            self._draft_plan = None
         for b in self._batch:
             try:
                 self.planner.finish(b)

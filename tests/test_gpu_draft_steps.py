@@ -1,0 +1,299 @@
+"""Models that check drafted tokens several at a time, end to end: append, tree attention, the accepted rows moved together, plain steps
+after them; over K and V pools, and over latent rows with prompts in the expanded form.
+
+The models run in float32, where every kernel sums in float32: their logits are a few hundred float32 roundings of two small layers away
+from the exact ones, 2^-24 each, so less than 1e-3 of the logits' scale by a wide margin.  The picks of the exact model (float64, on the
+CPU, the whole text at every step) lie at least 2e-3 of that scale apart, which each test asserts of its input: the tokens are equal.
+"""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from aicomp_amd.block_manager import StepPlanner
+from aicomp_amd.generation import LatentAttentionBackend, PagedAttentionBackend, ScheduleGeneration, accept_drafts
+from tiny_llama import TinyLlama
+
+pytestmark = pytest.mark.gpu
+VOCAB, NEW = 199, 24
+
+
+class TinyLatent:
+    """Two layers of latent attention with random weights: one plain form over the whole text, one over a backend."""
+
+    def __init__(self, hidden=192, layers=2, heads=5, n=24, d=16, c=64, v=40, seed=3):
+        g = torch.Generator().manual_seed(seed)
+        w = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64) / math.sqrt(s[-1])
+        self.heads, self.n, self.d, self.c, self.v, self.layers = heads, n, d, c, v, layers
+        self.embed, self.head = torch.randn(VOCAB, hidden, generator=g, dtype=torch.float64), w(VOCAB, hidden)
+        self.q = [w(heads * (n + d), hidden) for _ in range(layers)]
+        self.down = [w(c + d, hidden) for _ in range(layers)]
+        self.up = [w(heads, n + v, c) for _ in range(layers)]
+        self.o = [w(hidden, heads * v) for _ in range(layers)]
+        self.weight = [1 + 0.2 * torch.randn(c, generator=g, dtype=torch.float64) for _ in range(layers)]
+        self.inv_freq = 1.0 / 10000.0 ** (torch.arange(0, d, 2, dtype=torch.float64) / d)
+        self.scale = 1 / math.sqrt(n + d)
+
+    @staticmethod
+    def norm(x):
+        return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6)
+
+    def exact(self, ids):
+        """ids [S] -> logits [S, V] in float64."""
+        x, S = self.embed[ids], len(ids)
+        angle = torch.arange(S, dtype=torch.float64)[:, None] * self.inv_freq
+        def turn(t, cos, sin):
+            a, b = t.chunk(2, -1)
+            return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+        for i in range(self.layers):
+            h = self.norm(x)
+            q = (h @ self.q[i].T).view(S, self.heads, -1)
+            down = h @ self.down[i].T
+            row = self.norm(down[:, :self.c]) * self.weight[i]
+            up = torch.einsum("sc,hnc->shn", row, self.up[i])
+            k = torch.cat((up[..., :self.n], turn(down[:, self.c:], angle.cos(), angle.sin())[:, None].expand(S, self.heads, self.d)), -1)
+            q = torch.cat((q[..., :self.n], turn(q[..., self.n:], angle.cos()[:, None], angle.sin()[:, None])), -1)
+            score = torch.einsum("qhd,khd->hqk", q, k) * self.scale
+            score = score.masked_fill(torch.ones(S, S, dtype=torch.bool).triu(1), -math.inf)
+            x = x + torch.einsum("hqk,khv->qhv", score.softmax(-1), up[..., self.n:]).reshape(S, -1) @ self.o[i].T
+        return self.norm(x) @ self.head.T
+
+    def backend(self, num_blocks, device, max_positions):
+        b = LatentAttentionBackend(self.layers, num_blocks, self.c, self.d, self.inv_freq, self.scale, torch.float32, device, max_positions)
+        for i in range(self.layers):
+            b.set_layer(i, self.up[i][:, :self.n], self.up[i][:, self.n:], self.weight[i])
+        return b
+
+    def paged(self, ids, backend):
+        to = lambda t: t.to(ids.device, torch.float32)
+        x = to(self.embed)[ids]
+        for i in range(self.layers):
+            h = self.norm(x)
+            a = backend.attend(i, F.linear(h, to(self.q[i])).view(len(ids), self.heads, -1), F.linear(h, to(self.down[i])))
+            x = x + F.linear(a.flatten(1), to(self.o[i]))
+        return F.linear(self.norm(x), to(self.head))
+
+
+class Llama:
+    def __init__(self, **kw):
+        self.m = TinyLlama(vocab=VOCAB, seed=2, **kw).double()
+        self.m.inv_freq = self.m.inv_freq.float()
+
+    @torch.no_grad()
+    def exact(self, ids):
+        return self.m.forward_naive(torch.as_tensor(ids)[None])[0]
+
+    def backend(self, num_blocks, device, max_positions):
+        self.m = self.m.float().to(device)
+        return PagedAttentionBackend(self.m.layers, num_blocks, self.m.hkv, self.m.d, torch.float32, device, inv_freq=self.m.inv_freq,
+                                     max_positions=max_positions)
+
+    def paged(self, ids, backend):
+        return self.m.forward_paged(ids, backend.plan.positions, backend)
+
+
+def exact_texts(model, prompts):
+    texts = []
+    for p in prompts:
+        text = list(p)
+        for _ in range(NEW):
+            logits = model.exact(text)[-1]
+            top = logits.topk(2).values
+            assert float(top[0] - top[1]) > 2e-3 * float(logits.abs().max())
+            text.append(int(logits.argmax()))
+        texts.append(text)
+    return texts
+
+
+def drafts_for(text, at, g):
+    """A tree below the token ``text[at]``: each level holds the right continuation with a chance of 3 in 4, and wrong ones."""
+    tokens, parents, right = [text[at]], [-1], 0
+    for level in range(int(torch.randint(0, 5, (1,), generator=g))):
+        here = []
+        for _ in range(int(torch.randint(1, 4, (1,), generator=g))):
+            tokens.append(int(torch.randint(0, VOCAB, (1,), generator=g)))
+            parents.append(right if right is not None else int(torch.randint(0, len(tokens) - 1, (1,), generator=g)))
+            here.append(len(tokens) - 1)
+        hit = right is not None and at + level + 1 < len(text) and int(torch.randint(0, 4, (1,), generator=g)) > 0
+        if hit:
+            tokens[here[int(torch.randint(0, len(here), (1,), generator=g))]] = text[at + level + 1]
+        right = next((b for b in here if hit and tokens[b] == text[at + level + 1]), None)
+    return tokens, parents
+
+
+def generate(model, prompts, texts, device, chunk, seed):
+    """Prompts, then drafts until every text is long enough, with a plain step now and then."""
+    g = torch.Generator().manual_seed(seed)
+    planner = StepPlanner(num_blocks=64, max_seqs=8, max_seq_len=128, max_num_batched_tokens=96, prefill_chunk=chunk, device=device,
+                          check_plans=True)
+    backend = model.backend(64, device, 128)
+    gen = ScheduleGeneration(lambda ids, pos: model.paged(ids, backend), backend, planner)
+    lens = [len(p) for p in prompts]
+    ids = torch.zeros(len(prompts), max(lens), dtype=torch.int64)
+    for b, p in enumerate(prompts):
+        ids[b, :lens[b]] = torch.tensor(p)
+    got = [list(p) for p in prompts]
+    nxt = gen.prefill(ids.to(device), prompt_lens=lens).argmax(-1).tolist()
+    accepted = steps = 0
+    while min(len(t) - n for t, n in zip(got, lens)) < NEW:
+        steps += 1
+        if steps % 4 == 0:
+            logits = gen.decode_step(torch.tensor(nxt, device=device))
+            for b in range(len(got)):
+                got[b].append(nxt[b])
+            nxt = logits.argmax(-1).tolist()
+            continue
+        trees = []
+        for b, t in enumerate(got):
+            known = (texts[b] + [0] * 40)
+            tokens, parents = drafts_for(known, len(t), g) if len(t) < len(texts[b]) else ([nxt[b]], [-1])
+            tokens[0] = nxt[b]
+            trees.append((tokens, parents))
+        picks = [x.argmax(-1).tolist() for x in gen.draft_step([t for t, _ in trees], [p for _, p in trees])]
+        kept = []
+        for b, (tokens, parents) in enumerate(trees):
+            path, nxt[b] = accept_drafts(tokens, parents, picks[b])
+            got[b] += [tokens[i] for i in path]
+            kept.append(path)
+            accepted += len(path) - 1
+        gen.keep_drafts(kept)
+    assert accepted > 10                                       # (of the drafts, some were right)
+    gen.clear_cache()
+    assert planner.alloc.num_used == 0
+    return got
+
+
+def prompts_of(lens, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, VOCAB, (n,), generator=g).tolist() for n in lens]
+
+
+@pytest.mark.parametrize("chunk", [64, 16])
+@pytest.mark.parametrize("name", ["llama", "latent", "latent_expanded"])
+def test_drafts_give_the_tokens_of_single_steps(device, name, chunk):
+    model = Llama() if name == "llama" else TinyLatent() if name == "latent" else TinyLatent(n=32, v=48, seed=1)
+    prompts = prompts_of([37, 5, 61, 16], seed=11)
+    texts = exact_texts(model, prompts)
+    got = generate(model, prompts, texts, device, chunk, seed=chunk)
+    for have, want in zip(got, texts):
+        n = min(len(have), len(want))
+        assert have[:n] == want[:n]
+
+
+def test_a_step_left_open_ends_with_its_batch(device):
+    model = Llama()
+    backend = model.backend(16, device, 64)
+    planner = StepPlanner(num_blocks=16, max_seqs=2, max_seq_len=64, device=device)
+    gen = ScheduleGeneration(lambda ids, pos: model.paged(ids, backend), backend, planner)
+    with pytest.raises(ValueError, match="follows draft_step"):
+        gen.keep_drafts([])
+    prompt = torch.tensor([prompts_of([7], 1)[0]], device=device)
+    gen.prefill(prompt)
+    with pytest.raises(ValueError, match="one tree per sequence"):
+        gen.draft_step([[1], [2]], [[-1], [-1]])
+    with pytest.raises(ValueError, match="one parent per token"):
+        gen.draft_step([[1, 2]], [[-1]])
+    first = gen.draft_step([[3, 4]], [[-1, 0]])
+    with pytest.raises(ValueError, match="still open"):
+        gen.decode_step(torch.tensor([3], device=device))
+    gen.clear_cache()
+    gen.prefill(prompt)
+    again = gen.draft_step([[3, 4]], [[-1, 0]])
+    gen.keep_drafts([[0, 1]])
+    assert planner.context_len(0) == 9 and torch.equal(first[0], again[0])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_latent_attention_of_a_mixed_step(device, interleaved):
+    """One layer in bfloat16 with 20 heads of 128 + 64 over rows of 512 + 64: two fresh prompts, then a chunk behind one of them next to
+    a token of the other, then fresh prompts next to tokens, against the formula in float64 on the bfloat16 inputs.
+
+    Bound, from roundings of u = 2^-8 relative each, independent of one another: a sum of errors within +-c_i passes 7 sqrt(sum c_i^2)
+    with a chance of 2 e^-24.5 (Hoeffding), 1e-5 over all elements here.  A score: of the row and the multiplied query (absorbed), of the
+    row and the key made of it (expanded), of the rotated parts, ds = 7 u scale sqrt(2 sum_c q'_c^2 r_c^2 + sum_n q_n^2 k_n^2 + 2 sum_d ..);
+    the mean moves by (e^(2 ds) - 1) sum_j p_j |v_j - out|.  The value: the rows', the rounded mean's, the weights' and the expanded
+    values' own; the result's, u.
+    """
+    from aicomp_amd.block_manager import StepPlanner
+    H, N, D, C, V = 20, 128, 64, 512, 128
+    bf, g = torch.bfloat16, torch.Generator().manual_seed(4)
+    w_k = (torch.randn(H, N, C, generator=g) / math.sqrt(C)).to(bf)
+    w_v = (torch.randn(H, V, C, generator=g) / math.sqrt(C)).to(bf)
+    weight = 1 + 0.2 * torch.randn(C, generator=g)
+    inv = 1.0 / 10000.0 ** (torch.arange(0, D, 2, dtype=torch.float64) / D)
+    scale = 0.1 / math.sqrt(N + D)
+    backend = LatentAttentionBackend(1, 32, C, D, inv, scale, bf, device, 256, interleaved=interleaved)
+    with pytest.raises(RuntimeError, match="outside a step"):
+        backend.attend(0, torch.empty(1, H, N + D, dtype=bf, device=device), torch.empty(1, C + D, dtype=bf, device=device))
+    planner = StepPlanner(num_blocks=32, max_seqs=8, max_seq_len=256, max_num_batched_tokens=128, prefill_chunk=48, device=device,
+                          check_plans=True)
+    cos, sin = [t.double().cpu() for t in (backend.cos, backend.sin)]
+    query, latent = {}, {}
+
+    def turn(x, pos):
+        c, s = cos[pos], sin[pos]
+        if x.dim() == 3:
+            c, s = c[:, None], s[:, None]
+        if interleaved:
+            a, b = x[..., 0::2], x[..., 1::2]
+            return torch.stack((a * c - b * s, b * c + a * s), -1).flatten(-2)
+        a, b = x.chunk(2, -1)
+        return torch.cat((a * c - b * s, b * c + a * s), -1)
+
+    def run(plan):
+        backend.begin_step(plan)
+        if not backend._layers:
+            with pytest.raises(RuntimeError, match="no weights"):
+                backend.attend(0, None, None)
+            backend.set_layer(0, w_k, w_v, weight)
+        q = torch.randn(plan.total_new_tokens, H, N + D, generator=g).to(bf)
+        x = torch.randn(plan.total_new_tokens, C + D, generator=g).to(bf)
+        out = backend.attend(0, q.to(device), x.to(device)).double().cpu()
+        cu = plan.host_cu_q_lens
+        for r, sid in enumerate(plan.seq_ids):
+            mine, n = slice(int(cu[r]), int(cu[r + 1])), int(cu[r + 1] - cu[r])
+            latent[sid] = torch.cat((latent.get(sid, x[:0]), x[mine]))
+            L = len(latent[sid])
+            xs, pos = latent[sid].double(), torch.arange(L)
+            row = xs[:, :C] * torch.rsqrt(xs[:, :C].pow(2).mean(-1, keepdim=True) + 1e-6) * weight.double()
+            rk = turn(xs[:, C:], pos)
+            qs = q[mine].double()
+            qr = turn(qs[..., N:], pos[L - n:])
+            k, v = [torch.einsum("hnc,sc->shn", w.double(), row) for w in (w_k, w_v)]
+            see = torch.arange(L) <= torch.arange(L - n, L)[:, None]
+            score = scale * (torch.einsum("qhn,shn->hqs", qs[..., :N], k) + torch.einsum("qhd,sd->hqs", qr, rk))
+            p = score.masked_fill(~see, -math.inf).softmax(-1)
+            want = torch.einsum("hqs,shv->qhv", p, v)
+            u = 2.0 ** -8
+            qa = torch.einsum("qhn,hnc->qhc", qs[..., :N], w_k.double())
+            ds = (2 * torch.einsum("qhc,sc->qhs", qa ** 2, row ** 2) + torch.einsum("qhn,shn->qhs", qs[..., :N] ** 2, k ** 2)
+                  + 2 * torch.einsum("qhd,sd->qhs", qr ** 2, rk ** 2))
+            ds = 7 * u * scale * ds.masked_fill(~see[:, None], 0).amax(-1, keepdim=True).sqrt()
+            spread = torch.stack([torch.einsum("hs,shv->hv", p[:, i], (v - want[i]).abs()) for i in range(n)])
+            w2, o = w_v.double() ** 2, torch.einsum("hqs,sc->qhc", p, row)
+            of_rows = torch.einsum("hvc,qhc->qhv", w2, torch.einsum("hqs,sc->qhc", p ** 2, row ** 2))
+            of_mean = torch.einsum("hvc,qhc->qhv", w2, o ** 2)
+            of_values = torch.einsum("hqs,shv->qhv", p ** 2, v ** 2)
+            tol = 7 * u * (of_rows + of_mean + 2 * of_values).sqrt() + torch.expm1(2 * ds) * spread + u * want.abs()
+            err = (out[mine] - want).abs()
+            assert bool((err <= tol).all()), (sid, float((err / tol).max()))
+            assert float(tol.mean()) < 0.3 * float(v.pow(2).mean().sqrt())             # (no idle bound)
+
+    planner.add_request("a", 40)
+    planner.add_request("b", 60)
+    run(planner.schedule(decode=()))                           # fresh: a whole, 48 of b
+    run(planner.schedule())                                    # a's token, b's last 12
+    planner.add_request("c", 33)
+    planner.add_request("d", 1)
+    run(planner.schedule())                                    # c and d fresh, tokens of a and b
+    plan = planner.schedule_drafts({"a": [-1, 0, 0, 2], "b": [-1], "d": [-1, 0]})
+    backend.begin_step(plan)
+    assert torch.isfinite(backend.attend(0, torch.randn(7, H, N + D, generator=g).to(device, bf),
+                                         torch.randn(7, C + D, generator=g).to(device, bf))).all()
+    moved = planner.keep_drafts(plan, {"a": [0, 2]})
+    before = backend.pools[0].clone()
+    backend.keep_drafts(moved)
+    f = int(moved.first[0])
+    tab = plan.host_block_table[0]
+    assert torch.equal(backend.pools[0][tab[(f + 1) // 16], (f + 1) % 16], before[tab[(f + 2) // 16], (f + 2) % 16])
