@@ -4,6 +4,10 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 using namespace aicomp;
 
 static bool float_type(int dt) { return dt == AICOMP_KV_F32 || is_16bit_float(dt); }
@@ -213,6 +217,16 @@ int aicomp_kv_keep_rows(void* const* pools, int num_pools, int64_t row_bytes, in
                    block_size, (long long)num_blocks, max_blocks_per_seq);
     AICOMP_REQUIRE(row_bytes <= INT32_MAX / num_kv_heads && num_seqs <= 16777215, AICOMP_KV_EINVAL,
                    "%s: %d sequences, or %d heads of %lld bytes, exceed one launch", who, num_seqs, num_kv_heads, (long long)row_bytes);
+    // Two workgroups that moved the rows of one pool would read what the other has moved already
+    int64_t bytes = row_bytes;
+    AICOMP_REQUIRE(!__builtin_mul_overflow(bytes, (int64_t)num_kv_heads * block_size, &bytes) &&
+                   !__builtin_mul_overflow(bytes, num_blocks, &bytes), AICOMP_KV_EINVAL, "%s: pools of more than 2^63 bytes", who);
+    std::unique_ptr<uintptr_t[]> places(new (std::nothrow) uintptr_t[num_pools]);
+    AICOMP_REQUIRE(places, AICOMP_KV_EINVAL, "%s: no host memory for %d pools", who, num_pools);
+    std::copy((const uintptr_t*)pools, (const uintptr_t*)pools + num_pools, places.get());
+    if (!std::is_sorted(places.get(), places.get() + num_pools)) std::sort(places.get(), places.get() + num_pools);
+    for (int i = 1; i < num_pools; ++i)
+        AICOMP_REQUIRE(places[i] - places[i - 1] >= (uintptr_t)bytes, AICOMP_KV_EINVAL, "%s: two of the pools overlap", who);
     KeepRowsArgs a;
     a.pools = pools; a.num_pools = num_pools; a.row_bytes = row_bytes; a.hkv = num_kv_heads; a.bs = block_size; a.num_blocks = num_blocks;
     a.block_table = block_table; a.block_table_stride = block_table_stride; a.max_blocks = max_blocks_per_seq; a.first = first;

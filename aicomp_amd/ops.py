@@ -1251,9 +1251,10 @@ def keep_rows(pools: Sequence[torch.Tensor], block_table: torch.Tensor, first: t
     that of token ``first[s] + i`` for the i-th entry ``keep[cu_keep[s]:cu_keep[s+1]]``, in one launch on the current stream.
 
     ``pools``: the K and V pools ``[num_blocks, Hkv, block_size, D]`` of all layers, or pools of latent rows
-    ``[num_blocks, block_size, C + D]``, alike in shape and type.  ``block_table [S, max_blocks]`` int32 on the device; ``first [S]``,
-    ``keep [n]`` and ``cu_keep [S+1]`` int32: on the host they are checked (``keep`` ascends from 0 or more in every sequence) and copied,
-    on the device they are taken as they are.  Tokens beyond the table, or in blocks outside the pools, are left alone.
+    ``[num_blocks, block_size, C + D]``, alike in shape and type, none of them twice.  ``block_table [S, max_blocks]`` int32 on the
+    device; ``first [S]``, ``keep [n]`` and ``cu_keep [S+1]`` int32: on the host they are checked (``keep`` ascends from 0 or more in
+    every sequence) and copied, on the device they are taken as they are.  Tokens beyond the table, or in blocks outside the pools, are
+    left alone.
     """
     if _native("aicomp_kv_keep_rows") and _FAST.keep_rows(pools, block_table, first, keep, cu_keep):
         return

@@ -657,7 +657,7 @@ size_t aicomp_paged_tree_workspace_bytes(int num_seqs, int64_t total_q, int max_
  * What is left of a tree of drafts once some are accepted: in every pool, the row of token first[s] + keep[i] of sequence s becomes that
  * of token first[s] + i, for i-th entry of cu_keep[s] .. cu_keep[s+1], in one launch (per 128 pools).
  *   pools           HOST array of num_pools device pointers, pools [num_blocks, num_kv_heads, block_size, row] of row_bytes per row
- *                   (a pool of latent rows: num_kv_heads 1)
+ *                   (a pool of latent rows: num_kv_heads 1); pools that overlap, or one given twice, are refused
  *   first           [num_seqs] int32: the position of each tree's first draft
  *   keep, cu_keep   [total_keep] int32, strictly ascending from 0 or more within a sequence; [num_seqs+1] int32 prefix sums
  * A token beyond the table, or whose table entry is outside the pool, is neither read nor written.  No block of the pools may be

@@ -158,3 +158,12 @@ def test_tree_masks():
     for bad in ([0], [-1, 1], [-1, -2], [-1, 5]):
         with pytest.raises(ValueError, match="parent"):
             ops.tree_masks([bad])
+
+
+def test_a_pool_is_moved_once(lib):
+    """The second of two moves of one pool would start from what the first has moved already."""
+    bytes_ = 64 * 2 * 16 * 256
+    for pools in ((P, P), (P, P + bytes_ - 256), (P + bytes_ - 16, P)):
+        assert keep(lib, pools=(ctypes.c_void_p * 2)(*pools)) == EINVAL and "overlap" in err(lib)
+    assert keep(lib, pools=(ctypes.c_void_p * 4)(P, P + 2 * bytes_, P + bytes_, P + 2 * bytes_ - 1), n=4) == EINVAL and "overlap" in err(lib)
+    assert keep(lib, nb=2 ** 60) == EINVAL and "bytes" in err(lib)
