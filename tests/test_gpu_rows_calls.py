@@ -1,0 +1,436 @@
+"""The calls of latent rows, trees of drafts and accepted rows where calls go wrong: both host routes, recorded and replayed with other
+lengths, on other streams, from two threads, with many sequences, with offsets beyond 32 bits.  Tolerances: those of
+test_gpu_latent.py; the same call made another way gives the same bits, since no sum depends on an order that is left open."""
+import math
+import threading
+
+import pytest
+import torch
+
+from aicomp_amd import ops
+from oracle.rows_oracle import kept, masked_attention
+from test_gpu_latent import Case as Latent
+from test_gpu_latent import attention_bound, check, expect_prompt, parents_of, prompt_case
+from test_gpu_tree import Case as Tree
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32, FP8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+I32 = dict(dtype=torch.int32, device="cuda")
+
+
+def sums(lens):
+    return torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32)
+
+
+class Step:
+    """Buffers of one step of all five calls, with room for other lengths; ``load(i)`` fills them with the i-th set of inputs."""
+    MAX = 20                                                   # rows of a call
+
+    def __init__(self, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+        self.g = g
+        self.latent, self.query, self.w = r(self.MAX, 576), r(self.MAX, 16, 64), torch.ones(512, device="cuda")
+        angles = torch.randn(64, 32, generator=g)
+        self.cos, self.sin = angles.cos().cuda(), angles.sin().cuda()
+        self.pos, self.slots = torch.zeros(self.MAX, dtype=torch.int64, device="cuda"), torch.zeros(self.MAX, dtype=torch.int64, device="cuda")
+        self.pool, self.k, self.v = r(80, 16, 576), r(80, 2, 16, 128), r(80, 2, 16, 128)
+        self.table = torch.randperm(80, generator=g)[:60].view(3, 20).to(torch.int32).cuda()
+        self.lens, self.cu = torch.zeros(3, **I32), torch.zeros(4, **I32)
+        self.masks = torch.zeros(self.MAX, 1, dtype=torch.int64, device="cuda")
+        self.ql, self.qt, self.qp = r(self.MAX, 16, 576), r(self.MAX, 8, 128), r(self.MAX, 16, 192)
+        self.expanded, self.cuk = r(700, 16, 256), torch.zeros(4, **I32)
+        self.first, self.keep, self.cukeep = torch.zeros(3, **I32), torch.zeros(6, **I32), torch.zeros(4, **I32)
+        self.start = [t.clone() for t in (self.pool, self.k, self.v)]
+
+    def load(self, i):
+        g = torch.Generator().manual_seed(100 + i)
+        new = [[7, 1, 12], [1, 0, 3], [0, 20, 0], [5, 6, 9], [1, 1, 1]][i]
+        lens = [[300, 17, 40], [1, 0, 320], [5, 20, 0], [319, 100, 9], [33, 2, 150]][i]
+        self.latent.copy_(torch.randn(self.MAX, 576, generator=g))
+        for t in (self.query, self.ql, self.qt, self.qp):
+            t.copy_(torch.randn(t.shape, generator=g))
+        self.pos.copy_(torch.randint(0, 64, (self.MAX,), generator=g))
+        self.slots.copy_(torch.randperm(1280, generator=g)[:self.MAX])
+        self.lens.copy_(torch.tensor(lens)), self.cu.copy_(sums(new))
+        masks = torch.from_numpy(ops.tree_masks([parents_of(n, i) for n in new]))
+        self.masks.zero_()[:len(masks)].copy_(masks)
+        self.cuk.copy_(sums([max(n, n + 10 * i) for n in new]))
+        self.first.copy_(torch.tensor([max(0, c - n) for c, n in zip(lens, new)]))
+        keep = [list(range(n))[1::3][:2] for n in new]
+        self.keep.zero_()[:sum(map(len, keep))].copy_(torch.tensor([x for k in keep for x in k], dtype=torch.int32))
+        self.cukeep.copy_(sums([len(k) for k in keep]))
+        for t, s in zip((self.pool, self.k, self.v), self.start):
+            t.copy_(s)
+
+    def outs(self):
+        z = lambda *s: torch.full(s, 7.0, dtype=BF16, device="cuda")
+        return [z(self.MAX, 16, 64), z(self.MAX, 576), z(3, 16, 512), z(self.MAX, 16, 512), z(self.MAX, 16, 512), z(self.MAX, 8, 128),
+                z(self.MAX, 16, 128)]
+
+    def run(self, outs):
+        qo, rows, one, chunk, tree, kv, prompt = outs
+        ops.latent_kv_append(self.latent, self.w, self.cos, self.sin, self.pos, self.pool, self.slots, 1e-6, False, self.query, qo, rows)
+        ops.paged_latent_attn(one, self.ql[:3], self.pool, self.table, self.lens, 0.07)
+        ops.paged_latent_attn(chunk, self.ql, self.pool, self.table, self.lens, 0.07, self.cu, self.MAX)
+        ops.paged_latent_attn(tree, self.ql, self.pool, self.table, self.lens, 0.07, self.cu, self.MAX, self.masks)
+        ops.paged_tree_attn(kv, self.qt, self.k, self.v, self.table, self.lens, self.cu, self.masks, 0.09, self.MAX)
+        ops.latent_prompt_attn(prompt, self.qp, self.expanded[..., :128], self.latent_rows(), self.expanded[..., 128:], self.cu, self.cuk,
+                               0.07, self.MAX)
+        ops.keep_rows([self.k, self.v], self.table, self.first, self.keep, self.cukeep)
+        ops.keep_rows([self.pool], self.table, self.first, self.keep, self.cukeep)
+
+    def latent_rows(self):
+        return self.pool.view(-1, 576)[:700, 512:]
+
+    def eager(self, i):
+        self.load(i)
+        outs = self.outs()
+        self.run(outs)
+        torch.cuda.synchronize()
+        return [t.clone() for t in outs + [self.pool, self.k, self.v]]
+
+
+def same(got, want):
+    for n, (g, w) in enumerate(zip(got, want)):
+        assert torch.equal(g, w), f"result {n}: {int((g != w).sum())} of {g.numel()} elements differ"
+
+
+def test_both_routes_give_the_same(device, monkeypatch):
+    s = Step()
+    want = [s.eager(i) for i in range(5)]
+    monkeypatch.setattr(ops, "_FAST", None)
+    for i in range(5):
+        same(s.eager(i), want[i])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_recorded_step_replayed_with_other_lengths(device, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(ops, "_FAST", None)
+    s = Step(1)
+    want = [s.eager(i) for i in range(5)]
+    outs, side = s.outs(), torch.cuda.Stream()
+    s.load(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        s.run(outs)
+    for i in (0, 3, 1, 2, 4, 0):
+        s.load(i)
+        for t in outs:
+            t.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        same(outs + [s.pool, s.k, s.v], want[i])
+        same(Step(1).eager(3 - i % 3), want[3 - i % 3])        # (eager calls between the replays)
+
+
+def test_two_recorded_steps_side_by_side(device):
+    """Two graphs recorded on one stream, replayed on two at once: each has scratch of its own."""
+    steps, side = [Step(2), Step(3)], torch.cuda.Stream()
+    want = [[s.eager(i) for i in range(5)] for s in steps]
+    graphs, outs = [], [s.outs() for s in steps]
+    for s, o in zip(steps, outs):
+        s.load(0)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            s.run(o)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in (0, 3, 4, 2):
+        for s, o in zip(steps, outs):
+            s.load(i)
+            for t in o:
+                t.fill_(7.0)
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for s, o, w in zip(steps, outs, want):
+            same(o + [s.pool, s.k, s.v], w[i])
+
+
+def test_on_a_stream_of_its_own(device):
+    """Inputs written on a side stream, the calls and their results on it, no synchronization between."""
+    s = Step(4)
+    want = [s.eager(i) for i in range(5)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in (3, 0, 4):
+        with torch.cuda.stream(side):
+            busy = torch.randn(2048, 2048, device="cuda")
+            for _ in range(5):
+                busy = busy @ busy * 0.01
+            s.load(i)
+            outs = s.outs()
+            s.run(outs)
+            got = [t.clone() for t in outs + [s.pool, s.k, s.v]]
+        side.synchronize()
+        same(got, want[i])
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("pair", [("latent", "tree"), ("latent", "latent"), ("tree", "tree")], ids="-".join)
+def test_two_threads_on_one_stream(device, monkeypatch, pair, native):
+    """Calls of two launches with the stream's scratch between them: no call's second launch joins another's partial rows."""
+    if not native:
+        monkeypatch.setattr(ops, "_FAST", None)
+    L, T = Latent([3000, 1700, 40], [9, 5, 9], 16, seed=1).tree(), Tree([2500, 900], [9, 30], 8, 2, 128, seed=2)
+    cuda = {}
+    for name, c in (("latent", L), ("tree", T)):
+        cuda[name] = (c.q.cuda(), c.table.clamp(0, 10 ** 6).cuda(), torch.tensor(c.ctx, **I32), sums(c.new).cuda(),
+                      torch.from_numpy(ops.tree_masks(c.parents)).cuda())
+    pool, k, v = L.pool.cuda(), T.k.cuda(), T.v.cuda()
+
+    def latent():
+        q, table, lens, cu, masks = cuda["latent"]
+        return ops.paged_latent_attn(torch.empty_like(q[..., :512]), q, pool, table, lens, L.scale, cu, 9, masks)
+
+    def tree():
+        q, table, lens, cu, masks = cuda["tree"]
+        return ops.paged_tree_attn(torch.empty_like(q), q, k, v, table, lens, cu, masks, T.scale, 30)
+    calls = [{"latent": latent, "tree": tree}[name] for name in pair]
+    want, got, errors = [c() for c in calls], [[], []], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            for _ in range(60):
+                got[i].append(calls[i]())
+        except Exception as e:                                 # (reported by the test, not by the thread)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+
+
+def bad_calls():
+    """Calls that are refused, made on the device."""
+    z = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device="cuda")
+    i32 = lambda *v: torch.tensor(v, **I32)
+    q, o, pool, table, lens, cu = z(4, 16, 576), z(4, 16, 512), z(5, 16, 576), z(2, 3, dtype=torch.int32), i32(20, 9), i32(0, 3, 4)
+    masks = torch.ones(4, 1, dtype=torch.int64, device="cuda")
+    latent = lambda o=o, q=q, p=pool, t=table, c=lens, cu=cu, m=masks, n=3, s=0.1, l=0: ops.paged_latent_attn(o, q, p, t, c, s, cu, n, m, l)
+    qt, kp, ks = z(4, 8, 128), z(5, 2, 16, 128), torch.ones(2, device="cuda")
+    tree = lambda o=qt, q=qt, k=kp, v=kp, t=table, c=lens, cu=cu, m=masks, n=3, ks=None, s=0.1: ops.paged_tree_attn(
+        o.clone(), q, k, v, t, c, cu, m, s, n, ks, ks)
+    x, w, cos, pos, slots, qr = z(4, 576), torch.ones(512, device="cuda"), torch.ones(9, 32, device="cuda"), z(4, dtype=torch.int64), \
+        z(4, dtype=torch.int64), z(4, 16, 64)
+    append = lambda x=x, w=w, c=cos, s=cos, p=pos, pool=pool, sl=slots, q=qr, qo=None, r=None, e=1e-6: ops.latent_kv_append(
+        x, w, c, s, p, pool, sl, e, False, q, qo, r)
+    qp, key, value, rk, op, cuk = z(4, 2, 192), z(9, 2, 128), z(9, 2, 128), z(9, 64), z(4, 2, 128), i32(0, 5, 9)
+    prompt = lambda o=op, q=qp, k=key, r=rk, v=value, cu=cu, ck=cuk, s=0.1, n=3: ops.latent_prompt_attn(o, q, k, r, v, cu, ck, s, n)
+    move = lambda p=(kp, z(5, 2, 16, 128)), t=table, f=i32(3, 4), k=i32(1, 2), c=i32(0, 1, 2): ops.keep_rows(p, t, f, k, c)
+    wide = z(4, 16, 600)
+    return {
+        "latent type": lambda: latent(q=q.to(F16)), "latent pool type": lambda: latent(p=pool.to(F16)), "latent out shape": lambda: latent(o=z(4, 15, 512)),
+        "latent strides": lambda: latent(q=wide[..., :576]), "latent table type": lambda: latent(t=table.long()),
+        "latent lens": lambda: latent(c=lens[:1]), "latent cu": lambda: latent(cu=cu[:2]), "latent masks": lambda: latent(m=masks[:3]),
+        "latent mask type": lambda: latent(m=masks.int()), "latent mask words": lambda: latent(m=masks[:, :0]), "latent scale": lambda: latent(s=math.nan),
+        "latent max_q_len": lambda: latent(n=5), "latent longest": lambda: latent(l=-1), "latent rows": lambda: latent(cu=None, m=None),
+        "latent masks without cu": lambda: latent(q=q[:2], o=o[:2], cu=None, m=masks[:2]), "latent host": lambda: latent(c=lens.cpu()),
+        "latent width": lambda: latent(q=z(4, 16, 520), p=z(5, 16, 520)), "latent unaligned": lambda: latent(q=z(4 * 16 * 576 + 8)[4:-4].view(4, 16, 576)),
+        "tree type": lambda: tree(q=qt.to(F16)), "tree pools": lambda: tree(v=z(5, 2, 16, 64)), "tree heads": lambda: tree(o=z(4, 7, 128), q=z(4, 7, 128)),
+        "tree fp8 without scales": lambda: tree(k=kp.to(FP8), v=kp.to(FP8)), "tree scales": lambda: tree(k=kp.to(FP8), v=kp.to(FP8), ks=ks[:1]),
+        "tree masks": lambda: tree(m=masks[:1]), "tree max_q_len": lambda: tree(n=5), "tree strides": lambda: tree(q=z(4, 8, 256)[..., ::2]),
+        "append type": lambda: append(x=x.to(F16)), "append weight": lambda: append(w=w.to(BF16)), "append table": lambda: append(c=cos[:, :16], s=cos[:, :16]),
+        "append tables": lambda: append(s=cos[:8]), "append positions": lambda: append(p=pos.int()), "append slots": lambda: append(sl=slots[:3]),
+        "append query": lambda: append(q=z(4, 16, 32)), "append out": lambda: append(qo=z(4, 16, 32)), "append rows": lambda: append(r=z(4, 512)),
+        "append eps": lambda: append(e=-1.0), "append pool": lambda: append(pool=z(5, 16, 560)),
+        "prompt type": lambda: prompt(k=key.to(F16)), "prompt widths": lambda: prompt(r=z(9, 48)), "prompt heads": lambda: prompt(v=z(9, 3, 128)),
+        "prompt lens": lambda: prompt(ck=cuk[:2]), "prompt max_q_len": lambda: prompt(n=9), "prompt scale": lambda: prompt(s=math.inf),
+        "prompt strides": lambda: prompt(q=z(4, 2, 384)[..., ::2]), "prompt step": lambda: prompt(k=z(9, 2, 132)[..., :128]),
+        "keep shapes": lambda: move(p=(kp, z(5, 2, 16, 64))), "keep twice": lambda: move(p=(kp, kp)), "keep overlap": lambda: move(p=(kp[:4], kp[1:])),
+        "keep table": lambda: move(t=table[:1]), "keep first": lambda: move(f=i32(3, 4).long()), "keep sums": lambda: move(c=i32(0, 1)),
+        "keep devices": lambda: move(f=i32(3, 4).cpu()), "keep order": lambda: move(f=i32(3, 4).cpu(), k=torch.tensor([2, 1], dtype=torch.int32),
+                                                                                  c=torch.tensor([0, 2, 2], dtype=torch.int32)),
+    }
+
+
+def test_refusals_of_both_routes_are_alike(device, monkeypatch):
+    calls = bad_calls()
+    texts = {}
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError) as e:
+            call()
+            pytest.fail(f"{name} was not refused")
+        texts[name] = str(e.value)
+    monkeypatch.setattr(ops, "_FAST", None)
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError) as e:
+            call()
+        assert str(e.value) == texts[name], name
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------- heads, sequences, places
+@pytest.mark.parametrize("rows", ["chunk", "tree"])
+@pytest.mark.parametrize("H", [5, 6, 16, 24, 33, 64, 100])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_latent_rows_of_every_tile(dtype, H, rows):
+    """Tokens times heads from 5 to 1900 rows: every size of row tile, whole and cut."""
+    c = Latent([200, 37, 64, 33, 700, 2], [3, 1, 19, 4, 8, 2], H, dtype=dtype, seed=11)
+    if rows == "tree":
+        c.tree()
+    c.poison()
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("n", [257, 1100, 3000])
+def test_many_sequences(n):
+    """More sequences than a workgroup has threads, with lengths of none to a few tiles, and the last ones the longest."""
+    ctx = [(i * 7) % 40 for i in range(n)]
+    ctx[-1], ctx[-2], ctx[5] = 900, 0, 400
+    c = Latent(ctx, [1] * n, 2, seed=12)
+    c.check(c.run())
+    t = Tree(ctx, [min(i % 4, x) for i, x in enumerate(ctx)], 2, 1, 64, seed=13)
+    t.check(t.run(max_q_len=3))
+    cut = Latent(ctx, [i % 3 for i in range(n)], 2, seed=14)
+    cut.check(cut.run())
+
+
+def test_many_prompts():
+    lens = [(i * 7) % 50 for i in range(1030)]
+    q, expanded, latent = prompt_case(lens, lens, 2, seed=15)
+    cu = sums(lens).cuda()
+    out = torch.empty(*q.shape[:2], 128, dtype=BF16, device="cuda")
+    ops.latent_prompt_attn(out, q.cuda(), expanded.cuda()[..., :128], latent.cuda()[:, 512:], expanded.cuda()[..., 128:], cu, cu, 0.07,
+                           max(lens))
+    want, mean_abs, size = expect_prompt(q, expanded, latent, lens, lens, 128, 64, 0.07)
+    check(out.cpu(), want, attention_bound(want, mean_abs, size, 192, BF16))
+
+
+def test_a_bound_of_the_contexts_cuts_no_row():
+    c = Latent([3000, 10], [1, 1], 16, seed=16)
+    c.check(c.run(longest_context=1))
+    c = Latent([3000, 10], [5, 2], 24, seed=16)
+    c.check(c.run(longest_context=1))
+    t = Tree([3000, 10], [9, 3], 8, 2, 128, seed=17)
+    t.check(t.run(longest_context=1))
+
+
+def test_wider_masks_and_tables_than_needed():
+    t = Tree([300, 40], [70, 9], 8, 2, 64, seed=18)
+    masks = torch.from_numpy(ops.tree_masks(t.parents))
+    wide = torch.full((masks.shape[0], 6), -1, dtype=torch.int64)
+    wide[:, :2] = masks
+    table, t.table = t.table, torch.cat((t.table, torch.full((2, 30), 2 ** 31 - 1, dtype=torch.int32)), dim=1)
+    t.check(t.run(wide))
+    got = t.run(wide[:, :2])
+    t.table = t.table[:, :table.shape[1]]
+    assert torch.equal(got, t.run(wide[:, :2]))
+
+
+# Pools and rows beyond 2^31 elements and 2^32 bytes
+def test_a_latent_pool_beyond_32_bits():
+    blocks, C, D = 2 ** 31 // (16 * 576) + 4000, 512, 64
+    pool = torch.zeros(blocks, 16, C + D, dtype=BF16, device="cuda")
+    c = Latent([500, 70, 33], [1, 1, 1], 16, seed=19)
+    far = blocks - 1 - torch.arange(c.pool.shape[0])
+    c.table = far[c.table.long().clamp(0, c.pool.shape[0] - 1)].to(torch.int32)
+    pool[far.cuda()] = c.pool.cuda()
+    for new, tree in (([1, 1, 1], False), ([9, 5, 3], True)):
+        small = Latent([500, 70, 33], new, 16, seed=19)
+        if tree:
+            small.tree()
+        q = small.q.cuda()
+        out = torch.empty(q.shape[0], 16, C, dtype=BF16, device="cuda")
+        masks = torch.from_numpy(ops.tree_masks(small.parents)).cuda() if tree else None
+        ops.paged_latent_attn(out, q, pool, c.table.cuda(), torch.tensor(c.ctx, **I32), c.scale, sums(new).cuda() if tree else None,
+                              max(new), masks)
+        assert torch.equal(out.cpu(), small.run())
+    # appended and moved there too
+    slots = torch.arange(5, device="cuda") + blocks * 16 - 5
+    ops.latent_kv_append(pool[0, :5], None, torch.ones(9, 32, device="cuda"), torch.zeros(9, 32, device="cuda"), None, pool, slots)
+    row = torch.randn(5, C + D, device="cuda").to(BF16)
+    ops.latent_kv_append(row, None, torch.ones(9, 32, device="cuda"), torch.zeros(9, 32, device="cuda"), None, pool, slots)
+    assert torch.equal(pool[-1, -5:], row)
+    table = torch.tensor([[blocks - 1]], **I32)
+    ops.keep_rows([pool], table, torch.tensor([10], **I32), torch.tensor([2, 4], **I32), torch.tensor([0, 2], **I32))
+    assert torch.equal(pool[-1, 10], row[1]) and torch.equal(pool[-1, 11], row[3])
+
+
+@pytest.mark.parametrize("dtype,pool", [(BF16, None), (F16, FP8), (F32, None)])
+@pytest.mark.parametrize("new", [[3, 2], [9, 1], [33, 64]])
+def test_tree_pools_beyond_32_bits(dtype, pool, new):
+    c = Tree([500, 70], new, 16, 4, 128, dtype=dtype, pool=pool, seed=20)
+    want = c.run()
+    blocks, n = 2 ** 31 // (4 * 16 * 128) + 2000, c.k.shape[0]
+    far = blocks - 1 - torch.arange(n)
+    k = torch.zeros(blocks, 4, 16, 128, dtype=torch.uint8 if c.pool == FP8 else c.pool, device="cuda")
+    v = torch.zeros_like(k)
+    bits = lambda t: t.view(torch.uint8) if c.pool == FP8 else t
+    k[far.cuda()], v[far.cuda()] = bits(c.k).cuda(), bits(c.v).cuda()
+    if c.pool == FP8:
+        k, v = k.view(FP8), v.view(FP8)
+    out = torch.empty_like(c.q).cuda()
+    scales = {} if c.ks is None else {"k_scale": c.ks.cuda(), "v_scale": c.vs.cuda()}
+    ops.paged_tree_attn(out, c.q.cuda(), k, v, far[c.table.long().clamp(0, n - 1)].to(torch.int32).cuda(), torch.tensor(c.ctx, **I32),
+                        sums(new).cuda(), torch.from_numpy(ops.tree_masks(c.parents)).cuda(), c.scale, max(new), **scales)
+    assert torch.equal(out.cpu(), want)
+
+
+def test_rows_beyond_32_bits():
+    """More than 2^31 elements of queries: the last rows are those of a small call."""
+    n, H = 30000, 128
+    q = torch.zeros(n, H, 576, dtype=BF16, device="cuda")
+    assert q.numel() > 2 ** 31
+    tail = Latent([3, 40, 17, 1], [1] * 4, H, seed=21)
+    want = tail.run()
+    q[-4:] = tail.q.cuda()
+    out = torch.empty(n, H, 512, dtype=BF16, device="cuda")
+    table = torch.zeros(n, tail.table.shape[1], **I32)
+    table[-4:] = tail.table.cuda()
+    lens = torch.zeros(n, **I32)
+    lens[-4:] = torch.tensor(tail.ctx, **I32)
+    ops.paged_latent_attn(out, q, tail.pool.cuda(), table, lens, tail.scale)
+    w, mean_abs, size = tail.expect()
+    tol = attention_bound(w, mean_abs, size, 576, BF16)
+    check(out[-4:].cpu(), w, tol)
+    assert bool((out[:-4] == 0).all()) and bool(((want.double() - out[-4:].cpu().double()).abs() <= 2 * tol).all())
+
+
+def test_prompt_rows_beyond_32_bits():
+    """More than 2^31 elements of keys and values, of queries too: prompts of 40 tokens, the last ones checked."""
+    S, n, H = 1700, 40, 128
+    g = torch.Generator().manual_seed(22)
+    q, expanded = torch.zeros(S * n, H, 192, dtype=BF16, device="cuda"), torch.zeros(S * n, H, 256, dtype=BF16, device="cuda")
+    rk = torch.zeros(S * n, 64, dtype=BF16, device="cuda")
+    assert min(expanded.numel(), q.numel() * 4 // 3) > 2 ** 31
+    tq, te, tr = (torch.randn(2 * n, *s, generator=g).to(BF16) for s in ((H, 192), (H, 256), (64,)))
+    q[-2 * n:], expanded[-2 * n:], rk[-2 * n:] = tq.cuda(), te.cuda(), tr.cuda()
+    cu = (torch.arange(S + 1) * n).to(torch.int32).cuda()
+    out = torch.empty(S * n, H, 128, dtype=BF16, device="cuda")
+    ops.latent_prompt_attn(out, q, expanded[..., :128], rk, expanded[..., 128:], cu, cu, 0.07, n)
+    parts = []
+    see = torch.ones(n, n, dtype=torch.bool).tril()
+    for s in range(2):
+        rows = slice(s * n, (s + 1) * n)
+        k = torch.cat((te[rows, :, :128], tr[rows, None].expand(n, H, 64)), -1)
+        parts.append(masked_attention(tq[rows], k, te[rows, :, 128:], see, 0.07))
+    want, mean_abs, size = [torch.cat(x) for x in zip(*parts)]
+    check(out[-2 * n:].cpu(), want, attention_bound(want, mean_abs, size, 192, BF16))
+    assert bool((out[:-2 * n] == 0).all())
+
+
+def test_moves_of_random_trees():
+    """Many sequences, ascending entries of any gaps, pools of one token a block and of many."""
+    for bs, seed in ((1, 23), (16, 24), (48, 25)):
+        g = torch.Generator().manual_seed(seed)
+        S, width = 300, 96 // bs + 2
+        table = torch.randperm(S * width, generator=g).view(S, width).to(torch.int32)
+        firsts = torch.randint(0, 40, (S,), generator=g)
+        keep = [torch.randperm(50, generator=g)[:int(torch.randint(0, 12, (1,), generator=g))].sort().values.tolist() for _ in range(S)]
+        pool = torch.randn(S * width, 3, bs, 8, generator=g)
+        got = pool.cuda()
+        flat = torch.tensor([x for k in keep for x in k], dtype=torch.int32)
+        ops.keep_rows([got], table.cuda(), firsts.to(torch.int32).cuda(), flat.cuda(), sums([len(k) for k in keep]).cuda())
+        assert torch.equal(got.cpu(), kept(pool, table, firsts.tolist(), keep))
