@@ -189,22 +189,41 @@ row_join_kernel(RowParams p) {
     const int sub = blockIdx.x % (ROWS / PER), item = blockIdx.x / (ROWS / PER);
     const int rtile = item % p.row_tiles, kvh = item / p.row_tiles % p.hkv, seq = item / p.row_tiles / p.hkv;
     const Seq q = load_seq<ROWS, KT>(p, seq);
-    const int2 who = p.ws_items[item];
+    int2 who = p.ws_items[item];
+    who.x = __builtin_amdgcn_readfirstlane(who.x);
+    who.y = __builtin_amdgcn_readfirstlane(who.y);
     const int r = sub * PER + threadIdx.x / LPR, row = rtile * ROWS + r, col = threadIdx.x % LPR * 4;
     if (row >= q.n * p.group || who.y == 0) return;            // (no such row: its entry was not written)
     auto slot_of = [&](int k) { return 2 * (int64_t)(who.x + k) + (k == 0 ? 1 : 0); };
-    float top = NEG_BIG;
-    for (int k = 0; k <= who.y; ++k) top = fmaxf(top, p.ws_ml[slot_of(k) * ROWS + r].x);
+    // Pieces eight at a time, all their loads under way together (what they wait for is most of this kernel's time); a place behind the
+    // last piece repeats that one's and is not added.
+    constexpr int AT_ONCE = 8;
+    float top = NEG_BIG, sum = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int k = 0; k <= who.y; ++k) {
-        const float2 ml = p.ws_ml[slot_of(k) * ROWS + r];
-        const f32x4_t x = *(const f32x4_t*)(p.ws_acc + (slot_of(k) * ROWS + r) * DV + col);
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
-        sum = fmaf(f, ml.y, sum);
+    for (int first = 0; first <= who.y; first += AT_ONCE) {
+        float2 ml[AT_ONCE];
+        f32x4_t x[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int64_t at = slot_of(min(first + k, who.y)) * ROWS + r;
+            ml[k] = p.ws_ml[at];
+            x[k] = *(const f32x4_t*)(p.ws_acc + at * DV + col);
+        }
+        float m_new = top;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) m_new = fmaxf(m_new, ml[k].x);
+        const float alpha = __builtin_amdgcn_exp2f(top - m_new);
+        top = m_new;
+        sum *= alpha;
+        o *= alpha;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (first + k > who.y) break;                      // uniform
+            const float f = __builtin_amdgcn_exp2f(ml[k].x - top);
+            sum = fmaf(f, ml[k].y, sum);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[k][i], o[i]);
+        }
     }
     const float inv = (p.v_scale != nullptr ? p.v_scale[kvh] : 1.f) / sum;
     o *= inv;
