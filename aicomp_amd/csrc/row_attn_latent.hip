@@ -315,7 +315,7 @@ row_attn_latent_kernel(RowParams p) {
 
 template <typename E, int NC> void launch(const RowParams& p, int64_t items, hipStream_t stream) {
     hipLaunchKernelGGL((row_attn_latent_kernel<E, NC>), dim3((unsigned)p.workers), dim3(256), 0, stream, p);
-    if (p.workers > 1)
+    if (p.ws_items != nullptr)
         hipLaunchKernelGGL((row_join_kernel<E, DV, 16 * NC, KT>), dim3((unsigned)(items * (16 * NC * DV / 1024))), dim3(256), 0, stream, p);
 }
 

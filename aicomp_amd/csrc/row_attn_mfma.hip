@@ -325,6 +325,7 @@ struct RowPlan {
     bool shared;                       // row_attn_shared.hip
     int R, rows, keys;
     int workers, least, over, row_tiles;
+    bool single;
 };
 
 RowPlan row_plan(const RowAttnArgs& a) {
@@ -349,16 +350,25 @@ RowPlan row_plan(const RowAttnArgs& a) {
     // 60 us without, 55 with); where items are divided, as many workgroups as there are tiles for are worth more (one row of 700 tokens:
     // 17 us without, 21 with).
     const int64_t tiles = (span + r.keys - 1) / r.keys, most = latent || a.dk == 256 ? 256 : 512;
-    r.over = items * 4 >= most ? (r.shared ? 3 : 8) : 0;
+    const bool many = items * 4 >= most;
+    r.over = many ? (r.shared ? 3 : 8) : 0;
     r.least += r.over;
     r.workers = (int)std::min<int64_t>(most, (items * (tiles + r.over) + r.least - 1) / r.least);
+    // An item whole for every workgroup saves the second launch and the division, and costs what the longest item takes alone.  Measured
+    // at equal lengths, divided and whole: one row of 16 heads, 256 tokens 15.4 and 12.7 us, 512 15.9 and 15.4, 768 16.8 and 18.6; 128
+    // heads, 1 x 256 tokens 16.5 and 14.4, 1 x 512 17.5 and 20.3, 64 x 512 38.6 and 24.1; trees of 9 drafts for 8 KV heads of 4, one wave
+    // to the rows, 1 x 192 tokens 12.5 and 7.7, 1 x 384 11.7 and 10.5; of 2 drafts, 1 x 768 10.9 and 9.4, 8 x 768 14.4 and 11.3.
+    // Many items even out whatever their lengths are (400 rows of 1024 tokens: 16 heads 112 and 99 us, 128 heads 328 and 242).
+    const int64_t all = (int64_t)a.num_seqs * a.hkv * r.row_tiles, few = r.shared ? 256 : latent ? 384 : 768, some = r.shared || latent ? 512 : 768;
+    r.single = span <= (items >= 2 * most ? 1024 : many ? some : few) && all <= 2 * items;       // (few workgroups for no rows)
+    if (r.single) r.over = 0, r.workers = (int)std::min<int64_t>(all, INT32_MAX);
     return r;
 }
 
 template <typename E, bool FP8, int DK, int DV, bool LATENT, int R, int OCC>
 void launch_variant(const RowParams& p, int64_t join_items, hipStream_t stream) {
     hipLaunchKernelGGL((row_attn_kernel<E, FP8, DK, DV, LATENT, R, OCC>), dim3((unsigned)p.workers), dim3(256), 0, stream, p);
-    if (p.workers > 1)
+    if (p.ws_items != nullptr)
         hipLaunchKernelGGL((row_join_kernel<E, DV, 16 * R, KT>), dim3((unsigned)(join_items * (16 * R * DV / 1024))), dim3(256), 0, stream, p);
 }
 
@@ -384,7 +394,7 @@ bool row_attn_mfma_supported(const RowAttnArgs& a) {
 
 size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a) {
     const RowPlan r = row_plan(a);
-    return r.workers > 1 ? (size_t)2 * r.workers * r.rows * (a.dv + 2) * sizeof(float) + (size_t)a.num_seqs * a.hkv * r.row_tiles * sizeof(int2) : 0;
+    return r.workers > 1 && !r.single ? (size_t)2 * r.workers * r.rows * (a.dv + 2) * sizeof(float) + (size_t)a.num_seqs * a.hkv * r.row_tiles * sizeof(int2) : 0;
 }
 
 int launch_row_attn_mfma(const RowAttnArgs& a) {
@@ -394,10 +404,10 @@ int launch_row_attn_mfma(const RowAttnArgs& a) {
     p.block_table_stride = a.block_table_stride; p.context_lens = a.context_lens; p.cu_q_lens = a.cu_q_lens; p.masks = a.masks;
     p.mask_words = a.mask_words; p.num_seqs = a.num_seqs; p.rows = (int)a.rows; p.max_q_len = a.max_q_len; p.hq = a.hq; p.hkv = a.hkv;
     p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
-    p.v_scale = a.v_scale; p.workers = r.workers; p.least = r.least; p.over = r.over; p.row_tiles = r.row_tiles;
+    p.v_scale = a.v_scale; p.workers = r.workers; p.single = r.single; p.least = r.least; p.over = r.over; p.row_tiles = r.row_tiles;
     p.ws_acc = (float*)a.workspace;
     p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * r.rows * a.dv);
-    p.ws_items = r.workers > 1 ? (int2*)(p.ws_ml + (size_t)2 * r.workers * r.rows) : nullptr;
+    p.ws_items = r.workers > 1 && !r.single ? (int2*)(p.ws_ml + (size_t)2 * r.workers * r.rows) : nullptr;
     const int64_t items = (int64_t)a.num_seqs * a.hkv * r.row_tiles;
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, f16 = a.q_dtype == AICOMP_KV_F16;
     if (r.shared && a.dk == 576) launch_row_attn_latent(p, f16, r.R, items, a.stream);

@@ -286,7 +286,7 @@ row_attn_shared_kernel(RowParams p) {
 template <typename E, bool FP8, int D, int R, int OCC>
 void launch_variant(const RowParams& p, int64_t join_items, hipStream_t stream) {
     hipLaunchKernelGGL((row_attn_shared_kernel<E, FP8, D, R, OCC>), dim3((unsigned)p.workers), dim3(256), 0, stream, p);
-    if (p.workers > 1)
+    if (p.ws_items != nullptr)
         hipLaunchKernelGGL((row_join_kernel<E, D, 64 * R, KT>), dim3((unsigned)(join_items * (64 * R * D / 1024))), dim3(256), 0, stream, p);
 }
 

@@ -3,9 +3,11 @@
 //
 // All (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of equal length, whatever
 // the sequences' lengths are.  Before an item's key tiles the line has `over` places more, in which nothing is done: what the start and
-// the end of an item cost, in tiles, so that pieces of several items have fewer tiles.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by it; of others each
-// leaves (m, l, O) of its rows in the workspace: in its slot 0 where it does not have the item's first key tile, else in its slot 1.  Who
-// has the first tile says who has the others.
+// the end of an item cost, in tiles, so that pieces of several items have fewer tiles.  An item (sequence, KV head, row tile) that one
+// workgroup has whole is finished by it; of others each leaves (m, l, O) of its rows in the workspace: in its slot 0 where it does not have
+// the item's first key tile, else in its slot 1.  Who has the first tile says who has the others.
+//
+// Where contexts are short, every workgroup has one item whole (`single`): nothing to join, and no line to find one's place on.
 #pragma once
 
 #include "row_attn.h"
@@ -30,6 +32,7 @@ struct RowParams {
     const float* k_scale;
     const float* v_scale;
     int workers;                       // workgroups
+    bool single;                       // one for each (sequence, KV head, row tile)
     int least;                         // places that a workgroup has at least
     int over;                          // places of an item before its key tiles
     int row_tiles;                     // of the longest sequence (the join's grid)
@@ -87,6 +90,16 @@ struct PieceScratch {
 
 template <int ROWS, int KT, int THREADS>
 __device__ __forceinline__ bool piece_of(const RowParams& p, int worker, PieceScratch& sh, Piece& mine) {
+    if (p.single) {
+        const int of_seq = p.hkv * p.row_tiles;
+        mine.seq = (unsigned)worker / (unsigned)of_seq;
+        const int item = worker - mine.seq * of_seq, kvh = (unsigned)item / (unsigned)p.row_tiles, rtile = item - kvh * p.row_tiles;
+        mine.q = load_seq<ROWS, KT>(p, mine.seq);
+        mine.length = mine.end = mine.q.key_tiles;
+        mine.at = 0;
+        mine.off = (kvh * mine.q.row_tiles + rtile) * mine.q.key_tiles;
+        return rtile < mine.q.row_tiles;
+    }
     const int per = (p.num_seqs + THREADS - 1) / THREADS, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int first = min((int)threadIdx.x * per, p.num_seqs), last = min(first + per, p.num_seqs);
     Seq q;
