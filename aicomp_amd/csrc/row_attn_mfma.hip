@@ -334,11 +334,8 @@ RowPlan row_plan(const RowAttnArgs& a) {
     const int64_t rows = (int64_t)a.max_q_len * group;
     RowPlan r;
     r.shared = rows > (latent ? 16 : 32);
-    // latent rows: 16 R to a workgroup.  64 rows keep fewer registers for the products than 48 and are the better choice only where
-    // 48 would be two tiles
-    if (latent) r.R = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 || rows > 64 ? 3 : 4;
-    else r.R = r.shared ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
-    r.rows = (r.shared && !latent ? 64 : 16) * r.R;
+    r.R = r.shared ? (latent || rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
+    r.rows = (r.shared ? 64 : 16) * r.R;
     r.keys = r.shared ? 64 : 32;
     r.least = r.shared ? 2 : 4;
     r.row_tiles = (int)((rows + r.rows - 1) / r.rows);
@@ -410,7 +407,7 @@ int launch_row_attn_mfma(const RowAttnArgs& a) {
     p.ws_items = r.workers > 1 && !r.single ? (int2*)(p.ws_ml + (size_t)2 * r.workers * r.rows) : nullptr;
     const int64_t items = (int64_t)a.num_seqs * a.hkv * r.row_tiles;
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3, f16 = a.q_dtype == AICOMP_KV_F16;
-    if (r.shared && a.dk == 576) launch_row_attn_latent(p, f16, r.R, items, a.stream);
+    if (r.shared && a.dk == 576) launch_row_attn_latent(p, f16, items, a.stream);
     else if (r.shared) launch_row_attn_shared(p, f16, fp8, a.dk, r.R, items, a.stream);
     else if (a.dk == 576 && f16) launch_variant<F16Fmt, false, 576, 512, true, 1, 1>(p, items, a.stream);
     else if (a.dk == 576) launch_variant<Bf16Fmt, false, 576, 512, true, 1, 1>(p, items, a.stream);

@@ -43,7 +43,7 @@ struct RowParams {
 
 // d: head_dim; R: groups of 16 rows to a wave; items: of the join's grid
 void launch_row_attn_shared(const RowParams& p, bool f16, bool fp8, int d, int R, int64_t items, hipStream_t stream);
-void launch_row_attn_latent(const RowParams& p, bool f16, int groups, int64_t items, hipStream_t stream);
+void launch_row_attn_latent(const RowParams& p, bool f16, int64_t items, hipStream_t stream);
 
 namespace {
 
@@ -53,6 +53,10 @@ constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both
 
 #define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+
+// All waves of the workgroup meet, and what they wrote to LDS is there.  Unlike __syncthreads(), which waits for loads from memory too:
+// those under way stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A sequence as the line of work sees it.
 struct Seq {

@@ -434,3 +434,27 @@ def test_moves_of_random_trees():
         flat = torch.tensor([x for k in keep for x in k], dtype=torch.int32)
         ops.keep_rows([got], table.cuda(), firsts.to(torch.int32).cuda(), flat.cuda(), sums([len(k) for k in keep]).cuda())
         assert torch.equal(got.cpu(), kept(pool, table, firsts.tolist(), keep))
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 3.0])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scales_of_either_sign(dtype, scale):
+    """A scale below zero turns the order of the scores around, one of zero makes all weights alike, a large one leaves few."""
+    for H, new, tree in ((16, [1, 1, 1], False), (40, [1, 1, 1], False), (16, [9, 3, 1], True)):
+        c = Latent([300, 65, 7], new, H, dtype=dtype, seed=26)
+        if tree:
+            c.tree()
+        c.scale = scale
+        c.poison()
+        c.check(c.run())
+    for new in ([9, 1, 3], [70, 20, 7]):
+        t = Tree([300, 65, 7], new, 8, 2, 128, dtype=dtype, seed=27)
+        t.scale = scale
+        t.poison()
+        t.check(t.run())
+    q, expanded, latent = prompt_case([200, 70], [200, 33], 4, dtype=dtype, seed=28)
+    cu, cuk = sums([200, 33]).cuda(), sums([200, 70]).cuda()
+    out = torch.empty(*q.shape[:2], 128, dtype=dtype, device="cuda")
+    ops.latent_prompt_attn(out, q.cuda(), expanded.cuda()[..., :128], latent.cuda()[:, 512:], expanded.cuda()[..., 128:], cu, cuk, scale, 200)
+    want, mean_abs, size = expect_prompt(q, expanded, latent, [200, 70], [200, 33], 128, 64, scale)
+    check(out.cpu(), want, attention_bound(want, mean_abs, size, 192, dtype))
