@@ -89,10 +89,8 @@ row_attn_latent_kernel(RowParams p) {
         const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
         const int last_block = (q.ctx - 1) / BS;               // (blocks behind it are not this sequence's)
         // Wave w brings in block w of a tile, load i of 18.
-        auto block_of = [&](int t) -> const char* {
-            const int b = table[min(4 * t + w, last_block)];
-            return (const char*)p.k_pool + (int64_t)max(0, min(b, p.num_blocks - 1)) * BS * KROW;
-        };
+        auto block = [&](int b) { return (const char*)p.k_pool + (int64_t)max(0, min(b, p.num_blocks - 1)) * BS * KROW; };
+        auto block_of = [&](int t) { return block(table[min(4 * t + w, last_block)]); };
         // (a buffer of no bytes brings in nothing: the last tile's step has the same instructions as the others)
         auto buffer_of = [&](const char* from, bool there) {
             return __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, there ? BLOCK : 0, 0x00027000);
@@ -102,12 +100,9 @@ row_attn_latent_kernel(RowParams p) {
                                                      (i & 1) * 8 * KROW + (i >> 1) * 128, 0, 0);
         };
         const int t_end = min(it.t1, (q.ctx + KT - 1) / KT);   // (0 tiles where the context is none)
-        if (it.t0 < t_end) {
-            const auto from = buffer_of(block_of(t_end - 1), true);
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) load(from, buf0, i);
-        }
-        // The rows come by way of the second buffer, sixteen by each wave (rows beyond the last: that one, computed and not stored).
+        // The rows come by way of the second buffer, sixteen by each wave (rows beyond the last: that one, computed and not stored); before
+        // the first tile, whose place in the table is still to arrive.
+        const int entry = t_end > it.t0 ? table[min(4 * (t_end - 1) + w, last_block)] : 0;
         {
             const int here = min(row0 + 16 * w, nrows - 1);
             const char* from = (const char*)p.query + ((int64_t)q.begin * p.hq + here) * KROW;
@@ -115,6 +110,11 @@ row_attn_latent_kernel(RowParams p) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 __builtin_amdgcn_global_load_lds(GLOBAL_PTR(from + at[i & 1] + (i >> 1) * 128), LDS_PTR(buf1 + w * BLOCK + 1024 * i), 16, 0, 0);
+        }
+        if (it.t0 < t_end) {
+            const auto from = buffer_of(block(entry), true);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) load(from, buf0, i);
         }
         if (tid < 2) moved[tid] = 0;
         __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0)

@@ -356,8 +356,8 @@ RowPlan row_plan(const RowAttnArgs& a) {
     // heads, 1 x 256 tokens 16.5 and 14.4, 1 x 512 17.5 and 20.3, 64 x 512 38.6 and 24.1; trees of 9 drafts for 8 KV heads of 4, one wave
     // to the rows, 1 x 192 tokens 12.5 and 7.7, 1 x 384 11.7 and 10.5; of 2 drafts, 1 x 768 10.9 and 9.4, 8 x 768 14.4 and 11.3.
     // Many items even out whatever their lengths are (400 rows of 1024 tokens: 16 heads 112 and 99 us, 128 heads 328 and 242).
-    const int64_t all = (int64_t)a.num_seqs * a.hkv * r.row_tiles, few = r.shared ? 256 : latent ? 384 : 768, some = r.shared || latent ? 512 : 768;
-    r.single = span <= (items >= 2 * most ? 1024 : many ? some : few) && all <= 2 * items;       // (few workgroups for no rows)
+    const int64_t all = (int64_t)a.num_seqs * a.hkv * r.row_tiles, few = r.shared ? 256 : latent ? 384 : 768;
+    r.single = span <= (items >= 2 * most ? 1024 : many ? 768 : few) && all <= 2 * items;       // (few workgroups for no rows)
     if (r.single) r.over = 0, r.workers = (int)std::min<int64_t>(all, INT32_MAX);
     return r;
 }
