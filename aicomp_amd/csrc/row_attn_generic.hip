@@ -5,6 +5,9 @@
 // bytes at a time, so that the lines are taken whole from the L1), the tile's weights go through LDS, and the output's
 // columns are divided among the threads in quads, the keys of a tile among as many threads as there are quads to spare.  An online
 // softmax in float32, exponents in base 2.  Keys that the row does not see are neither multiplied nor read.
+//
+// Bound by the reads of every (row, head) for itself, out of the caches: 16 rows of 16 heads over 1024 latent rows of float32 387 us, of
+// bfloat16 in blocks of 32 tokens 310 (in blocks of 16, on the matrix cores, 21).
 #include "row_attn.h"
 
 #include <algorithm>

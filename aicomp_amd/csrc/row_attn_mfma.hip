@@ -9,9 +9,11 @@
 // The reference moves when a score passes it by 2^8, so most tiles leave O as it is.  Rows of a tile are swizzled in 16-byte chunks
 // (chunk c of key k at c ^ f(k)), so that both reads spread over the banks.  Tiles come from the pool straight into LDS.
 //
-// Work is divided evenly: all (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of
-// equal length, whatever the sequences' lengths are.  An item (sequence, KV head, row tile) that one workgroup has whole is finished by
-// it; of others it leaves (m, l, O) in the workspace, and a second kernel joins them.
+// How the work is divided: row_line.h.  Calls of more rows to a sequence and KV head are row_attn_latent.hip's (latent rows, above 16) and
+// row_attn_shared.hip's (trees, above 32): there a key that one wave reads serves too few rows.
+//
+// Bound by latency in small calls (one row of 16 heads over 700 latent rows 16 us, of which 4.5 are the second launch) and by HBM in
+// large ones: 64 rows of 16 heads over 512 .. 4096 latent rows 49 us, 3.5 TB/s of the 5.1 that a large copy reaches.
 #include "row_line.h"
 
 #include <algorithm>
@@ -353,9 +355,9 @@ RowPlan row_plan(const RowAttnArgs& a) {
     r.workers = (int)std::min<int64_t>(most, (items * (tiles + r.over) + r.least - 1) / r.least);
     // An item whole for every workgroup saves the second launch and the division, and costs what the longest item takes alone.  Measured
     // at equal lengths, divided and whole: one row of 16 heads, 256 tokens 15.4 and 12.7 us, 512 15.9 and 15.4, 768 16.8 and 18.6; 128
-    // heads, 1 x 256 tokens 16.5 and 14.4, 1 x 512 17.5 and 20.3, 64 x 512 38.6 and 24.1; trees of 9 drafts for 8 KV heads of 4, one wave
-    // to the rows, 1 x 192 tokens 12.5 and 7.7, 1 x 384 11.7 and 10.5; of 2 drafts, 1 x 768 10.9 and 9.4, 8 x 768 14.4 and 11.3.
-    // Many items even out whatever their lengths are (400 rows of 1024 tokens: 16 heads 112 and 99 us, 128 heads 328 and 242).
+    // heads, 1 x 256 tokens 17.3 and 14.8, 1 x 512 17.5 and 20.9, 64 x 512 37.7 and 25.9, 64 x 768 42.7 and 32.3; trees of 9 drafts for
+    // 8 KV heads of 4, 1 x 192 tokens 12.5 and 7.7, 1 x 384 11.7 and 10.5; of 2 drafts, 1 x 768 10.9 and 9.4, 8 x 768 14.4 and 11.3.
+    // Many items even out whatever their lengths are (400 x 1024 tokens: 128 heads 234 and 193 us, trees of 9 drafts 356 and 317).
     const int64_t all = (int64_t)a.num_seqs * a.hkv * r.row_tiles, few = r.shared ? 256 : latent ? 384 : 768;
     r.single = span <= (items >= 2 * most ? 1024 : many ? 768 : few) && all <= 2 * items;       // (few workgroups for no rows)
     if (r.single) r.over = 0, r.workers = (int)std::min<int64_t>(all, INT32_MAX);

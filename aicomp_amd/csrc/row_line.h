@@ -1,5 +1,5 @@
-// The line of work of the matrix-core kernels of row_attn.h (row_attn_mfma.hip, row_attn_shared.hip): which piece of it a workgroup has,
-// what a row sees of a tile, and how the pieces of an item are joined.
+// The line of work of the matrix-core kernels of row_attn.h (row_attn_mfma.hip, row_attn_shared.hip, row_attn_latent.hip): which piece of
+// it a workgroup has, what a row sees of a tile, and how the pieces of an item are joined.
 //
 // All (sequence, KV head, row tile, key tile) in this order are one line, of which every workgroup has a piece of equal length, whatever
 // the sequences' lengths are.  Before an item's key tiles the line has `over` places more, in which nothing is done: what the start and
