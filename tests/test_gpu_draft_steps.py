@@ -297,3 +297,41 @@ def test_latent_attention_of_a_mixed_step(device, interleaved):
     f = int(moved.first[0])
     tab = plan.host_block_table[0]
     assert torch.equal(backend.pools[0][tab[(f + 1) // 16], (f + 1) % 16], before[tab[(f + 2) // 16], (f + 2) % 16])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_trees_through_normed_layers(device, interleaved):
+    """A tree that is a line, through a layer with head norms: what a chunk of the same tokens gives, and the same rows in the pools.  Both
+    sum in float32: a score of 64 products of normed heads, |scale q k| <= 8 max |w_q w_k| < 20, is off by at most 110 * 2^-24 * 20, a weight
+    by twice that relatively, 2^-11.9, and the mean of values by less than 2^-10.9 of the largest, on either side: 2^-9.9 between the two.
+    A layer with a score rule refuses the tree."""
+    g = torch.Generator().manual_seed(6)
+    inv = 1.0 / 10000.0 ** (torch.arange(0, 64, 2, dtype=torch.float32) / 64)
+    mk = lambda n, h: torch.randn(n, h, 64, generator=g).to(device)
+    weights = 1 + 0.2 * torch.randn(2, 64, generator=g)
+    first, rest = [[mk(n, h) for h in (8, 2, 2)] for n in (20, 7)]
+    got = []
+    for tree in (False, True):
+        planner = StepPlanner(num_blocks=8, max_seqs=2, max_seq_len=64, max_num_batched_tokens=64, device=device, check_plans=True)
+        backend = PagedAttentionBackend(1, 8, 2, 64, torch.float32, device, inv_freq=inv, max_positions=64, interleaved=interleaved)
+        backend.set_head_norm(0, weights[0], weights[1], 1e-6)
+        planner.add_request("a", 20 if tree else 27)
+        if not tree:
+            planner.prefill_chunk = 20
+        backend.begin_step(planner.schedule())
+        backend.attend(0, *first)
+        plan = planner.schedule_drafts({"a": list(range(-1, 6))}) if tree else planner.schedule()
+        backend.begin_step(plan)
+        got.append(backend.attend(0, *rest))
+        if tree:
+            moved = planner.keep_drafts(plan, {"a": list(range(7))})
+            assert not moved.moves
+            backend.keep_drafts(moved)
+        got.append([backend.k_pools[0].clone(), backend.v_pools[0].clone()])
+    bound = 2.0 ** -9.9 * float(max(first[2].abs().max(), rest[2].abs().max()))
+    assert float((got[0] - got[2]).abs().max()) <= bound
+    assert torch.equal(got[1][0], got[3][0]) and torch.equal(got[1][1], got[3][1])
+    backend.set_score_rule(0, softcap=30.0)
+    backend.begin_step(planner.schedule_drafts({"a": [-1]}))
+    with pytest.raises(RuntimeError, match="without one"):
+        backend.attend(0, mk(1, 8), mk(1, 2), mk(1, 2))
