@@ -594,7 +594,8 @@ int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const flo
  *                   was cached before them, and draft b of its sequence if bit b % 64 of its word b / 64 is set
  *   longest_context what the caller knows of context_lens (0: nothing); it sizes the call and bounds nothing
  *   workspace       aicomp_paged_latent_workspace_bytes(...) bytes (max_q_len 1 without cu_q_lens), 16-byte aligned, needing no
- *                   initialisation; may be NULL where that is 0.  Calls that may overlap need separate ones
+ *                   initialisation; may be NULL where that is 0.  Calls that may overlap need separate ones.  The bytes are those of a
+ *                   call with these arguments: a smaller longest_context never needs more, but a call of fewer rows may need more
  * A row that sees nothing is zero, as are the rows of a sequence whose context is shorter than its tokens here.  Keys that a row does
  * not see may hold anything; a row that sees an element that is not finite may be not a number as a whole.
  * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16.  Matrix cores: 16 bits, 512 + 64, blocks of 16.

@@ -458,3 +458,47 @@ def test_scales_of_either_sign(dtype, scale):
     ops.latent_prompt_attn(out, q.cuda(), expanded.cuda()[..., :128], latent.cuda()[:, 512:], expanded.cuda()[..., 128:], cu, cuk, scale, 200)
     want, mean_abs, size = expect_prompt(q, expanded, latent, [200, 70], [200, 33], 128, 64, scale)
     check(out.cpu(), want, attention_bound(want, mean_abs, size, 192, dtype))
+
+
+# ------------------------------------------------- calls whose items are divided among workgroups (longer contexts)
+@pytest.mark.parametrize("n", [257, 1100, 3000])
+def test_many_sequences_divided(n):
+    """As above, with a context that no workgroup has whole."""
+    ctx = [(i * 7) % 40 for i in range(n)]
+    ctx[-1], ctx[-2], ctx[5], ctx[n // 2] = 1500, 0, 400, 2100
+    c = Latent(ctx, [1] * n, 2, seed=12)
+    c.check(c.run())
+    t = Tree(ctx, [min(i % 4, x) for i, x in enumerate(ctx)], 2, 1, 64, seed=13)
+    t.check(t.run(max_q_len=3))
+    cut = Latent(ctx, [i % 3 for i in range(n)], 12, seed=14)
+    cut.check(cut.run())
+    wide = Tree(ctx, [min(i % 4, x) for i, x in enumerate(ctx)], 16, 1, 64, seed=15)
+    wide.check(wide.run())
+
+
+@pytest.mark.parametrize("new", [[3, 1, 4, 2], [8, 7, 5, 1], [16, 2, 9, 3], [30, 31, 1, 40]])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype,pool", [(BF16, None), (F16, None), (BF16, FP8), (F16, FP8)])
+def test_trees_divided(dtype, pool, d, new):
+    c = Tree([3000, 900, 20, 1300], new, 8, 2, d, dtype=dtype, pool=pool, seed=29, rows_behind=2)
+    c.poison()
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("rows", ["one", "chunk", "tree"])
+@pytest.mark.parametrize("H", [4, 17, 33, 64, 65, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_latent_rows_divided(dtype, H, rows):
+    c = Latent([3000, 900, 20, 1300, 0, 64], [1] * 6 if rows == "one" else [3, 1, 4, 9, 1, 2], H, dtype=dtype, seed=30)
+    if rows == "tree":
+        c.tree()
+    c.poison()
+    c.check(c.run())
+
+
+def test_the_same_rows_whole_and_divided():
+    """The bound of the contexts changes how a call is laid out, not what it gives: each within the tolerance, both of one formula."""
+    for c in (Latent([700, 300, 90], [1, 1, 1], 16, seed=31), Latent([700, 300, 90], [5, 3, 9], 16, seed=32).tree(),
+              Tree([700, 300, 90], [5, 3, 9], 8, 2, 128, seed=33), Tree([700, 300, 90], [40, 3, 9], 8, 2, 128, seed=34)):
+        for longest in (0, 1, 100, 700, 10 ** 6):
+            c.check(c.run(longest_context=longest))
