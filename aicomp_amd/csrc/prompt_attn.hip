@@ -264,6 +264,7 @@ prompt_attn_kernel(PromptParams p) {
         };
 #pragma unroll
         for (int u = 0; u < VAHEAD; ++u) val[u] = value_of(u);
+        __builtin_amdgcn_s_setprio(2);                             // (before the other wave's softmax: 8192 tokens 358 and 351 us)
 #pragma unroll
         for (int u = 0; u < 2 * NJ; ++u) {
             if (u + VAHEAD < 2 * NJ) val[(u + VAHEAD) % (VAHEAD + 1)] = value_of(u + VAHEAD);
@@ -272,6 +273,7 @@ prompt_attn_kernel(PromptParams p) {
             for (int c = 0; c < R; ++c) O[c][u >> 1] = E::mfma(__builtin_bit_cast(uint4, val[u % (VAHEAD + 1)]), pf[c][u & 1], O[c][u >> 1]);
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
     };
 
     // A weight of 0 times a value that is not finite is not 0.  In tiles that not all queries here see whole, a wave looks through the

@@ -347,10 +347,11 @@ RowPlan row_plan(const RowAttnArgs& a) {
     const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / r.rows + a.num_seqs);
     // What an item's start and end cost, in key tiles, counts where workgroups have several items (64 rows of 512 .. 4096 tokens, 16 heads:
     // 60 us without, 55 with); where items are divided, as many workgroups as there are tiles for are worth more (one row of 700 tokens:
-    // 17 us without, 21 with).
+    // 17 us without, 21 with).  32 rows of 128 heads over 512 .. 4096 latent rows: 54 us with one tile's worth, 49.5 with three, 47.2 with six,
+    // 49 with ten; trees of 16 .. 64 drafts over as many tokens 117 with three, 119 with one, 117 with six.
     const int64_t tiles = (span + r.keys - 1) / r.keys, most = latent || a.dk == 256 ? 256 : 512;
     const bool many = items * 4 >= most;
-    r.over = many ? (r.shared ? 3 : 8) : 0;
+    r.over = many ? (!r.shared ? 8 : latent ? 6 : 3) : 0;
     r.least += r.over;
     r.workers = (int)std::min<int64_t>(most, (items * (tiles + r.over) + r.least - 1) / r.least);
     // An item whole for every workgroup saves the second launch and the division, and costs what the longest item takes alone.  Measured
