@@ -1,5 +1,5 @@
 // Attention of query rows over cached or expanded latent rows on the vector ALU: every type, head and row size.  The path of what
-// the matrix-core kernels do not take: float32, other sizes than theirs, other blocks than of 16 tokens.
+// the matrix-core kernels do not take: float32, other sizes than theirs, blocks of fewer than 16 tokens or of no power of two.
 //
 // One workgroup per (query row, head).  Tiles of 256 keys: a thread has one key's score (a row of the pool is read by one thread, 16
 // bytes at a time, so that the lines are taken whole from the L1), the tile's weights go through LDS, and the output's
@@ -7,7 +7,7 @@
 // softmax in float32, exponents in base 2.  Keys that the row does not see are neither multiplied nor read.
 //
 // Bound by the reads of every (row, head) for itself, out of the caches: 16 rows of 16 heads over 1024 latent rows of float32 387 us, of
-// bfloat16 in blocks of 32 tokens 310 (in blocks of 16, on the matrix cores, 21).
+// bfloat16 in blocks of 48 tokens 310 (in blocks of 16, on the matrix cores, 21).
 #include "row_attn.h"
 
 #include <algorithm>

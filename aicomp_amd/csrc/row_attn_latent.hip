@@ -1,5 +1,5 @@
 // Attention of many query rows over latent rows of 512 + 64 elements (row_attn.h) on the matrix cores: more than 16 (token, head) pairs
-// to a sequence; 16 bits, blocks of 16 tokens.
+// to a sequence; 16 bits, blocks of 16, 32, 64 .. tokens.
 //
 // An output of 512 elements is too much of a wave's registers for more than 32 rows, and a row of 1152 bytes too much of LDS for every
 // wave to have tiles of its own.  So four waves, one to a SIMD with all its registers, share 64 rows and tiles of 64 keys, two of those in
@@ -92,10 +92,9 @@ row_attn_latent_kernel(RowParams p) {
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
         const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
-        const int last_block = (q.ctx - 1) / BS;               // (blocks behind it are not this sequence's)
-        // Wave w brings in block w of a tile, load i of 18.
-        auto block = [&](int b) { return (const char*)p.k_pool + (int64_t)max(0, min(b, p.num_blocks - 1)) * BS * KROW; };
-        auto block_of = [&](int t) { return block(table[min(4 * t + w, last_block)]); };
+        // Wave w brings in 16 rows of a tile, by 18 loads.
+        auto block = [&](int entry, int t) { return (const char*)p.k_pool + place_of(p, entry, 0, 4 * t + w) * BLOCK; };
+        auto block_of = [&](int t) { return block(table[entry_of(p, q, 4 * t + w)], t); };
         // (a buffer of no bytes brings in nothing: the last tile's step has the same instructions as the others)
         auto buffer_of = [&](const char* from, bool there) {
             return __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, there ? BLOCK : 0, 0x00027000);
@@ -107,7 +106,7 @@ row_attn_latent_kernel(RowParams p) {
         const int t_end = min(it.t1, (q.ctx + KT - 1) / KT);   // (0 tiles where the context is none)
         // The rows come by way of the second buffer, sixteen by each wave (rows beyond the last: that one, computed and not stored); before
         // the first tile, whose place in the table is still to arrive.
-        const int entry = t_end > it.t0 ? table[min(4 * (t_end - 1) + w, last_block)] : 0;
+        const int entry = t_end > it.t0 ? table[entry_of(p, q, 4 * (t_end - 1) + w)] : 0;
         {
             const int here = min(row0 + 16 * w, nrows - 1);
             const char* from = (const char*)p.query + ((int64_t)q.begin * p.hq + here) * KROW;
@@ -117,7 +116,7 @@ row_attn_latent_kernel(RowParams p) {
                 __builtin_amdgcn_global_load_lds(GLOBAL_PTR(from + at[i & 1] + (i >> 1) * 128), LDS_PTR(buf1 + w * BLOCK + 1024 * i), 16, 0, 0);
         }
         if (it.t0 < t_end) {
-            const auto from = buffer_of(block(entry), true);
+            const auto from = buffer_of(block(entry, t_end - 1), true);
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) load(from, buf0, i);
         }

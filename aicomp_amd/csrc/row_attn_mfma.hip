@@ -1,5 +1,5 @@
 // Attention of query rows over cached rows (row_attn.h) on the matrix cores: latent rows of 512 + 64 elements, trees of drafts over K and
-// V pools of head_dim 64, 128 and 256; 16-bit rows, and fp8 ones under them; blocks of 16 tokens.
+// V pools of head_dim 64, 128 and 256; 16-bit rows, and fp8 ones under them; blocks of 16, 32, 64 .. tokens.
 //
 // The rows of a sequence and KV head, (token, head) pairs one after the other, are cut into tiles of 16 R rows, and the keys into
 // tiles of 32.  A workgroup has a row tile; its four waves take the key tiles in turn, each with its own piece of LDS, its own running
@@ -88,10 +88,9 @@ row_attn_kernel(RowParams p) {
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
         const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
-        const int last_block = (q.ctx - 1) / BS;                           // (blocks behind it are not this sequence's)
-        auto block_base = [&](int t, int half) -> int64_t {                // element index of the block's first row
-            const int b = table[min(2 * t + half, last_block)];
-            return ((int64_t)max(0, min(b, p.num_blocks - 1)) * p.hkv + kvh) * (BS * DK);
+        auto block_base = [&](int t, int half) -> int64_t {                // element index of the first of the 16 rows
+            const int g = 2 * t + half;
+            return place_of(p, table[entry_of(p, q, g)], kvh, g) * (BS * DK);
         };
         auto fetch_dma = [&](int t) __attribute__((always_inline)) {
             if constexpr (!FP8) {
@@ -341,7 +340,7 @@ RowPlan row_plan(const RowAttnArgs& a) {
     r.keys = r.shared ? 64 : 32;
     r.least = r.shared ? 2 : 4;
     r.row_tiles = (int)((rows + r.rows - 1) / r.rows);
-    int64_t span = (int64_t)a.max_blocks * BS;
+    int64_t span = (int64_t)a.max_blocks * a.bs;
     if (a.longest_context > 0) span = std::min<int64_t>(span, a.longest_context);
     // (rows in all bound the row tiles too, where one long sequence is among many short ones)
     const int64_t items = a.hkv * std::min<int64_t>((int64_t)a.num_seqs * r.row_tiles, a.rows * group / r.rows + a.num_seqs);
@@ -382,14 +381,14 @@ template <typename E, bool FP8> void launch_tree(const RowParams& p, const RowPl
 
 // (the join's grid holds less than 2^32 threads; a workgroup's place in a launch and a row are 32 bits)
 bool row_attn_mfma_supported(const RowAttnArgs& a) {
-    if (a.bs != BS || !is_16bit_float(a.q_dtype) || a.num_blocks > INT32_MAX) return false;
+    if (a.bs < BS || (a.bs & (a.bs - 1)) != 0 || !is_16bit_float(a.q_dtype) || a.num_blocks > INT32_MAX) return false;
     const bool latent = a.dk == 576 && a.dv == 512 && a.v_row == 576 && a.hkv == 1;
     if (!latent && (a.dk != a.dv || (a.dk != 64 && a.dk != 128 && a.dk != 256))) return false;
     const int64_t rows = (int64_t)a.max_q_len * (a.hq / a.hkv), wgs = (rows + 127) * a.hkv * a.num_seqs / 2;
     if (rows > INT32_MAX / 2 || a.rows > INT32_MAX || wgs >= ((int64_t)1 << 24) || (int64_t)a.num_seqs * a.hkv >= ((int64_t)1 << 24)) return false;
     const RowPlan r = row_plan(a);                             // (the whole line, contexts as long as the table)
     return (int64_t)a.num_seqs * a.hkv * r.row_tiles < ((int64_t)1 << 24) &&
-           (int64_t)a.num_seqs * a.hkv * r.row_tiles * (((int64_t)a.max_blocks * BS + r.keys - 1) / r.keys + r.over) < ((int64_t)1 << 30);
+           (int64_t)a.num_seqs * a.hkv * r.row_tiles * (((int64_t)a.max_blocks * a.bs + r.keys - 1) / r.keys + r.over) < ((int64_t)1 << 30);
 }
 
 size_t row_attn_mfma_workspace_bytes(const RowAttnArgs& a) {
@@ -403,7 +402,7 @@ int launch_row_attn_mfma(const RowAttnArgs& a) {
     p.out = a.out; p.query = a.query; p.k_pool = a.k_pool; p.v_pool = a.v_pool; p.block_table = a.block_table;
     p.block_table_stride = a.block_table_stride; p.context_lens = a.context_lens; p.cu_q_lens = a.cu_q_lens; p.masks = a.masks;
     p.mask_words = a.mask_words; p.num_seqs = a.num_seqs; p.rows = (int)a.rows; p.max_q_len = a.max_q_len; p.hq = a.hq; p.hkv = a.hkv;
-    p.group = a.hq / a.hkv; p.max_blocks = a.max_blocks; p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
+    p.group = a.hq / a.hkv; p.span = a.max_blocks * a.bs; p.shift = __builtin_ctz(a.bs / BS); p.num_blocks = (int)a.num_blocks; p.mul = a.scale * LOG2E; p.k_scale = a.k_scale;
     p.v_scale = a.v_scale; p.workers = r.workers; p.single = r.single; p.least = r.least; p.over = r.over; p.row_tiles = r.row_tiles;
     p.ws_acc = (float*)a.workspace;
     p.ws_ml = (float2*)(p.ws_acc + (size_t)2 * r.workers * r.rows * a.dv);

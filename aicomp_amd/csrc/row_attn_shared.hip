@@ -1,5 +1,5 @@
 // Attention of many query rows over cached rows (row_attn.h) on the matrix cores: trees of drafts whose rows are more than two groups
-// of 16 to a KV head, over K and V pools of head_dim 64, 128 and 256; blocks of 16 tokens.
+// of 16 to a KV head, over K and V pools of head_dim 64, 128 and 256; blocks of 16, 32, 64 .. tokens.
 //
 // Where row_attn_mfma.hip has every wave stream keys of its own for all rows of the workgroup, here the four waves have rows of
 // their own, 16 R each, and share the tiles of 64 keys, which are brought into LDS while the tile before is computed: a key is
@@ -91,11 +91,10 @@ row_attn_shared_kernel(RowParams p) {
 
         typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
         const const_i32_ptr table = (const_i32_ptr)(p.block_table + (int64_t)mine.seq * p.block_table_stride);
-        const int last_block = (q.ctx - 1) / BS;               // (blocks behind it are not this sequence's)
         // wave w brings in block w of a tile
         auto block_base = [&](int t) -> int64_t {              // element index of its first row
-            const int b = table[min(4 * t + w, last_block)];
-            return ((int64_t)max(0, min(b, p.num_blocks - 1)) * p.hkv + kvh) * (BS * D);
+            const int g = 4 * t + w;
+            return place_of(p, table[entry_of(p, q, g)], kvh, g) * (BS * D);
         };
         auto fetch_dma = [&](int t, unsigned char* kb, unsigned char* vb) __attribute__((always_inline)) {
             const int64_t base = block_base(t) * 2;

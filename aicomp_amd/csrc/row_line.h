@@ -27,7 +27,8 @@ struct RowParams {
     int mask_words;
     int num_seqs;
     int rows, max_q_len;
-    int hq, hkv, group, max_blocks, num_blocks;
+    int hq, hkv, group, num_blocks;
+    int span, shift;                   // tokens of a table's row; a block has 16 << shift
     float mul;                         // scale * log2(e)
     const float* k_scale;
     const float* v_scale;
@@ -47,7 +48,7 @@ void launch_row_attn_latent(const RowParams& p, bool f16, int64_t items, hipStre
 
 namespace {
 
-constexpr int BS = 16;                 // tokens per block
+constexpr int BS = 16;                 // tokens that are looked up together: a block, or a part of one
 constexpr float NEG_BIG = -1.0e30f;
 constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both formats' range
 
@@ -72,12 +73,20 @@ template <int ROWS, int KT> __device__ __forceinline__ Seq load_seq(const RowPar
     q.begin = p.cu_q_lens ? max(0, p.cu_q_lens[s]) : s;
     q.n = p.cu_q_lens ? min(min(p.cu_q_lens[s + 1], p.rows) - q.begin, p.max_q_len) : 1;
     q.n = max(0, q.n);
-    q.ctx = min(p.context_lens[s], p.max_blocks * BS);
+    q.ctx = min(p.context_lens[s], p.span);
     q.prior = q.ctx - q.n;
     if (q.prior < 0) q.ctx = 0;
     q.row_tiles = (q.n * p.group + ROWS - 1) / ROWS;
     q.key_tiles = max(1, (q.ctx + KT - 1) / KT);
     return q;
+}
+
+// Which entry of a table's row has the g-th 16 tokens, and where they are in the pool, in units of 16 rows.
+__device__ __forceinline__ int entry_of(const RowParams& p, const Seq& q, int g) {
+    return min(g >> p.shift, (q.ctx - 1) >> (4 + p.shift));    // (entries behind the last one are not this sequence's)
+}
+__device__ __forceinline__ int64_t place_of(const RowParams& p, int entry, int kvh, int g) {
+    return (((int64_t)max(0, min(entry, p.num_blocks - 1)) * p.hkv + kvh) << p.shift) + (g & ((1 << p.shift) - 1));
 }
 
 // A workgroup's piece of the line: places at .. end - 1, the first of them place `off` of sequence `seq`, `q`.  (A line is less than 2^31

@@ -502,3 +502,29 @@ def test_the_same_rows_whole_and_divided():
               Tree([700, 300, 90], [5, 3, 9], 8, 2, 128, seed=33), Tree([700, 300, 90], [40, 3, 9], 8, 2, 128, seed=34)):
         for longest in (0, 1, 100, 700, 10 ** 6):
             c.check(c.run(longest_context=longest))
+
+
+@pytest.mark.parametrize("longest", [0, 100])
+@pytest.mark.parametrize("bs", [32, 64, 128, 512])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_blocks_of_more_tokens(dtype, bs, longest):
+    """Blocks of several groups of 16 tokens, ending inside a tile and inside a block, in every matrix-core form; others (48) beside them."""
+    ctx = [700, 33, 300, 0, bs, bs + 1, 64]
+    for H, new, tree in ((16, [1] * 7, False), (40, [1] * 7, False), (12, [9, 1, 5, 1, 3, 1, 2], True), (16, [9, 1, 5, 1, 3, 1, 2], False)):
+        c = Latent(ctx, new, H, bs=bs, dtype=dtype, seed=35)
+        if tree:
+            c.tree()
+        c.poison()
+        c.check(c.run(longest_context=longest))
+    for d, pool, new in ((64, None, [9, 1, 5, 1, 3, 1, 2]), (128, FP8, [4, 1, 5, 1, 3, 1, 2]), (128, None, [40, 1, 5, 1, 3, 1, 2]),
+                         (64, FP8, [40, 1, 5, 1, 3, 1, 2]), (256, None, [9, 1, 5, 1, 3, 1, 2])):
+        t = Tree(ctx, new, 8, 2, d, bs=bs, dtype=dtype, pool=pool, seed=36)
+        t.poison()
+        t.check(t.run(longest_context=longest))
+
+
+def test_matrix_cores_take_larger_blocks(device):
+    from helpers import kernels_of
+    for bs, name in ((16, "row_attn_kernel"), (64, "row_attn_kernel"), (48, "rows_generic_kernel"), (8, "rows_generic_kernel")):
+        c = Latent([100, 30], [1, 1], 16, bs=bs, seed=37)
+        assert any(name in k for k in kernels_of(c.run)), bs
