@@ -598,7 +598,8 @@ int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const flo
  *                   call with these arguments: a smaller longest_context never needs more, but a call of fewer rows may need more
  * A row that sees nothing is zero, as are the rows of a sequence whose context is shorter than its tokens here.  Keys that a row does
  * not see may hold anything; a row that sees an element that is not finite may be not a number as a whole.
- * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16.  Matrix cores: 16 bits, 512 + 64, blocks of 16.
+ * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16.  Matrix cores: 16 bits, 512 + 64, blocks
+ * of 16, 32, 64 .. tokens.
  */
 int aicomp_paged_latent_attn(void* out, const void* query, const void* pool,
                              const int32_t* block_table, int64_t block_table_stride,
@@ -639,7 +640,8 @@ int aicomp_latent_prompt_attn(void* out, const void* query,
  * already, see what was cached before them, and each other by tree_masks (as in aicomp_paged_latent_attn).
  *   out, query, pools, block_table, context_lens, cu_q_lens, scales   as in aicomp_paged_prefill_attn
  *   longest_context, workspace   as in aicomp_paged_latent_attn, with aicomp_paged_tree_workspace_bytes
- * head_dim 64, 128 or 256; any block size; f32/f32, bf16/bf16, f16/f16, bf16/fp8, f16/fp8 (query / pool); pointers 16-byte aligned.
+ * head_dim 64, 128 or 256; any block size (matrix cores, for 16-bit queries: 16, 32, 64 .. tokens); f32/f32, bf16/bf16, f16/f16, bf16/fp8,
+ * f16/fp8 (query / pool); pointers 16-byte aligned.
  */
 int aicomp_paged_tree_attn(void* out, const void* query, const void* k_pool, const void* v_pool,
                            const int32_t* block_table, int64_t block_table_stride,
