@@ -42,6 +42,7 @@ row_attn_kernel(RowParams p) {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * TILE];
     __shared__ PieceScratch scratch;
     __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];             // of each wave
+    __shared__ float factor[4][ROWS];                          // of a wave's output in the whole
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -292,28 +293,32 @@ row_attn_kernel(RowParams p) {
 #pragma unroll
                 for (int j = 0; j < CH / 16; ++j)
                     *(f32x4_t*)(joint + (w * ROWS + 16 * c + r16) * (CH + 4) + 16 * j + 4 * g4) = O[c][ch * (CH / 16) + j];
+            if (ch == 0 && tid < ROWS) {
+                float top = sm_m[0][tid], sum = 0.f;
+#pragma unroll
+                for (int k = 1; k < 4; ++k) top = fmaxf(top, sm_m[k][tid]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum = fmaf(__builtin_amdgcn_exp2f(sm_m[k][tid] - top), sm_l[k][tid], sum);
+                // (sum 0: nothing was seen, and O is 0)
+                const float inv = !it.whole ? 1.f : sum == 0.f ? 0.f : (FP8 ? p.v_scale[kvh] : 1.f) / sum;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) factor[k][tid] = __builtin_amdgcn_exp2f(sm_m[k][tid] - top) * inv;
+                if (!it.whole) p.ws_ml[it.slot * ROWS + tid] = make_float2(top, sum);
+            }
             __syncthreads();
-#pragma unroll
-            for (int i0 = 0; i0 < ROWS * (CH / 4); i0 += 256) {
-                const int i = i0 + tid, r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
-                float top = sm_m[0][r], sum = 0.f;
-#pragma unroll
-                for (int k = 1; k < 4; ++k) top = fmaxf(top, sm_m[k][r]);
+            // (not unrolled: a call of one tile runs this once, and waits for its instructions)
+#pragma unroll 1
+            for (int i = tid; i < ROWS * (CH / 4); i += 256) {
+                const int r = i / (CH / 4), col = i % (CH / 4) * 4, row = rtile * ROWS + r;
+                if (row >= nrows) break;
                 f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float f = __builtin_amdgcn_exp2f(sm_m[k][r] - top);
-                    sum = fmaf(f, sm_l[k][r], sum);
-                    o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col) * f;
-                }
-                if (row >= nrows) continue;
+                for (int k = 0; k < 4; ++k) o += *(const f32x4_t*)(joint + (k * ROWS + r) * (CH + 4) + col) * factor[k][r];
                 if (!it.whole) {
                     *(f32x4_t*)(p.ws_acc + (it.slot * ROWS + r) * DV + ch * CH + col) = o;
-                    if (ch == 0 && col == 0) p.ws_ml[it.slot * ROWS + r] = make_float2(top, sum);
                 } else {
-                    const float inv = sum == 0.f ? 0.f : (FP8 ? p.v_scale[kvh] : 1.f) / sum;   // (0: nothing was seen, and O is 0)
                     uint16_t* dst = (uint16_t*)p.out + ((int64_t)(q.begin + row / p.group) * p.hq + kvh * p.group + row % p.group) * DV;
-                    *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv));
+                    *(uint2*)(dst + ch * CH + col) = make_uint2(E::pack(o[0], o[1]), E::pack(o[2], o[3]));
                 }
             }
         }
