@@ -212,7 +212,8 @@ int aicomp_kv_keep_rows(void* const* pools, int num_pools, int64_t row_bytes, in
     for (int i = 0; i < num_pools; ++i)
         AICOMP_REQUIRE(pools[i], AICOMP_KV_EINVAL, "%s: pool %d is a null pointer", who, i);
     AICOMP_REQUIRE(row_bytes > 0 && row_bytes <= INT32_MAX && num_kv_heads > 0 && block_size > 0 && num_blocks > 0 &&
-                   max_blocks_per_seq > 0 && block_table_stride >= max_blocks_per_seq && total_keep <= INT32_MAX, AICOMP_KV_EINVAL,
+                   max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size <= INT32_MAX &&
+                   block_table_stride >= max_blocks_per_seq && total_keep <= INT32_MAX - 64, AICOMP_KV_EINVAL,
                    "%s: bad sizes (row of %lld bytes, Hkv %d, BS %d, blocks %lld, table %d)", who, (long long)row_bytes, num_kv_heads,
                    block_size, (long long)num_blocks, max_blocks_per_seq);
     AICOMP_REQUIRE(row_bytes <= INT32_MAX / num_kv_heads && num_seqs <= 16777215, AICOMP_KV_EINVAL,

@@ -7,8 +7,8 @@
 // the chain of a sequence is a quarter of its entries.
 //
 // A copy of pieces of some hundred bytes: bound by the launch and by four dependent loads for one sequence, by them and the pieces' places
-// all over HBM for many.  One sequence, 4 of 9 drafts in 64 pools: 5.4 us; 64 sequences, 8 of 32 in 32 pools: 22 us, 2.6 TB/s (eight entries at
-// a time brought nothing).
+// all over HBM for many.  One sequence, 4 of 9 drafts in 64 pools: 5.3 us; 64 sequences, 8 of 32 in 32 pools: 18.8 us, 3.1 TB/s (one pool to
+// a workgroup 20.9, two 19.9; eight entries at a time 20.8).
 #include "row_attn.h"
 
 #include <algorithm>
@@ -19,6 +19,7 @@ namespace {
 
 constexpr int MAX_POOLS = 128;             // per launch: 1 KB of arguments
 constexpr int AHEAD = 4;
+constexpr int TOGETHER = 4;                // pools of a workgroup, which looks the rows' places up once
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -33,7 +34,7 @@ struct KeepParams {
     int hkv, bs, max_blocks;
 };
 
-// Workgroup (sequence, pool, slice of the row's vectors); V = the widest vector that the rows and the pools' alignment allow
+// Workgroup (sequence, four pools, slice of the row's vectors); V = the widest vector that the rows and the pools' alignment allow
 template <typename V>
 __global__ void __launch_bounds__(128)
 keep_rows_kernel(KeepParams p) {
@@ -42,28 +43,38 @@ keep_rows_kernel(KeepParams p) {
     const int col = blockIdx.z * 128 + threadIdx.x;
     if (col >= p.hkv * p.vecs) return;
     const int head = col / p.vecs, v = col - head * p.vecs;
-    V* pool = (V*)p.pools[blockIdx.y];
+    // (behind the last pool it is there again: the same thread then reads and writes the same twice)
+    V* pool[TOGETHER];
+#pragma unroll
+    for (int j = 0; j < TOGETHER; ++j) pool[j] = (V*)p.pools[blockIdx.y * TOGETHER + j];
     const int32_t* table = p.block_table + seq * p.block_table_stride;
     const int64_t first = p.first[seq], limit = (int64_t)p.max_blocks * p.bs;
     // the vector of a token of this sequence, -1 where it has none
     auto at = [&](int64_t token) -> int64_t {
         if (token < 0 || token >= limit) return -1;
-        const int64_t blk = table[token / p.bs];
+        const uint32_t entry = (uint32_t)token / (uint32_t)p.bs;            // (64-bit divisions: 3 of 21 us)
+        const int64_t blk = table[entry];
         if (blk < 0 || blk >= p.num_blocks) return -1;
-        return ((blk * p.hkv + head) * p.bs + token % p.bs) * p.vecs + v;
+        return ((blk * p.hkv + head) * p.bs + ((uint32_t)token - entry * p.bs)) * p.vecs + v;
     };
     for (int i = begin; i < end; i += AHEAD) {
         int64_t from[AHEAD], to[AHEAD];
-        V held[AHEAD];
+        V held[TOGETHER][AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             from[k] = i + k < end ? at(first + p.keep[i + k]) : -1;
             to[k] = i + k < end ? at(first + (i + k - begin)) : -1;
-            if (from[k] >= 0) held[k] = pool[from[k]];
+            if (from[k] >= 0) {
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) held[j][k] = pool[j][from[k]];
+            }
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-            if (from[k] >= 0 && to[k] >= 0 && from[k] != to[k]) pool[to[k]] = held[k];
+            if (from[k] >= 0 && to[k] >= 0 && from[k] != to[k]) {
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) pool[j][to[k]] = held[j][k];
+            }
     }
 }
 
@@ -83,7 +94,7 @@ int launch_keep_rows(const KeepRowsArgs& a) {
     for (int first = 0; first < a.num_pools; first += MAX_POOLS) {
         const int n = std::min(a.num_pools - first, MAX_POOLS);
         for (int i = 0; i < MAX_POOLS; ++i) p.pools[i] = a.pools[first + std::min(i, n - 1)];
-        const dim3 grid((unsigned)a.num_seqs, (unsigned)n, (unsigned)slices);
+        const dim3 grid((unsigned)a.num_seqs, (unsigned)((n + TOGETHER - 1) / TOGETHER), (unsigned)slices);
         if (width == 16) hipLaunchKernelGGL(keep_rows_kernel<u32x4>, grid, dim3(128), 0, a.stream, p);
         else if (width == 4) hipLaunchKernelGGL(keep_rows_kernel<uint32_t>, grid, dim3(128), 0, a.stream, p);
         else hipLaunchKernelGGL(keep_rows_kernel<uint8_t>, grid, dim3(128), 0, a.stream, p);

@@ -167,3 +167,10 @@ def test_a_pool_is_moved_once(lib):
         assert keep(lib, pools=(ctypes.c_void_p * 2)(*pools)) == EINVAL and "overlap" in err(lib)
     assert keep(lib, pools=(ctypes.c_void_p * 4)(P, P + 2 * bytes_, P + bytes_, P + 2 * bytes_ - 1), n=4) == EINVAL and "overlap" in err(lib)
     assert keep(lib, nb=2 ** 60) == EINVAL and "bytes" in err(lib)
+
+
+def test_sizes_that_pass_32_bits_are_refused(lib):
+    """A kernel's loop over the entries, and a token's place in its table, are 32 bits."""
+    pools = (ctypes.c_void_p * 2)(P, P + 2 ** 30)
+    assert keep(lib, pools=pools, total=2 ** 31 - 1) == EINVAL and keep(lib, pools=pools, total=2 ** 31 - 8) == EINVAL
+    assert keep(lib, pools=pools, mb=2 ** 27, stride=2 ** 27) == EINVAL and "sizes" in err(lib)
