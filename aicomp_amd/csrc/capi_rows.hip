@@ -10,20 +10,23 @@
 
 using namespace aicomp;
 
+// tokens that a 32-bit place counts, with a tile beyond the last
+static const int64_t MAX_TOKENS = INT32_MAX - 1023;
+
 static bool float_type(int dt) { return dt == AICOMP_KV_F32 || is_16bit_float(dt); }
 
 // What both paged calls check; the sizes of a row are the caller's.
 static int check_rows(const RowAttnArgs& a, const char* who) {
     AICOMP_REQUIRE(a.hq > 0 && a.hkv > 0 && a.hq % a.hkv == 0 && a.hq <= 65535, AICOMP_KV_EINVAL,
                    "%s: %d query heads are not a multiple of %d KV heads, or more than 65535", who, a.hq, a.hkv);
-    AICOMP_REQUIRE(a.bs > 0 && a.max_blocks > 0 && a.num_blocks > 0 && (int64_t)a.max_blocks * a.bs <= INT32_MAX, AICOMP_KV_EINVAL,
+    AICOMP_REQUIRE(a.bs > 0 && a.max_blocks > 0 && a.num_blocks > 0 && (int64_t)a.max_blocks * a.bs <= MAX_TOKENS, AICOMP_KV_EINVAL,
                    "%s: bad sizes (block_size %d, max_blocks %d, num_blocks %lld)", who, a.bs, a.max_blocks, (long long)a.num_blocks);
     AICOMP_REQUIRE(a.block_table_stride >= a.max_blocks, AICOMP_KV_EINVAL, "%s: block table stride %lld < width %d", who,
                    (long long)a.block_table_stride, a.max_blocks);
     AICOMP_REQUIRE(isfinite(3.f * a.scale), AICOMP_KV_EINVAL, "%s: scale must be finite (got %g)", who, (double)a.scale);
     AICOMP_REQUIRE(a.longest_context >= 0, AICOMP_KV_EINVAL, "%s: negative longest context", who);
     if (a.cu_q_lens != nullptr)
-        AICOMP_REQUIRE(a.max_q_len > 0 && a.max_q_len <= a.rows && a.rows <= INT32_MAX, AICOMP_KV_EINVAL,
+        AICOMP_REQUIRE(a.max_q_len > 0 && a.max_q_len <= a.rows && a.rows <= MAX_TOKENS, AICOMP_KV_EINVAL,
                        "%s: max_q_len %d out of range (total %lld)", who, a.max_q_len, (long long)a.rows);
     else
         AICOMP_REQUIRE(a.rows == a.num_seqs, AICOMP_KV_EINVAL, "%s: without cu_q_lens there is one row per sequence", who);
@@ -177,7 +180,7 @@ int aicomp_latent_prompt_attn(void* out, const void* query, const void* key, int
     if (num_seqs == 0 || total_q == 0) return AICOMP_KV_OK;
     AICOMP_REQUIRE(out && query && cu_q_lens && cu_k_lens && (total_k == 0 || (key && rope_key && value)), AICOMP_KV_EINVAL,
                    "%s: null pointer", who);
-    AICOMP_REQUIRE(num_heads > 0 && num_heads <= 65535 && total_q <= INT32_MAX && total_k <= INT32_MAX, AICOMP_KV_EINVAL,
+    AICOMP_REQUIRE(num_heads > 0 && num_heads <= 65535 && total_q <= MAX_TOKENS && total_k <= MAX_TOKENS, AICOMP_KV_EINVAL,
                    "%s: bad sizes (heads %d, rows %lld, keys %lld)", who, num_heads, (long long)total_q, (long long)total_k);
     AICOMP_REQUIRE(nope_dim > 0 && nope_dim % 16 == 0 && rope_dim > 0 && rope_dim % 16 == 0 && value_dim > 0 && value_dim % 16 == 0,
                    AICOMP_KV_EUNSUPPORTED, "%s: heads of %d + %d key and %d value elements are not multiples of 16", who, nope_dim,
@@ -212,8 +215,8 @@ int aicomp_kv_keep_rows(void* const* pools, int num_pools, int64_t row_bytes, in
     for (int i = 0; i < num_pools; ++i)
         AICOMP_REQUIRE(pools[i], AICOMP_KV_EINVAL, "%s: pool %d is a null pointer", who, i);
     AICOMP_REQUIRE(row_bytes > 0 && row_bytes <= INT32_MAX && num_kv_heads > 0 && block_size > 0 && num_blocks > 0 &&
-                   max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size <= INT32_MAX &&
-                   block_table_stride >= max_blocks_per_seq && total_keep <= INT32_MAX - 64, AICOMP_KV_EINVAL,
+                   max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size <= MAX_TOKENS &&
+                   block_table_stride >= max_blocks_per_seq && total_keep <= MAX_TOKENS, AICOMP_KV_EINVAL,
                    "%s: bad sizes (row of %lld bytes, Hkv %d, BS %d, blocks %lld, table %d)", who, (long long)row_bytes, num_kv_heads,
                    block_size, (long long)num_blocks, max_blocks_per_seq);
     AICOMP_REQUIRE(row_bytes <= INT32_MAX / num_kv_heads && num_seqs <= 16777215, AICOMP_KV_EINVAL,

@@ -174,3 +174,7 @@ def test_sizes_that_pass_32_bits_are_refused(lib):
     pools = (ctypes.c_void_p * 2)(P, P + 2 ** 30)
     assert keep(lib, pools=pools, total=2 ** 31 - 1) == EINVAL and keep(lib, pools=pools, total=2 ** 31 - 8) == EINVAL
     assert keep(lib, pools=pools, mb=2 ** 27, stride=2 ** 27) == EINVAL and "sizes" in err(lib)
+    for call in (latent, tree):
+        assert call(lib, mb=2 ** 27 - 1, stride=2 ** 27) == EINVAL and "sizes" in err(lib)
+        assert call(lib, total=2 ** 31 - 9) == EINVAL and "max_q_len" in err(lib)
+    assert prompt(lib, keys=2 ** 31 - 1) == EINVAL and prompt(lib, total=2 ** 31 - 500) == EINVAL and "sizes" in err(lib)
