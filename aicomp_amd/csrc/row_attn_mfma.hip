@@ -343,7 +343,9 @@ RowPlan row_plan(const RowAttnArgs& a) {
     r.R = r.shared ? (latent || rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
     r.rows = (r.shared ? 64 : 16) * r.R;
     r.keys = r.shared ? 64 : 32;
-    r.least = r.shared ? 2 : 4;
+    // (8 skewed sequences of 2055 .. 6511 latent rows, 48 rows each: two tiles at least 37 us, three 29, four 34; trees of 36 .. 49 drafts over
+    // 500 tokens two 17.7, three 22)
+    r.least = !r.shared ? 4 : latent ? 3 : 2;
     r.row_tiles = (int)((rows + r.rows - 1) / r.rows);
     int64_t span = (int64_t)a.max_blocks * a.bs;
     if (a.longest_context > 0) span = std::min<int64_t>(span, a.longest_context);
