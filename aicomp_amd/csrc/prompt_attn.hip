@@ -8,8 +8,8 @@
 // Two tiles of 40 KB are 80 KB, so that two workgroups share a CU and one's products run beside the other's exponentials.
 // The reference of a query moves when a score passes it by 2^8 (row_attn_mfma.hip).
 //
-// Bound by the matrix cores: 8192 tokens of 16 heads 334 us, 1.03 PFLOP/s of the 1.27 that a large library product of the card reaches; 12
-// prompts of 37 .. 1500 tokens behind 0 .. 2048, 16 heads, 205 us, 0.79 PFLOP/s (tiles that are partly masked, queries beyond the last).
+// Bound by the matrix cores: 8192 tokens of 16 heads 321 us, 1.07 PFLOP/s of the 1.27 that a large library product of the card reaches; 12
+// prompts of 37 .. 1500 tokens behind 0 .. 2048, 16 heads, 200 us, 0.81 PFLOP/s (tiles that are partly masked, queries beyond the last).
 #include "row_attn.h"
 
 #include <algorithm>
@@ -264,7 +264,7 @@ prompt_attn_kernel(PromptParams p) {
         };
 #pragma unroll
         for (int u = 0; u < VAHEAD; ++u) val[u] = value_of(u);
-        __builtin_amdgcn_s_setprio(2);                             // (before the other wave's softmax: 8192 tokens 358 and 351 us)
+        __builtin_amdgcn_s_setprio(2);                             // (before the other wave's softmax: 8192 tokens 333 and 321 us)
 #pragma unroll
         for (int u = 0; u < 2 * NJ; ++u) {
             if (u + VAHEAD < 2 * NJ) val[(u + VAHEAD) % (VAHEAD + 1)] = value_of(u + VAHEAD);

@@ -16,7 +16,7 @@
 //
 // The division of the work is that of row_line.h; values that are not finite are marked as in row_attn_mfma.hip.
 //
-// 32 rows of 128 heads over 512 .. 4096 latent rows: 49 us, 407 TFLOP/s, of which the second launch 9.  A tile takes 4600 cycles, its products
+// 32 rows of 128 heads over 512 .. 4096 latent rows: 46 us, 437 TFLOP/s, of which the second launch 9.  A tile takes 4600 cycles, its products
 // 2200: the scores 1700 (LDS, which gives a key to two waves and takes in the next tile), weights 1150, the output 1300; an item's start
 // and end some 7 us, its partial output in float32, 128 KB, among them.  Tiles of 48 rows by products of 16 x 16 x 32, a wave having all
 // rows and 16 keys: 4550 cycles a tile, 59 us.

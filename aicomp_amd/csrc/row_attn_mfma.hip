@@ -12,8 +12,8 @@
 // How the work is divided: row_line.h.  Calls of more rows to a sequence and KV head are row_attn_latent.hip's (latent rows, above 16) and
 // row_attn_shared.hip's (trees, above 32): there a key that one wave reads serves too few rows.
 //
-// Bound by latency in small calls (one row of 16 heads over 700 latent rows 16 us, of which 4.5 are the second launch) and by HBM in
-// large ones: 64 rows of 16 heads over 512 .. 4096 latent rows 49 us, 3.5 TB/s of the 5.1 that a large copy reaches.
+// Bound by latency in small calls (one row of 16 heads over 700 latent rows 15.3 us, of which 4.4 are the second launch) and by HBM in
+// large ones: 64 rows of 16 heads over 512 .. 4096 latent rows 48 us, 3.6 TB/s of the 5.1 that a large copy reaches.
 #include "row_line.h"
 
 #include <algorithm>
