@@ -448,17 +448,22 @@ class ScheduleGeneration:
     @torch.no_grad()
     def draft_step(self, tokens: Sequence[Sequence[int]], parents: Sequence[Sequence[int]]) -> List[torch.Tensor]:
         """A tree of drafted tokens per sequence, ``tokens[b]`` with ``parents[b]`` (``StepPlanner.schedule_drafts``): the logits after
-        every draft, one ``[n, V]`` tensor per batch row.  ``keep_drafts`` has to follow."""
+        every draft, one ``[n, V]`` tensor per batch row.  ``keep_drafts`` has to follow.  If the model raises, the step is closed and
+        no draft stays."""
         if len(tokens) != len(self._batch) or len(parents) != len(self._batch):
             raise ValueError(f"draft_step needs one tree per sequence: got {len(tokens)} for batch {len(self._batch)}")
         if any(len(t) != len(p) for t, p in zip(tokens, parents)):
             raise ValueError("draft_step needs one parent per token")
         plan = self.planner.schedule_drafts({b: p for b, p in zip(self._batch, parents)})
-        ids = torch.as_tensor([int(x) for row in tokens for x in row], dtype=torch.int64).to(self.backend.device)
-        self.backend.begin_step(plan)
-        logits = self.model(ids, plan.positions)
+        try:
+            ids = torch.as_tensor([int(x) for row in tokens for x in row], dtype=torch.int64).to(self.backend.device)
+            self.backend.begin_step(plan)
+            logits = list(self.model(ids, plan.positions).split([len(t) for t in tokens]))
+        except BaseException:
+            self.planner.keep_drafts(plan, {})
+            raise
         self._draft_plan = plan
-        return list(logits.split([len(t) for t in tokens]))
+        return logits
 
     def keep_drafts(self, kept: Sequence[Sequence[int]]) -> None:
         """The drafts of the last ``draft_step`` that stay, one path per batch row (``accept_drafts``)."""
