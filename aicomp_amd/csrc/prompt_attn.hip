@@ -23,6 +23,7 @@ constexpr int NOPE = 128, ROPE = 64, DV = 128;
 constexpr int KT = 64;                 // keys per tile
 constexpr int NS = (NOPE + ROPE) / 32, NJ = DV / 16, NH = KT / 16;
 constexpr float NEG_BIG = -1.0e30f, SLACK = 8.f;
+constexpr float FAR = 0x1p26f;         // a reference beyond which its own rounding, 2^2 there, is no longer small beside SLACK
 
 #define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
@@ -126,6 +127,7 @@ prompt_attn_kernel(PromptParams p) {
     }
     float m[R], l[R];
     f32x4_t O[R][NJ];
+    uint32_t far = 0;                                              // bit c: some reference of group c is beyond FAR
 #pragma unroll
     for (int c = 0; c < R; ++c) {
         m[c] = NEG_BIG; l[c] = 0.f;
@@ -237,12 +239,27 @@ prompt_attn_kernel(PromptParams p) {
             if (__ballot(mx > m[c] + SLACK)) {                     // wave-uniform
                 const float m_new = fmaxf(m[c], mx), alpha = __builtin_amdgcn_exp2f(m[c] - m_new);
                 m[c] = m_new;
+                if (__ballot(fabsf(m_new) > FAR && m_new > NEG_BIG)) far |= 1u << c;
                 l[c] *= alpha;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) O[c][j] *= alpha;
             }
+            // The reference is a rounded product: against the exact ones of an fma, all weights of a row are off by its rounding.  Where that
+            // would leave the range of 16 bits, the products are rounded too.
+            float factor = p.mul, ref = m[c];
+            if (far >> c & 1) {                                    // wave-uniform
+#pragma clang fp contract(off)
+                const bool mine = fabsf(m[c]) > FAR;               // (by row: another one keeps what it has in its other tiles)
 #pragma unroll
-            for (int e = 0; e < 4 * NH; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], p.mul, -m[c]));
+                for (int e = 0; e < 4 * NH; ++e) {
+                    const float s = x[e] * p.mul;
+                    x[e] = mine ? s - m[c] : x[e];
+                }
+                factor = mine ? 1.f : p.mul;
+                ref = mine ? 0.f : m[c];
+            }
+#pragma unroll
+            for (int e = 0; e < 4 * NH; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], factor, -ref));
 #pragma unroll
             for (int hp = 0; hp < NH / 2; ++hp) {
                 pf[c][hp] = make_uint4(E::pack(x[8 * hp], x[8 * hp + 1]), E::pack(x[8 * hp + 2], x[8 * hp + 3]),

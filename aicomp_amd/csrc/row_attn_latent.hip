@@ -136,6 +136,7 @@ row_attn_latent_kernel(RowParams p) {
 
         // of rows n and 32 + n; l: of the wave's half of the rows and keys
         float m[2] = {NEG_BIG, NEG_BIG}, l = 0.f;
+        bool far = false;                                      // some reference of the wave's half of the rows is beyond FAR
         f32x16_t O[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -198,7 +199,7 @@ row_attn_latent_kernel(RowParams p) {
             }
             // element e: key 8 (e / 4) + 4 h + e % 4 of the wave's, row n
             float factor = mul;
-            if (masked) {                                      // (nothing is left to multiply: the factor may be 0)
+            if (masked || far) {                               // (nothing is left to multiply: the factor may be 0)
                 factor = 1.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sa[e] = win >> (8 * (e >> 2) + (e & 3)) & 1 ? sa[e] * mul : -INFINITY;
@@ -247,7 +248,17 @@ row_attn_latent_kernel(RowParams p) {
                     const float m_new = fmaxf(fmaxf(top[0][32 * r + n], top[1][32 * r + n]), m[r]);
                     const float alpha = __builtin_amdgcn_exp2f(m[r] - m_new);
                     m[r] = m_new;
-                    if (r == rh) l *= alpha;
+                    if (r == rh) {
+                        l *= alpha;
+                        // The reference is a rounded product: against the exact ones of an fma, all weights of a row are off by its
+                        // rounding.  Where that would leave the range of 16 bits, the products are rounded too.
+                        if (!far && __ballot(fabsf(m_new) > FAR && m_new > NEG_BIG)) {     // (alike in the two waves of a row)
+                            far = true;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sa[e] *= factor;
+                            factor = 1.f;
+                        }
+                    }
                     if (t == t_first) continue;                // (nothing to scale)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {

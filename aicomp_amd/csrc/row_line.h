@@ -51,6 +51,7 @@ namespace {
 constexpr int BS = 16;                 // tokens that are looked up together: a block, or a part of one
 constexpr float NEG_BIG = -1.0e30f;
 constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both formats' range
+constexpr float FAR = 0x1p26f;         // a reference beyond which its own rounding, 2^2 there, is no longer small beside that
 
 #define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
