@@ -22,7 +22,7 @@ namespace {
 constexpr int NOPE = 128, ROPE = 64, DV = 128;
 constexpr int KT = 64;                 // keys per tile
 constexpr int NS = (NOPE + ROPE) / 32, NJ = DV / 16, NH = KT / 16;
-constexpr float NEG_BIG = -1.0e30f, SLACK = 8.f;
+constexpr float NEG_BIG = -0x1.fffffep127f, SLACK = 8.f;         // (no score is below: the first that a row sees moves its reference)
 constexpr float FAR = 0x1p26f;         // a reference beyond which its own rounding, 2^2 there, is no longer small beside SLACK
 
 #define GLOBAL_PTR(p) ((const __attribute__((address_space(1))) void*)(p))
@@ -338,7 +338,7 @@ prompt_attn_kernel(PromptParams p) {
         l[c] += __shfl_xor(l[c], 32);
         const int row = row0 + 16 * c + r16;
         if (row >= n) continue;
-        const float inv = 1.f / l[c];                              // (a query sees itself: at least 2^-8, or not a number)
+        const float inv = 1.f / l[c];                              // (a query sees itself: at least 2^-8; not a number of a score that is not finite)
         uint16_t* o = out + (int64_t)row * p.heads * DV + 4 * g4;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)

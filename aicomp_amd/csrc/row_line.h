@@ -49,7 +49,7 @@ void launch_row_attn_latent(const RowParams& p, bool f16, int64_t items, hipStre
 namespace {
 
 constexpr int BS = 16;                 // tokens that are looked up together: a block, or a part of one
-constexpr float NEG_BIG = -1.0e30f;
+constexpr float NEG_BIG = -0x1.fffffep127f;                    // no score is below it: the first that a row sees moves its reference
 constexpr float SLACK = 8.f;           // a weight is at most 2^8: exact in both formats' range
 constexpr float FAR = 0x1p26f;         // a reference beyond which its own rounding, 2^2 there, is no longer small beside that
 

@@ -166,3 +166,29 @@ def test_prompts(name, dtype, exponent, sign):
         pytest.skip("float32 prompts have one kernel, whatever their number of heads")
     run_prompt(name, dtype, exponent, sign)
     run_prompt(name, dtype, exponent, sign, alike=True)
+
+
+# Nothing a row sees is within 1e30 = 2^99.7 of zero.  The sums of products that a score is made of are larger than it, by up to ln 2 / 0.07
+# = 2^3.3 here, and by 9 / 4 = 2^1.2 where all elements are the largest: of scores of 2^122 they stay below 2^126.5, inside float32; of
+# 2^125 they would not, and a sum that is infinite tells nothing of its keys.
+LAST = [(dtype, exponent, sign) for dtype in (BF16, F32) for exponent in (110, 122) for sign in (1, -1)]
+
+
+@pytest.mark.parametrize("dtype,exponent,sign", LAST)
+@pytest.mark.parametrize("name", LATENT)
+def test_latent_rows_to_the_end_of_float32(name, dtype, exponent, sign):
+    run_latent(name, dtype, exponent, sign)
+
+
+@pytest.mark.parametrize("dtype,exponent,sign", LAST)
+@pytest.mark.parametrize("name", TREE)
+def test_trees_to_the_end_of_float32(name, dtype, exponent, sign):
+    run_tree(name, dtype, exponent, sign)
+    run_tree(name, dtype, exponent, sign, alike=True)
+
+
+@pytest.mark.parametrize("dtype,exponent,sign", LAST)
+@pytest.mark.parametrize("name", PROMPT)
+def test_prompts_to_the_end_of_float32(name, dtype, exponent, sign):
+    run_prompt(name, dtype, exponent, sign)
+    run_prompt(name, dtype, exponent, sign, alike=True)
