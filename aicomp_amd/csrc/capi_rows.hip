@@ -13,6 +13,9 @@ using namespace aicomp;
 // tokens that a 32-bit place counts, with a tile beyond the last
 static const int64_t MAX_TOKENS = INT32_MAX - 1023;
 
+// Whether a key of two parts fits, whose sum may pass 32 bits.
+static bool key_fits(int a, int b) { return (int64_t)a + b <= MAX_KEY; }
+
 static bool float_type(int dt) { return dt == AICOMP_KV_F32 || is_16bit_float(dt); }
 
 // What both paged calls check; the sizes of a row are the caller's.
@@ -96,6 +99,7 @@ int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const flo
 
 size_t aicomp_paged_latent_workspace_bytes(int num_seqs, int64_t total_q, int max_q_len, int num_heads, int latent_dim, int rope_dim,
                                            int block_size, int max_blocks_per_seq, int dtype, int longest_context) {
+    if (latent_dim <= 0 || rope_dim < 0 || latent_dim > MAX_VALUE || !key_fits(latent_dim, rope_dim)) return 0;
     RowAttnArgs a;
     memset(&a, 0, sizeof(a));
     a.num_seqs = num_seqs; a.rows = total_q; a.max_q_len = max_q_len; a.hq = num_heads; a.hkv = 1; a.dk = latent_dim + rope_dim;
@@ -115,6 +119,8 @@ int aicomp_paged_latent_attn(void* out, const void* query, const void* pool, con
     AICOMP_REQUIRE(out && query && pool && block_table && context_lens, AICOMP_KV_EINVAL, "%s: null pointer", who);
     AICOMP_REQUIRE(latent_dim > 0 && latent_dim % 16 == 0 && rope_dim >= 0 && rope_dim % 16 == 0, AICOMP_KV_EUNSUPPORTED,
                    "%s: latent and rotated parts of %d and %d elements are not multiples of 16", who, latent_dim, rope_dim);
+    AICOMP_REQUIRE(latent_dim <= MAX_VALUE && key_fits(latent_dim, rope_dim), AICOMP_KV_EUNSUPPORTED,
+                   "%s: rows of %d + %d elements, at most %d of the latent part and %d in all", who, latent_dim, rope_dim, MAX_VALUE, MAX_KEY);
     AICOMP_REQUIRE(float_type(dtype), AICOMP_KV_EUNSUPPORTED, "%s: rows must be float32, bfloat16 or float16 (got %d)", who, dtype);
     RowAttnArgs a;
     memset(&a, 0, sizeof(a));
@@ -185,6 +191,8 @@ int aicomp_latent_prompt_attn(void* out, const void* query, const void* key, int
     AICOMP_REQUIRE(nope_dim > 0 && nope_dim % 16 == 0 && rope_dim > 0 && rope_dim % 16 == 0 && value_dim > 0 && value_dim % 16 == 0,
                    AICOMP_KV_EUNSUPPORTED, "%s: heads of %d + %d key and %d value elements are not multiples of 16", who, nope_dim,
                    rope_dim, value_dim);
+    AICOMP_REQUIRE(key_fits(nope_dim, rope_dim) && value_dim <= MAX_VALUE, AICOMP_KV_EUNSUPPORTED,
+                   "%s: heads of %d + %d key and %d value elements, at most %d and %d", who, nope_dim, rope_dim, value_dim, MAX_KEY, MAX_VALUE);
     AICOMP_REQUIRE(float_type(dtype), AICOMP_KV_EUNSUPPORTED, "%s: rows must be float32, bfloat16 or float16 (got %d)", who, dtype);
     AICOMP_REQUIRE(max_q_len > 0 && max_q_len <= total_q, AICOMP_KV_EINVAL, "%s: max_q_len %d out of range (total %lld)", who, max_q_len,
                    (long long)total_q);

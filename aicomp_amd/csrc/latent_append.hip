@@ -17,6 +17,7 @@ namespace aicomp {
 namespace {
 
 constexpr int MAX_LATENT = 1024;           // two chunks of eight elements to a lane
+constexpr int MAX_ROPE = 65536;            // (a row's elements are counted in 32 bits)
 
 struct LatentAppendParams {
     LatentAppendArgs a;
@@ -73,7 +74,7 @@ latent_append_kernel(LatentAppendParams p) {
     const uint32_t item = (blockIdx.x - p.latent_wgs) * 256 + threadIdx.x;
     if (item >= p.items) return;
     const uint32_t per = a.rope_dim / 16, row = item / per, c = item - row * per;       // lanes to a row
-    const uint32_t rows = (a.q_in ? a.heads : 0) + 1;                                   // of a token; row 0 is the shared key
+    const uint32_t rows = (a.q_in ? (uint32_t)a.heads : 0) + 1;                         // of a token; row 0 is the shared key
     const int64_t t = row / rows;
     const int h = (int)(row - (uint32_t)t * rows) - 1;
     const int a_col = 8 * c, b_col = a_col + a.rope_dim / 2;
@@ -136,13 +137,17 @@ latent_append_kernel(LatentAppendParams p) {
 }  // namespace
 
 int launch_latent_append(const LatentAppendArgs& a) {
-    AICOMP_REQUIRE(a.latent_dim <= MAX_LATENT, AICOMP_KV_EUNSUPPORTED, "latent_kv_append: latent part of %d elements, at most %d",
-                   a.latent_dim, MAX_LATENT);
+    AICOMP_REQUIRE(a.latent_dim <= MAX_LATENT && a.rope_dim <= MAX_ROPE, AICOMP_KV_EUNSUPPORTED,
+                   "latent_kv_append: latent and rotated parts of %d and %d elements, at most %d and %d", a.latent_dim, a.rope_dim, MAX_LATENT,
+                   MAX_ROPE);
     LatentAppendParams p;
     p.a = a;
-    const int64_t items = a.num_tokens * ((a.q_in ? a.heads : 0) + 1) * (a.rope_dim / 16);
+    const int64_t rows = a.num_tokens < ((int64_t)1 << 32) ? a.num_tokens * ((a.q_in ? (int64_t)a.heads : 0) + 1) : INT64_MAX;
+    const int64_t items = rows < ((int64_t)1 << 32) ? rows * (a.rope_dim / 16) : INT64_MAX;
+    AICOMP_REQUIRE(items < UINT32_MAX - 256, AICOMP_KV_EINVAL, "latent_kv_append: %lld tokens of %d heads exceed one launch",
+                   (long long)a.num_tokens, a.heads);
     const int64_t latent_wgs = (a.num_tokens + 3) / 4, wgs = latent_wgs + (items + 255) / 256;
-    AICOMP_REQUIRE(items < UINT32_MAX - 256 && wgs * 256 <= UINT32_MAX, AICOMP_KV_EINVAL,
+    AICOMP_REQUIRE(wgs * 256 <= UINT32_MAX, AICOMP_KV_EINVAL,
                    "latent_kv_append: %lld tokens of %d heads exceed one launch", (long long)a.num_tokens, a.heads);
     p.latent_wgs = (uint32_t)latent_wgs;
     p.items = (uint32_t)items;

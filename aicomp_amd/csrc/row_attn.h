@@ -11,6 +11,8 @@
 
 namespace aicomp {
 
+constexpr int MAX_KEY = 1280, MAX_VALUE = 1024;     // elements of a key and of a value row, which the entry points hold to
+
 struct RowAttnArgs {
     void* out;                  // [rows, hq, dv]
     const void* query;          // [rows, hq, dk]

@@ -16,8 +16,6 @@ namespace aicomp {
 
 namespace {
 
-constexpr int MAX_DK = 1280, MAX_DV = 1024;
-
 // four elements as floats
 template <typename T> __device__ __forceinline__ float4 load_quad(const T* p);
 template <> __device__ __forceinline__ float4 load_quad<float>(const float* p) { return *(const float4*)p; }
@@ -124,7 +122,7 @@ template <typename KV_T> struct DenseRows {
 template <typename Q_T, typename KV_T, typename ROWS>
 __global__ void __launch_bounds__(256)
 rows_generic_kernel(ROWS r, int64_t row0) {
-    __shared__ __attribute__((aligned(16))) float q[MAX_DK];
+    __shared__ __attribute__((aligned(16))) float q[MAX_KEY];
     __shared__ float weight[256];
     __shared__ float4 sums[256];
     __shared__ float red[4];
@@ -213,8 +211,6 @@ template <typename T> void launch_dense(const PromptAttnArgs& a) {
 }  // namespace
 
 int launch_rows_generic(const RowAttnArgs& a) {
-    AICOMP_REQUIRE(a.dk % 16 == 0 && a.dv % 16 == 0 && a.dk <= MAX_DK && a.dv <= MAX_DV, AICOMP_KV_EUNSUPPORTED,
-                   "rows of %d key and %d value elements are not multiples of 16 up to %d and %d", a.dk, a.dv, MAX_DK, MAX_DV);
     const bool fp8 = a.kv_dtype == AICOMP_KV_FP8_E4M3;
     if (a.q_dtype == AICOMP_KV_F32) launch_paged<float, float>(a);
     else if (a.q_dtype == AICOMP_KV_BF16) { if (fp8) launch_paged<bf16_t, fp8_t>(a); else launch_paged<bf16_t, bf16_t>(a); }
@@ -224,9 +220,6 @@ int launch_rows_generic(const RowAttnArgs& a) {
 }
 
 int launch_prompt_generic(const PromptAttnArgs& a) {
-    AICOMP_REQUIRE(a.nope % 16 == 0 && a.rope % 16 == 0 && a.dv % 16 == 0 && a.nope + a.rope <= MAX_DK && a.dv <= MAX_DV,
-                   AICOMP_KV_EUNSUPPORTED, "heads of %d + %d key and %d value elements are not multiples of 16 up to %d and %d", a.nope,
-                   a.rope, a.dv, MAX_DK, MAX_DV);
     if (a.dtype == AICOMP_KV_F32) launch_dense<float>(a);
     else if (a.dtype == AICOMP_KV_BF16) launch_dense<bf16_t>(a);
     else launch_dense<f16_t>(a);
