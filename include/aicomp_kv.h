@@ -569,8 +569,8 @@ int aicomp_kv_copy_blocks(void* const* pools, int num_pools, int64_t block_bytes
  *   q_in, q_out     [T, num_heads, rope_dim], element (t,h,d) at t*token_stride + h*head_stride + d; q_out may be q_in; both NULL: none
  *   rows_out        the rows once more, row t at t*rows_stride; NULL: not wanted
  *   slot_mapping    [T] int64 as in aicomp_kv_append (a row outside the pool is not stored; queries and rows_out are written)
- * Computed in float32 and rounded once.  F32, BF16, F16; latent_dim (at most 1024) and rope_dim multiples of 16; pointers and strides
- * 16-byte aligned.
+ * Computed in float32 and rounded once.  F32, BF16, F16; latent_dim at most 1024 and rope_dim at most 65536, multiples of 16; pointers
+ * and strides 16-byte aligned.
  */
 int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const float* weight, float eps,
                             const float* cos, const float* sin, int64_t table_stride, int64_t table_rows,
@@ -597,9 +597,10 @@ int aicomp_latent_kv_append(const void* latent, int64_t latent_stride, const flo
  *                   initialisation; may be NULL where that is 0.  Calls that may overlap need separate ones.  The bytes are those of a
  *                   call with these arguments: a smaller longest_context never needs more, but a call of fewer rows may need more
  * A row that sees nothing is zero, as are the rows of a sequence whose context is shorter than its tokens here.  Keys that a row does
- * not see may hold anything; a row that sees an element that is not finite may be not a number as a whole.
- * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16.  Matrix cores: 16 bits, 512 + 64, blocks
- * of 16, 32, 64 .. tokens.
+ * not see may hold anything; a row that sees an element that is not finite may be not a number as a whole.  Scores are float32: a row
+ * that sees one whose sum leaves that range may be not a number too, or zero.
+ * F32, BF16, F16; any block size; latent_dim (at most 1024) and rope_dim multiples of 16, latent_dim + rope_dim at most 1280.  Matrix
+ * cores: 16 bits, 512 + 64, blocks of 16, 32, 64 .. tokens.
  */
 int aicomp_paged_latent_attn(void* out, const void* query, const void* pool,
                              const int32_t* block_table, int64_t block_table_stride,
@@ -624,7 +625,8 @@ size_t aicomp_paged_latent_workspace_bytes(int num_seqs, int64_t total_q, int ma
  *                   the keys, the queries the last of its keys; one with fewer keys than queries gets zero rows, rows behind the last
  *                   sequence are left as they are
  *   max_q_len       bound of the sequences' queries
- * F32, BF16, F16; dims multiples of 16.  Matrix cores: 16 bits, 128 + 64 and 128.  Pointers and strides 16-byte aligned.
+ * F32, BF16, F16; dims multiples of 16, nope_dim + rope_dim at most 1280, value_dim at most 1024.  Matrix cores: 16 bits, 128 + 64 and
+ * 128.  Pointers and strides 16-byte aligned.  What is not finite: as in aicomp_paged_latent_attn.
  */
 int aicomp_latent_prompt_attn(void* out, const void* query,
                               const void* key, int64_t key_token_stride, int64_t key_head_stride,

@@ -1,5 +1,8 @@
-"""The largest rows of latent caches that the C ABI takes, and sizes whose sums and products pass the integers
+"""The largest rows of latent caches that the C ABI takes, as the header states them, and sizes whose sums and products pass the integers
 they are held in: refused on the host, before any device work (runs without a GPU; the pointers are never followed)."""
+import os
+import re
+
 import pytest
 
 from test_rows_validation import BF16, EINVAL, EUNSUPPORTED, F16, F32, append, err, latent, lib, prompt, tree  # noqa: F401
@@ -35,3 +38,9 @@ def test_tokens_and_heads_of_an_append(lib):
     for heads in (2 ** 31 - 1, 2 ** 31 - 2):
         for n in (2, 5, 2 ** 33):
             assert append(lib, heads=heads, n=n) == EINVAL and "one launch" in err(lib), (heads, n)
+
+def test_the_header_states_them():
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "aicomp_kv.h")).read()
+    text = re.sub(r"\s+\*?\s*", " ", text)
+    assert "latent_dim + rope_dim at most 1280" in text and "nope_dim + rope_dim at most 1280, value_dim at most 1024" in text
+    assert "rope_dim at most 65536" in text
