@@ -19,7 +19,8 @@ kernels read (``block_table``, ``context_lens``, ``slot_mapping``,
                     (``schedule_drafts``, ``keep_drafts``).  ``schedule()`` returns a ``StepPlan`` whose
                     tensors are already on the device: the whole plan is
                     packed into one pinned staging buffer and moved with a
-                    single asynchronous copy.  A step of one token per
+                    single asynchronous copy (the masks of a step of drafts
+                    by a second, blocking one).  A step of one token per
                     running sequence is selected, packed and uploaded by
                     ``csrc/fast_call.cpp`` where that is built.
 
@@ -353,7 +354,8 @@ class StepPlan:
 
 @dataclass
 class KeptDrafts:
-    """What ``StepPlanner.keep_drafts`` leaves to do in the pools: the arguments of ``ops.keep_rows``, the lengths on the host."""
+    """What ``StepPlanner.keep_drafts`` leaves to do in the pools: the arguments of ``ops.keep_rows``, the lists on the host, where they
+    are checked and from where they are copied."""
     block_table: torch.Tensor             # the plan's
     first: torch.Tensor                   # [S] int32: the position of each tree's first draft
     keep: torch.Tensor                    # int32: the drafts kept, ascending in every sequence

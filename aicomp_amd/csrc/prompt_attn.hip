@@ -9,7 +9,7 @@
 // The reference of a query moves when a score passes it by 2^8 (row_attn_mfma.hip).
 //
 // Bound by the matrix cores: 8192 tokens of 16 heads 321 us, 1.07 PFLOP/s of the 1.27 that a large library product of the card reaches; 12
-// prompts of 37 .. 1500 tokens behind 0 .. 2048, 16 heads, 200 us, 0.81 PFLOP/s (tiles that are partly masked, queries beyond the last).
+// prompts of 37 .. 1500 tokens behind 0 .. 2048, 16 heads, 203 us, 0.80 PFLOP/s (tiles that are partly masked, queries beyond the last).
 #include "row_attn.h"
 
 #include <algorithm>
@@ -60,7 +60,9 @@ prompt_attn_kernel(PromptParams p) {
     // Ragged prompts: a tile costs the keys that its last query sees, which differ several-fold, and workgroups start in the order of
     // the grid.  So the one in place i takes the tile of rank i, the dearest first.  Every workgroup finds it for itself: a tile's rank
     // is how many tiles of each sequence are dearer, which follows from the sequence's lengths.  (12 prompts of 37 .. 1500 behind 0 ..
-    // 2048, 16 heads: 235 us in the order of the grid, 200 so.)
+    // 2048, 16 heads: 254 us in the order of the grid, 223 so; 16 of 37 .. 300 behind 0 .. 300, 64 heads, 88 and 91.)  The table and the
+    // tests are of 16 sequences.  More would gain as much (measured in a copy, 17 of 37 .. 1500: 316 and 287; 40 of 37 .. 700: 395 and 317;
+    // 64 of 37 .. 124: 153 and 135) and take the order of the grid so far.
     const int nseq = gridDim.y, ntile = gridDim.z;
     if (nseq > 1 && nseq <= 16 && nseq * ntile <= 512) {                   // grid-uniform
         int* const tab = (int*)k0;                                         // [nseq][3]: context, prior, tiles; then the one found

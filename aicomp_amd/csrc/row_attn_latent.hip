@@ -12,7 +12,11 @@
 //
 // With one wave to a SIMD nothing hides what a wave waits for, or issues beside the products: products of 32 x 32 x 16, so that there are
 // few of them and each covers the reads ahead and the next tile's loads, one of which goes out every other product or so (all eighteen
-// at once hold the wave up for as long as the scores take).
+// at once hold the wave up for as long as the scores take).  395 of a wave's 512 registers are taken; what else might be begun beside a
+// tile's softmax has room there.
+//
+// Causal chunks are taken like trees: an item has the keys of the whole context, those behind its last row too, which are masked.  2048 tokens
+// of a new prompt, 16 heads: 199 us, about half of the products for nothing; 512 tokens behind 4096: 96 us, 0.80 PFLOP/s.
 //
 // The division of the work is that of row_line.h; values that are not finite are marked as in row_attn_mfma.hip.
 //

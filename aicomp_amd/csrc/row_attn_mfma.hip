@@ -340,6 +340,8 @@ RowPlan row_plan(const RowAttnArgs& a) {
     const int64_t rows = (int64_t)a.max_q_len * group;
     RowPlan r;
     r.shared = rows > (latent ? 16 : 32);
+    // (two groups to a wave at head_dim 256 too, where they spill: row_attn_shared.hip; here over fp8 pools 17 registers, 32 trees of 4 .. 8
+    // drafts, 8 KV heads of 4, over 512 .. 4096 tokens 93 us, 3.3 TB/s)
     r.R = r.shared ? (latent || rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : 2;
     r.rows = (r.shared ? 64 : 16) * r.R;
     r.keys = r.shared ? 64 : 32;

@@ -8,7 +8,12 @@
 //
 // Bound by LDS, which gives every key and value to four waves (1024 cycles of a tile of 128 rows and head_dim 128, its products 1024 too),
 // and by the partial outputs: 32 trees of 16 .. 64 drafts, 8 KV heads of 4, over 512 .. 4096 tokens 112 us, 456 TFLOP/s, of which the
-// second launch 15 (without loads 82, loads alone 84).  One tree of 24 drafts over 700 tokens: 11 us, of which the second launch 4.5.
+// second launch 15 (without loads 82, loads alone 84); over fp8 pools 105; head_dim 64 70, and 68 over fp8.  One tree of 24 drafts over 700
+// tokens: 11 us, of which the second launch 4.5.
+//
+// Two groups of rows to a wave at head_dim 256 are more than its registers hold: 17 of them go by way of memory, 45 over fp8 pools (2 at head_dim
+// 128).  They are right all the same in 16 bits, where a key serves twice the rows: the 32 trees 276 us, with one group 347 (back to back
+// over two sets of pools; over fp8 pools 295 and 276).
 #include "row_line.h"
 
 namespace aicomp {

@@ -237,10 +237,10 @@ class LatentAttentionBackend:
 
     A token's cache row is one latent vector of ``latent_dim`` elements, normed, and ``rope_dim`` rotated ones, shared by all heads.
     ``set_layer`` gives a layer its norm and the two halves of its up-projection, ``w_k [H, N, C]`` (latent to a head's key) and
-    ``w_v [H, V, C]`` (to its value); they are laid out once.  Prompts that start a sequence are attended in the expanded form (keys and
-    values of every head made by one product, ``ops.latent_prompt_attn``) where N, D and V are multiples of 16; all other rows, one token per
-    sequence, later chunks and trees of drafts, over the latent rows themselves, ``w_k`` multiplied into the queries and ``w_v`` into
-    the output.
+    ``w_v [H, V, C]`` (to its value); they are laid out once.  In a step all of whose chunks start their sequences, they are attended in
+    the expanded form (keys and values of every head made by one product, ``ops.latent_prompt_attn``) where N, D and V are multiples of
+    16.  All other rows, one token per sequence, trees of drafts, later chunks and what starts beside one, are attended over the latent
+    rows themselves, ``w_k`` multiplied into the queries and ``w_v`` into the output; the two forms differ by their roundings.
     """
 
     def __init__(self, num_layers: int, num_blocks: int, latent_dim: int, rope_dim: int, inv_freq: torch.Tensor,

@@ -1124,11 +1124,11 @@ def paged_latent_attn(out: torch.Tensor, query: torch.Tensor, pool: torch.Tensor
     """Attention over paged latent rows, absorbed: ``out[t, h] = softmax(scale q[t, h] . row_j) row_j[:C]``.
 
     ``query [T, H, C + D]`` (each head's key projection multiplied in already, its rotated part behind), ``out [T, H, C]``, ``pool
-    [num_blocks, block_size, C + D]``, C and D multiples of 16, C at most 1024 and C + D at most 1280.  One token per sequence; or, with ``cu_q_lens [S+1]``, the last tokens of each sequence, causal,
-    or by ``tree_masks [T, words]`` (``tree_masks``) the drafts of a tree over what is cached before them.  A row that sees nothing is
-    zero; rows behind the last sequence are left as they are.  ``max_q_len``: the host's bound of the sequences' tokens (``None``: read
-    back from ``cu_q_lens``); ``longest_context``: its bound of ``context_lens`` (0: the table's width), which sizes the call and cuts
-    no row.  In place on ``out``, on the current stream.
+    [num_blocks, block_size, C + D]``, C and D multiples of 16, C at most 1024 and C + D at most 1280.  One token per sequence; or,
+    with ``cu_q_lens [S+1]``, the last tokens of each sequence, causal, or by ``tree_masks [T, words]`` (``tree_masks``) the drafts of a
+    tree over what is cached before them.  A row that sees nothing is zero; rows behind the last sequence are left as they are.
+    ``max_q_len``: the host's bound of the sequences' tokens (``None``: read back from ``cu_q_lens``); ``longest_context``: its bound of
+    ``context_lens`` (0: the table's width), which sizes the call and cuts no row.  In place on ``out``, on the current stream.
     """
     if _native("aicomp_paged_latent_attn") and _FAST.paged_latent_attn(out, query, pool, block_table, context_lens, scale, cu_q_lens,
                                                                        1 if cu_q_lens is None else max_q_len, tree_masks, longest_context):
@@ -1204,9 +1204,9 @@ def latent_prompt_attn(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     """Causal attention of prompts over expanded latent rows: head h's key is ``key[u, h]`` with ``rope_key[u]`` behind it.
 
     ``query [Tq, H, N + D]``, ``key [Tk, H, N]``, ``rope_key [Tk, D]`` (shared by the heads), ``value [Tk, H, V]``, ``out [Tq, H, V]``;
-    multiples of 16, N + D at most 1280 and V at most 1024; key, value and rope_key may be slices of wider tensors.  Tokens ``cu_q_lens[s]:cu_q_lens[s+1]`` are the last of the keys
-    ``cu_k_lens[s]:cu_k_lens[s+1]`` of sequence s; one with fewer keys than queries gets zero rows, and rows behind the last sequence are
-    left as they are.  ``max_q_len``: the host's bound of the sequences' queries (``None``: read back).  In place on ``out``, on the
+    multiples of 16, N + D at most 1280 and V at most 1024; key, value and rope_key may be slices of wider tensors.  Tokens
+    ``cu_q_lens[s]:cu_q_lens[s+1]`` are the last of the keys ``cu_k_lens[s]:cu_k_lens[s+1]`` of sequence s; one with fewer keys than
+    queries gets zero rows, and rows behind the last sequence are left as they are.  ``max_q_len``: the host's bound of the sequences' queries (``None``: read back).  In place on ``out``, on the
     current stream.
     """
     if _native("aicomp_latent_prompt_attn") and _FAST.latent_prompt_attn(out, query, key, rope_key, value, cu_q_lens, cu_k_lens, scale,
