@@ -79,6 +79,15 @@ def test_trees_of_large_tiles_divided(device, d, dtype, pool):
     c.check(got[0])
 
 
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (12, 4), (16, 1)])
+@pytest.mark.parametrize("dtype,pool", [(BF16, None), (F16, None), (F32, None), (BF16, FP8), (F16, FP8)])
+def test_long_trees_of_other_heads(hq, hkv, dtype, pool):
+    for d in (64, 128, 256):
+        c = Tree([4100, 700], [9, 64], hq, hkv, d, dtype=dtype, pool=pool, seed=47, rows_behind=3)
+        c.poison()
+        c.check(c.run(max_q_len=64, longest_context=4100))
+
+
 def test_large_tiles_of_trees_beside_drafts_that_are_not_finite():
     ctx, new = TREES
     for dtype, pool, which in ((BF16, None, "v"), (F16, None, "v"), (F16, FP8, "v"), (BF16, None, "k")):
