@@ -257,6 +257,7 @@ row_attn_latent_kernel(RowParams p) {
                         // The reference is a rounded product: against the exact ones of an fma, all weights of a row are off by its
                         // rounding.  Where that would leave the range of 16 bits, the products are rounded too.
                         if (!far && __ballot(fabsf(m_new) > FAR && m_new > NEG_BIG)) {     // (alike in the two waves of a row)
+#pragma clang fp contract(off)
                             far = true;
 #pragma unroll
                             for (int e = 0; e < 16; ++e) sa[e] *= factor;

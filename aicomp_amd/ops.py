@@ -1206,8 +1206,8 @@ def latent_prompt_attn(out: torch.Tensor, query: torch.Tensor, key: torch.Tensor
     ``query [Tq, H, N + D]``, ``key [Tk, H, N]``, ``rope_key [Tk, D]`` (shared by the heads), ``value [Tk, H, V]``, ``out [Tq, H, V]``;
     multiples of 16, N + D at most 1280 and V at most 1024; key, value and rope_key may be slices of wider tensors.  Tokens
     ``cu_q_lens[s]:cu_q_lens[s+1]`` are the last of the keys ``cu_k_lens[s]:cu_k_lens[s+1]`` of sequence s; one with fewer keys than
-    queries gets zero rows, and rows behind the last sequence are left as they are.  ``max_q_len``: the host's bound of the sequences' queries (``None``: read back).  In place on ``out``, on the
-    current stream.
+    queries gets zero rows, and rows behind the last sequence are left as they are.  ``max_q_len``: the host's bound of the sequences'
+    queries (``None``: read back).  In place on ``out``, on the current stream.
     """
     if _native("aicomp_latent_prompt_attn") and _FAST.latent_prompt_attn(out, query, key, rope_key, value, cu_q_lens, cu_k_lens, scale,
                                                                          max_q_len):
